@@ -381,6 +381,110 @@ int lvar_window_key_scores(lvar_tensor_t q, lvar_tensor_t k, const int64_t* wind
                            float* scores, int B, int H, int Lq, int Lk, int head_dim,
                            int pool_kernel_size, int max_pool, float scale, void* stream);
 
+/*
+ * ---- Norms, rotation and a paged key/value cache ----
+ *
+ * A paged cache: rows of head_dim keys or values in pages [num_pages, kv_heads, page_size, head_dim], either bf16 (k_exp and
+ * v_exp NULL) or e4m3 codes with one power of two per row, value = code * 2^(byte - 127), bytes uint8
+ * [num_pages, kv_heads, page_size] with unit stride along the page.  k and v share the strides (in elements; rows 16-byte
+ * aligned), k_exp and v_exp theirs (multiples of 4, 4-byte aligned bases).  page_size is a power of two from 16 to 1024, head_dim 64, 128 or 256.
+ * page_table int32 [B, max_pages]: token n of sequence b is row n % page_size of page page_table[b, n / page_size].  Entries
+ * outside [0, num_pages) name no page: such a token is not written, reads as zeros and takes no part in an attention.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+  int64_t stride_page, stride_head, stride_row;
+  int64_t exp_stride_page, exp_stride_head;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int num_pages, kv_heads, page_size, head_dim, max_pages;
+} lvar_paged_cache_t;
+
+/* Factors on normalised heads: fp32 or bf16 (dtype 0 / 1), [heads, head_dim] by strides: stride_head 0 = shared by the heads,
+ * stride_col 0 or 1 (0: one factor per head; 1: 16-byte aligned rows).  ptr NULL: none. */
+typedef struct {
+  const void* ptr;
+  int64_t stride_head;
+  int stride_col;
+  int dtype;
+} lvar_weight_t;
+
+#define LVAR_NORM_NONE 0
+#define LVAR_NORM_L2 1   /* x / max(|x|, eps) */
+#define LVAR_NORM_RMS 2  /* x / sqrt(mean(x^2) + eps) */
+
+/*
+ * The norm and the rotation: y = R(w * norm(x)).  The first rot_dim columns (a multiple of 16, at most head_dim) are rotated in pairs
+ * (2i, 2i+1) if interleaved, else (i, i + rot_dim/2), by the angles whose cosines and sines are rows of cos and sin (fp32
+ * [table_rows, rot_dim/2], row stride table_stride, 16-byte aligned rows; NULL: no rotation).  positions (int32, or int64 if
+ * positions64; strides in elements, 0 broadcasts) gives the row of each token, clamped to the table; NULL: the token's number
+ * in the call, plus start[b] where there is one.
+ */
+typedef struct {
+  int norm;
+  float eps;
+  lvar_weight_t q_weight, k_weight;
+  const float* cos;
+  const float* sin;
+  int64_t table_stride;
+  int table_rows, rot_dim, interleaved;
+  const void* positions;
+  int64_t pos_stride_b, pos_stride_row;
+  int positions64;
+} lvar_norm_rope_t;
+
+/*
+ * oq, ok = the norm and rotation of q [B,H,L,d] and k [B,kv_heads,L,d] (bf16 views), contiguous bf16.  head_dim 16, 32, 64, 128 or 256.
+ * The eager counterpart: L2 norm, learned factor and rotary embedding of models/sparvar/basic_sparvar.py:326-342.
+ */
+int lvar_qk_norm_rope_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, void* oq, void* ok, int B, int H, int kv_heads,
+                          int L, int head_dim, void* stream);
+
+/*
+ * Gradients of lvar_qk_norm_rope_fwd: from q, k and the contiguous bf16 gradients gq, gk of its outputs, dq and dk (bf16 views) and
+ * the weight gradients dqw, dkw (NULL: not wanted; contiguous, [heads or 1, head_dim or 1] as the weight's strides say, of its type).
+ * scratch: lvar_qk_norm_rope_bwd_scratch_bytes() (16-byte aligned; needed for weight gradients only), written and read by this call.
+ * Sums over tokens are formed in a fixed order.
+ */
+int64_t lvar_qk_norm_rope_bwd_scratch_bytes(int B, int H, int kv_heads, int L, int head_dim);
+int lvar_qk_norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, const void* gq, const void* gk, lvar_tensor_t dq,
+                          lvar_tensor_t dk, void* dqw, void* dkw, void* scratch, int64_t scratch_bytes, int B, int H,
+                          int kv_heads, int L, int head_dim, void* stream);
+
+/*
+ * Writes the L tokens of k and v [B,kv_heads,L,d] (bf16 views) to positions start[b] .. of the cache (int32 start[B]; counts int32 [B]
+ * or NULL: only the first counts[b] tokens of a sequence).  With how and oq (both or neither), k is normalised and rotated on its way,
+ * and so are the queries q [B,H,L,d], into oq (contiguous bf16, all L rows).  e4m3 caches: the byte of a row is the smallest one
+ * from 1 on with max|x| <= 448 * 2^(byte - 127), codes are rounded to nearest even from fp32, infinities become NaN.  Positions outside
+ * the table are dropped.  Two tokens of one call that go to the same row leave it undefined.
+ */
+int lvar_kv_cache_append(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, const lvar_norm_rope_t* how, void* oq, lvar_paged_cache_t cache,
+                         const int32_t* start, const int32_t* counts, int B, int H, int L, void* stream);
+
+/*
+ * Tokens start[b] .. start[b] + max_len - 1 of the cache (start NULL: 0) as contiguous bf16 k, v [B,kv_heads,max_len,d]; zeros from
+ * lengths[b] on.
+ */
+int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int32_t* lengths, void* k, void* v, int B, int max_len,
+                       void* stream);
+
+/*
+ * Attention of the newest Lq tokens q [B,H,Lq,d] (bf16 view) over the first lengths[b] tokens of the cache, which hold them already:
+ * o = softmax(q k^T scale) v (contiguous bf16), M and L fp32 [B,H,Lq] as everywhere here.  causal: row i of sequence b sees tokens
+ * j < lengths[b] - n + i + 1, n = counts[b] (NULL: Lq) its new tokens; rows i >= n, and rows that see no token, get o = 0, M = -inf, L = 1.
+ * Query head h reads key/value head h / (H / kv_heads).  Lengths are clamped to max_len (at most max_pages * page_size).
+ * workspace: lvar_paged_attn_workspace_bytes() (16-byte aligned, its contents need no preparation; calls that overlap in time
+ * need one each); without one, or with a smaller one, no sequence is cut and long ones are slow.  Results depend on the lengths of all
+ * sequences of the call in the last bits (they decide where sequences are cut), not on timing.
+ */
+int64_t lvar_paged_attn_workspace_bytes(int B, int H, int kv_heads, int Lq, int max_len, int head_dim);
+int lvar_paged_attn_fwd(lvar_tensor_t q, lvar_paged_cache_t cache, const int32_t* lengths, const int32_t* counts, void* o, float* M,
+                        float* L, void* workspace, int64_t workspace_bytes, int B, int H, int Lq, int max_len, int causal,
+                        float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,8 @@ EXPORTED_SYMBOLS = (
     "lvar_block_sparse_attn_ws_fwd", "lvar_block_sparse_attn_static_fwd",
     "lvar_block_topk_lists", "lvar_topk_token_lists", "lvar_topk_union_lists", "lvar_remap_concat_lists", "lvar_mask_to_lists",
     "lvar_window_key_scores",
+    "lvar_qk_norm_rope_fwd", "lvar_qk_norm_rope_bwd_scratch_bytes", "lvar_qk_norm_rope_bwd", "lvar_kv_cache_append", "lvar_kv_cache_read",
+    "lvar_paged_attn_workspace_bytes", "lvar_paged_attn_fwd",
 )
 
 
@@ -29,6 +31,23 @@ class LvarTensor(C.Structure):
 
 class LvarWorkspace(C.Structure):
     _fields_ = [("ptr", C.c_void_p), ("bytes", C.c_int64), ("min_share_tiles", C.c_int), ("min_piece_tiles", C.c_int)]
+
+
+class LvarPagedCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+                ("stride_page", C.c_int64), ("stride_head", C.c_int64), ("stride_row", C.c_int64),
+                ("exp_stride_page", C.c_int64), ("exp_stride_head", C.c_int64), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("num_pages", C.c_int), ("kv_heads", C.c_int), ("page_size", C.c_int), ("head_dim", C.c_int), ("max_pages", C.c_int)]
+
+
+class LvarWeight(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride_head", C.c_int64), ("stride_col", C.c_int), ("dtype", C.c_int)]
+
+
+class LvarNormRope(C.Structure):
+    _fields_ = [("norm", C.c_int), ("eps", C.c_float), ("q_weight", LvarWeight), ("k_weight", LvarWeight), ("cos", C.c_void_p), ("sin", C.c_void_p),
+                ("table_stride", C.c_int64), ("table_rows", C.c_int), ("rot_dim", C.c_int), ("interleaved", C.c_int), ("positions", C.c_void_p),
+                ("pos_stride_b", C.c_int64), ("pos_stride_row", C.c_int64), ("positions64", C.c_int)]
 
 
 class LvarError(RuntimeError):
@@ -108,6 +127,21 @@ def load() -> C.CDLL:
     lib.lvar_mask_to_lists.argtypes = [P, I64, P, I64, P, I, I, I, P]
     lib.lvar_window_key_scores.restype = I
     lib.lvar_window_key_scores.argtypes = [T, T, P, I, P, I, I, I, I, I, I, I, F, P]
+    N, G = LvarNormRope, LvarPagedCache
+    lib.lvar_qk_norm_rope_fwd.restype = I
+    lib.lvar_qk_norm_rope_fwd.argtypes = [T, T, N, P, P, I, I, I, I, I, P]
+    lib.lvar_qk_norm_rope_bwd_scratch_bytes.restype = I64
+    lib.lvar_qk_norm_rope_bwd_scratch_bytes.argtypes = [I, I, I, I, I]
+    lib.lvar_qk_norm_rope_bwd.restype = I
+    lib.lvar_qk_norm_rope_bwd.argtypes = [T, T, N, P, P, T, T, P, P, P, I64, I, I, I, I, I, P]
+    lib.lvar_kv_cache_append.restype = I
+    lib.lvar_kv_cache_append.argtypes = [T, T, T, P, P, G, P, P, I, I, I, P]
+    lib.lvar_kv_cache_read.restype = I
+    lib.lvar_kv_cache_read.argtypes = [G, P, P, P, P, I, I, P]
+    lib.lvar_paged_attn_workspace_bytes.restype = I64
+    lib.lvar_paged_attn_workspace_bytes.argtypes = [I, I, I, I, I, I]
+    lib.lvar_paged_attn_fwd.restype = I
+    lib.lvar_paged_attn_fwd.argtypes = [T, G, P, P, P, P, P, P, I64, I, I, I, I, I, F, P]
     _lib = lib
     return lib
 

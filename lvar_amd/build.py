@@ -18,12 +18,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "liblvar_sparse_attn.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-SOURCES = ["attn_fwd.hip", "colsum.hip", "rowlse.hip", "blockscore.hip", "masklist.hip", "listbuild.hip", "windowscore.hip", "capi.hip"]
+SOURCES = ["attn_fwd.hip", "colsum.hip", "rowlse.hip", "blockscore.hip", "masklist.hip", "listbuild.hip", "windowscore.hip", "capi.hip",
+           "normrope.hip", "kvread.hip", "pagedattn.hip", "kvcapi.hip"]
 ARCH = "gfx950"
 # -packed-fp32-ops is switched off: hipcc must not form v_pk_{add,mul,fma}_f32 from float code
 # -fno-honor-nans -mno-amdgpu-ieee: max/min map to single v_max/v_max3 without NaN-quieting copies
 HIPCC_FLAGS = ["-O3", f"--offload-arch={ARCH}", "-fPIC", "-std=c++17", "-fno-honor-nans", "-mno-amdgpu-ieee",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# these keep NaN as NaN (a cache may hold some in places that nobody reads, and what is read has to show them)
+HONOR_NANS = ("normrope.hip", "kvread.hip", "pagedattn.hip", "kvcapi.hip")
 
 
 def _hipcc() -> str:
@@ -50,7 +53,8 @@ def build_library(verbose: bool = False) -> str:
 
     def compile_one(pair):
         src, obj = pair
-        return _run([hipcc, *HIPCC_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj])
+        flags = [f for f in HIPCC_FLAGS if src not in HONOR_NANS or f not in ("-fno-honor-nans", "-mno-amdgpu-ieee")]
+        return _run([hipcc, *flags, "-c", os.path.join(CSRC, src), "-o", obj])
 
     with ThreadPoolExecutor(max_workers=min(4, len(SOURCES))) as ex:
         outs = list(ex.map(compile_one, zip(SOURCES, objs)))
