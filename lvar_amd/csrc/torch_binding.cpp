@@ -4,6 +4,7 @@
 //   fast_*                            the operators of lvar_amd.sparse_attn_ops and the two steps of SparseDiffAttn for
 //                                     well-formed inputs on the current device; every other input returns None and takes
 //                                     the Python path, which raises the errors
+//                                     (and of lvar_amd.kv_cache_ops, qk_norm_rope with its gradients)
 //   register_dense_attn(ns)           defines and implements the torch-library op
 //                                     `<ns>::dense_attn(Tensor q, Tensor k, Tensor v) -> Tensor[]`
 //                                     natively, as the reference registers torch.ops.chipmunk.dense_attn
@@ -15,7 +16,9 @@
 //
 // The module does not link the C-ABI library: bind() receives the entry points' addresses from the Python
 // side (which has loaded the library with ctypes), so both paths always call the same library.
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <memory>
 #include <optional>
 #include <string>
@@ -24,6 +27,7 @@
 #include <torch/library.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/core/DeviceGuard.h>
@@ -38,7 +42,9 @@ namespace {
   X(lvar_lse2_from_stats) X(lvar_colsum_fwd) X(lvar_csp_attn_fwd) X(lvar_csp_attn_upsample_fwd)                           \
   X(lvar_csp_attn_remap_fwd)                                                                                              \
   X(lvar_block_sparse_attn_fwd) X(lvar_block_topk_lists) X(lvar_topk_token_lists) X(lvar_topk_union_lists)                \
-  X(lvar_remap_concat_lists) X(lvar_mask_to_lists) X(lvar_window_key_scores)
+  X(lvar_remap_concat_lists) X(lvar_mask_to_lists) X(lvar_window_key_scores)                                              \
+  X(lvar_qk_norm_rope_fwd) X(lvar_qk_norm_rope_bwd_scratch_bytes) X(lvar_qk_norm_rope_bwd) X(lvar_kv_cache_append)        \
+  X(lvar_kv_cache_read) X(lvar_paged_attn_workspace_bytes) X(lvar_paged_attn_fwd)
 struct Api {
 #define LVAR_FIELD(name) decltype(&::name) name = nullptr;
   LVAR_ENTRIES(LVAR_FIELD)
@@ -498,6 +504,292 @@ LVAR_FAST(fast_window_keys) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- norms with rotation, the paged cache, attention over it (lvar_amd.kv_cache_ops) ----
+
+// a tensor or None; false: neither
+bool optional_tensor(PyObject* o, const at::Tensor*& t) {
+  t = o == Py_None ? nullptr : tensor(o);
+  return o == Py_None || t;
+}
+
+bool wants_grad(const at::Tensor* t) { return t && t->requires_grad() && at::GradMode::is_enabled(); }
+
+// int32 [B] on the device, or nothing
+bool per_sequence(const at::Tensor* t, int64_t B, int dev) { return !t || (packed(t, dev, at::kInt) && t->dim() == 1 && t->size(0) == B); }
+const int32_t* ints(const at::Tensor* t) { return t ? t->data_ptr<int32_t>() : nullptr; }
+
+bool same_strides(const at::Tensor& a, const at::Tensor& b, int64_t dims) {
+  for (int64_t i = 0; i < dims; i++)
+    if (a.size(i) != b.size(i) || (a.size(i) > 1 && a.stride(i) != b.stride(i))) return false;
+  return true;
+}
+
+// a[0..4]: k, v, k_exp, v_exp, page table (the entry points check alignments and limits)
+bool cache_ok(PyObject* const* a, int64_t B, int dev, lvar_paged_cache_t& c) {
+  const at::Tensor *k = tensor(a[0]), *v = tensor(a[1]), *table = tensor(a[4]), *ke, *ve;
+  if (!k || !v || !table || !optional_tensor(a[2], ke) || !optional_tensor(a[3], ve)) return false;
+  const bool f8 = k->scalar_type() == at::kFloat8_e4m3fn;
+  if ((!f8 && k->scalar_type() != at::kBFloat16) || v->scalar_type() != k->scalar_type() || k->dim() != 4 || v->dim() != 4) return false;
+  if (!k->is_cuda() || k->get_device() != dev || !v->is_cuda() || v->get_device() != dev || !same_strides(*k, *v, 4)) return false;
+  if (k->stride(3) != 1 || v->stride(3) != 1 || k->numel() == 0) return false;
+  for (int i = 0; i < 4; i++) if (k->size(i) > INT32_MAX) return false;
+  c = {};
+  if (f8) {
+    if (!ke || !ve) return false;
+    for (const at::Tensor* e : {ke, ve}) {
+      if (!e->is_cuda() || e->get_device() != dev || e->scalar_type() != at::kByte || e->dim() != 3 || e->stride(2) != 1) return false;
+      for (int i = 0; i < 3; i++) if (e->size(i) != k->size(i)) return false;
+    }
+    if (!same_strides(*ke, *ve, 3)) return false;
+    c.k_exp = ke->data_ptr<uint8_t>(); c.v_exp = ve->data_ptr<uint8_t>();
+    c.exp_stride_page = ke->size(0) > 1 ? ke->stride(0) : 0; c.exp_stride_head = ke->size(1) > 1 ? ke->stride(1) : 0;
+  } else if (ke || ve) {
+    return false;
+  }
+  if (!table->is_cuda() || table->get_device() != dev || table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) != B ||
+      table->size(1) <= 0 || table->size(1) > INT32_MAX || (table->stride(1) != 1 && table->size(1) > 1))
+    return false;
+  c.k = k->data_ptr(); c.v = v->data_ptr();
+  c.stride_page = k->size(0) > 1 ? k->stride(0) : 0; c.stride_head = k->size(1) > 1 ? k->stride(1) : 0; c.stride_row = k->stride(2);
+  c.page_table = table->data_ptr<int32_t>(); c.table_stride = B > 1 ? table->stride(0) : 0;
+  c.num_pages = static_cast<int>(k->size(0)); c.kv_heads = static_cast<int>(k->size(1)); c.page_size = static_cast<int>(k->size(2));
+  c.head_dim = static_cast<int>(k->size(3)); c.max_pages = static_cast<int>(table->size(1));
+  return true;
+}
+
+bool weight_ok(const at::Tensor* w, int64_t heads, int64_t d, int dev, lvar_weight_t& v) {
+  v = {};
+  if (!w) return true;
+  if (!w->is_cuda() || w->get_device() != dev || (w->scalar_type() != at::kFloat && w->scalar_type() != at::kBFloat16)) return false;
+  const int64_t n = w->dim(), rows = n == 2 ? w->size(0) : 1, cols = n == 2 ? w->size(1) : n == 1 ? w->size(0) : 0;
+  if ((n != 1 && n != 2) || (rows != 1 && rows != heads) || (cols != d && (cols != 1 || n == 1))) return false;
+  if ((rows > 1 && w->stride(0) == 0) || (cols > 1 && w->stride(n - 1) != 1)) return false;
+  v.ptr = w->data_ptr(); v.stride_head = rows > 1 ? w->stride(0) : 0; v.stride_col = cols > 1 ? 1 : 0; v.dtype = w->scalar_type() == at::kBFloat16;
+  return true;
+}
+
+// what a call says about the norm and the rotation, apart from the weights
+struct How {
+  lvar_norm_rope_t h;
+  const at::Tensor *cos, *sin, *positions;
+};
+
+// a: cos, sin, positions, q_weight, k_weight, norm, eps, interleaved
+bool how_ok(PyObject* const* a, const at::Tensor& q, const at::Tensor& k, int dev, bool needs_rows, How& w, const at::Tensor*& wq, const at::Tensor*& wk) {
+  const int64_t B = q.size(0), L = q.size(2), d = q.size(3);
+  w.h = {};
+  if (!optional_tensor(a[0], w.cos) || !optional_tensor(a[1], w.sin) || !optional_tensor(a[2], w.positions) || !optional_tensor(a[3], wq) || !optional_tensor(a[4], wk)) return false;
+  if (a[5] == Py_None) { w.h.norm = LVAR_NORM_NONE; w.h.eps = 0.f; }
+  else if (PyUnicode_Check(a[5]) && PyUnicode_CompareWithASCIIString(a[5], "l2") == 0) { w.h.norm = LVAR_NORM_L2; w.h.eps = 1e-12f; }
+  else if (PyUnicode_Check(a[5]) && PyUnicode_CompareWithASCIIString(a[5], "rms") == 0) { w.h.norm = LVAR_NORM_RMS; w.h.eps = 1e-6f; }
+  else return false;
+  double eps;
+  bool inter;
+  if (a[6] != Py_None) { if (!as_double(a[6], eps)) return false; w.h.eps = static_cast<float>(eps); }
+  if (!as_bool(a[7], inter)) return false;
+  if (!w.cos != !w.sin) return false;
+  if (w.cos) {
+    for (const at::Tensor* t : {w.cos, w.sin})
+      if (!t->is_cuda() || t->get_device() != dev || t->scalar_type() != at::kFloat || t->dim() != 2 || t->stride(1) != 1 || t->requires_grad()) return false;
+    if (w.cos->sizes() != w.sin->sizes() || w.cos->stride(0) != w.sin->stride(0) || w.cos->size(0) <= 0 || w.cos->size(0) > INT32_MAX || 2 * w.cos->size(1) > d) return false;
+    if (needs_rows && !w.positions && w.cos->size(0) < L) return false;
+    w.h.cos = w.cos->data_ptr<float>(); w.h.sin = w.sin->data_ptr<float>(); w.h.table_stride = w.cos->stride(0);
+    w.h.table_rows = static_cast<int>(w.cos->size(0)); w.h.rot_dim = static_cast<int>(2 * w.cos->size(1)); w.h.interleaved = inter;
+  }
+  if (w.positions) {
+    const at::Tensor& p = *w.positions;
+    const int64_t n = p.dim();
+    if (!p.is_cuda() || p.get_device() != dev || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong)) return false;
+    if ((n != 1 && n != 2) || p.size(n - 1) != L || (n == 2 && p.size(0) != B)) return false;
+    w.h.positions = p.data_ptr(); w.h.positions64 = p.scalar_type() == at::kLong;
+    w.h.pos_stride_b = n == 2 && B > 1 ? p.stride(0) : 0; w.h.pos_stride_row = p.stride(n - 1);
+  }
+  return weight_ok(wq, q.size(1), d, dev, w.h.q_weight) && weight_ok(wk, k.size(1), d, dev, w.h.k_weight);
+}
+
+// q and k of a norm on the current device
+bool qk_ok(const at::Tensor* q, const at::Tensor* k, int& dev, void*& stream) {
+  if (!bound || !q || !k || !q->is_cuda()) return false;
+  dev = q->get_device();
+  if (!rows_ok(q, dev) || !rows_ok(k, dev) || q->numel() == 0 || k->numel() == 0) return false;
+  if (q->size(0) != k->size(0) || q->size(2) != k->size(2) || q->size(3) != k->size(3) || q->size(1) % k->size(1) != 0) return false;
+  for (int i = 0; i < 3; i++) if (q->size(i) > INT32_MAX) return false;
+  if (c10::hip::current_device() != dev) return false;
+  stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  return true;
+}
+
+int dim(const at::Tensor& t, int i) { return static_cast<int>(t.size(i)); }
+
+int norm_rope_launch(const at::Tensor& q, const at::Tensor& k, const lvar_norm_rope_t& h, at::Tensor& oq, at::Tensor& ok, int dev, void* stream) {
+  oq = empty(q.sizes(), at::kBFloat16, dev);
+  ok = empty(k.sizes(), at::kBFloat16, dev);
+  return api.lvar_qk_norm_rope_fwd(view(q), view(k), h, oq.data_ptr(), ok.data_ptr(), dim(q, 0), dim(q, 1), dim(k, 1), dim(q, 2), dim(q, 3), stream);
+}
+
+// memory for a gradient of t in t's own order of axes, if the kernels can write it
+at::Tensor rows_like(const at::Tensor& t) {
+  at::Tensor g = at::empty_like(t);
+  const auto st = g.strides();
+  return st[3] == 1 && ((st[0] | st[1] | st[2]) & 7) == 0 ? g : at::empty(t.sizes(), t.options());
+}
+
+// The C call's arguments that are not tensors travel in `h`; its pointers are set anew from the saved tensors.
+struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
+  using Maybe = std::optional<at::Tensor>;   // (undefined tensors are no inputs)
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const Maybe& wq,
+                                                const Maybe& wk, const Maybe& cos, const Maybe& sin, const Maybe& positions, const lvar_norm_rope_t* h,
+                                                int64_t stream) {
+    auto some = [](const Maybe& t) { return t.value_or(at::Tensor()); };
+    ctx->save_for_backward({q, k, some(wq), some(wk), some(cos), some(sin), some(positions)});
+    ctx->saved_data["how"] = std::string(reinterpret_cast<const char*>(h), sizeof(*h));
+    at::Tensor oq, ok;
+    const int st = norm_rope_launch(q, k, *h, oq, ok, q.get_device(), reinterpret_cast<void*>(stream));
+    TORCH_CHECK(st == LVAR_OK, "lvar_qk_norm_rope_fwd failed with status ", st);
+    return {oq, ok};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope can be differentiated once: its gradients have no graph (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3], &cos = saved[4], &sin = saved[5], &positions = saved[6];
+    lvar_norm_rope_t h;
+    const std::string how = ctx->saved_data["how"].toStringRef();
+    std::memcpy(&h, how.data(), sizeof(h));
+    if (wq.defined()) h.q_weight.ptr = wq.data_ptr();
+    if (wk.defined()) h.k_weight.ptr = wk.data_ptr();
+    if (cos.defined()) { h.cos = cos.data_ptr<float>(); h.sin = sin.data_ptr<float>(); }
+    if (positions.defined()) h.positions = positions.data_ptr();
+    const int dev = q.get_device();
+    const c10::DeviceGuard guard(q.device());
+    auto rows = [](const at::Tensor& g) {
+      at::Tensor c = g.contiguous();
+      return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) ? c.clone() : c;
+    };
+    const at::Tensor gq = rows(grads[0]), gk = rows(grads[1]);
+    at::Tensor dq = rows_like(q), dk = rows_like(k), dwq, dwk, scratch;
+    if (wq.defined() && wq.requires_grad()) dwq = at::empty(wq.sizes(), wq.options());
+    if (wk.defined() && wk.requires_grad()) dwk = at::empty(wk.sizes(), wk.options());
+    const int B = dim(q, 0), H = dim(q, 1), Hkv = dim(k, 1), L = dim(q, 2), d = dim(q, 3);
+    int64_t bytes = 0;
+    if (dwq.defined() || dwk.defined()) {
+      bytes = api.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d);
+      if (bytes > 0) scratch = empty({bytes}, at::kByte, dev);
+    }
+    auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const int st = api.lvar_qk_norm_rope_bwd(view(q), view(k), h, gq.data_ptr(), gk.data_ptr(), view(dq), view(dk), ptr(dwq), ptr(dwk), ptr(scratch), bytes, B, H,
+                                             Hkv, L, d, c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream());
+    TORCH_CHECK(st == LVAR_OK, "lvar_qk_norm_rope_bwd failed with status ", st);
+    return {dq, dk, dwq, dwk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// (q, k, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved) -> (q, k)
+LVAR_FAST(fast_qk_norm_rope) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q = n == 10 ? tensor(a[0]) : nullptr, *k = n == 10 ? tensor(a[1]) : nullptr, *wq, *wk;
+  int dev;
+  void* stream;
+  How w;
+  LVAR_NEED(qk_ok(q, k, dev, stream) && how_ok(a + 2, *q, *k, dev, true, w, wq, wk));
+  at::Tensor oq, ok;
+  if (wants_grad(q) || wants_grad(k) || wants_grad(wq) || wants_grad(wk)) {
+    // (declined before a graph is built: what the entry point would refuse raises in the Python path)
+    LVAR_NEED(std::isfinite(w.h.eps) && w.h.eps >= 0.f && (!w.cos || (w.h.rot_dim % 16 == 0 && w.h.rot_dim > 0 && w.h.table_stride % 4 == 0 &&
+              ((reinterpret_cast<uintptr_t>(w.h.cos) | reinterpret_cast<uintptr_t>(w.h.sin)) & 15u) == 0)));
+    for (const auto* x : {&w.h.q_weight, &w.h.k_weight})
+      LVAR_NEED(!x->stride_col || ((reinterpret_cast<uintptr_t>(x->ptr) & 15u) == 0 && x->stride_head % 8 == 0));
+    const int64_t d = q->size(3);
+    LVAR_NEED((d == 16 || d == 32 || d == 64 || d == 128 || d == 256) && q->size(0) <= 65535 && q->size(1) <= 16384 && q->size(0) * q->size(2) <= (1ll << 30));
+    auto some = [](const at::Tensor* t) { return t ? std::optional<at::Tensor>(*t) : std::nullopt; };
+    auto r = NormRopeFunction::apply(*q, *k, some(wq), some(wk), some(w.cos), some(w.sin), some(w.positions), &w.h, reinterpret_cast<int64_t>(stream));
+    return tuple(std::move(r[0]), std::move(r[1]));
+  }
+  LVAR_NEED(norm_rope_launch(*q, *k, w.h, oq, ok, dev, stream) == LVAR_OK);
+  return tuple(std::move(oq), std::move(ok));
+  END_HANDLE_TH_ERRORS
+}
+
+// (cache k, v, k_exp, v_exp, page table, start, counts, q | None, k, v[, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved]) -> q, or True
+LVAR_FAST(fast_kv_append) {
+  HANDLE_TH_ERRORS
+  LVAR_NEED(n == 10 || n == 18);
+  const bool fused = n == 18;
+  const at::Tensor *q = fused ? tensor(a[7]) : tensor(a[8]), *k = tensor(a[8]), *v = tensor(a[9]), *start = tensor(a[5]), *counts, *wq = nullptr, *wk = nullptr;
+  int dev;
+  void* stream;
+  LVAR_NEED(qk_ok(q, k, dev, stream) && rows_ok(v, dev) && v->sizes() == k->sizes() && start && optional_tensor(a[6], counts));
+  const int64_t B = k->size(0);
+  lvar_paged_cache_t c;
+  LVAR_NEED(per_sequence(start, B, dev) && per_sequence(counts, B, dev) && cache_ok(a, B, dev, c) && c.kv_heads == k->size(1) && c.head_dim == k->size(3));
+  How w;
+  if (fused) LVAR_NEED(how_ok(a + 10, *q, *k, dev, false, w, wq, wk));
+  LVAR_NEED(!wants_grad(q) && !wants_grad(k) && !wants_grad(v) && !wants_grad(wq) && !wants_grad(wk));
+  at::Tensor oq;
+  if (fused) oq = empty(q->sizes(), at::kBFloat16, dev);
+  LVAR_NEED(api.lvar_kv_cache_append(view(*q), view(*k), view(*v), fused ? &w.h : nullptr, fused ? oq.data_ptr() : nullptr, c, ints(start), ints(counts),
+                                     static_cast<int>(B), dim(*q, 1), dim(*k, 2), stream) == LVAR_OK);
+  if (!fused) Py_RETURN_TRUE;
+  return THPVariable_Wrap(std::move(oq));
+  END_HANDLE_TH_ERRORS
+}
+
+// a length bound: None = everything that the table can name
+bool as_bound(PyObject* o, const lvar_paged_cache_t& c, bool clamp, int64_t& v) {
+  const int64_t reach = static_cast<int64_t>(c.max_pages) * c.page_size;
+  if (o == Py_None) v = reach;
+  else if (!as_long(o, v)) return false;
+  if (clamp) v = std::min(v, reach);
+  return v >= 0 && v <= INT32_MAX;
+}
+
+// (cache k, v, k_exp, v_exp, page table, lengths, max_len, start) -> (k, v)
+LVAR_FAST(fast_kv_read) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *k = n == 8 ? tensor(a[0]) : nullptr, *table = n == 8 ? tensor(a[4]) : nullptr, *start;
+  LVAR_NEED(bound && k && table && k->is_cuda() && table->dim() == 2 && optional_tensor(a[7], start));
+  const int dev = k->get_device();
+  const int64_t B = table->size(0);
+  const at::Tensor* lengths = tensor(a[5]);
+  lvar_paged_cache_t c;
+  int64_t most;
+  LVAR_NEED(lengths && c10::hip::current_device() == dev && cache_ok(a, B, dev, c) && per_sequence(lengths, B, dev) && per_sequence(start, B, dev) &&
+            as_bound(a[6], c, false, most) && most > 0 && B > 0 && B <= 65535);
+  at::Tensor ko = empty({B, c.kv_heads, most, c.head_dim}, at::kBFloat16, dev), vo = empty({B, c.kv_heads, most, c.head_dim}, at::kBFloat16, dev);
+  LVAR_NEED(api.lvar_kv_cache_read(c, ints(start), ints(lengths), ko.data_ptr(), vo.data_ptr(), static_cast<int>(B), static_cast<int>(most),
+                                   c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream()) == LVAR_OK);
+  return tuple(std::move(ko), std::move(vo));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, cache k, v, k_exp, v_exp, page table, lengths, counts, scale, causal, max_len) -> (o, M, L)
+LVAR_FAST(fast_paged_attn) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q = n == 11 ? tensor(a[0]) : nullptr, *counts;
+  LVAR_NEED(bound && q && q->is_cuda());
+  Qkv x{};
+  x.dev = q->get_device();
+  LVAR_NEED(rows_ok(q, x.dev) && q->numel() > 0 && c10::hip::current_device() == x.dev && !wants_grad(q) && optional_tensor(a[7], counts));
+  for (int i = 0; i < 3; i++) LVAR_NEED(q->size(i) <= INT32_MAX);
+  x.B = dim(*q, 0); x.H = dim(*q, 1); x.Lq = dim(*q, 2); x.d = dim(*q, 3);
+  const at::Tensor* lengths = tensor(a[6]);
+  lvar_paged_cache_t c;
+  float scale;
+  bool causal;
+  int64_t most;
+  LVAR_NEED(lengths && cache_ok(a + 1, x.B, x.dev, c) && c.head_dim == x.d && x.H % c.kv_heads == 0 && per_sequence(lengths, x.B, x.dev) &&
+            per_sequence(counts, x.B, x.dev) && as_scale(a[8], x.d, scale) && as_bool(a[9], causal) && as_bound(a[10], c, true, most));
+  const int64_t bytes = api.lvar_paged_attn_workspace_bytes(x.B, x.H, c.kv_heads, x.Lq, static_cast<int>(most), x.d);
+  LVAR_NEED(bytes >= 0);
+  at::Tensor o = empty_o(x), M, L, ws;
+  empty_stats(x, M, L);
+  if (bytes > 0) ws = empty({bytes}, at::kByte, x.dev);
+  LVAR_NEED(api.lvar_paged_attn_fwd(view(*q), c, ints(lengths), ints(counts), o.data_ptr(), M.data_ptr<float>(), L.data_ptr<float>(), bytes > 0 ? ws.data_ptr() : nullptr,
+                                    bytes, x.B, x.H, x.Lq, static_cast<int>(most), causal ? 1 : 0, scale,
+                                    c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(x.dev)).stream()) == LVAR_OK);
+  return tuple(std::move(o), std::move(M), std::move(L));
+  END_HANDLE_TH_ERRORS
+}
+
 // rows are read with 16-byte accesses: anything else is copied into a plain tensor first
 at::Tensor as_plain(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.dim() == 4, name, " must be [B,H,L,d], got ", t.sizes());
@@ -548,6 +840,7 @@ PyMethodDef fast_methods[] = {
     LVAR_METHOD(fast_dense_attn), LVAR_METHOD(fast_dense_colsum_attn), LVAR_METHOD(fast_colsum), LVAR_METHOD(fast_csp_attn),
     LVAR_METHOD(fast_full_step), LVAR_METHOD(fast_sparse_step), LVAR_METHOD(fast_block_sparse_attn), LVAR_METHOD(fast_block_topk_lists),
     LVAR_METHOD(fast_topk_token_lists), LVAR_METHOD(fast_remap_concat_lists), LVAR_METHOD(fast_mask_to_lists), LVAR_METHOD(fast_window_keys),
+    LVAR_METHOD(fast_qk_norm_rope), LVAR_METHOD(fast_kv_append), LVAR_METHOD(fast_kv_read), LVAR_METHOD(fast_paged_attn),
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

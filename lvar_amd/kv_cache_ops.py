@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from .sparse_attn_ops import ShapeError, _on_device, _prep, _ptr, _require, _scale, _stream, _view
+from .sparse_attn_ops import ShapeError, _native, _on_device, _plain_scale, _prep, _ptr, _require, _scale, _stream, _view
 
 __all__ = ["PagedKVCache", "qk_norm_rope", "qk_norm_rope_append", "kv_cache_append", "kv_cache_read", "paged_attn", "ShapeError"]
 
@@ -212,8 +212,9 @@ class _NormRope(torch.autograd.Function):
         return _norm_rope_launch(q, k, wq, wk, cos, sin, positions, norm, eps, interleaved)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
+        if torch.is_grad_enabled():
+            raise RuntimeError("qk_norm_rope can be differentiated once: its gradients have no graph (create_graph)")
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         norm, eps, interleaved = ctx.how
         B, H, L, d = q.shape
@@ -249,6 +250,11 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
     with ``interleaved=False``; token i takes row i, or row ``positions[i]`` / ``positions[b,i]`` (clamped to the table).
     ``head_dim`` 16, 32, 64, 128 or 256.  All in fp32, rounded once.  Differentiable in q, k and the weights (once); the
     reference's counterpart is models/sparvar/basic_sparvar.py:326-342, eager."""
+    fast = _native()
+    if fast is not None:
+        r = fast.fast_qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved)
+        if r is not None:
+            return r
     q, k = _prep(q, "q"), _prep(k, "k")
     cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
     _require(q.shape[3] in (16, 32, 64, 128, 256), lambda: f"head_dim must be 16, 32, 64, 128 or 256, got {q.shape[3]}")
@@ -287,6 +293,9 @@ def kv_cache_append(cache: PagedKVCache, k, v, page_table, start, counts=None) -
     ``counts`` int32 ``[B]`` limits a padded batch to the first ``counts[b]`` tokens.  An 8-bit cache gets, per token and
     head, the smallest power of two with ``max|x| <= 448 * 2^e`` and codes rounded to nearest even; infinities become NaN there.
     Positions outside the page table are dropped.  Two tokens of one call that go to the same row leave it undefined."""
+    fast = _native()
+    if fast is not None and fast.fast_kv_append(cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, start, counts, None, k, v):
+        return
     _no_gradient("kv_cache_append", k, v)
     k, v = _prep(k, "k"), _prep(v, "v")
     start, counts = _append_args(cache, k, v, page_table, start, counts)
@@ -299,6 +308,12 @@ def qk_norm_rope_append(cache: PagedKVCache, q, k, v, page_table, start, cos=Non
     """:func:`qk_norm_rope` on q and k and :func:`kv_cache_append` of the keys and of ``v``, in one launch; returns the queries.
     Without ``positions`` token i of sequence b takes row ``start[b] + i`` of the tables.  The keys are rounded once, from fp32 to
     the cache's type."""
+    fast = _native()
+    if fast is not None:
+        r = fast.fast_kv_append(cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, start, counts, q, k, v, cos, sin, positions, q_weight, k_weight,
+                                norm, eps, interleaved)
+        if r is not None:
+            return r
     _no_gradient("qk_norm_rope_append", q, k, v, q_weight, k_weight)
     q, k, v = _prep(q, "q"), _prep(k, "k"), _prep(v, "v")
     cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
@@ -315,6 +330,11 @@ def kv_cache_read(cache: PagedKVCache, page_table, lengths, max_len: Optional[in
     """Tokens ``start[b] ..`` (default 0) of every sequence as contiguous bf16 ``(k, v)`` ``[B,Hkv,max_len,d]``, the form that the
     dense and sparse attention operators take; zeros from position ``lengths[b]`` on.  ``max_len`` defaults to all that the page
     table can name.  Exact: every cached value is a bf16 value."""
+    fast = _native()
+    if fast is not None:
+        r = fast.fast_kv_read(cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, lengths, max_len, start)
+        if r is not None:
+            return r
     device = cache.k.device
     B = page_table.shape[0]
     arg = _cache_arg(cache, page_table, B, device)
@@ -338,6 +358,11 @@ def paged_attn(q, cache: PagedKVCache, page_table, lengths, scale=None, causal: 
     (default Lq) new tokens; otherwise all ``lengths[b]``.  Rows ``i >= counts[b]`` of a padded batch and rows that see no token
     get ``o = 0, M = -inf, L = 1``.  ``max_len`` bounds the lengths (longer ones are clamped to it; default: all that the page table
     can name): a small bound lets the launch do without the pass that joins the parts of long sequences."""
+    fast = _native()
+    if fast is not None:
+        r = fast.fast_paged_attn(q, cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, lengths, counts, _plain_scale(scale), causal, max_len)
+        if r is not None:
+            return r[0], (r[1], r[2])
     _no_gradient("paged_attn", q)
     q = _prep(q, "q")
     B, H, Lq, d = q.shape

@@ -189,6 +189,32 @@ def test_norm_rope_broadcast_inputs_and_one_output():
     assert bool(((dx.double().cpu() - want.sum((0, 1), keepdim=True)).abs() <= 2 * BF16 * want.abs().sum((0, 1), keepdim=True)).all())
 
 
+@pytest.mark.parametrize("binding", [True, False])
+def test_norm_rope_host_paths(binding, monkeypatch):
+    """The compiled and the Python host path give the same bits and refuse a second derivative."""
+    from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
+    q, k, _ = (t.cuda() for t in projection(2, 6, 2, 9, 64, seed=1))
+    w = weight("full", 6, 64, 2).cuda().requires_grad_()
+    cos, sin = (t.cuda() for t in tables(9, 16))
+    q = q.requires_grad_()
+    o = kv.qk_norm_rope(q, k, cos, sin, q_weight=w, norm="rms")
+    assert o[0].requires_grad
+    with torch.no_grad():
+        assert all(torch.equal(x, y) for x, y in zip(o, kv.qk_norm_rope(q, k, cos, sin, q_weight=w, norm="rms")))
+    g = [torch.ones_like(x) for x in o]
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(o, (q, w), g, create_graph=True)
+    o = kv.qk_norm_rope(q, k, cos, sin, q_weight=w, norm="rms")
+    dq, dw = torch.autograd.grad(o, (q, w), g)
+    assert dq.stride() == torch.empty_like(q).stride()
+    monkeypatch.setattr(kv, "_native", lambda: None)
+    o2 = kv.qk_norm_rope(q, k, cos, sin, q_weight=w, norm="rms")
+    dq2, dw2 = torch.autograd.grad(o2, (q, w), g)
+    assert torch.equal(dq, dq2) and torch.equal(dw, dw2) and all(torch.equal(x, y) for x, y in zip(o, o2))
+
+
 def test_norm_rope_leaves_nothing_for_empty_calls():
     from lvar_amd import kv_cache_ops as kv
     q = torch.zeros(2, 4, 0, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
@@ -618,10 +644,33 @@ def test_image_schedule(dtype):
     assert scores.shape == (B, H, total)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_host_paths_give_the_same(dtype, monkeypatch):
+    from lvar_amd import kv_cache_ops as kv
+    B, H, Hkv, L, d, page, P = 2, 4, 2, 21, 128, 32, 20
+    table = table_for(B, P // B, P, 1).cuda()
+    start, lens = torch.tensor([250, 3], dtype=torch.int32, device="cuda"), torch.tensor([271, 24], dtype=torch.int32, device="cuda")
+    cos, sin = (t.cuda() for t in tables(300, d // 2))
+    q, k, v = (t.cuda() for t in projection(B, H, Hkv, L, d, seed=3))
+    got = []
+    for native in (kv._native, lambda: None):
+        monkeypatch.setattr(kv, "_native", native)
+        c = to_gpu(make_cache(P, Hkv, page, d, dtype, 5))
+        kv.kv_cache_append(c, v, k, table, start)
+        oq = kv.qk_norm_rope_append(c, q, k, v, table, start, cos, sin, counts=lens - start)
+        o, (M, L_) = kv.paged_attn(oq, c, table, lens, causal=True, counts=lens - start)
+        got.append((oq, *kv.kv_cache_read(c, table, lens, L, start), o, M, L_, *(t.view(torch.uint8) for t in c if t is not None)))
+    for a, b in zip(*got):
+        assert a.dtype == b.dtype and torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
 # ---- refusals ----
 
-def test_refusals_on_the_device():
+@pytest.mark.parametrize("binding", [True, False])
+def test_refusals_on_the_device(binding, monkeypatch):
     from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
     x = rand(2, 2, 3, 64).cuda()
     c = kv.PagedKVCache.alloc(4, 2, 64, 16)
     c8 = kv.PagedKVCache.alloc(4, 2, 64, 16, torch.float8_e4m3fn)
