@@ -87,6 +87,7 @@ struct PagedAttnParams {
   int rt;                         // row tiles per key/value head
   int target, min_share;          // pieces aimed at, fewest 128-key stages of one
   int slot_rows;
+  int64_t ws_head;                // floats ahead of the partial results
 };
 
 int launch_norm_rope(const NormRopeParams& p, int head_dim, bool append, hipStream_t s);

@@ -10,9 +10,14 @@
 // and no barrier in the key loop: a wave waits for nothing but its own loads, and the loads of the next 32 keys are in
 // flight while it computes.
 //
-// The work is (sequence, key/value head, row tile) x stages of 128 keys (32 per wave of a workgroup).  It is cut into pieces
-// of about equal length by the lengths that only the device knows: every workgroup scans the lengths and finds its piece.
-// The pieces of one tile are joined by a second kernel, in order, so results do not depend on timing.
+// A workgroup's four waves are RW row waves times 4 / RW key waves: the row waves take 16 * NT rows each and read the same keys (from
+// L1 and L2 after the first), the key waves take turns at 32 keys.  More than 32 rows per wave would need over 256 registers, one
+// wave per SIMD, and nobody left to compute while it waits (64 rows per wave, 8 sequences of up to 4001 tokens with 61 new ones:
+// 105 us).
+//
+// The work is (sequence, key/value head, row tile) x stages of 128 keys.  It is cut into pieces of about equal length by the
+// lengths that only the device knows: every workgroup scans the lengths and finds its piece.  The pieces of one tile are joined by
+// a second kernel, in order, so results do not depend on timing.
 #include "kvcache.h"
 
 namespace lvar {
@@ -42,6 +47,8 @@ __device__ __forceinline__ float cross_sum(float x) {
   return __builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
+
 // ---- the plan: which piece of which sequence a workgroup takes ----
 
 struct Piece {
@@ -49,35 +56,36 @@ struct Piece {
   int n, piece;         // pieces per tile of this sequence, which one
   int tile, head;       // row tile, key/value head
   int slot;             // place of its partial result (n > 1)
+  int first_slot;       // of those of its sequence
 };
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
+// inclusive prefix sum over a wave
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp_mov<0x111>(x);                                                   // row_shr 1, 2, 4, 8: inside rows of 16
+  x += dpp_mov<0x112>(x);
+  x += dpp_mov<0x114>(x);
+  x += dpp_mov<0x118>(x);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);           // row_bcast 15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);           // row_bcast 31 to rows 2 and 3
   return x;
 }
-__device__ __forceinline__ int wave_scan(int x, int lane) {   // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  return x;
-}
+__device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
 
 __device__ __forceinline__ int stages_of(int len) { return len > 0 ? (len + PA_STAGE - 1) / PA_STAGE : 1; }
 
+__device__ __forceinline__ const __attribute__((address_space(4))) int32_t* as_constant(const int32_t* p) {
+  return (const __attribute__((address_space(4))) int32_t*)(p);
+}
+
 // New tokens of sequence b; the rows behind them get an empty result.
-__device__ __forceinline__ int fresh_of(const PagedAttnParams& p, int b) { return p.counts ? max(0, min(p.counts[b], p.Lq)) : p.Lq; }
+__device__ __forceinline__ int fresh_of(const PagedAttnParams& p, int b) { return p.counts ? max(0, min(as_constant(p.counts)[b], p.Lq)) : p.Lq; }
 
 // Length of sequence b within what the table can name.
 __device__ __forceinline__ int length_of(const PagedAttnParams& p, int b) { return max(0, min(p.lengths[b], p.max_len)); }
 
 // Stages of a piece: the work spread over `target` pieces, but no less than min_share stages each.  (The launch has checked that
 // the stages of all tiles together fit 31 bits.)
-__device__ __forceinline__ int share_of(const PagedAttnParams& p, int lane) {
-  uint32_t total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) total += wave_sum(b0 + lane < p.B ? stages_of(length_of(p, b0 + lane)) : 0);
+__device__ __forceinline__ int share_of(const PagedAttnParams& p, uint32_t total) {
   total *= (uint32_t)(p.cache.kv_heads * p.rt);
   return max((int)((total - 1) / (uint32_t)p.target) + 1, p.min_share);
 }
@@ -85,59 +93,83 @@ __device__ __forceinline__ int share_of(const PagedAttnParams& p, int lane) {
 // Pieces of a tile of `stages` > 0 stages.
 __device__ __forceinline__ int pieces_of(int stages, int share) { return (int)((uint32_t)(stages - 1) / (uint32_t)share) + 1; }
 
-// The piece with number `item`; false behind the last one.  All lanes of a wave call it and get the same answer.
-__device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int item, int lane, Piece& out) {
-  const int share = share_of(p, lane), units = p.cache.kv_heads * p.rt;
-  int before = 0, slots = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
+// The piece of workgroup `wg`; false for the workgroups that are left over.  All lanes of a wave call it and get the same answer, in
+// scalar registers.  Workgroups are dealt to the 8 XCDs in turn; each XCD takes a run of pieces, row tiles over the same keys next to
+// each other in one L2.
+__device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int lane, Piece& out) {
+  const int units = p.cache.kv_heads * p.rt;
+  const int len0 = lane < p.B ? length_of(p, lane) : 0;      // (the first 64 sequences are looked at once)
+  uint32_t total = last_lane(wave_scan(lane < p.B ? stages_of(len0) : 0));
+  for (int b0 = 64; b0 < p.B; b0 += 64) total += last_lane(wave_scan(b0 + lane < p.B ? stages_of(length_of(p, b0 + lane)) : 0));
+  const int share = share_of(p, total);
+  auto look = [&](int b0, int& len, int& st, int& n) {
     const int b = b0 + lane;
-    int len = 0, st = 0, n = 0;
+    len = st = n = 0;
     if (b < p.B) {
-      len = length_of(p, b);
+      len = b0 == 0 ? len0 : length_of(p, b);
       st = stages_of(len);
       n = pieces_of(st, share);
     }
+  };
+  int len, st, n, pieces = 0;
+  for (int b0 = (p.B - 1) & ~63; b0 >= 0; b0 -= 64) {        // (ends with the first 64 in len, st, n)
+    look(b0, len, st, n);
+    pieces += last_lane(wave_scan(n));
+  }
+  pieces *= units;
+  const int per = (pieces + 7) >> 3, item = (wg & 7) * per + (wg >> 3);
+  if ((wg >> 3) >= per || item >= pieces) return false;
+  int before = 0, slots = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    if (b0 > 0) look(b0, len, st, n);
     const int mine = n * units, cut = n > 1 ? mine : 0;
-    const int upto = wave_scan(mine, lane), cuts = wave_scan(cut, lane);
+    const int upto = wave_scan(mine), cuts = wave_scan(cut);
     const uint64_t hit = __ballot(before + upto > item);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       out.b = b0 + l;
-      out.len = __shfl(len, l, 64);
-      out.stages = __shfl(st, l, 64);
-      out.n = __shfl(n, l, 64);
-      const int rest = item - before - __shfl(upto - mine, l, 64);
-      out.slot = slots + __shfl(cuts - cut, l, 64) + rest;
-      out.tile = rest % p.rt;               // row tiles of the same keys next to each other
+      out.len = __builtin_amdgcn_readlane(len, l);
+      out.stages = __builtin_amdgcn_readlane(st, l);
+      out.n = __builtin_amdgcn_readlane(n, l);
+      const int rest = item - before - __builtin_amdgcn_readlane(upto - mine, l);
+      out.first_slot = slots + __builtin_amdgcn_readlane(cuts - cut, l);
+      out.slot = out.first_slot + rest;
+      out.tile = rest % p.rt;
       const int hp = rest / p.rt;
       out.piece = hp % out.n;
       out.head = hp / out.n;
       return true;
     }
-    before += __shfl(upto, 63, 64);
-    slots += __shfl(cuts, 63, 64);
+    before += last_lane(upto);
+    slots += last_lane(cuts);
   }
   return false;
 }
 
-template <int D, int NT, bool F8, int WAVES_PER_SIMD>
+template <int D, int NT, int RW, bool F8, int WAVES_PER_SIMD>
 __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const PagedAttnParams p) {
   constexpr int KS = D / 32;                  // steps of the contraction over the head dimension
   constexpr int CH = D < 128 ? 1 : D / 128;   // chunks of 128 (64) output columns
   constexpr int NE = D < 128 ? D / 16 : 8;    // columns of a chunk per lane and value row
   constexpr int CW = 16 * NE;                 // columns of a chunk
   constexpr int LDO = CW + 4;
+  constexpr int KW = PA_WAVES / RW;           // key waves
   __shared__ float so[PA_WAVES][16][LDO];
   __shared__ float sm[PA_WAVES][NT * 16], sl[PA_WAVES][NT * 16];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % RW, kw = wave / RW;
   const int qi = lane & 15, g = lane >> 4;
-  // consecutive pieces (tiles over the same keys) to the same XCD: workgroups are dealt to the 8 of them in turn
-  const int per = (gridDim.x + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   Piece w;
-  if ((int)(blockIdx.x >> 3) >= per || !find_piece(p, item, lane, w)) return;
+  if (!find_piece(p, blockIdx.x, lane, w)) return;
+  if (w.n > 1 && w.piece + w.tile + w.head == 0 && threadIdx.x == 0) {
+    ((int*)p.ws)[2 * w.b] = w.n;            // for the join
+    ((int*)p.ws)[2 * w.b + 1] = w.first_slot;
+  } else if (p.ws && w.n == 1 && w.tile + w.head == 0 && threadIdx.x == 0) {
+    ((int*)p.ws)[2 * w.b] = 1;
+  }
 
-  const int rows = p.G * p.Lq, row0 = w.tile * NT * 16;
+  const int rows = p.G * p.Lq, tile0 = w.tile * NT * RW * 16, row0 = tile0 + rw * NT * 16;
   const int fresh = fresh_of(p, w.b);
 
   // queries as the second operand, and how many keys each may see
@@ -163,22 +195,24 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     most = max(most, __shfl_xor(most, d, 64));
     least = min(least, __shfl_xor(least, d, 64));
   }
-  most = __builtin_amdgcn_readfirstlane(most);
+  most = row0 < rows ? __builtin_amdgcn_readfirstlane(most) : 0;   // a wave without rows has nothing to do
   least = __builtin_amdgcn_readfirstlane(least);
 
   const int s0 = (int)((int64_t)w.stages * w.piece / w.n), s1 = (int)((int64_t)w.stages * (w.piece + 1) / w.n);
   const int k_end = min(s1 * PA_STAGE, most);
 
   f32x4 o[NT][CH][NE] = {};
-  float m[NT], l[NT];
+  // m: what the exponentials count from, the same for the four lanes of a query; top: the largest score of this lane, times 1 / c
+  float m[NT], l[NT], top[NT];
 #pragma unroll
-  for (int t = 0; t < NT; t++) { m[t] = -INFINITY; l[t] = 0.f; }
+  for (int t = 0; t < NT; t++) { m[t] = top[t] = -INFINITY; l[t] = 0.f; }
 
   const uint8_t* kb = p.cache.k + w.head * p.cache.s_head;
   const uint8_t* vb = p.cache.v + w.head * p.cache.s_head;
   const uint8_t* keb = F8 ? p.cache.k_exp + w.head * p.cache.e_head : nullptr;
   const uint8_t* veb = F8 ? p.cache.v_exp + w.head * p.cache.e_head : nullptr;
-  const int32_t* table = p.cache.table + w.b * p.cache.table_stride;
+  // through the constant address space: scalar loads, which do not stand in the queue of the vector loads
+  const __attribute__((address_space(4))) int32_t* table = as_constant(p.cache.table + w.b * p.cache.table_stride);
   const int mask = (1 << p.cache.shift) - 1;
   const int sr = (int)p.cache.s_row;
 
@@ -188,12 +222,9 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
   u32x2 vc[F8 ? CH : 1][F8 ? 8 : 1];            // e4m3
   uint32_t ke[2], ve[2];
 
-  // page of the 16 keys from `key` on, -1: none
-  auto page_of = [&](int key) {
-    const int at = min(key >> p.cache.shift, p.cache.max_pages - 1);
-    const int pg = table[at];
-    return key < k_end && pg >= 0 && pg < p.cache.num_pages ? pg : -1;
-  };
+  // table entry for the 16 keys from `key` on (in the table whatever the key), and the page that it names, -1: none
+  auto entry_of = [&](int key) { return table[min(key >> p.cache.shift, p.cache.max_pages - 1)]; };
+  auto page_of = [&](int key, int entry) { return key < k_end && entry >= 0 && entry < p.cache.num_pages ? entry : -1; };
   auto load_k = [&](int key, const int* pg) {
 #pragma unroll
     for (int j = 0; j < 2; j++) {
@@ -230,17 +261,19 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     }
   };
 
-  int key = s0 * PA_STAGE + wave * 32;
-  int pg[2] = {-1, -1};
+  constexpr int STEP = 32 * KW;
+  int key = s0 * PA_STAGE + kw * 32;
+  int pg[2] = {-1, -1}, entry[2] = {0, 0};   // entry: of the next 32 keys
   if (key < k_end) {
-    pg[0] = page_of(key); pg[1] = page_of(key + 16);
+    pg[0] = page_of(key, entry_of(key)); pg[1] = page_of(key + 16, entry_of(key + 16));
     load_k(key, pg);
     load_v(key, pg);
+    entry[0] = entry_of(key + STEP); entry[1] = entry_of(key + STEP + 16);
   }
   while (key < k_end) {
-    const int next = key + PA_STAGE;
-    int npg[2] = {-1, -1};
-    if (next < k_end) { npg[0] = page_of(next); npg[1] = page_of(next + 16); }
+    const int next = key + STEP;
+    const int npg[2] = {page_of(next, entry[0]), page_of(next + 16, entry[1])};
+    entry[0] = entry_of(next + STEP); entry[1] = entry_of(next + STEP + 16);
     const bool ragged = key + 32 > least || pg[0] < 0 || pg[1] < 0;
 
     // scores
@@ -276,7 +309,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) a = mfma16(ka[j][ks], qf[t][ks], a);
 #pragma unroll
-        for (int r = 0; r < 4; r++) s[4 * j + r] = a[r] * p.c;
+        for (int r = 0; r < 4; r++) s[4 * j + r] = a[r];
       }
       if (ragged) {
 #pragma unroll
@@ -285,11 +318,13 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
           for (int r = 0; r < 4; r++)
             if (pg[j] < 0 || key + 16 * j + 4 * g + r >= limit[t]) s[4 * j + r] = -INFINITY;
       }
-      float mt = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(s[0], s[1]), __builtin_fmaxf(s[2], s[3])),
-                                 __builtin_fmaxf(__builtin_fmaxf(s[4], s[5]), __builtin_fmaxf(s[6], s[7])));
-      mt = __builtin_fmaxf(cross_max(mt), m[t]);
-      if (__any(mt > m[t])) {
-        const float f = mt == -INFINITY ? 1.f : fast_exp2(m[t] - mt);
+      float mt = max3(max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), __builtin_fmaxf(s[6], s[7]));
+      top[t] = __builtin_fmaxf(top[t], mt);
+      // The reference moves when a score is more than 2^8 above it (or is the first): sums and outputs stay far from the ends of
+      // 32-bit range, and the exchange between lanes and the rescaling of the outputs are rare.
+      if (__any(mt * p.c > m[t] + 8.f)) {
+        mt = __builtin_fmaxf(cross_max(mt) * p.c, m[t]);
+        const float f = m[t] == -INFINITY ? 0.f : fast_exp2(m[t] - mt);
         l[t] *= f;
 #pragma unroll
         for (int c = 0; c < CH; c++)
@@ -297,10 +332,10 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
           for (int e = 0; e < NE; e++) o[t][c][e] *= f;
         m[t] = mt;
       }
-      const float ms = mt == -INFINITY ? 0.f : mt;
+      const float ms = m[t] == -INFINITY ? 0.f : m[t];
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        s[e] = fast_exp2(s[e] - ms);
+        s[e] = fast_exp2(__builtin_fmaf(s[e], p.c, -ms));
         l[t] += s[e];
       }
       // p is rounded to bf16 for the matrix instruction (its sum is not): 2^-9 per term, independent signs
@@ -353,20 +388,24 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     key = next;
   }
 
-  // the four waves' results become one
+  // The key waves' results become one.  A row's sums are first put on the scale of its true maximum (the M of the result).
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    const float ls = cross_sum(l[t]);
-    if (lane < 16) { sm[wave][t * 16 + qi] = m[t]; sl[wave][t * 16 + qi] = ls; }
+    const float mx = cross_max(top[t]) * p.c, ls = cross_sum(l[t]);
+    // (no finite score: nothing, or NaN that has to stay one)
+    const float f = m[t] == -INFINITY ? 1.f : fast_exp2(m[t] - mx);
+    if (lane < 16) { sm[wave][t * 16 + qi] = mx; sl[wave][t * 16 + qi] = ls * f; }
+    m[t] = f;
+    top[t] = mx;
   }
   __syncthreads();
-  float* slot = w.n > 1 ? p.ws + (int64_t)w.slot * p.slot_rows * (D + 2) : nullptr;
-#pragma unroll
+  float* part = w.n > 1 ? p.ws + p.ws_head + (int64_t)w.slot * p.slot_rows * (D + 2) : nullptr;
+  #pragma unroll
   for (int t = 0; t < NT; t++) {
-    float top = -INFINITY;
+    float best = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < PA_WAVES; x++) top = __builtin_fmaxf(top, sm[x][t * 16 + qi]);
-    const float f = m[t] == -INFINITY ? 0.f : fast_exp2(m[t] - top);
+    for (int x = 0; x < KW; x++) best = __builtin_fmaxf(best, sm[x * RW + rw][t * 16 + qi]);
+    const float f = top[t] == -INFINITY ? 1.f : m[t] * fast_exp2(top[t] - best);
 #pragma unroll
     for (int c = 0; c < CH; c++) {
       if (t + c > 0) __syncthreads();
@@ -378,28 +417,27 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
           *(f32x4*)&so[wave][qi][(4 * g + r) * NE + e] = y;
         }
       __syncthreads();
-      // thread: query tid / 16, columns NE * (tid % 16) ..
-      const int query = threadIdx.x >> 4, col = (threadIdx.x & 15) * NE, r = row0 + t * 16 + query;
-      float y[NE] = {};
+      // thread: query tid / 16 of every row wave, columns NE * (tid % 16) ..
+      const int query = threadIdx.x >> 4, col = (threadIdx.x & 15) * NE;
 #pragma unroll
-      for (int x = 0; x < PA_WAVES; x++)
+      for (int rx = 0; rx < RW; rx++) {
+        const int at = rx * NT * 16 + t * 16 + query, r = tile0 + at;   // row of the tile, of the head
+        if (r >= rows) break;
+        float y[NE] = {}, qm = -INFINITY, ql = 0.f;
 #pragma unroll
-        for (int e = 0; e < NE; e++) y[e] += so[x][query][col + e];
-      float qm = -INFINITY, ql = 0.f;
+        for (int x = 0; x < KW; x++) qm = __builtin_fmaxf(qm, sm[x * RW + rx][t * 16 + query]);
 #pragma unroll
-      for (int x = 0; x < PA_WAVES; x++) qm = __builtin_fmaxf(qm, sm[x][t * 16 + query]);
+        for (int x = 0; x < KW; x++) {
 #pragma unroll
-      for (int x = 0; x < PA_WAVES; x++) {
-        // (no finite score: the sum is 0, or NaN where a score was)
-        const float mx = sm[x][t * 16 + query];
-        ql += sl[x][t * 16 + query] * (mx == -INFINITY ? 1.f : fast_exp2(mx - qm));
-      }
-      if (r < rows) {
-        if (slot) {
-          float* at = slot + (t * 16 + query) * (D + 2);
-          if (c == 0 && (threadIdx.x & 15) == 0) { at[D] = qm; at[D + 1] = ql; }
+          for (int e = 0; e < NE; e++) y[e] += so[x * RW + rx][query][col + e];
+          const float mx = sm[x * RW + rx][t * 16 + query];
+          ql += sl[x * RW + rx][t * 16 + query] * (mx == -INFINITY ? 1.f : fast_exp2(mx - qm));
+        }
+        if (part) {
+          float* to = part + at * (D + 2);
+          if (c == 0 && (threadIdx.x & 15) == 0) { to[D] = qm; to[D + 1] = ql; }
 #pragma unroll
-          for (int e = 0; e < NE; e += 2) *(f32x2*)(at + c * CW + col + e) = f32x2{y[e], y[e + 1]};
+          for (int e = 0; e < NE; e += 2) *(f32x2*)(to + c * CW + col + e) = f32x2{y[e], y[e + 1]};
         } else {
           const int i = r / p.G;
           const int64_t out = ((int64_t)w.b * p.H + w.head * p.G + (r - i * p.G)) * p.Lq + i;
@@ -417,79 +455,87 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
   }
 }
 
-// Joins the pieces of the tiles that were cut: a workgroup per (sequence, key/value head, row), 8 groups of lanes along the pieces.
-template <int D>
+// Joins the pieces of the tiles that were cut, in order.  A workgroup takes 512 / (D / 4) groups of D / 4 lanes: RPB rows with
+// GR / RPB groups each along the pieces.
+template <int D, int RPB>
 __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p, int tile_rows) {
-  constexpr int LPR = D / 4, GR = 512 / LPR;
-  __shared__ float so[GR][D];
+  constexpr int LPR = D / 4, GR = 512 / LPR, GP = GR / RPB;
+  static_assert(GR % RPB == 0, "groups per row");
+  __shared__ float so[GP > 1 ? GR : 1][D];
   __shared__ float sm[GR], sl[GR];
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
-  const int tile = row / tile_rows, units = p.cache.kv_heads * p.rt;
-  // slots ahead of this sequence
-  const int share = share_of(p, lane);
-  int n = 0, slots = 0;
-  for (int b0 = 0; b0 <= b; b0 += 64) {
-    const int x = b0 + lane;
-    const int k = x < p.B ? pieces_of(stages_of(length_of(p, x)), share) : 0;
-    slots += wave_sum(x < b && k > 1 ? k * units : 0);
-    if (b < b0 + 64) n = __shfl(k, b - b0, 64);
-  }
+  const int head = blockIdx.y, b = blockIdx.z;
+  const int n = ((const int*)p.ws)[2 * b];
   if (n <= 1) return;
-  const float* first = p.ws + ((int64_t)slots + (int64_t)head * n * p.rt + tile) * p.slot_rows * (D + 2) + (row - tile * tile_rows) * (D + 2);
+  const int first_slot = ((const int*)p.ws)[2 * b + 1];
+  const int l = threadIdx.x % LPR, g = threadIdx.x / LPR, x0 = g / RPB;
+  const int rows = p.G * p.Lq, row = blockIdx.x * RPB + g % RPB, rc = min(row, rows - 1);
+  const int tile = rc / tile_rows;
+  const float* first = p.ws + p.ws_head + ((int64_t)(first_slot + head * n * p.rt + tile) * p.slot_rows + (rc - tile * tile_rows)) * (D + 2);
   const int64_t step = (int64_t)p.rt * p.slot_rows * (D + 2);
-  const int l = threadIdx.x % LPR, g = threadIdx.x / LPR;
   float top = -INFINITY;
-  for (int x = g; x < n; x += GR) top = __builtin_fmaxf(top, first[x * step + D]);
-  if (l == 0) sm[g] = top;
-  __syncthreads();
+  for (int x = x0; x < n; x += GP) top = __builtin_fmaxf(top, first[x * step + D]);
+  if constexpr (GP > 1) {
+    if (l == 0) sm[g] = top;
+    __syncthreads();
 #pragma unroll
-  for (int x = 0; x < GR; x++) top = __builtin_fmaxf(top, sm[x]);
+    for (int x = 0; x < GP; x++) top = __builtin_fmaxf(top, sm[x * RPB + g % RPB]);
+  }
   float y[4] = {}, sum = 0.f;
 #pragma unroll 4
-  for (int x = g; x < n; x += GR) {
+  for (int x = x0; x < n; x += GP) {
     const float* at = first + x * step;
     const float mx = at[D], lx = at[D + 1];
     const f32x2 a = *(const f32x2*)(at + l * 4), c = *(const f32x2*)(at + l * 4 + 2);
-    const float f = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
+    const float f = mx == -INFINITY ? 1.f : fast_exp2(mx - top);   // (no finite score: zeros, or NaN that stays one)
     y[0] += a[0] * f; y[1] += a[1] * f; y[2] += c[0] * f; y[3] += c[1] * f;
-    sum += mx == -INFINITY ? lx : lx * f;
+    sum += lx * f;
   }
-  if (l == 0) sl[g] = sum;
+  if constexpr (GP > 1) {
+    if (l == 0) sl[g] = sum;
 #pragma unroll
-  for (int e = 0; e < 4; e++) so[g][l * 4 + e] = y[e];
-  __syncthreads();
+    for (int e = 0; e < 4; e++) so[g][l * 4 + e] = y[e];
+    __syncthreads();
+    if (g >= RPB) return;
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < GP; x++) {
+      sum += sl[x * RPB + g];
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] += so[x * RPB + g][l * 4 + e];
+    }
+  }
+  if (row >= rows) return;
   const int i = row / p.G;
   const int64_t out = ((int64_t)b * p.H + head * p.G + (row - i * p.G)) * p.Lq + i;
-  float all = 0.f;
-#pragma unroll
-  for (int x = 0; x < GR; x++) all += sl[x];
-  const bool none = i >= fresh_of(p, b) || (top == -INFINITY && all == 0.f);
-  for (int col = threadIdx.x; col < D; col += 512) {
-    float s = 0.f;
-#pragma unroll
-    for (int x = 0; x < GR; x++) s += so[x][col];
-    p.o[out * D + col] = (bf16_t)(none ? 0.f : s / all);
-  }
-  if (threadIdx.x == 0) { p.M[out] = none ? -INFINITY : top; p.L[out] = none ? 1.f : all; }
+  const bool none = i >= fresh_of(p, b) || (top == -INFINITY && sum == 0.f);
+  const float inv = 1.f / sum;
+  const u32x2 u = {pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)};
+  *(u32x2*)(p.o + out * D + l * 4) = none ? u32x2{0u, 0u} : u;
+  if (l == 0) { p.M[out] = none ? -INFINITY : top; p.L[out] = none ? 1.f : sum; }
 }
 
 // ---- launch ----
 
-struct Shape { int nt, rt, rows, target, min_share; };
+struct Shape { int nt, rw, rt, rows, target, min_share; };
 
+// Rows per tile: 16 up to 16 rows of a key/value head, else 32, 64 or 128.
 static Shape shape_of(int H, int Hkv, int Lq, int head_dim) {
   Shape s;
   const int64_t rows = (int64_t)(H / Hkv) * Lq;
-  const int widest = head_dim == 256 ? 2 : 4;
-  s.nt = rows <= 16 ? 1 : rows <= 32 ? 2 : widest;
-  s.rt = (int)((rows + 16 * s.nt - 1) / (16 * s.nt));
-  s.rows = (int)(rows < 16 * s.nt ? rows : 16 * s.nt);
-  const int resident = s.nt == 1 ? 3 : s.nt == 2 ? 2 : 1;   // workgroups per compute unit that the registers allow
-  s.target = device_cus() * resident;
+  s.nt = rows <= 16 || head_dim == 256 ? 1 : 2;
+  const int per = 16 * s.nt;
+  s.rw = rows <= per ? 1 : rows <= 2 * per ? 2 : 4;
+  const int tile = per * s.rw;
+  s.rt = (int)((rows + tile - 1) / tile);
+  s.rows = (int)(rows < tile ? rows : tile);
+  s.target = device_cus() * (s.nt == 1 && head_dim < 256 ? 3 : 2);   // workgroups that the registers let a compute unit hold
   s.min_share = 2;
   return s;
 }
+
+static int64_t ws_head_floats(int B) { return ((int64_t)2 * B + 63) / 64 * 64; }   // pieces and first slot of every sequence
 
 // Partial results are kept for tiles that are cut only; such a tile has n < 2 * stages / share pieces, so that there are fewer
 // than 2 * target of them in all.
@@ -497,26 +543,41 @@ int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head
   const Shape s = shape_of(H, Hkv, Lq, head_dim);
   if (s.target <= 0) return LVAR_ELAUNCH;
   if ((max_len + PA_STAGE - 1) / PA_STAGE <= s.min_share) return 0;   // nothing can be cut
-  return 2ll * s.target * s.rows * (head_dim + 2) * 4;
+  return 4 * (ws_head_floats(B) + 2ll * s.target * s.rows * (head_dim + 2));
 }
 
-template <int D, int NT, bool F8, int W>
-static void launch_one(const PagedAttnParams& p, int grid, hipStream_t s) {
-  hipLaunchKernelGGL((paged_attn_kernel<D, NT, F8, W>), dim3(grid), dim3(PA_T), 0, s, p);
+template <int D, int NT, int RW, int W>
+static void launch_rw(const PagedAttnParams& p, int grid, hipStream_t s) {
+  if (p.cache.k_exp) hipLaunchKernelGGL((paged_attn_kernel<D, NT, RW, true, W>), dim3(grid), dim3(PA_T), 0, s, p);
+  else hipLaunchKernelGGL((paged_attn_kernel<D, NT, RW, false, W>), dim3(grid), dim3(PA_T), 0, s, p);
+}
+
+template <int D, int RPB>
+static void launch_join(const PagedAttnParams& p, int tile_rows, hipStream_t s) {
+  hipLaunchKernelGGL((paged_join_kernel<D, RPB>), dim3((p.G * p.Lq + RPB - 1) / RPB, p.cache.kv_heads, p.B), dim3(512), 0, s, p, tile_rows);
 }
 
 template <int D>
-static int launch_d(const PagedAttnParams& p, int nt, hipStream_t s) {
-  const bool f8 = p.cache.k_exp != nullptr;
+static int launch_d(const PagedAttnParams& p, const Shape& h, hipStream_t s) {
   const int64_t items = (int64_t)p.B * p.cache.kv_heads * p.rt + (p.ws ? p.target : 0);
   if (items > 0x7ffffff0) return LVAR_EINVAL;
   const int grid = (int)((items + 7) / 8 * 8);
-  if (nt == 1) f8 ? launch_one<D, 1, true, D == 256 ? 2 : 3>(p, grid, s) : launch_one<D, 1, false, D == 256 ? 2 : 3>(p, grid, s);
-  else if (nt == 2) f8 ? launch_one<D, 2, true, D == 256 ? 1 : 2>(p, grid, s) : launch_one<D, 2, false, D == 256 ? 1 : 2>(p, grid, s);
-  else if constexpr (D < 256) f8 ? launch_one<D, 4, true, 1>(p, grid, s) : launch_one<D, 4, false, 1>(p, grid, s);
+  if (h.nt == 1) {
+    constexpr int W = D == 256 ? 2 : 3;
+    if (h.rw == 1) launch_rw<D, 1, 1, W>(p, grid, s);
+    else if constexpr (D == 256) { if (h.rw == 2) launch_rw<D, 1, 2, W>(p, grid, s); else launch_rw<D, 1, 4, W>(p, grid, s); }
+  } else if constexpr (D < 256) {
+    if (h.rw == 1) launch_rw<D, 2, 1, 2>(p, grid, s);
+    else if (h.rw == 2) launch_rw<D, 2, 2, 2>(p, grid, s);
+    else launch_rw<D, 2, 4, 2>(p, grid, s);
+  }
   if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
   if (p.ws) {
-    hipLaunchKernelGGL((paged_join_kernel<D>), dim3(p.G * p.Lq, p.cache.kv_heads, p.B), dim3(512), 0, s, p, 16 * nt);
+    // few rows: all groups along the pieces of one row; many: a group per row
+    constexpr int GR = 512 / (D / 4);
+    const int tile_rows = 16 * h.nt * h.rw;
+    if ((int64_t)p.G * p.Lq * p.cache.kv_heads * p.B <= 4 * device_cus()) launch_join<D, 1>(p, tile_rows, s);
+    else launch_join<D, GR>(p, tile_rows, s);
     if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
   }
   return LVAR_OK;
@@ -528,11 +589,12 @@ int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s) {
   p.rt = h.rt;
   p.target = h.target;
   p.slot_rows = h.rows;
+  p.ws_head = ws_head_floats(p.B);
   // without room for partial results every tile stays whole: a share longer than any sequence
   p.min_share = p.ws ? h.min_share : 0x7fffffff;
-  if (head_dim == 128) return launch_d<128>(p, h.nt, s);
-  if (head_dim == 64) return launch_d<64>(p, h.nt, s);
-  if (head_dim == 256) return launch_d<256>(p, h.nt, s);
+  if (head_dim == 128) return launch_d<128>(p, h, s);
+  if (head_dim == 64) return launch_d<64>(p, h, s);
+  if (head_dim == 256) return launch_d<256>(p, h, s);
   return LVAR_EUNSUPPORTED;
 }
 
