@@ -47,6 +47,17 @@ __device__ __forceinline__ float cross_sum(float x) {
   return __builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]);
 }
 
+// bf16 values of 8 codes times a power of two (exact)
+__device__ __forceinline__ u32x4 scaled8(u32x2 c, float scale) {
+  u32x4 r;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    r[2 * h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[h], scale, false));
+    r[2 * h + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[h], scale, true));
+  }
+  return r;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
 
 // ---- the plan: which piece of which sequence a workgroup takes ----
@@ -83,11 +94,10 @@ __device__ __forceinline__ int fresh_of(const PagedAttnParams& p, int b) { retur
 // Length of sequence b within what the table can name.
 __device__ __forceinline__ int length_of(const PagedAttnParams& p, int b) { return max(0, min(p.lengths[b], p.max_len)); }
 
-// Stages of a piece: the work spread over `target` pieces, but no less than min_share stages each.  (The launch has checked that
-// the stages of all tiles together fit 31 bits.)
-__device__ __forceinline__ int share_of(const PagedAttnParams& p, uint32_t total) {
-  total *= (uint32_t)(p.cache.kv_heads * p.rt);
-  return max((int)((total - 1) / (uint32_t)p.target) + 1, p.min_share);
+// Stages of a piece: `total` stages spread over `target` pieces, but no less than min_share stages each.  (The launch has checked
+// that the stages of all tiles together fit 31 bits.)
+__device__ __forceinline__ int share_of(const PagedAttnParams& p, uint32_t total, uint32_t target) {
+  return max((int)((total - 1) / target) + 1, p.min_share);
 }
 
 // Pieces of a tile of `stages` > 0 stages.
@@ -101,7 +111,8 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
   const int len0 = lane < p.B ? length_of(p, lane) : 0;      // (the first 64 sequences are looked at once)
   uint32_t total = last_lane(wave_scan(lane < p.B ? stages_of(len0) : 0));
   for (int b0 = 64; b0 < p.B; b0 += 64) total += last_lane(wave_scan(b0 + lane < p.B ? stages_of(length_of(p, b0 + lane)) : 0));
-  const int share = share_of(p, total);
+  total *= (uint32_t)units;
+  int share = share_of(p, total, p.target);
   auto look = [&](int b0, int& len, int& st, int& n) {
     const int b = b0 + lane;
     len = st = n = 0;
@@ -111,12 +122,23 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
       n = pieces_of(st, share);
     }
   };
-  int len, st, n, pieces = 0;
-  for (int b0 = (p.B - 1) & ~63; b0 >= 0; b0 -= 64) {        // (ends with the first 64 in len, st, n)
-    look(b0, len, st, n);
-    pieces += last_lane(wave_scan(n));
+  int len, st, n, pieces;
+  auto count = [&]() {
+    pieces = 0;
+    for (int b0 = (p.B - 1) & ~63; b0 >= 0; b0 -= 64) {      // (ends with the first 64 in len, st, n)
+      look(b0, len, st, n);
+      pieces += last_lane(wave_scan(n));
+    }
+    pieces *= units;
+  };
+  count();
+  // One round of workgroups if the rounding up of the pieces lets it be one; otherwise pieces half as long, whose second and third
+  // rounds even out (one sequence of 131071 tokens, 752 pieces in one round: 54 us, in two 56; 32 ragged ones 401 us with one round
+  // and a bit, 388 with finer pieces).
+  if (pieces > p.target) {
+    share = share_of(p, total, 2 * p.target);
+    count();
   }
-  pieces *= units;
   const int per = (pieces + 7) >> 3, item = (wg & 7) * per + (wg >> 3);
   if ((wg >> 3) >= per || item >= pieces) return false;
   int before = 0, slots = 0;
@@ -146,6 +168,102 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
   return false;
 }
 
+// What the join needs to know of a sequence, from one of its workgroups.
+__device__ __forceinline__ void write_plan(const PagedAttnParams& p, const Piece& w) {
+  if (!p.ws || w.piece + w.tile + w.head != 0 || threadIdx.x != 0) return;
+  ((int*)p.ws)[2 * w.b] = w.n;
+  ((int*)p.ws)[2 * w.b + 1] = w.first_slot;
+}
+
+// The end of both kernels.  `so` holds, per wave, 16 rows (16-row group t of the wave's NT) of COLS output columns from col0 on, on
+// the scale of the row's maximum over the key waves; sm and sl every wave's maxima and sums.  Adds up the key waves and writes the
+// result, or the partial result of a piece.
+template <int D, int NT, int RW, int COLS>
+__device__ __forceinline__ void write_rows(const PagedAttnParams& p, const Piece& w, int fresh, int t, int col0, const float* so, int ldo,
+                                           const float (*sm)[NT * 16], const float (*sl)[NT * 16]) {
+  constexpr int KW = PA_WAVES / RW, NC = COLS / 16;
+  const int rows = p.G * p.Lq, tile0 = w.tile * NT * RW * 16;
+  float* part = w.n > 1 ? p.ws + p.ws_head + (int64_t)w.slot * p.slot_rows * (D + 2) : nullptr;
+  // thread: query tid / 16 of every row wave, NC columns
+  const int query = threadIdx.x >> 4, col = (threadIdx.x & 15) * NC;
+#pragma unroll
+  for (int rx = 0; rx < RW; rx++) {
+    const int at = rx * NT * 16 + t * 16 + query, r = tile0 + at;   // row of the tile, of the head
+    if (r >= rows) break;
+    float y[NC] = {}, qm = -INFINITY, ql = 0.f;
+#pragma unroll
+    for (int x = 0; x < KW; x++) qm = __builtin_fmaxf(qm, sm[x * RW + rx][t * 16 + query]);
+#pragma unroll
+    for (int x = 0; x < KW; x++) {
+#pragma unroll
+      for (int e = 0; e < NC; e++) y[e] += so[((x * RW + rx) * 16 + query) * ldo + col + e];
+      const float mx = sm[x * RW + rx][t * 16 + query];
+      ql += sl[x * RW + rx][t * 16 + query] * (mx == -INFINITY ? 1.f : fast_exp2(mx - qm));
+    }
+    if (part) {
+      float* to = part + at * (D + 2);
+      if (col0 == 0 && col == 0) { to[D] = qm; to[D + 1] = ql; }
+#pragma unroll
+      for (int e = 0; e < NC; e += 2) *(f32x2*)(to + col0 + col + e) = f32x2{y[e], y[e + 1]};
+    } else {
+      const int i = r / p.G;
+      const int64_t out = ((int64_t)w.b * p.H + w.head * p.G + (r - i * p.G)) * p.Lq + i;
+      const bool none = i >= fresh || (qm == -INFINITY && ql == 0.f);
+      const float inv = 1.f / ql;
+#pragma unroll
+      for (int e = 0; e < NC; e += 4) {
+        const u32x2 u = {pack_bf16(y[e] * inv, y[e + 1] * inv), pack_bf16(y[e + 2] * inv, y[e + 3] * inv)};
+        *(u32x2*)(p.o + out * D + col0 + col + e) = none ? u32x2{0u, 0u} : u;
+      }
+      if (col0 == 0 && col == 0) { p.M[out] = none ? -INFINITY : qm; p.L[out] = none ? 1.f : ql; }
+    }
+  }
+}
+
+// Keys that row r of a head sees, and whether that is fewer for earlier rows.  (Rows behind the last one, and padded rows, go along
+// with the last one: what they compute is not written.)
+__device__ __forceinline__ int limit_of(const PagedAttnParams& p, const Piece& w, int fresh, int r) {
+  const int i = min(r, p.G * p.Lq - 1) / p.G;
+  return fresh == 0 ? 0 : p.causal ? max(0, w.len - fresh + min(i, fresh - 1) + 1) : w.len;
+}
+
+// One step of the running softmax of 16 rows over the NS scores of a lane: afterwards s holds the exponentials.  m: what they count
+// from, the same for the four lanes of a query; l: their sum in this lane; top: its largest score.  The reference moves when
+// a score is more than 2^8 above it (or is the first): sums and outputs stay far from the ends of 32-bit range, and the exchange
+// between lanes and the rescaling of the outputs are rare.
+template <int NS, int NO>
+__device__ __forceinline__ void softmax_step(float* s, float c, float& m, float& l, float& top, f32x4* o) {
+  float mt = __builtin_fmaxf(s[0], s[1]);
+#pragma unroll
+  for (int e = 2; e < NS; e += 2) mt = max3(mt, s[e], s[e + 1]);
+  top = __builtin_fmaxf(top, mt);
+  if (__any(mt * c > m + 8.f)) {
+    mt = __builtin_fmaxf(cross_max(mt) * c, m);
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - mt);
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < NO; e++) o[e] *= f;
+    m = mt;
+  }
+  const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int e = 0; e < NS; e++) {
+    s[e] = fast_exp2(__builtin_fmaf(s[e], c, -ms));
+    l += s[e];
+  }
+}
+
+// Puts a wave's sums on the scale of its true maximum (the M of the result): writes both, and returns the factor for its outputs
+// in m and the maximum in top.
+__device__ __forceinline__ void settle(float c, int lane, float& m, float& l, float& top, float* sm, float* sl) {
+  const float mx = cross_max(top) * c, ls = cross_sum(l);
+  // (no finite score: nothing, or NaN that has to stay one)
+  const float f = m == -INFINITY ? 1.f : fast_exp2(m - mx);
+  if (lane < 16) { sm[lane] = mx; sl[lane] = ls * f; }
+  m = f;
+  top = mx;
+}
+
 template <int D, int NT, int RW, bool F8, int WAVES_PER_SIMD>
 __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const PagedAttnParams p) {
   constexpr int KS = D / 32;                  // steps of the contraction over the head dimension
@@ -162,12 +280,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
   const int qi = lane & 15, g = lane >> 4;
   Piece w;
   if (!find_piece(p, blockIdx.x, lane, w)) return;
-  if (w.n > 1 && w.piece + w.tile + w.head == 0 && threadIdx.x == 0) {
-    ((int*)p.ws)[2 * w.b] = w.n;            // for the join
-    ((int*)p.ws)[2 * w.b + 1] = w.first_slot;
-  } else if (p.ws && w.n == 1 && w.tile + w.head == 0 && threadIdx.x == 0) {
-    ((int*)p.ws)[2 * w.b] = 1;
-  }
+  write_plan(p, w);
 
   const int rows = p.G * p.Lq, tile0 = w.tile * NT * RW * 16, row0 = tile0 + rw * NT * 16;
   const int fresh = fresh_of(p, w.b);
@@ -185,8 +298,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
       const int d = F8 ? (ks >> 1) * 64 + g * 16 + (ks & 1) * 8 : ks * 32 + g * 8;
       qf[t][ks] = *(const u32x4*)(q + d);
     }
-    // (columns behind the last row, and padded rows, go along with the last one: what they compute is not written)
-    limit[t] = fresh == 0 ? 0 : p.causal ? max(0, w.len - fresh + min(i, fresh - 1) + 1) : w.len;
+    limit[t] = limit_of(p, w, fresh, r);
     most = max(most, limit[t]);
     least = min(least, limit[t]);
   }
@@ -202,7 +314,6 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
   const int k_end = min(s1 * PA_STAGE, most);
 
   f32x4 o[NT][CH][NE] = {};
-  // m: what the exponentials count from, the same for the four lanes of a query; top: the largest score of this lane, times 1 / c
   float m[NT], l[NT], top[NT];
 #pragma unroll
   for (int t = 0; t < NT; t++) { m[t] = top[t] = -INFINITY; l[t] = 0.f; }
@@ -318,26 +429,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
           for (int r = 0; r < 4; r++)
             if (pg[j] < 0 || key + 16 * j + 4 * g + r >= limit[t]) s[4 * j + r] = -INFINITY;
       }
-      float mt = max3(max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), __builtin_fmaxf(s[6], s[7]));
-      top[t] = __builtin_fmaxf(top[t], mt);
-      // The reference moves when a score is more than 2^8 above it (or is the first): sums and outputs stay far from the ends of
-      // 32-bit range, and the exchange between lanes and the rescaling of the outputs are rare.
-      if (__any(mt * p.c > m[t] + 8.f)) {
-        mt = __builtin_fmaxf(cross_max(mt) * p.c, m[t]);
-        const float f = m[t] == -INFINITY ? 0.f : fast_exp2(m[t] - mt);
-        l[t] *= f;
-#pragma unroll
-        for (int c = 0; c < CH; c++)
-#pragma unroll
-          for (int e = 0; e < NE; e++) o[t][c][e] *= f;
-        m[t] = mt;
-      }
-      const float ms = m[t] == -INFINITY ? 0.f : m[t];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        s[e] = fast_exp2(__builtin_fmaf(s[e], p.c, -ms));
-        l[t] += s[e];
-      }
+      softmax_step<8, CH * NE>(s, p.c, m[t], l[t], top[t], &o[t][0][0]);
       // p is rounded to bf16 for the matrix instruction (its sum is not): 2^-9 per term, independent signs
       pf[t] = pack8u(s);
     }
@@ -388,19 +480,11 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     key = next;
   }
 
-  // The key waves' results become one.  A row's sums are first put on the scale of its true maximum (the M of the result).
+  // the key waves' results become one
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const float mx = cross_max(top[t]) * p.c, ls = cross_sum(l[t]);
-    // (no finite score: nothing, or NaN that has to stay one)
-    const float f = m[t] == -INFINITY ? 1.f : fast_exp2(m[t] - mx);
-    if (lane < 16) { sm[wave][t * 16 + qi] = mx; sl[wave][t * 16 + qi] = ls * f; }
-    m[t] = f;
-    top[t] = mx;
-  }
+  for (int t = 0; t < NT; t++) settle(p.c, lane, m[t], l[t], top[t], &sm[wave][t * 16], &sl[wave][t * 16]);
   __syncthreads();
-  float* part = w.n > 1 ? p.ws + p.ws_head + (int64_t)w.slot * p.slot_rows * (D + 2) : nullptr;
-  #pragma unroll
+#pragma unroll
   for (int t = 0; t < NT; t++) {
     float best = -INFINITY;
 #pragma unroll
@@ -417,41 +501,191 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
           *(f32x4*)&so[wave][qi][(4 * g + r) * NE + e] = y;
         }
       __syncthreads();
-      // thread: query tid / 16 of every row wave, columns NE * (tid % 16) ..
-      const int query = threadIdx.x >> 4, col = (threadIdx.x & 15) * NE;
+      write_rows<D, NT, RW, CW>(p, w, fresh, t, c * CW, &so[0][0][0], LDO, sm, sl);
+    }
+  }
+}
+
+// ---- many rows per key/value head ----
+
+// The same with keys and values staged in LDS, where the waves of a workgroup share them: RW row waves of 16 * NT rows, 4 / RW key
+// waves of 32 keys of a tile of KT.  A quarter of the tile goes through the registers of each wave (requested a tile ahead,
+// converted there if it is e4m3, masked there if nobody may see it), into the buffer that nobody reads: one barrier per tile.
+// 16-byte pieces of a row change places by their row number so that 16 keys (first product) and 16 rows of 32 bytes (transposing
+// reads of the second) lie in different banks.
+template <int D, int NT, int RW, bool F8>
+__global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnParams p) {
+  constexpr int KT = D == 256 ? 32 : 64, KW = PA_WAVES / RW, KS = D / 32, NB = D / 16;
+  constexpr int RB = 2 * D, BUF = KT * RB;                  // bytes of a row, of a tile of keys or values
+  constexpr int LPW = D / 8, RPI = 64 / LPW, NI = KT / 4 / RPI;   // fills: lanes per row, rows per load, loads per wave
+  constexpr int HALVES = KT / (32 * KW);                    // runs of 32 keys per wave and tile
+  static_assert(HALVES >= 1, "a wave takes 32 keys");
+  constexpr int LDO = D + 4;
+  extern __shared__ __align__(16) char smem[];              // [2 buffers][keys, values][BUF]; then the outputs
+  __shared__ float sm[PA_WAVES][NT * 16], sl[PA_WAVES][NT * 16];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % RW, kw = wave / RW;
+  const int qi = lane & 15, g = lane >> 4;
+  Piece w;
+  if (!find_piece(p, blockIdx.x, lane, w)) return;
+  write_plan(p, w);
+
+  const int rows = p.G * p.Lq, tile0 = w.tile * NT * RW * 16, row0 = tile0 + rw * NT * 16;
+  const int fresh = fresh_of(p, w.b);
+  const int s0 = (int)((int64_t)w.stages * w.piece / w.n), s1 = (int)((int64_t)w.stages * (w.piece + 1) / w.n);
+  // limits do not fall from row to row: the last row of the tile, and of the wave, has the largest
+  const int k_end = min(s1 * PA_STAGE, limit_of(p, w, fresh, min(tile0 + NT * RW * 16, rows) - 1));
+  const int least = limit_of(p, w, fresh, row0);
+  const int mine = row0 < rows ? limit_of(p, w, fresh, row0 + NT * 16 - 1) : 0;   // a wave without rows only fills
+
+  u32x4 qf[NT][KS];
+  int limit[NT];
 #pragma unroll
-      for (int rx = 0; rx < RW; rx++) {
-        const int at = rx * NT * 16 + t * 16 + query, r = tile0 + at;   // row of the tile, of the head
-        if (r >= rows) break;
-        float y[NE] = {}, qm = -INFINITY, ql = 0.f;
+  for (int t = 0; t < NT; t++) {
+    const int r = row0 + t * 16 + qi, rc = min(r, rows - 1), i = rc / p.G, h = w.head * p.G + (rc - i * p.G);
+    const bf16_t* q = p.q + w.b * p.q_sb + h * p.q_sh + i * p.q_sr;
 #pragma unroll
-        for (int x = 0; x < KW; x++) qm = __builtin_fmaxf(qm, sm[x * RW + rx][t * 16 + query]);
+    for (int ks = 0; ks < KS; ks++) qf[t][ks] = *(const u32x4*)(q + ks * 32 + g * 8);
+    limit[t] = limit_of(p, w, fresh, r);
+  }
+
+  f32x4 o[NT][NB] = {};
+  float m[NT], l[NT], top[NT];
 #pragma unroll
-        for (int x = 0; x < KW; x++) {
+  for (int t = 0; t < NT; t++) { m[t] = top[t] = -INFINITY; l[t] = 0.f; }
+
+  // fills
+  const uint8_t* kb = p.cache.k + w.head * p.cache.s_head;
+  const uint8_t* vb = p.cache.v + w.head * p.cache.s_head;
+  const uint8_t* keb = F8 ? p.cache.k_exp + w.head * p.cache.e_head : nullptr;
+  const uint8_t* veb = F8 ? p.cache.v_exp + w.head * p.cache.e_head : nullptr;
+  const __attribute__((address_space(4))) int32_t* table = as_constant(p.cache.table + w.b * p.cache.table_stride);
+  const int mask = (1 << p.cache.shift) - 1, sr = (int)p.cache.s_row;
+  const int fr = lane / LPW, fc = lane % LPW;               // row of a load, 16-byte piece (of bf16) of the row
+  auto entry_of = [&](int key) { return table[min(key >> p.cache.shift, p.cache.max_pages - 1)]; };
+  auto page_of = [&](int key, int entry) { return key < k_end && entry >= 0 && entry < p.cache.num_pages ? entry : -1; };
+  u32x4 stage[F8 ? 1 : 2][F8 ? 1 : NI];
+  u32x2 code[F8 ? 2 : 1][F8 ? NI : 1];
+  uint32_t byte[2][NI];
+  int spage = -1;                                           // page of the staged quarter
+  auto request = [&](int key) {                             // key: first of the tile
+    const int first = key + wave * (KT / 4);
+    spage = page_of(first, entry_of(first));
+    const int64_t pp = spage < 0 ? 0 : spage;
+    const int slot = first & mask;
+    const int64_t base = pp * p.cache.s_page + (int64_t)slot * p.cache.s_row;
 #pragma unroll
-          for (int e = 0; e < NE; e++) y[e] += so[x * RW + rx][query][col + e];
-          const float mx = sm[x * RW + rx][t * 16 + query];
-          ql += sl[x * RW + rx][t * 16 + query] * (mx == -INFINITY ? 1.f : fast_exp2(mx - qm));
-        }
-        if (part) {
-          float* to = part + at * (D + 2);
-          if (c == 0 && (threadIdx.x & 15) == 0) { to[D] = qm; to[D + 1] = ql; }
-#pragma unroll
-          for (int e = 0; e < NE; e += 2) *(f32x2*)(to + c * CW + col + e) = f32x2{y[e], y[e + 1]};
-        } else {
-          const int i = r / p.G;
-          const int64_t out = ((int64_t)w.b * p.H + w.head * p.G + (r - i * p.G)) * p.Lq + i;
-          const bool none = i >= fresh || (qm == -INFINITY && ql == 0.f);
-          const float inv = 1.f / ql;
-#pragma unroll
-          for (int e = 0; e < NE; e += 4) {
-            const u32x2 u = {pack_bf16(y[e] * inv, y[e + 1] * inv), pack_bf16(y[e + 2] * inv, y[e + 3] * inv)};
-            *(u32x2*)(p.o + out * D + c * CW + col + e) = none ? u32x2{0u, 0u} : u;
-          }
-          if (c == 0 && (threadIdx.x & 15) == 0) { p.M[out] = none ? -INFINITY : qm; p.L[out] = none ? 1.f : ql; }
-        }
+    for (int x = 0; x < NI; x++) {
+      const uint32_t off = (x * RPI + fr) * sr + fc * (F8 ? 8 : 16);
+      if constexpr (F8) {
+        code[0][x] = *(const u32x2*)(kb + base + off);
+        code[1][x] = *(const u32x2*)(vb + base + off);
+        byte[0][x] = (keb + pp * p.cache.e_page + slot)[x * RPI + fr];
+        byte[1][x] = (veb + pp * p.cache.e_page + slot)[x * RPI + fr];
+      } else {
+        stage[0][x] = *(const u32x4*)(kb + base + off);
+        stage[1][x] = *(const u32x4*)(vb + base + off);
       }
     }
+  };
+  auto deposit = [&](int key, int buf) {
+    const int first = key + wave * (KT / 4);
+    const bool ragged = first + KT / 4 > k_end || spage < 0;
+#pragma unroll
+    for (int x = 0; x < NI; x++) {
+      const int row = wave * (KT / 4) + x * RPI + fr;
+      const int kc = fc ^ (D == 64 ? (row >> 1) & 7 : row & 15), vc = fc ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1);
+      u32x4 kx, vx;
+      if constexpr (F8) {
+        kx = scaled8(code[0][x], exp_value(byte[0][x]));
+        vx = scaled8(code[1][x], exp_value(byte[1][x]));
+      } else {
+        kx = stage[0][x];
+        vx = stage[1][x];
+      }
+      // rows of keys nobody may see hold anything, NaN too, and 0 * NaN is not 0
+      if (ragged && (spage < 0 || key + row >= k_end)) vx = u32x4{0u, 0u, 0u, 0u};
+      *(u32x4*)(smem + (2 * buf) * BUF + row * RB + kc * 16) = kx;
+      *(u32x4*)(smem + (2 * buf + 1) * BUF + row * RB + vc * 16) = vx;
+    }
+  };
+
+  // addresses of the reads: constants of a product's steps are exclusive-ored in, rows added
+  const int ka = qi * RB + (g ^ (D == 64 ? (qi >> 1) & 3 : qi & 3)) * 16 + ((D == 64 ? qi >> 3 : qi >> 2) << 6);
+  const int vrow = 4 * g + (qi >> 2);
+  const int va = vrow * RB + (D == 64 ? (vrow >> 1) & 3 : vrow & 7) * 32 + (qi & 3) * 8;
+
+  const int k0 = s0 * PA_STAGE;
+  if (k0 < k_end) {
+    request(k0);
+    deposit(k0, 0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int key = k0; key < k_end; key += KT, buf ^= 1) {
+    const bool more = key + KT < k_end;
+    if (more) request(key + KT);
+    const char *kt = smem + 2 * buf * BUF, *vt = kt + BUF;
+#pragma unroll
+    for (int hh = 0; hh < HALVES; hh++) {
+      const int run = (kw * HALVES + hh) * 32, first = key + run;
+      if (first >= mine) continue;
+      int pg[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) pg[j] = page_of(first + 16 * j, entry_of(first + 16 * j));
+      const bool ragged = first + 32 > least || pg[0] < 0 || pg[1] < 0;
+      u32x4 pf[NT];
+      f32x4 a[NT][2] = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const u32x4 kx = *(const u32x4*)(kt + ((ka ^ (ks * 64)) + (run + 16 * j) * RB));
+#pragma unroll
+          for (int t = 0; t < NT; t++) a[t][j] = mfma16(kx, qf[t][ks], a[t][j]);
+        }
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float s[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[e] = a[t][e >> 2][e & 3];
+        if (ragged) {
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (pg[e >> 2] < 0 || first + 16 * (e >> 2) + 4 * g + (e & 3) >= limit[t]) s[e] = -INFINITY;
+        }
+        softmax_step<8, NB>(s, p.c, m[t], l[t], top[t], o[t]);
+        pf[t] = pack8u(s);
+      }
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        const char* at = vt + ((va ^ (n * 32)) + run * RB);
+        const u32x2 lo = __builtin_bit_cast(u32x2, lds_read_tr(at)), hi = __builtin_bit_cast(u32x2, lds_read_tr(at + 16 * RB));
+        const u32x4 vx = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[t][n] = mfma16(vx, pf[t], o[t][n]);
+      }
+    }
+    if (more) deposit(key + KT, buf ^ 1);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int t = 0; t < NT; t++) settle(p.c, lane, m[t], l[t], top[t], &sm[wave][t * 16], &sl[wave][t * 16]);
+  __syncthreads();
+  float* so = (float*)smem;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    float best = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < KW; x++) best = __builtin_fmaxf(best, sm[x * RW + rw][t * 16 + qi]);
+    const float f = top[t] == -INFINITY ? 1.f : m[t] * fast_exp2(top[t] - best);
+    if (t > 0) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NB; n++) *(f32x4*)&so[(wave * 16 + qi) * LDO + n * 16 + 4 * g] = o[t][n] * f;
+    __syncthreads();
+    write_rows<D, NT, RW, D>(p, w, fresh, t, 0, so, LDO, sm, sl);
   }
 }
 
@@ -518,38 +752,52 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p
 
 // ---- launch ----
 
-struct Shape { int nt, rw, rt, rows, target, min_share; };
+struct Shape { int nt, rw, rt, rows, target, min_share; bool staged; };
 
-// Rows per tile: 16 up to 16 rows of a key/value head, else 32, 64 or 128.
+// Rows per tile: 16 up to 16 rows of a key/value head, 32 up to 32 (each wave reads keys for itself), more with staged tiles: 64 up to
+// 64 rows, then 128 (head_dim 256: 64 from 17 rows on, its outputs take twice the registers).
 static Shape shape_of(int H, int Hkv, int Lq, int head_dim) {
   Shape s;
   const int64_t rows = (int64_t)(H / Hkv) * Lq;
   s.nt = rows <= 16 || head_dim == 256 ? 1 : 2;
-  const int per = 16 * s.nt;
-  s.rw = rows <= per ? 1 : rows <= 2 * per ? 2 : 4;
-  const int tile = per * s.rw;
+  s.staged = rows > 16 * s.nt;
+  s.rw = !s.staged ? 1 : rows <= 64 && head_dim < 256 ? 2 : 4;
+  const int tile = 16 * s.nt * s.rw;
   s.rt = (int)((rows + tile - 1) / tile);
   s.rows = (int)(rows < tile ? rows : tile);
-  s.target = device_cus() * (s.nt == 1 && head_dim < 256 ? 3 : 2);   // workgroups that the registers let a compute unit hold
+  s.target = device_cus() * (s.nt == 1 && head_dim < 256 ? 3 : 2);   // workgroups that a compute unit holds
   s.min_share = 2;
   return s;
 }
 
 static int64_t ws_head_floats(int B) { return ((int64_t)2 * B + 63) / 64 * 64; }   // pieces and first slot of every sequence
 
-// Partial results are kept for tiles that are cut only; such a tile has n < 2 * stages / share pieces, so that there are fewer
-// than 2 * target of them in all.
+// Partial results are kept for tiles that are cut only; such a tile has n < 2 * stages / share pieces, and a share is at least the
+// 2 * target-th part of all stages, so that there are fewer than 4 * target of them in all.
 int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim) {
   const Shape s = shape_of(H, Hkv, Lq, head_dim);
   if (s.target <= 0) return LVAR_ELAUNCH;
   if ((max_len + PA_STAGE - 1) / PA_STAGE <= s.min_share) return 0;   // nothing can be cut
-  return 4 * (ws_head_floats(B) + 2ll * s.target * s.rows * (head_dim + 2));
+  return 4 * (ws_head_floats(B) + 4ll * s.target * s.rows * (head_dim + 2));
 }
 
-template <int D, int NT, int RW, int W>
-static void launch_rw(const PagedAttnParams& p, int grid, hipStream_t s) {
-  if (p.cache.k_exp) hipLaunchKernelGGL((paged_attn_kernel<D, NT, RW, true, W>), dim3(grid), dim3(PA_T), 0, s, p);
-  else hipLaunchKernelGGL((paged_attn_kernel<D, NT, RW, false, W>), dim3(grid), dim3(PA_T), 0, s, p);
+template <int D, int NT, int W>
+static void launch_direct(const PagedAttnParams& p, int grid, hipStream_t s) {
+  if (p.cache.k_exp) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, true, W>), dim3(grid), dim3(PA_T), 0, s, p);
+  else hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, false, W>), dim3(grid), dim3(PA_T), 0, s, p);
+}
+
+template <int D, int NT, int RW, bool F8>
+static bool launch_staged(const PagedAttnParams& p, int grid, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int kTiles = 4 * (D == 256 ? 32 : 64) * 2 * D, kOut = PA_WAVES * 16 * (D + 4) * 4, kBytes = kTiles > kOut ? kTiles : kOut;
+  if (!ensure_lds_limit((const void*)&paged_tile_kernel<D, NT, RW, F8>, kBytes, done)) return false;
+  hipLaunchKernelGGL((paged_tile_kernel<D, NT, RW, F8>), dim3(grid), dim3(PA_T), kBytes, s, p);
+  return true;
+}
+template <int D, int NT, int RW>
+static bool launch_staged(const PagedAttnParams& p, int grid, hipStream_t s) {
+  return p.cache.k_exp ? launch_staged<D, NT, RW, true>(p, grid, s) : launch_staged<D, NT, RW, false>(p, grid, s);
 }
 
 template <int D, int RPB>
@@ -559,19 +807,18 @@ static void launch_join(const PagedAttnParams& p, int tile_rows, hipStream_t s) 
 
 template <int D>
 static int launch_d(const PagedAttnParams& p, const Shape& h, hipStream_t s) {
-  const int64_t items = (int64_t)p.B * p.cache.kv_heads * p.rt + (p.ws ? p.target : 0);
+  const int64_t items = (int64_t)p.B * p.cache.kv_heads * p.rt + (p.ws ? 2ll * p.target : 0);
   if (items > 0x7ffffff0) return LVAR_EINVAL;
   const int grid = (int)((items + 7) / 8 * 8);
-  if (h.nt == 1) {
-    constexpr int W = D == 256 ? 2 : 3;
-    if (h.rw == 1) launch_rw<D, 1, 1, W>(p, grid, s);
-    else if constexpr (D == 256) { if (h.rw == 2) launch_rw<D, 1, 2, W>(p, grid, s); else launch_rw<D, 1, 4, W>(p, grid, s); }
-  } else if constexpr (D < 256) {
-    if (h.rw == 1) launch_rw<D, 2, 1, 2>(p, grid, s);
-    else if (h.rw == 2) launch_rw<D, 2, 2, 2>(p, grid, s);
-    else launch_rw<D, 2, 4, 2>(p, grid, s);
+  bool ok = true;
+  if constexpr (D == 256) {
+    if (!h.staged) launch_direct<D, 1, 2>(p, grid, s);
+    else ok = launch_staged<D, 1, 4>(p, grid, s);
+  } else {
+    if (!h.staged) h.nt == 1 ? launch_direct<D, 1, 3>(p, grid, s) : launch_direct<D, 2, 2>(p, grid, s);
+    else ok = h.rw == 2 ? launch_staged<D, 2, 2>(p, grid, s) : launch_staged<D, 2, 4>(p, grid, s);
   }
-  if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
+  if (!ok || hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
   if (p.ws) {
     // few rows: all groups along the pieces of one row; many: a group per row
     constexpr int GR = 512 / (D / 4);
