@@ -132,9 +132,13 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
     pieces *= units;
   };
   count();
-  // One round of workgroups if the rounding up of the pieces lets it be one; otherwise pieces half as long, whose second and third
-  // rounds even out (one sequence of 131071 tokens, 752 pieces in one round: 54 us, in two 56; 32 ragged ones 401 us with one round
-  // and a bit, 388 with finer pieces).
+  // One round of workgroups, with pieces up to 3 / 8 longer if that makes it one; otherwise pieces half as long, whose second and third
+  // rounds even out.
+  const int even = share;
+  for (int tries = 0; tries < 3 && pieces > p.target; tries++) {
+    share += max(1, even >> 3);
+    count();
+  }
   if (pieces > p.target) {
     share = share_of(p, total, 2 * p.target);
     count();
@@ -508,8 +512,12 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
 
 // ---- many rows per key/value head ----
 
+__device__ __forceinline__ u32x2 read_tr(LVAR_LDS const char* p) {   // see lds_read_tr
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LVAR_LDS bf16x4*)p));
+}
+
 // The same with keys and values staged in LDS, where the waves of a workgroup share them: RW row waves of 16 * NT rows, 4 / RW key
-// waves of 32 keys of a tile of KT.  A quarter of the tile goes through the registers of each wave (requested a tile ahead,
+// waves of 32 keys of a tile of KT.  A quarter of the tile goes through the registers of each wave (requested two tiles ahead,
 // converted there if it is e4m3, masked there if nobody may see it), into the buffer that nobody reads: one barrier per tile.
 // 16-byte pieces of a row change places by their row number so that 16 keys (first product) and 16 rows of 32 bytes (transposing
 // reads of the second) lie in different banks.
@@ -523,6 +531,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
   constexpr int LDO = D + 4;
   extern __shared__ __align__(16) char smem[];              // [2 buffers][keys, values][BUF]; then the outputs
   __shared__ float sm[PA_WAVES][NT * 16], sl[PA_WAVES][NT * 16];
+  __shared__ uint8_t missing[2][4];                         // quarters of a tile without a page (or behind the last key)
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave % RW, kw = wave / RW;
@@ -565,86 +574,86 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
   const int fr = lane / LPW, fc = lane % LPW;               // row of a load, 16-byte piece (of bf16) of the row
   auto entry_of = [&](int key) { return table[min(key >> p.cache.shift, p.cache.max_pages - 1)]; };
   auto page_of = [&](int key, int entry) { return key < k_end && entry >= 0 && entry < p.cache.num_pages ? entry : -1; };
-  u32x4 stage[F8 ? 1 : 2][F8 ? 1 : NI];
-  u32x2 code[F8 ? 2 : 1][F8 ? NI : 1];
-  uint32_t byte[2][NI];
-  int spage = -1;                                           // page of the staged quarter
-  auto request = [&](int key) {                             // key: first of the tile
-    const int first = key + wave * (KT / 4);
-    spage = page_of(first, entry_of(first));
-    const int64_t pp = spage < 0 ? 0 : spage;
+  struct Fill {                                             // a wave's quarter of a tile on its way
+    u32x4 row[F8 ? 1 : 2][F8 ? 1 : NI];
+    u32x2 code[F8 ? 2 : 1][F8 ? NI : 1];
+    uint32_t byte[F8 ? 2 : 1][F8 ? NI : 1];
+    int page;
+  };
+  // Quarter of the tile from `key` on; behind the last tile that one again (nobody reads it): no branch stands between the loads
+  // of one tile and the next, so that the wait for one never waits for the other.
+  const int k0 = s0 * PA_STAGE, last = k_end > k0 ? (k_end - 1) / KT * KT : k0;
+  auto quarter_of = [&](int key) { return min(key, last) + wave * (KT / 4); };
+  auto request = [&](Fill& f, int key, int entry) {
+    const int first = quarter_of(key);
+    f.page = page_of(first, entry);
+    const int64_t pp = f.page < 0 ? 0 : f.page;
     const int slot = first & mask;
     const int64_t base = pp * p.cache.s_page + (int64_t)slot * p.cache.s_row;
 #pragma unroll
     for (int x = 0; x < NI; x++) {
       const uint32_t off = (x * RPI + fr) * sr + fc * (F8 ? 8 : 16);
       if constexpr (F8) {
-        code[0][x] = *(const u32x2*)(kb + base + off);
-        code[1][x] = *(const u32x2*)(vb + base + off);
-        byte[0][x] = (keb + pp * p.cache.e_page + slot)[x * RPI + fr];
-        byte[1][x] = (veb + pp * p.cache.e_page + slot)[x * RPI + fr];
+        f.code[0][x] = *(const u32x2*)(kb + base + off);
+        f.code[1][x] = *(const u32x2*)(vb + base + off);
+        f.byte[0][x] = (keb + pp * p.cache.e_page + slot)[x * RPI + fr];
+        f.byte[1][x] = (veb + pp * p.cache.e_page + slot)[x * RPI + fr];
       } else {
-        stage[0][x] = *(const u32x4*)(kb + base + off);
-        stage[1][x] = *(const u32x4*)(vb + base + off);
+        f.row[0][x] = *(const u32x4*)(kb + base + off);
+        f.row[1][x] = *(const u32x4*)(vb + base + off);
       }
     }
   };
-  auto deposit = [&](int key, int buf) {
-    const int first = key + wave * (KT / 4);
-    const bool ragged = first + KT / 4 > k_end || spage < 0;
+  auto deposit = [&](const Fill& f, int key, int buf) {
+    const int first = quarter_of(key);
+    const bool ragged = first + KT / 4 > k_end || f.page < 0;
 #pragma unroll
     for (int x = 0; x < NI; x++) {
       const int row = wave * (KT / 4) + x * RPI + fr;
       const int kc = fc ^ (D == 64 ? (row >> 1) & 7 : row & 15), vc = fc ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1);
       u32x4 kx, vx;
       if constexpr (F8) {
-        kx = scaled8(code[0][x], exp_value(byte[0][x]));
-        vx = scaled8(code[1][x], exp_value(byte[1][x]));
+        kx = scaled8(f.code[0][x], exp_value(f.byte[0][x]));
+        vx = scaled8(f.code[1][x], exp_value(f.byte[1][x]));
       } else {
-        kx = stage[0][x];
-        vx = stage[1][x];
+        kx = f.row[0][x];
+        vx = f.row[1][x];
       }
       // rows of keys nobody may see hold anything, NaN too, and 0 * NaN is not 0
-      if (ragged && (spage < 0 || key + row >= k_end)) vx = u32x4{0u, 0u, 0u, 0u};
+      if (ragged && (f.page < 0 || first + x * RPI + fr >= k_end)) vx = u32x4{0u, 0u, 0u, 0u};
       *(u32x4*)(smem + (2 * buf) * BUF + row * RB + kc * 16) = kx;
       *(u32x4*)(smem + (2 * buf + 1) * BUF + row * RB + vc * 16) = vx;
     }
+    if (lane == 0) missing[buf][wave] = f.page < 0;
   };
 
   // addresses of the reads: constants of a product's steps are exclusive-ored in, rows added
   const int ka = qi * RB + (g ^ (D == 64 ? (qi >> 1) & 3 : qi & 3)) * 16 + ((D == 64 ? qi >> 3 : qi >> 2) << 6);
   const int vrow = 4 * g + (qi >> 2);
   const int va = vrow * RB + (D == 64 ? (vrow >> 1) & 3 : vrow & 7) * 32 + (qi & 3) * 8;
+  LVAR_LDS const char *const lds = (LVAR_LDS const char*)smem, *kp[KS], *vp[NB];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) kp[ks] = lds + (ka ^ (ks * 64)) + kw * HALVES * 32 * RB;
+#pragma unroll
+  for (int n = 0; n < NB; n++) vp[n] = lds + (va ^ (n * 32)) + kw * HALVES * 32 * RB;
 
-  const int k0 = s0 * PA_STAGE;
-  if (k0 < k_end) {
-    request(k0);
-    deposit(k0, 0);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int key = k0; key < k_end; key += KT, buf ^= 1) {
-    const bool more = key + KT < k_end;
-    if (more) request(key + KT);
-    const char *kt = smem + 2 * buf * BUF, *vt = kt + BUF;
+  auto compute = [&](int key, int buf) {
+    const uint32_t gone = *(const uint32_t*)missing[buf];
 #pragma unroll
     for (int hh = 0; hh < HALVES; hh++) {
       const int run = (kw * HALVES + hh) * 32, first = key + run;
       if (first >= mine) continue;
-      int pg[2];
-#pragma unroll
-      for (int j = 0; j < 2; j++) pg[j] = page_of(first + 16 * j, entry_of(first + 16 * j));
-      const bool ragged = first + 32 > least || pg[0] < 0 || pg[1] < 0;
       u32x4 pf[NT];
       f32x4 a[NT][2] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ks++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          const u32x4 kx = *(const u32x4*)(kt + ((ka ^ (ks * 64)) + (run + 16 * j) * RB));
+          const u32x4 kx = *(LVAR_LDS const u32x4*)(kp[ks] + 2 * buf * BUF + (hh * 32 + 16 * j) * RB);
 #pragma unroll
           for (int t = 0; t < NT; t++) a[t][j] = mfma16(kx, qf[t][ks], a[t][j]);
         }
+      const bool ragged = first + 32 > least || __builtin_amdgcn_readfirstlane(gone) != 0;
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         float s[8];
@@ -652,22 +661,42 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
         for (int e = 0; e < 8; e++) s[e] = a[t][e >> 2][e & 3];
         if (ragged) {
 #pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (pg[e >> 2] < 0 || first + 16 * (e >> 2) + 4 * g + (e & 3) >= limit[t]) s[e] = -INFINITY;
+          for (int e = 0; e < 8; e++) {
+            const int at = run + 16 * (e >> 2);             // of the tile: the 16 keys of one page
+            if (((gone >> (at / (KT / 4) * 8)) & 1) || key + at + 4 * g + (e & 3) >= limit[t]) s[e] = -INFINITY;
+          }
         }
         softmax_step<8, NB>(s, p.c, m[t], l[t], top[t], o[t]);
         pf[t] = pack8u(s);
       }
 #pragma unroll
       for (int n = 0; n < NB; n++) {
-        const char* at = vt + ((va ^ (n * 32)) + run * RB);
-        const u32x2 lo = __builtin_bit_cast(u32x2, lds_read_tr(at)), hi = __builtin_bit_cast(u32x2, lds_read_tr(at + 16 * RB));
+        LVAR_LDS const char* at = vp[n] + (2 * buf + 1) * BUF + hh * 32 * RB;
+        const u32x2 lo = read_tr(at), hi = read_tr(at + 16 * RB);
         const u32x4 vx = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
         for (int t = 0; t < NT; t++) o[t][n] = mfma16(vx, pf[t], o[t][n]);
       }
     }
-    if (more) deposit(key + KT, buf ^ 1);
+  };
+
+  // (the table entry that the next request needs is loaded ahead of a barrier: scalar loads and LDS reads share a counter)
+  Fill f0, f1;
+  request(f0, k0, entry_of(quarter_of(k0)));
+  request(f1, k0 + KT, entry_of(quarter_of(k0 + KT)));
+  deposit(f0, k0, 0);
+  int entry = entry_of(quarter_of(k0 + 2 * KT));
+  __syncthreads();
+  for (int key = k0; key < k_end; key += 2 * KT) {
+    request(f0, key + 2 * KT, entry);
+    compute(key, 0);
+    deposit(f1, key + KT, 1);
+    entry = entry_of(quarter_of(key + 3 * KT));
+    __syncthreads();
+    request(f1, key + 3 * KT, entry);
+    if (key + KT < k_end) compute(key + KT, 1);
+    deposit(f0, key + 2 * KT, 0);
+    entry = entry_of(quarter_of(key + 4 * KT));
     __syncthreads();
   }
 
