@@ -517,7 +517,7 @@ __device__ __forceinline__ u32x2 read_tr(LVAR_LDS const char* p) {   // see lds_
 }
 
 // The same with keys and values staged in LDS, where the waves of a workgroup share them: RW row waves of 16 * NT rows, 4 / RW key
-// waves of 32 keys of a tile of KT.  A quarter of the tile goes through the registers of each wave (requested two tiles ahead,
+// waves of 32 keys of a tile of KT.  A quarter of the tile goes through the registers of each wave (requested a tile ahead,
 // converted there if it is e4m3, masked there if nobody may see it), into the buffer that nobody reads: one barrier per tile.
 // 16-byte pieces of a row change places by their row number so that 16 keys (first product) and 16 rows of 32 bytes (transposing
 // reads of the second) lie in different banks.
@@ -681,22 +681,21 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
   };
 
   // (the table entry that the next request needs is loaded ahead of a barrier: scalar loads and LDS reads share a counter)
-  Fill f0, f1;
-  request(f0, k0, entry_of(quarter_of(k0)));
-  request(f1, k0 + KT, entry_of(quarter_of(k0 + KT)));
-  deposit(f0, k0, 0);
-  int entry = entry_of(quarter_of(k0 + 2 * KT));
+  Fill f;
+  request(f, k0, entry_of(quarter_of(k0)));
+  deposit(f, k0, 0);
+  int entry = entry_of(quarter_of(k0 + KT));
   __syncthreads();
   for (int key = k0; key < k_end; key += 2 * KT) {
-    request(f0, key + 2 * KT, entry);
+    request(f, key + KT, entry);
     compute(key, 0);
-    deposit(f1, key + KT, 1);
-    entry = entry_of(quarter_of(key + 3 * KT));
+    deposit(f, key + KT, 1);
+    entry = entry_of(quarter_of(key + 2 * KT));
     __syncthreads();
-    request(f1, key + 3 * KT, entry);
+    request(f, key + 2 * KT, entry);
     if (key + KT < k_end) compute(key + KT, 1);
-    deposit(f0, key + 2 * KT, 0);
-    entry = entry_of(quarter_of(key + 4 * KT));
+    deposit(f, key + 2 * KT, 0);
+    entry = entry_of(quarter_of(key + 3 * KT));
     __syncthreads();
   }
 
