@@ -645,14 +645,23 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
       if (first >= mine) continue;
       u32x4 pf[NT];
       f32x4 a[NT][2] = {};
+      // (all reads of a run of steps ahead of its products: a wave has one other to hide their time behind)
+      constexpr int KG = KS > 4 ? 4 : KS;
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++)
+      for (int k1 = 0; k1 < KS; k1 += KG) {
+        u32x4 kx[KG][2];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const u32x4 kx = *(LVAR_LDS const u32x4*)(kp[ks] + 2 * buf * BUF + (hh * 32 + 16 * j) * RB);
+        for (int ks = 0; ks < KG; ks++)
 #pragma unroll
-          for (int t = 0; t < NT; t++) a[t][j] = mfma16(kx, qf[t][ks], a[t][j]);
-        }
+          for (int j = 0; j < 2; j++) kx[ks][j] = *(LVAR_LDS const u32x4*)(kp[k1 + ks] + 2 * buf * BUF + (hh * 32 + 16 * j) * RB);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < KG; ks++)
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) a[t][j] = mfma16(kx[ks][j], qf[t][k1 + ks], a[t][j]);
+      }
       const bool ragged = first + 32 > least || __builtin_amdgcn_readfirstlane(gone) != 0;
 #pragma unroll
       for (int t = 0; t < NT; t++) {
@@ -669,13 +678,24 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
         softmax_step<8, NB>(s, p.c, m[t], l[t], top[t], o[t]);
         pf[t] = pack8u(s);
       }
+      u32x4 vx[2][4];
+      auto read4 = [&](int n0, u32x4* to) {
 #pragma unroll
-      for (int n = 0; n < NB; n++) {
-        LVAR_LDS const char* at = vp[n] + (2 * buf + 1) * BUF + hh * 32 * RB;
-        const u32x2 lo = read_tr(at), hi = read_tr(at + 16 * RB);
-        const u32x4 vx = {lo[0], lo[1], hi[0], hi[1]};
+        for (int n = 0; n < 4; n++) {
+          LVAR_LDS const char* at = vp[n0 + n] + (2 * buf + 1) * BUF + hh * 32 * RB;
+          const u32x2 lo = read_tr(at), hi = read_tr(at + 16 * RB);
+          to[n] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+      };
+      read4(0, vx[0]);
 #pragma unroll
-        for (int t = 0; t < NT; t++) o[t][n] = mfma16(vx, pf[t], o[t][n]);
+      for (int n0 = 0; n0 < NB; n0 += 4) {
+        if (n0 + 4 < NB) read4(n0 + 4, vx[(n0 / 4 + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+          for (int t = 0; t < NT; t++) o[t][n0 + n] = mfma16(vx[(n0 / 4) & 1][n], pf[t], o[t][n0 + n]);
       }
     }
   };
