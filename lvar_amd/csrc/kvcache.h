@@ -37,7 +37,7 @@ struct NormRopeParams {
   bf16_t *oq, *ok;               // contiguous [B,H,L,d], [B,Hkv,L,d]; ok null: k goes into the cache
   WeightView wq, wk;
   int norm;
-  float eps;
+  float eps, inv_eps;            // inv_eps: set at launch
   const float *cos, *sin;        // [table_rows, rot/2], null: no rotation
   int64_t cs_row;
   int table_rows, rot, interleaved;
@@ -45,6 +45,8 @@ struct NormRopeParams {
   int64_t pos_sb, pos_sl;
   int pos64;
   int B, H, Hkv, L;
+  uint32_t div_mul;              // division by L, set at launch
+  int div_s1, div_s2;
   // append
   PagedView cache;
   const int32_t *start, *counts;  // [B]; counts null: L
@@ -90,9 +92,9 @@ struct PagedAttnParams {
   int64_t ws_head;                // floats ahead of the partial results
 };
 
-int launch_norm_rope(const NormRopeParams& p, int head_dim, bool append, hipStream_t s);
+int launch_norm_rope(NormRopeParams p, int head_dim, bool append, hipStream_t s);
 int norm_rope_bwd_blocks(int B, int H, int Hkv, int L, int head_dim);
-int launch_norm_rope_bwd(const NormRopeParams& p, int head_dim, hipStream_t s);
+int launch_norm_rope_bwd(NormRopeParams p, int head_dim, hipStream_t s);
 int launch_weight_grad(const WeightGradParams& w, hipStream_t s);
 int launch_kv_read(const KvReadParams& p, int head_dim, hipStream_t s);
 int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim);

@@ -14,6 +14,14 @@ namespace lvar {
 
 constexpr int NR_T = 256;
 
+// Results of large launches go past the L2s, whoever reads them next mostly sits on another XCD: 2 x 16 x 4096 rows of q and of k
+// 28.3 -> 26.4 us, their gradients over 10521 tokens 240 -> 220.
+template <bool STREAM>
+__device__ __forceinline__ void put(bf16_t* to, u32x4 x) {
+  if constexpr (STREAM) __builtin_nontemporal_store(x, (u32x4*)to);
+  else *(u32x4*)to = x;
+}
+
 struct Angles {
   float c[8], s[8];   // pairs of the lane: 4 of them (interleaved) or 8 (halves)
   bool on;            // the lane's columns are among the rotated ones
@@ -89,15 +97,27 @@ __device__ __forceinline__ void load_weight(const WeightView& w, int head, int l
   }
 }
 
-// r of a row with this sum of squares; `flat`: |x| <= eps, where the l2 norm is a division by eps
+// r of a row with this sum of squares; `flat`: |x| <= eps, where the l2 norm is a division by eps.  The reciprocal root is the
+// hardware's, off by one step of fp32 at most (sums below its normal range scaled into it): with roots and quotients rounded
+// to nearest, a quarter of the instructions of a row went into these two lines.
 template <int D>
 __device__ __forceinline__ float norm_factor(const NormRopeParams& p, float ss, bool& flat) {
   flat = false;
   if (p.norm == NORM_NONE) return 1.f;
-  if (p.norm == NORM_RMS) return 1.f / __builtin_sqrtf(ss * (1.f / D) + p.eps);
-  const float n = __builtin_sqrtf(ss);
-  flat = n <= p.eps;
-  return 1.f / (flat ? p.eps : n);
+  if (p.norm == NORM_RMS) ss = ss * (1.f / D) + p.eps;
+  const bool tiny = ss < 0x1p-100f;
+  const float r = __builtin_amdgcn_rsqf(tiny ? ss * 0x1p100f : ss) * (tiny ? 0x1p50f : 1.f);
+  if (p.norm == NORM_L2 && ss * r <= p.eps) {   // ss * r = |x| (0 * inf, the norm of a zero row, is NaN)
+    flat = true;
+  }
+  if (p.norm == NORM_L2 && ss == 0.f) flat = true;
+  return flat ? p.inv_eps : r;
+}
+
+// t / L by a multiplication (see division_by): 31-bit t
+__device__ __forceinline__ int sequence_of(const NormRopeParams& p, int t) {
+  const uint32_t h = __umulhi(p.div_mul, (uint32_t)t);
+  return (int)((h + (((uint32_t)t - h) >> p.div_s1)) >> p.div_s2);
 }
 
 __device__ __forceinline__ int64_t table_row(const NormRopeParams& p, int b, int i, int64_t base) {
@@ -109,17 +129,26 @@ __device__ __forceinline__ int64_t table_row(const NormRopeParams& p, int b, int
   return pos < 0 ? 0 : pos >= p.table_rows ? p.table_rows - 1 : pos;
 }
 
+// chunks of HC heads: those of q (unless keys are written as they are), of k, and when appending of v
+template <int HC>
+__host__ __device__ __forceinline__ int chunks_of(const NormRopeParams& p, bool append) {
+  const int nk = (p.Hkv + HC - 1) / HC;
+  return (append && p.ready ? 0 : (p.H + HC - 1) / HC) + (append ? 2 * nk : nk);
+}
+
 template <int D, int HC, bool APPEND>
 __global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p) {
   constexpr int LPR = D / 8, RPB = NR_T / LPR;
   const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
-  const int T = p.B * p.L, t_own = blockIdx.x * RPB + g;
+  // heads fastest: the rows of a token lie next to each other in a fused projection (heads slowest, so that workgroups in flight
+  // read 1 KiB pieces 12 KiB apart: 140 us where this takes 126, 4 x 10521 tokens of 32 heads)
+  const int T = p.B * p.L, chunks_all = chunks_of<HC>(p, APPEND), t_own = (int)(blockIdx.x / chunks_all) * RPB + g;
   const bool live = t_own < T;
   const int t = live ? t_own : T - 1;
-  const int b = t / p.L, i = t - b * p.L;
+  const int b = sequence_of(p, t), i = t - b * p.L;
   // chunks of heads: those of q, then k, then v
   const int nq = APPEND && p.ready ? 0 : (p.H + HC - 1) / HC, nk = (p.Hkv + HC - 1) / HC;
-  int c = blockIdx.y;
+  int c = blockIdx.x % chunks_all;
   const int which = c < nq ? 0 : c < nq + nk ? 1 : 2;
   c -= which == 0 ? 0 : which == 1 ? nq : nq + nk;
   const int heads = which == 0 ? p.H : p.Hkv, h0 = c * HC;
@@ -165,7 +194,7 @@ __global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p)
     }
     if (!APPEND || which == 0) {
       bf16_t* out = which == 0 ? p.oq : p.ok;
-      if (live) *(u32x4*)(out + (((int64_t)b * heads + head) * p.L + i) * D + lane * 8) = pack8u(f);
+      if (live) put<(HC > 1)>(out + (((int64_t)b * heads + head) * p.L + i) * D + lane * 8, pack8u(f));
     } else {
       const int64_t at = page * p.cache.s_page + head * p.cache.s_head + slot * p.cache.s_row;
       uint8_t* pages = which == 1 ? p.cache.k : p.cache.v;
@@ -186,25 +215,36 @@ __global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p)
   }
 }
 
+// Constants of the division of 32-bit numbers by L (rounded-up reciprocal, Granlund and Montgomery 1994, figure 4.1).
+static void division_by(NormRopeParams& p) {
+  const uint32_t L = (uint32_t)p.L;
+  int l = 0;
+  while ((1ull << l) < L) l++;
+  p.div_mul = (uint32_t)(((1ull << 32) * ((1ull << l) - L)) / L + 1);
+  p.div_s1 = l < 1 ? l : 1;
+  p.div_s2 = l - 1 > 0 ? l - 1 : 0;
+}
+
 template <int D, int HC>
 static void launch_fwd(const NormRopeParams& p, bool append, hipStream_t s) {
   constexpr int RPB = NR_T / (D / 8);
-  const int nk = (p.Hkv + HC - 1) / HC, nq = append && p.ready ? 0 : (p.H + HC - 1) / HC;
-  const dim3 grid((p.B * p.L + RPB - 1) / RPB, nq + nk + (append ? nk : 0));
+  const dim3 grid((uint32_t)chunks_of<HC>(p, append) * (uint32_t)((p.B * p.L + RPB - 1) / RPB));
   if (append) hipLaunchKernelGGL((norm_rope_kernel<D, HC, true>), grid, dim3(NR_T), 0, s, p);
   else hipLaunchKernelGGL((norm_rope_kernel<D, HC, false>), grid, dim3(NR_T), 0, s, p);
 }
 
 template <int D>
 static void launch_fwd_d(const NormRopeParams& p, bool append, hipStream_t s) {
-  // Four heads per workgroup once such workgroups fill the chip, one head before that.
+  // Four heads per workgroup once such workgroups are four per compute unit, one head before that (latency is the time there).
   constexpr int RPB = NR_T / (D / 8);
-  const int64_t tiles = (int64_t)(p.B * p.L + RPB - 1) / RPB, heads = p.H + p.Hkv;
-  if (tiles * ((heads + 3) / 4) >= 8ll * device_cus()) launch_fwd<D, 4>(p, append, s);
+  const int64_t tiles = (int64_t)(p.B * p.L + RPB - 1) / RPB;
+  if (tiles * chunks_of<4>(p, append) >= 4ll * device_cus()) launch_fwd<D, 4>(p, append, s);
   else launch_fwd<D, 1>(p, append, s);
 }
 
-int launch_norm_rope(const NormRopeParams& p, int head_dim, bool append, hipStream_t s) {
+int launch_norm_rope(NormRopeParams p, int head_dim, bool append, hipStream_t s) {
+  division_by(p);
+  p.inv_eps = 1.f / p.eps;
   switch (head_dim) {
     case 16: if (append) return LVAR_EUNSUPPORTED; launch_fwd_d<16>(p, append, s); break;
     case 32: if (append) return LVAR_EUNSUPPORTED; launch_fwd_d<32>(p, append, s); break;
@@ -218,7 +258,7 @@ int launch_norm_rope(const NormRopeParams& p, int head_dim, bool append, hipStre
 
 // ---- backward ----
 
-constexpr int NB_HC = 4;   // heads of a workgroup
+constexpr int NB_HC = 2;   // heads of a workgroup
 
 // Workgroup (blk, chunk): tokens blk * RPB + g, + nblk * RPB, ... of up to 4 heads of q or of k.  The weight gradients of its
 // heads stay in registers over all its tokens and meet in LDS once, in a fixed order: row `blk` of the partial sums.
@@ -228,9 +268,10 @@ __global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParam
   __shared__ float red[DW ? RPB * D : 1];
   const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
   const int T = p.B * p.L;
-  const int nq = (p.H + HC - 1) / HC;
-  const bool isq = (int)blockIdx.y < nq;
-  const int h0 = (isq ? (int)blockIdx.y : (int)blockIdx.y - nq) * HC;
+  const int nq = (p.H + HC - 1) / HC, nc = chunks_of<HC>(p, false);
+  const int blk = blockIdx.x / nc, own = blockIdx.x % nc;
+  const bool isq = own < nq;
+  const int h0 = (isq ? own : own - nq) * HC;
   const int heads = isq ? p.H : p.Hkv;
   const bf16_t *x = isq ? p.q : p.k, *gy = isq ? p.gq : p.gk;
   bf16_t* dx = isq ? p.dq : p.dk;
@@ -240,10 +281,10 @@ __global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParam
   float* part = isq ? p.pq : p.pk;
 
   float acc[DW ? HC : 1][8] = {};
-  for (int t0 = blockIdx.x * RPB; t0 < T; t0 += p.nblk * RPB) {
+  for (int t0 = blk * RPB; t0 < T; t0 += p.nblk * RPB) {
     const bool live = t0 + g < T;
     const int t = live ? t0 + g : T - 1;
-    const int b = t / p.L, i = t - b * p.L;
+    const int b = sequence_of(p, t), i = t - b * p.L;
     u32x4 xin[HC], gin[HC];
 #pragma unroll
     for (int j = 0; j < HC; j++) {
@@ -282,7 +323,7 @@ __global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParam
       if (p.norm == NORM_NONE || flat) dot = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; e++) gu[e] = r * (gu[e] - n[e] * dot);
-      if (live) *(u32x4*)(dx + b * db + head * dh + i * dr + lane * 8) = pack8u(gu);
+      if (live) put<true>(dx + b * db + head * dh + i * dr + lane * 8, pack8u(gu));
     }
   }
   if constexpr (DW) {
@@ -301,7 +342,7 @@ __global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParam
 #pragma unroll
       for (int e = 0; e < 8; e++) red[g * D + lane * 8 + e] = acc[j][e];
       __syncthreads();
-      const int64_t at = shared ? (int64_t)blockIdx.x * chunks + chunk : (int64_t)blockIdx.x * heads + h0 + j;
+      const int64_t at = shared ? (int64_t)blk * chunks + chunk : (int64_t)blk * heads + h0 + j;
       for (int col = threadIdx.x; col < D; col += NR_T) {
         float sum = 0.f;
         for (int r = 0; r < RPB; r++) sum += red[r * D + col];
@@ -324,10 +365,28 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const WeightGradParam
   const float* part = w.part[k] + (int64_t)blockIdx.x * w.D;
   const int64_t rs = (int64_t)w.heads[k] * w.D;
   float sum = 0.f;
-  for (int col = (scalar ? 0 : blockIdx.y * 32) + cl; col < w.D; col += 32) {
-#pragma unroll 8
-    for (int r = rl; r < w.rows[k]; r += 32) sum += part[r * rs + col];
-    if (!scalar) break;
+  // (loads in runs of 8 whose end is clamped and not branched over: they are in flight together)
+  if (scalar) {
+    const int n = w.rows[k] * w.D, shift = 31 - __builtin_clz(w.D);
+    for (int at = threadIdx.x; at < n; at += 8 * 1024) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int x = min(at + u * 1024, n - 1);
+        v[u] = part[(x >> shift) * rs + (x & (w.D - 1))];
+      }
+#pragma unroll
+      for (int u = 0; u < 8; u++) sum += at + u * 1024 < n ? v[u] : 0.f;
+    }
+  } else {
+    const int col = blockIdx.y * 32 + cl;
+    for (int r = rl; r < w.rows[k]; r += 8 * 32) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) v[u] = part[min(r + u * 32, w.rows[k] - 1) * rs + min(col, w.D - 1)];
+#pragma unroll
+      for (int u = 0; u < 8; u++) sum += r + u * 32 < w.rows[k] ? v[u] : 0.f;
+    }
   }
   red[rl][cl] = sum;
   __syncthreads();
@@ -358,12 +417,14 @@ int norm_rope_bwd_blocks(int B, int H, int Hkv, int L, int head_dim) {
 
 template <int D>
 static void launch_bwd(const NormRopeParams& p, hipStream_t s) {
-  const dim3 grid(p.nblk, (p.H + NB_HC - 1) / NB_HC + (p.Hkv + NB_HC - 1) / NB_HC);
+  const dim3 grid((uint32_t)chunks_of<NB_HC>(p, false) * (uint32_t)p.nblk);
   if (p.pq || p.pk) hipLaunchKernelGGL((norm_rope_bwd_kernel<D, true>), grid, dim3(NR_T), 0, s, p);
   else hipLaunchKernelGGL((norm_rope_bwd_kernel<D, false>), grid, dim3(NR_T), 0, s, p);
 }
 
-int launch_norm_rope_bwd(const NormRopeParams& p, int head_dim, hipStream_t s) {
+int launch_norm_rope_bwd(NormRopeParams p, int head_dim, hipStream_t s) {
+  division_by(p);
+  p.inv_eps = 1.f / p.eps;
   switch (head_dim) {
     case 16: launch_bwd<16>(p, s); break;
     case 32: launch_bwd<32>(p, s); break;
