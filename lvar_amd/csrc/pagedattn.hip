@@ -100,8 +100,11 @@ __device__ __forceinline__ int share_of(const PagedAttnParams& p, uint32_t total
   return max((int)((total - 1) / target) + 1, p.min_share);
 }
 
-// Pieces of a tile of `stages` > 0 stages.
-__device__ __forceinline__ int pieces_of(int stages, int share) { return (int)((uint32_t)(stages - 1) / (uint32_t)share) + 1; }
+// Pieces of a tile of `stages` > 0 stages.  Up to PA_WHOLE stages stay in one: a workgroup on its own takes 1.3 us per stage, the join 4.3.
+constexpr int PA_WHOLE = 5;
+__device__ __forceinline__ int pieces_of(int stages, int share) {
+  return stages <= PA_WHOLE ? 1 : (int)((uint32_t)(stages - 1) / (uint32_t)share) + 1;
+}
 
 // The piece of workgroup `wg`; false for the workgroups that are left over.  All lanes of a wave call it and get the same answer, in
 // scalar registers.  Workgroups are dealt to the 8 XCDs in turn; each XCD takes a run of pieces, row tiles over the same keys next to
@@ -655,6 +658,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
 #pragma unroll
           for (int j = 0; j < 2; j++) kx[ks][j] = *(LVAR_LDS const u32x4*)(kp[k1 + ks] + 2 * buf * BUF + (hh * 32 + 16 * j) * RB);
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int ks = 0; ks < KG; ks++)
 #pragma unroll
@@ -662,6 +666,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
 #pragma unroll
             for (int t = 0; t < NT; t++) a[t][j] = mfma16(kx[ks][j], qf[t][k1 + ks], a[t][j]);
       }
+      __builtin_amdgcn_s_setprio(0);
       const bool ragged = first + 32 > least || __builtin_amdgcn_readfirstlane(gone) != 0;
 #pragma unroll
       for (int t = 0; t < NT; t++) {
@@ -688,6 +693,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
         }
       };
       read4(0, vx[0]);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int n0 = 0; n0 < NB; n0 += 4) {
         if (n0 + 4 < NB) read4(n0 + 4, vx[(n0 / 4 + 1) & 1]);
@@ -697,6 +703,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
 #pragma unroll
           for (int t = 0; t < NT; t++) o[t][n0 + n] = mfma16(vx[(n0 / 4) & 1][n], pf[t], o[t][n0 + n]);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
   };
 
@@ -754,38 +761,45 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p
   const int tile = rc / tile_rows;
   const float* first = p.ws + p.ws_head + ((int64_t)(first_slot + head * n * p.rt + tile) * p.slot_rows + (rc - tile * tile_rows)) * (D + 2);
   const int64_t step = (int64_t)p.rt * p.slot_rows * (D + 2);
-  float top = -INFINITY;
-  for (int x = x0; x < n; x += GP) top = __builtin_fmaxf(top, first[x * step + D]);
-  if constexpr (GP > 1) {
-    if (l == 0) sm[g] = top;
-    __syncthreads();
+  // a running maximum, sum and output per group, four pieces in flight
+  float top = -INFINITY, sum = 0.f;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int x = x0; x < n; x += 4 * GP) {
+    float mx[4], lx[4];
+    f32x2 lo[4], hi[4];
 #pragma unroll
-    for (int x = 0; x < GP; x++) top = __builtin_fmaxf(top, sm[x * RPB + g % RPB]);
-  }
-  float y[4] = {}, sum = 0.f;
-#pragma unroll 4
-  for (int x = x0; x < n; x += GP) {
-    const float* at = first + x * step;
-    const float mx = at[D], lx = at[D + 1];
-    const f32x2 a = *(const f32x2*)(at + l * 4), c = *(const f32x2*)(at + l * 4 + 2);
-    const float f = mx == -INFINITY ? 1.f : fast_exp2(mx - top);   // (no finite score: zeros, or NaN that stays one)
-    y[0] += a[0] * f; y[1] += a[1] * f; y[2] += c[0] * f; y[3] += c[1] * f;
-    sum += lx * f;
+    for (int u = 0; u < 4; u++) {
+      const float* at = first + min(x + u * GP, n - 1) * step;
+      mx[u] = at[D]; lx[u] = at[D + 1];
+      lo[u] = *(const f32x2*)(at + l * 4); hi[u] = *(const f32x2*)(at + l * 4 + 2);
+    }
+    float best = top;
+#pragma unroll
+    for (int u = 0; u < 4; u++) best = __builtin_fmaxf(best, mx[u]);   // (a piece that is looked at twice does not change it)
+    const float fade = top == -INFINITY ? 1.f : fast_exp2(top - best);
+    y *= fade; sum *= fade; top = best;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      if (x + u * GP >= n) break;
+      const float f = mx[u] == -INFINITY ? 1.f : fast_exp2(mx[u] - top);   // (no finite score: zeros, or NaN that stays one)
+      y += f32x4{lo[u][0], lo[u][1], hi[u][0], hi[u][1]} * f;
+      sum += lx[u] * f;
+    }
   }
   if constexpr (GP > 1) {
-    if (l == 0) sl[g] = sum;
-#pragma unroll
-    for (int e = 0; e < 4; e++) so[g][l * 4 + e] = y[e];
+    if (l == 0) { sm[g] = top; sl[g] = sum; }
+    *(f32x4*)&so[g][l * 4] = y;
     __syncthreads();
     if (g >= RPB) return;
-    sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = 0.f;
+    for (int x = 0; x < GP; x++) top = __builtin_fmaxf(top, sm[x * RPB + g]);
+    sum = 0.f;
+    y = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < GP; x++) {
-      sum += sl[x * RPB + g];
-#pragma unroll
-      for (int e = 0; e < 4; e++) y[e] += so[x * RPB + g][l * 4 + e];
+      const float mx = sm[x * RPB + g], f = mx == -INFINITY ? 1.f : fast_exp2(mx - top);
+      sum += sl[x * RPB + g] * f;
+      y += *(const f32x4*)&so[x * RPB + g][l * 4] * f;
     }
   }
   if (row >= rows) return;
@@ -825,7 +839,7 @@ static int64_t ws_head_floats(int B) { return ((int64_t)2 * B + 63) / 64 * 64; }
 int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim) {
   const Shape s = shape_of(H, Hkv, Lq, head_dim);
   if (s.target <= 0) return LVAR_ELAUNCH;
-  if ((max_len + PA_STAGE - 1) / PA_STAGE <= s.min_share) return 0;   // nothing can be cut
+  if ((max_len + PA_STAGE - 1) / PA_STAGE <= PA_WHOLE) return 0;   // nothing can be cut
   return 4 * (ws_head_floats(B) + 4ll * s.target * s.rows * (head_dim + 2));
 }
 
