@@ -86,7 +86,7 @@ struct PagedAttnParams {
   int max_len;                    // lengths are clamped to it
   float c;                        // scale * log2(e)
   // set at launch
-  int rt;                         // row tiles per key/value head
+  int rt, tile_rows;              // row tiles per key/value head, rows of one
   int target, min_share;          // pieces aimed at, fewest 128-key stages of one
   int slot_rows;
   int64_t ws_head;                // floats ahead of the partial results

@@ -66,6 +66,7 @@ struct Piece {
   int b, len, stages;   // sequence, its length, its stages
   int n, piece;         // pieces per tile of this sequence, which one
   int tile, head;       // row tile, key/value head
+  int rt;               // row tiles with new tokens among their rows
   int slot;             // place of its partial result (n > 1)
   int first_slot;       // of those of its sequence
 };
@@ -89,7 +90,12 @@ __device__ __forceinline__ const __attribute__((address_space(4))) int32_t* as_c
 }
 
 // New tokens of sequence b; the rows behind them get an empty result.
-__device__ __forceinline__ int fresh_of(const PagedAttnParams& p, int b) { return p.counts ? max(0, min(as_constant(p.counts)[b], p.Lq)) : p.Lq; }
+__device__ __forceinline__ int fresh_of(const PagedAttnParams& p, int b) { return p.counts ? max(0, min(p.counts[b], p.Lq)) : p.Lq; }
+
+// Row tiles that hold new tokens of sequence b (at least one; the rows behind them are written by its last one).
+__device__ __forceinline__ int tiles_of(const PagedAttnParams& p, int b) {
+  return p.rt == 1 || !p.counts ? p.rt : max(1, (fresh_of(p, b) * p.G + p.tile_rows - 1) / p.tile_rows);
+}
 
 // Length of sequence b within what the table can name.
 __device__ __forceinline__ int length_of(const PagedAttnParams& p, int b) { return max(0, min(p.lengths[b], p.max_len)); }
@@ -110,30 +116,34 @@ __device__ __forceinline__ int pieces_of(int stages, int share) {
 // scalar registers.  Workgroups are dealt to the 8 XCDs in turn; each XCD takes a run of pieces, row tiles over the same keys next to
 // each other in one L2.
 __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int lane, Piece& out) {
-  const int units = p.cache.kv_heads * p.rt;
-  const int len0 = lane < p.B ? length_of(p, lane) : 0;      // (the first 64 sequences are looked at once)
-  uint32_t total = last_lane(wave_scan(lane < p.B ? stages_of(len0) : 0));
-  for (int b0 = 64; b0 < p.B; b0 += 64) total += last_lane(wave_scan(b0 + lane < p.B ? stages_of(length_of(p, b0 + lane)) : 0));
-  total *= (uint32_t)units;
-  int share = share_of(p, total, p.target);
-  auto look = [&](int b0, int& len, int& st, int& n) {
+  // (the first 64 sequences are loaded once)
+  const int len0 = lane < p.B ? length_of(p, lane) : 0, tiles0 = lane < p.B ? tiles_of(p, lane) : 0;
+  int len, st, tiles, n, pieces, share = 0x7fffffff;
+  auto look = [&](int b0) {
     const int b = b0 + lane;
-    len = st = n = 0;
-    if (b < p.B) {
-      len = b0 == 0 ? len0 : length_of(p, b);
-      st = stages_of(len);
-      n = pieces_of(st, share);
+    len = b0 == 0 ? len0 : 0;
+    tiles = b0 == 0 ? tiles0 : 0;
+    if (b0 > 0 && b < p.B) {
+      len = length_of(p, b);
+      tiles = tiles_of(p, b);
     }
+    st = b < p.B ? stages_of(len) : 0;
+    n = b < p.B ? pieces_of(st, share) : 0;
   };
-  int len, st, n, pieces;
+  uint32_t total = 0;
   auto count = [&]() {
     pieces = 0;
-    for (int b0 = (p.B - 1) & ~63; b0 >= 0; b0 -= 64) {      // (ends with the first 64 in len, st, n)
-      look(b0, len, st, n);
-      pieces += last_lane(wave_scan(n));
+    total = 0;
+    for (int b0 = (p.B - 1) & ~63; b0 >= 0; b0 -= 64) {      // (ends with the first 64 in len, st, tiles, n)
+      look(b0);
+      pieces += last_lane(wave_scan(n * tiles));
+      total += last_lane(wave_scan(st * tiles));
     }
-    pieces *= units;
+    pieces *= p.cache.kv_heads;
+    total *= (uint32_t)p.cache.kv_heads;
   };
+  count();
+  share = share_of(p, total, p.target);
   count();
   // One round of workgroups, with pieces up to 3 / 8 longer if that makes it one; otherwise pieces half as long, whose second and third
   // rounds even out.
@@ -150,8 +160,8 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
   if ((wg >> 3) >= per || item >= pieces) return false;
   int before = 0, slots = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    if (b0 > 0) look(b0, len, st, n);
-    const int mine = n * units, cut = n > 1 ? mine : 0;
+    if (b0 > 0) look(b0);
+    const int mine = n * tiles * p.cache.kv_heads, cut = n > 1 ? mine : 0;
     const int upto = wave_scan(mine), cuts = wave_scan(cut);
     const uint64_t hit = __ballot(before + upto > item);
     if (hit) {
@@ -160,11 +170,12 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
       out.len = __builtin_amdgcn_readlane(len, l);
       out.stages = __builtin_amdgcn_readlane(st, l);
       out.n = __builtin_amdgcn_readlane(n, l);
+      out.rt = __builtin_amdgcn_readlane(tiles, l);
       const int rest = item - before - __builtin_amdgcn_readlane(upto - mine, l);
       out.first_slot = slots + __builtin_amdgcn_readlane(cuts - cut, l);
       out.slot = out.first_slot + rest;
-      out.tile = rest % p.rt;
-      const int hp = rest / p.rt;
+      out.tile = rest % out.rt;
+      const int hp = rest / out.rt;
       out.piece = hp % out.n;
       out.head = hp / out.n;
       return true;
@@ -173,6 +184,19 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
     slots += last_lane(cuts);
   }
   return false;
+}
+
+// The rows of a padded batch behind the last tile with new tokens: empty results, from the first piece of that tile.
+template <int D>
+__device__ __forceinline__ void write_padding(const PagedAttnParams& p, const Piece& w) {
+  if (w.rt == p.rt || w.piece > 0 || w.tile != w.rt - 1) return;
+  const int rows = p.G * p.Lq;
+  for (int x = w.rt * p.tile_rows * (D / 8) + threadIdx.x; x < rows * (D / 8); x += PA_T) {
+    const int r = x / (D / 8), i = r / p.G;
+    const int64_t out = ((int64_t)w.b * p.H + w.head * p.G + (r - i * p.G)) * p.Lq + i;
+    *(u32x4*)(p.o + out * D + x % (D / 8) * 8) = u32x4{0u, 0u, 0u, 0u};
+    if (x % (D / 8) == 0) { p.M[out] = -INFINITY; p.L[out] = 1.f; }
+  }
 }
 
 // What the join needs to know of a sequence, from one of its workgroups.
@@ -314,7 +338,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     most = max(most, __shfl_xor(most, d, 64));
     least = min(least, __shfl_xor(least, d, 64));
   }
-  most = row0 < rows ? __builtin_amdgcn_readfirstlane(most) : 0;   // a wave without rows has nothing to do
+  most = row0 < fresh * p.G ? __builtin_amdgcn_readfirstlane(most) : 0;   // a wave without new rows has nothing to do
   least = __builtin_amdgcn_readfirstlane(least);
 
   const int s0 = (int)((int64_t)w.stages * w.piece / w.n), s1 = (int)((int64_t)w.stages * (w.piece + 1) / w.n);
@@ -511,6 +535,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
       write_rows<D, NT, RW, CW>(p, w, fresh, t, c * CW, &so[0][0][0], LDO, sm, sl);
     }
   }
+  write_padding<D>(p, w);
 }
 
 // ---- many rows per key/value head ----
@@ -549,7 +574,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
   // limits do not fall from row to row: the last row of the tile, and of the wave, has the largest
   const int k_end = min(s1 * PA_STAGE, limit_of(p, w, fresh, min(tile0 + NT * RW * 16, rows) - 1));
   const int least = limit_of(p, w, fresh, row0);
-  const int mine = row0 < rows ? limit_of(p, w, fresh, row0 + NT * 16 - 1) : 0;   // a wave without rows only fills
+  const int mine = row0 < fresh * p.G ? limit_of(p, w, fresh, row0 + NT * 16 - 1) : 0;   // a wave without new rows only fills
 
   u32x4 qf[NT][KS];
   int limit[NT];
@@ -742,12 +767,13 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
     __syncthreads();
     write_rows<D, NT, RW, D>(p, w, fresh, t, 0, so, LDO, sm, sl);
   }
+  write_padding<D>(p, w);
 }
 
 // Joins the pieces of the tiles that were cut, in order.  A workgroup takes 512 / (D / 4) groups of D / 4 lanes: RPB rows with
 // GR / RPB groups each along the pieces.
 template <int D, int RPB>
-__global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p, int tile_rows) {
+__global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p) {
   constexpr int LPR = D / 4, GR = 512 / LPR, GP = GR / RPB;
   static_assert(GR % RPB == 0, "groups per row");
   __shared__ float so[GP > 1 ? GR : 1][D];
@@ -757,10 +783,11 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p
   if (n <= 1) return;
   const int first_slot = ((const int*)p.ws)[2 * b + 1];
   const int l = threadIdx.x % LPR, g = threadIdx.x / LPR, x0 = g / RPB;
-  const int rows = p.G * p.Lq, row = blockIdx.x * RPB + g % RPB, rc = min(row, rows - 1);
-  const int tile = rc / tile_rows;
-  const float* first = p.ws + p.ws_head + ((int64_t)(first_slot + head * n * p.rt + tile) * p.slot_rows + (rc - tile * tile_rows)) * (D + 2);
-  const int64_t step = (int64_t)p.rt * p.slot_rows * (D + 2);
+  const int rt = tiles_of(p, b), rows = min(p.G * p.Lq, rt * p.tile_rows);   // (the rows behind these are written)
+  if ((int)blockIdx.x * RPB >= rows) return;
+  const int row = blockIdx.x * RPB + g % RPB, rc = min(row, rows - 1), tile = rc / p.tile_rows;
+  const float* first = p.ws + p.ws_head + ((int64_t)(first_slot + head * n * rt + tile) * p.slot_rows + (rc - tile * p.tile_rows)) * (D + 2);
+  const int64_t step = (int64_t)rt * p.slot_rows * (D + 2);
   // a running maximum, sum and output per group, four pieces in flight
   float top = -INFINITY, sum = 0.f;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
@@ -863,8 +890,8 @@ static bool launch_staged(const PagedAttnParams& p, int grid, hipStream_t s) {
 }
 
 template <int D, int RPB>
-static void launch_join(const PagedAttnParams& p, int tile_rows, hipStream_t s) {
-  hipLaunchKernelGGL((paged_join_kernel<D, RPB>), dim3((p.G * p.Lq + RPB - 1) / RPB, p.cache.kv_heads, p.B), dim3(512), 0, s, p, tile_rows);
+static void launch_join(const PagedAttnParams& p, hipStream_t s) {
+  hipLaunchKernelGGL((paged_join_kernel<D, RPB>), dim3((p.G * p.Lq + RPB - 1) / RPB, p.cache.kv_heads, p.B), dim3(512), 0, s, p);
 }
 
 template <int D>
@@ -884,9 +911,8 @@ static int launch_d(const PagedAttnParams& p, const Shape& h, hipStream_t s) {
   if (p.ws) {
     // few rows: all groups along the pieces of one row; many: a group per row
     constexpr int GR = 512 / (D / 4);
-    const int tile_rows = 16 * h.nt * h.rw;
-    if ((int64_t)p.G * p.Lq * p.cache.kv_heads * p.B <= 4 * device_cus()) launch_join<D, 1>(p, tile_rows, s);
-    else launch_join<D, GR>(p, tile_rows, s);
+    if ((int64_t)p.G * p.Lq * p.cache.kv_heads * p.B <= 4 * device_cus()) launch_join<D, 1>(p, s);
+    else launch_join<D, GR>(p, s);
     if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
   }
   return LVAR_OK;
@@ -896,6 +922,7 @@ int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s) {
   const Shape h = shape_of(p.H, p.cache.kv_heads, p.Lq, head_dim);
   if (h.target <= 0) return LVAR_ELAUNCH;
   p.rt = h.rt;
+  p.tile_rows = 16 * h.nt * h.rw;
   p.target = h.target;
   p.slot_rows = h.rows;
   p.ws_head = ws_head_floats(p.B);
