@@ -89,13 +89,14 @@ __device__ __forceinline__ const __attribute__((address_space(4))) int32_t* as_c
   return (const __attribute__((address_space(4))) int32_t*)(p);
 }
 
-// New tokens of sequence b; the rows behind them get an empty result.
-__device__ __forceinline__ int fresh_of(const PagedAttnParams& p, int b) { return p.counts ? max(0, min(p.counts[b], p.Lq)) : p.Lq; }
+// New tokens of a sequence by its entry of `counts`; the rows behind them get an empty result.
+__device__ __forceinline__ int fresh_by(const PagedAttnParams& p, int count) { return max(0, min(count, p.Lq)); }
+// The same of sequence b, the same one for all lanes: a scalar load.
+__device__ __forceinline__ int fresh_of(const PagedAttnParams& p, int b) { return p.counts ? fresh_by(p, as_constant(p.counts)[b]) : p.Lq; }
 
-// Row tiles that hold new tokens of sequence b (at least one; the rows behind them are written by its last one).
-__device__ __forceinline__ int tiles_of(const PagedAttnParams& p, int b) {
-  return p.rt == 1 || !p.counts ? p.rt : max(1, (fresh_of(p, b) * p.G + p.tile_rows - 1) / p.tile_rows);
-}
+// Row tiles that hold new tokens (at least one; the rows behind them are written by the last one).
+__device__ __forceinline__ int tiles_by(const PagedAttnParams& p, int fresh) { return max(1, (fresh * p.G + p.tile_rows - 1) / p.tile_rows); }
+__device__ __forceinline__ int tiles_of(const PagedAttnParams& p, int b) { return p.rt == 1 || !p.counts ? p.rt : tiles_by(p, fresh_by(p, p.counts[b])); }
 
 // Length of sequence b within what the table can name.
 __device__ __forceinline__ int length_of(const PagedAttnParams& p, int b) { return max(0, min(p.lengths[b], p.max_len)); }
@@ -116,6 +117,31 @@ __device__ __forceinline__ int pieces_of(int stages, int share) {
 // scalar registers.  Workgroups are dealt to the 8 XCDs in turn; each XCD takes a run of pieces, row tiles over the same keys next to
 // each other in one L2.
 __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int lane, Piece& out) {
+  auto take = [&](int pieces, int& item) {
+    const int per = (pieces + 7) >> 3;
+    item = (wg & 7) * per + (wg >> 3);
+    return (wg >> 3) < per && item < pieces;
+  };
+  auto split = [&](int rest) {              // of the pieces of a sequence
+    out.tile = rest % out.rt;
+    const int hp = rest / out.rt;
+    out.piece = hp % out.n;
+    out.head = hp / out.n;
+  };
+  int item;
+  if (!p.ws && (p.rt == 1 || !p.counts)) {
+    // nothing is cut and all sequences have the same tiles: no need to look at the others (0.6 us of the 5 us of the smallest calls)
+    const int units = p.cache.kv_heads * p.rt;
+    if (!take(p.B * units, item)) return false;
+    out.b = item / units;
+    out.len = max(0, min(as_constant(p.lengths)[out.b], p.max_len));
+    out.stages = stages_of(out.len);
+    out.n = 1;
+    out.rt = p.rt;
+    out.slot = out.first_slot = 0;
+    split(item - out.b * units);
+    return true;
+  }
   // (the first 64 sequences are loaded once)
   const int len0 = lane < p.B ? length_of(p, lane) : 0, tiles0 = lane < p.B ? tiles_of(p, lane) : 0;
   int len, st, tiles, n, pieces, share = 0x7fffffff;
@@ -131,18 +157,19 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
     n = b < p.B ? pieces_of(st, share) : 0;
   };
   uint32_t total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    look(b0);
+    total += last_lane(wave_scan(st * tiles));
+  }
+  total *= (uint32_t)p.cache.kv_heads;
   auto count = [&]() {
     pieces = 0;
-    total = 0;
     for (int b0 = (p.B - 1) & ~63; b0 >= 0; b0 -= 64) {      // (ends with the first 64 in len, st, tiles, n)
       look(b0);
       pieces += last_lane(wave_scan(n * tiles));
-      total += last_lane(wave_scan(st * tiles));
     }
     pieces *= p.cache.kv_heads;
-    total *= (uint32_t)p.cache.kv_heads;
   };
-  count();
   share = share_of(p, total, p.target);
   count();
   // One round of workgroups, with pieces up to 3 / 8 longer if that makes it one; otherwise pieces half as long, whose second and third
@@ -156,8 +183,7 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
     share = share_of(p, total, 2 * p.target);
     count();
   }
-  const int per = (pieces + 7) >> 3, item = (wg & 7) * per + (wg >> 3);
-  if ((wg >> 3) >= per || item >= pieces) return false;
+  if (!take(pieces, item)) return false;
   int before = 0, slots = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (b0 > 0) look(b0);
@@ -174,10 +200,7 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
       const int rest = item - before - __builtin_amdgcn_readlane(upto - mine, l);
       out.first_slot = slots + __builtin_amdgcn_readlane(cuts - cut, l);
       out.slot = out.first_slot + rest;
-      out.tile = rest % out.rt;
-      const int hp = rest / out.rt;
-      out.piece = hp % out.n;
-      out.head = hp / out.n;
+      split(rest);
       return true;
     }
     before += last_lane(upto);
@@ -783,7 +806,7 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p
   if (n <= 1) return;
   const int first_slot = ((const int*)p.ws)[2 * b + 1];
   const int l = threadIdx.x % LPR, g = threadIdx.x / LPR, x0 = g / RPB;
-  const int rt = tiles_of(p, b), rows = min(p.G * p.Lq, rt * p.tile_rows);   // (the rows behind these are written)
+  const int fresh = fresh_of(p, b), rt = tiles_by(p, fresh), rows = min(p.G * p.Lq, rt * p.tile_rows);   // (the rows behind these are written)
   if ((int)blockIdx.x * RPB >= rows) return;
   const int row = blockIdx.x * RPB + g % RPB, rc = min(row, rows - 1), tile = rc / p.tile_rows;
   const float* first = p.ws + p.ws_head + ((int64_t)(first_slot + head * n * rt + tile) * p.slot_rows + (rc - tile * p.tile_rows)) * (D + 2);
@@ -832,7 +855,7 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p
   if (row >= rows) return;
   const int i = row / p.G;
   const int64_t out = ((int64_t)b * p.H + head * p.G + (row - i * p.G)) * p.Lq + i;
-  const bool none = i >= fresh_of(p, b) || (top == -INFINITY && sum == 0.f);
+  const bool none = i >= fresh || (top == -INFINITY && sum == 0.f);
   const float inv = 1.f / sum;
   const u32x2 u = {pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)};
   *(u32x2*)(p.o + out * D + l * 4) = none ? u32x2{0u, 0u} : u;
