@@ -87,7 +87,7 @@ struct PagedAttnParams {
   float c;                        // scale * log2(e)
   // set at launch
   int rt, tile_rows;              // row tiles per key/value head, rows of one
-  int target, min_share;          // pieces aimed at, fewest 128-key stages of one
+  int target, finer, min_share, whole;   // pieces of one round, of several; fewest 128-key stages of one; tiles up to this many stay whole
   int slot_rows;
   int64_t ws_head;                // floats ahead of the partial results
 };

@@ -107,10 +107,9 @@ __device__ __forceinline__ int share_of(const PagedAttnParams& p, uint32_t total
   return max((int)((total - 1) / target) + 1, p.min_share);
 }
 
-// Pieces of a tile of `stages` > 0 stages.  Up to PA_WHOLE stages stay in one: a workgroup on its own takes 1.3 us per stage, the join 4.3.
-constexpr int PA_WHOLE = 5;
-__device__ __forceinline__ int pieces_of(int stages, int share) {
-  return stages <= PA_WHOLE ? 1 : (int)((uint32_t)(stages - 1) / (uint32_t)share) + 1;
+// Pieces of a tile of `stages` > 0 stages; tiles of up to `whole` stages stay in one.
+__device__ __forceinline__ int pieces_of(const PagedAttnParams& p, int stages, int share) {
+  return stages <= p.whole ? 1 : (int)((uint32_t)(stages - 1) / (uint32_t)share) + 1;
 }
 
 // The piece of workgroup `wg`; false for the workgroups that are left over.  All lanes of a wave call it and get the same answer, in
@@ -154,7 +153,7 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
       tiles = tiles_of(p, b);
     }
     st = b < p.B ? stages_of(len) : 0;
-    n = b < p.B ? pieces_of(st, share) : 0;
+    n = b < p.B ? pieces_of(p, st, share) : 0;
   };
   uint32_t total = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
@@ -172,15 +171,14 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
   };
   share = share_of(p, total, p.target);
   count();
-  // One round of workgroups, with pieces up to 3 / 8 longer if that makes it one; otherwise pieces half as long, whose second and third
-  // rounds even out.
+  // One round of workgroups, with pieces up to 3 / 8 longer if that makes it one; otherwise fine pieces, whose last round is short.
   const int even = share;
   for (int tries = 0; tries < 3 && pieces > p.target; tries++) {
     share += max(1, even >> 3);
     count();
   }
   if (pieces > p.target) {
-    share = share_of(p, total, 2 * p.target);
+    share = share_of(p, total, p.finer);
     count();
   }
   if (!take(pieces, item)) return false;
@@ -864,11 +862,13 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p
 
 // ---- launch ----
 
-struct Shape { int nt, rw, rt, rows, target, min_share; bool staged; };
+constexpr int PA_LEAST = 2;   // fewest stages of a share
+
+struct Shape { int nt, rw, rt, rows, whole, finer; bool staged; };
 
 // Rows per tile: 16 up to 16 rows of a key/value head, 32 up to 32 (each wave reads keys for itself), more with staged tiles: 64 up to
 // 64 rows, then 128 (head_dim 256: 64 from 17 rows on, its outputs take twice the registers).
-static Shape shape_of(int H, int Hkv, int Lq, int head_dim) {
+static Shape shape_of(int B, int H, int Hkv, int Lq, int head_dim) {
   Shape s;
   const int64_t rows = (int64_t)(H / Hkv) * Lq;
   s.nt = rows <= 16 || head_dim == 256 ? 1 : 2;
@@ -877,20 +877,35 @@ static Shape shape_of(int H, int Hkv, int Lq, int head_dim) {
   const int tile = 16 * s.nt * s.rw;
   s.rt = (int)((rows + tile - 1) / tile);
   s.rows = (int)(rows < tile ? rows : tile);
-  s.target = device_cus() * (s.nt == 1 && head_dim < 256 ? 3 : 2);   // workgroups that a compute unit holds
-  s.min_share = 2;
+  // A workgroup on its own takes 1.2 us per stage, the join 4: tiles of up to 5 stages are not cut (512 tokens of one sequence 9.7 -> 8.2
+  // us), and where uncut tiles are half as many as compute units, none of up to 10 (16 x 768 tokens 15.5 -> 11.9, 32 x 1280 37.9
+  // -> 32.6; not of the staged tiles, whose stages take two to four times as long).
+  s.whole = !s.staged && (int64_t)B * Hkv * s.rt >= device_cus() / 2 ? 10 : 5;
+  s.finer = device_cus() * (s.staged ? 4 : 6);
   return s;
+}
+
+// Pieces of one round, per compute unit.  A workgroup is bound by latency, about 1.2 us per stage, and as many are wanted as fill the
+// memory's bandwidth: more only add to what is joined.  That is one per compute unit with stages of 64 KiB or more (bf16, head_dim
+// 128), two with half of that, three with less; and two, all that fit, where row tiles share keys and the matrix units are the bound.
+// Two instead of one: 8 x 4096 keys in bf16 with 8 new tokens 30.6 -> 33.2 us, 131071 keys in e4m3 61.1 -> 57.5, 4 x 256 rows 50.0 -> 45.8.
+static int round_of(const Shape& s, int head_dim, bool f8) {
+  const int stage = 2 * PA_STAGE * head_dim * (f8 ? 1 : 2);
+  const int per = stage >= 65536 ? 1 : stage >= 32768 ? 2 : s.staged ? 2 : 3;
+  return device_cus() * (s.staged && s.rt > 1 && head_dim < 256 ? 2 : per);
 }
 
 static int64_t ws_head_floats(int B) { return ((int64_t)2 * B + 63) / 64 * 64; }   // pieces and first slot of every sequence
 
 // Partial results are kept for tiles that are cut only; such a tile has n < 2 * stages / share pieces, and a share is at least the
-// 2 * target-th part of all stages, so that there are fewer than 4 * target of them in all.
+// `finer`-th part of all stages, so that there are fewer than 2 * finer of them in all; nor are there more than pieces of the shortest share.
 int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim) {
-  const Shape s = shape_of(H, Hkv, Lq, head_dim);
-  if (s.target <= 0) return LVAR_ELAUNCH;
-  if ((max_len + PA_STAGE - 1) / PA_STAGE <= PA_WHOLE) return 0;   // nothing can be cut
-  return 4 * (ws_head_floats(B) + 4ll * s.target * s.rows * (head_dim + 2));
+  const Shape s = shape_of(B, H, Hkv, Lq, head_dim);
+  if (s.finer <= 0) return LVAR_ELAUNCH;
+  const int64_t stages = ((int64_t)max_len + PA_STAGE - 1) / PA_STAGE;
+  if (stages <= s.whole) return 0;   // nothing can be cut
+  const int64_t most = (int64_t)B * Hkv * s.rt * ((stages + PA_LEAST - 1) / PA_LEAST), slots = most < 2ll * s.finer ? most : 2ll * s.finer;
+  return 4 * (ws_head_floats(B) + slots * s.rows * (head_dim + 2));
 }
 
 template <int D, int NT, int W>
@@ -919,7 +934,7 @@ static void launch_join(const PagedAttnParams& p, hipStream_t s) {
 
 template <int D>
 static int launch_d(const PagedAttnParams& p, const Shape& h, hipStream_t s) {
-  const int64_t items = (int64_t)p.B * p.cache.kv_heads * p.rt + (p.ws ? 2ll * p.target : 0);
+  const int64_t items = (int64_t)p.B * p.cache.kv_heads * p.rt + (p.ws ? p.finer : 0);
   if (items > 0x7ffffff0) return LVAR_EINVAL;
   const int grid = (int)((items + 7) / 8 * 8);
   bool ok = true;
@@ -942,15 +957,17 @@ static int launch_d(const PagedAttnParams& p, const Shape& h, hipStream_t s) {
 }
 
 int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s) {
-  const Shape h = shape_of(p.H, p.cache.kv_heads, p.Lq, head_dim);
-  if (h.target <= 0) return LVAR_ELAUNCH;
+  const Shape h = shape_of(p.B, p.H, p.cache.kv_heads, p.Lq, head_dim);
+  if (h.finer <= 0) return LVAR_ELAUNCH;
   p.rt = h.rt;
   p.tile_rows = 16 * h.nt * h.rw;
-  p.target = h.target;
+  p.target = round_of(h, head_dim, p.cache.k_exp != nullptr);
+  p.finer = h.finer;
+  p.whole = h.whole;
   p.slot_rows = h.rows;
   p.ws_head = ws_head_floats(p.B);
   // without room for partial results every tile stays whole: a share longer than any sequence
-  p.min_share = p.ws ? h.min_share : 0x7fffffff;
+  p.min_share = p.ws ? PA_LEAST : 0x7fffffff;
   if (head_dim == 128) return launch_d<128>(p, h, s);
   if (head_dim == 64) return launch_d<64>(p, h, s);
   if (head_dim == 256) return launch_d<256>(p, h, s);
