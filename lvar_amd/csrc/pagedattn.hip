@@ -3,17 +3,18 @@
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp2(q_i . k_j * scale * log2e - M_i),  j < limit_i
 //
 // The rows that share a key/value head (its query heads times the new tokens) are the columns of 16-wide MFMA tiles: with
-// S^T = K Q^T the four scores a lane holds are those of keys 4g .. 4g+3 for one query (g = lane / 16), which is the layout that
-// the second product O^T = V^T P^T wants its P in, so that scores never leave their lane.  Keys go from memory straight into
-// the matrix operand (16 lanes x 64 bytes of 16 rows per load); values are loaded as whole rows (16 lanes cover one row), eight
-// rows of a lane are regrouped by byte permutes into pairs of keys, and output columns come out as runs of 32 per lane.  No LDS
-// and no barrier in the key loop: a wave waits for nothing but its own loads, and the loads of the next 32 keys are in
-// flight while it computes.
+// S^T = K Q^T the scores a lane holds are those of keys 4g .. 4g+3 of 16 for one query (g = lane / 16), which is the layout that
+// the second product O^T = V^T P^T wants its P in, so that scores never leave their lane.  Two kernels:
 //
-// A workgroup's four waves are RW row waves times 4 / RW key waves: the row waves take 16 * NT rows each and read the same keys (from
-// L1 and L2 after the first), the key waves take turns at 32 keys.  More than 32 rows per wave would need over 256 registers, one
-// wave per SIMD, and nobody left to compute while it waits (64 rows per wave, 8 sequences of up to 4001 tokens with 61 new ones:
-// 105 us).
+//   paged_attn_kernel   up to 32 rows, where the cache is read once and its bandwidth is the bound.  Keys go from memory straight into
+//     the matrix operand (16 lanes x 64 bytes of 16 rows per load); values are loaded as whole rows (16 lanes cover one row), eight rows
+//     of a lane are regrouped by byte permutes into pairs of keys, and output columns come out as runs of 32 per lane.  No
+//     LDS and no barrier in the key loop: a wave waits for nothing but its own loads, the loads of its next 32 keys are in flight
+//     while it computes, and the four waves take turns at 32 keys.  32 sequences of up to 32768 tokens, 32 query heads over 8 of
+//     128: 2.2 GB of bf16 in 390 us (5.7 TB/s; a copy moves 5.2); 131071 tokens in e4m3: 0.27 GB in 55 us.
+//   paged_tile_kernel   more rows: keys and values staged in LDS, where the waves share them.  4 x 256 rows of 16 heads over 2521
+//     tokens: 45 .. 50 us, 420 .. 470 TFLOP/s.  (With 64 rows per wave and no LDS there is one wave per SIMD and nobody left to
+//     compute while it waits: 105 us where this takes 38, 8 sequences of up to 4001 tokens with up to 61 new ones.)
 //
 // The work is (sequence, key/value head, row tile) x stages of 128 keys.  It is cut into pieces of about equal length by the
 // lengths that only the device knows: every workgroup scans the lengths and finds its piece.  The pieces of one tile are joined by
@@ -316,25 +317,23 @@ __device__ __forceinline__ void settle(float c, int lane, float& m, float& l, fl
   top = mx;
 }
 
-template <int D, int NT, int RW, bool F8, int WAVES_PER_SIMD>
+template <int D, int NT, bool F8, int WAVES_PER_SIMD>
 __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const PagedAttnParams p) {
   constexpr int KS = D / 32;                  // steps of the contraction over the head dimension
   constexpr int CH = D < 128 ? 1 : D / 128;   // chunks of 128 (64) output columns
   constexpr int NE = D < 128 ? D / 16 : 8;    // columns of a chunk per lane and value row
   constexpr int CW = 16 * NE;                 // columns of a chunk
   constexpr int LDO = CW + 4;
-  constexpr int KW = PA_WAVES / RW;           // key waves
   __shared__ float so[PA_WAVES][16][LDO];
   __shared__ float sm[PA_WAVES][NT * 16], sl[PA_WAVES][NT * 16];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rw = wave % RW, kw = wave / RW;
   const int qi = lane & 15, g = lane >> 4;
   Piece w;
   if (!find_piece(p, blockIdx.x, lane, w)) return;
   write_plan(p, w);
 
-  const int rows = p.G * p.Lq, tile0 = w.tile * NT * RW * 16, row0 = tile0 + rw * NT * 16;
+  const int rows = p.G * p.Lq, row0 = w.tile * NT * 16;
   const int fresh = fresh_of(p, w.b);
 
   // queries as the second operand, and how many keys each may see
@@ -359,7 +358,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     most = max(most, __shfl_xor(most, d, 64));
     least = min(least, __shfl_xor(least, d, 64));
   }
-  most = row0 < fresh * p.G ? __builtin_amdgcn_readfirstlane(most) : 0;   // a wave without new rows has nothing to do
+  most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
 
   const int s0 = (int)((int64_t)w.stages * w.piece / w.n), s1 = (int)((int64_t)w.stages * (w.piece + 1) / w.n);
@@ -424,8 +423,8 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     }
   };
 
-  constexpr int STEP = 32 * KW;
-  int key = s0 * PA_STAGE + kw * 32;
+  constexpr int STEP = 32 * PA_WAVES;
+  int key = s0 * PA_STAGE + wave * 32;
   int pg[2] = {-1, -1}, entry[2] = {0, 0};   // entry: of the next 32 keys
   if (key < k_end) {
     pg[0] = page_of(key, entry_of(key)); pg[1] = page_of(key + 16, entry_of(key + 16));
@@ -532,7 +531,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     key = next;
   }
 
-  // the key waves' results become one
+  // the waves' results become one
 #pragma unroll
   for (int t = 0; t < NT; t++) settle(p.c, lane, m[t], l[t], top[t], &sm[wave][t * 16], &sl[wave][t * 16]);
   __syncthreads();
@@ -540,7 +539,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
   for (int t = 0; t < NT; t++) {
     float best = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < KW; x++) best = __builtin_fmaxf(best, sm[x * RW + rw][t * 16 + qi]);
+    for (int x = 0; x < PA_WAVES; x++) best = __builtin_fmaxf(best, sm[x][t * 16 + qi]);
     const float f = top[t] == -INFINITY ? 1.f : m[t] * fast_exp2(top[t] - best);
 #pragma unroll
     for (int c = 0; c < CH; c++) {
@@ -553,7 +552,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
           *(f32x4*)&so[wave][qi][(4 * g + r) * NE + e] = y;
         }
       __syncthreads();
-      write_rows<D, NT, RW, CW>(p, w, fresh, t, c * CW, &so[0][0][0], LDO, sm, sl);
+      write_rows<D, NT, 1, CW>(p, w, fresh, t, c * CW, &so[0][0][0], LDO, sm, sl);
     }
   }
   write_padding<D>(p, w);
@@ -580,7 +579,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
   constexpr int LDO = D + 4;
   extern __shared__ __align__(16) char smem[];              // [2 buffers][keys, values][BUF]; then the outputs
   __shared__ float sm[PA_WAVES][NT * 16], sl[PA_WAVES][NT * 16];
-  __shared__ uint8_t missing[2][4];                         // quarters of a tile without a page (or behind the last key)
+  __shared__ __align__(4) uint8_t missing[2][4];             // quarters of a tile without a page (or behind the last key)
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave % RW, kw = wave / RW;
@@ -910,8 +909,8 @@ int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head
 
 template <int D, int NT, int W>
 static void launch_direct(const PagedAttnParams& p, int grid, hipStream_t s) {
-  if (p.cache.k_exp) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, true, W>), dim3(grid), dim3(PA_T), 0, s, p);
-  else hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, false, W>), dim3(grid), dim3(PA_T), 0, s, p);
+  if (p.cache.k_exp) hipLaunchKernelGGL((paged_attn_kernel<D, NT, true, W>), dim3(grid), dim3(PA_T), 0, s, p);
+  else hipLaunchKernelGGL((paged_attn_kernel<D, NT, false, W>), dim3(grid), dim3(PA_T), 0, s, p);
 }
 
 template <int D, int NT, int RW, bool F8>

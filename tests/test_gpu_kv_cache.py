@@ -608,6 +608,146 @@ def test_gradients_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
 
 
+PADDED_CASES = [
+    # B, H, Hkv, Lq, lengths, d, page, causal, counts: padding that leaves whole row tiles without a token, cut and uncut sequences
+    (4, 8, 1, 64, [1500, 70, 40, 900], 128, 64, True, [64, 3, 0, 17]),
+    (4, 8, 1, 64, [1500, 70, 40, 900], 64, 16, False, [1, 64, 64, 16]),
+    (3, 4, 1, 50, [900, 2000, 10], 256, 32, True, [50, 1, 0]),
+    (70, 4, 1, 40, [(i * 31) % 300 for i in range(70)], 64, 16, True, [(i * 7) % 45 - 2 for i in range(70)]),
+]
+
+
+@pytest.mark.parametrize("case", PADDED_CASES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_paged_attn_padded_batches(case, dtype):
+    B, H, Hkv, Lq, lengths, d, page, causal, counts = case
+    attn_case(B, H, Hkv, Lq, lengths, d, page, dtype, causal, counts, seed=7)
+
+
+@pytest.mark.parametrize("Lq,H,Hkv,d,lengths", [(17, 2, 2, 64, [130, 64]), (33, 1, 1, 128, [700, 65]), (16, 3, 1, 128, [129, 48]), (129, 1, 1, 64, [300, 129]), (65, 2, 1, 256, [190, 1000]),
+                                                (257, 1, 1, 128, [257, 900])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_paged_attn_row_tiles(Lq, H, Hkv, d, lengths, dtype):
+    """Rows around the ends of tiles of 16, 32, 64 and 128."""
+    for causal in (True, False):
+        attn_case(2, H, Hkv, Lq, lengths, d, 16, dtype, causal, seed=Lq)
+
+
+@pytest.mark.parametrize("Lq", [1, 20, 70])
+def test_leftover_bytes_of_any_value(Lq):
+    """Codes and scale bytes of rows nobody has written: every byte there is, NaN and infinities among them, on pages that are shared and on one that is missing."""
+    from lvar_amd import kv_cache_ops as kv
+    B, H, d, page, n = 2, 2, 128, 32, 330
+    P, per = 30, 12
+    g = torch.Generator().manual_seed(1)
+    shape = (P, H, page, d)
+    raw = [torch.randint(0, 256, shape, generator=g, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2)]
+    exps = [torch.randint(0, 256, shape[:3], generator=g, dtype=torch.uint8) for _ in range(2)]
+    cache = kv.PagedKVCache(*raw, *exps)
+    table = table_for(B, per, P, 2)
+    lens = torch.tensor([n, 97], dtype=torch.int32)
+    x = [rand(B, H, n, d, seed=3 + i) for i in range(2)]
+    pages = [ref.append(c, e, table, y, torch.zeros(B, dtype=torch.int32), lens) for c, e, y in ((cache.k, cache.k_exp, x[0]), (cache.v, cache.v_exp, x[1]))]
+    cache = kv.PagedKVCache(pages[0][0], pages[1][0], pages[0][1], pages[1][1])
+    table[1, 1] = -1
+    q = rand(B, H, Lq, d, seed=9)
+    k, there = ref.read(cache.k, cache.k_exp, table, lens, n)
+    v, _ = ref.read(cache.v, cache.v_exp, table, lens, n)
+    for causal in (False, True):
+        o, (M, L) = kv.paged_attn(q.cuda(), to_gpu(cache), table.cuda(), lens.cuda(), causal=causal)
+        check_attn(o, M, L, *ref.paged_attn(q, k, v, there, lens, d ** -0.5, causal), q, k, d ** -0.5, n)
+
+
+def test_paged_attn_operands_of_other_layouts():
+    """Queries with a head axis of stride 0 and as a slice of longer rows; one page table, one row, for all sequences; lengths as a slice."""
+    from lvar_amd import kv_cache_ops as kv
+    B, H, Hkv, d, page, n = 3, 4, 2, 64, 16, 90
+    cache = kv.PagedKVCache.alloc(8, Hkv, d, page)
+    one = torch.arange(6, dtype=torch.int32, device="cuda").view(1, 6)
+    x = [rand(1, Hkv, n, d, seed=i).cuda() for i in range(2)]
+    kv.kv_cache_append(cache, *x, one, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    table = one.expand(B, 6)
+    lens = torch.tensor([[90, 0], [33, 0], [64, 0]], dtype=torch.int32, device="cuda")[:, 0]
+    wide = rand(B, 1, 2, 2 * d, seed=5).cuda()
+    q = wide[..., d:].expand(B, H, 2, d)
+    o, (M, L) = kv.paged_attn(q, cache, table, lens, causal=True)
+    o2, (M2, L2) = kv.paged_attn(q.contiguous(), cache, table.contiguous(), lens.contiguous(), causal=True)
+    assert torch.equal(o, o2) and torch.equal(M, M2) and torch.equal(L, L2) and torch.equal(o[:, 0], o[:, 1])
+    k, v = (t.double().cpu().expand(B, Hkv, n, d) for t in x)
+    check_attn(o, M, L, *ref.paged_attn(q.cpu(), k, v, torch.ones(B, n, dtype=torch.bool), lens.cpu(), d ** -0.5, True), q.cpu(), k, d ** -0.5, n)
+
+
+@pytest.mark.parametrize("Lq", [1, 24, 100])
+def test_entry_point_without_workspace(Lq):
+    """No workspace: no sequence is cut, the same result but for the order of the sums; a workspace that is too small is not used."""
+    from lvar_amd import _lib, kv_cache_ops as kv
+    o, M, L, args = attn_case(2, 4, 2, Lq, [1800, 300], 128, 32, torch.bfloat16, True, seed=3)
+    q, cache, table, lens = args[:4]
+    lib = _lib.load()
+    need = lib.lvar_paged_attn_workspace_bytes(2, 4, 2, Lq, 1800, 128)
+    assert need > 0
+    small = torch.full((1024,), 7, dtype=torch.uint8, device="cuda")
+    for ws, size in ((None, 0), (small.data_ptr(), 1024)):
+        o2, M2, L2 = torch.full_like(o, 9), torch.full_like(M, 9), torch.full_like(L, 9)
+        st = lib.lvar_paged_attn_fwd(kv._view(q), kv._cache_arg(cache, table, 2, q.device), lens.data_ptr(), None, o2.data_ptr(), M2.data_ptr(), L2.data_ptr(), ws, size,
+                                     2, 4, Lq, 1 << 30, 1, 128 ** -0.5, kv._stream(q))
+        assert st == 0
+        # two roundings of the same sum; maxima are exact, the sums' terms differ by the reference that they count from
+        assert torch.equal(M2, M) and torch.allclose(L2, L, rtol=2e-5) and float((o2.float() - o.float()).abs().max()) <= 2 * BF16 * float(o.float().abs().max())
+    assert bool((small == 7).all())
+
+
+def test_staged_tiles_first_called_under_capture():
+    """Tiles of many rows raise their kernel's LDS limit on the first call; that call may be a captured one."""
+    from lvar_amd import kv_cache_ops as kv
+    cache = kv.PagedKVCache.alloc(40, 1, 256, 16)
+    x = [rand(1, 1, 600, 256, seed=i).cuda() for i in range(2)]
+    table, lens = torch.arange(40, dtype=torch.int32, device="cuda").view(1, 40), torch.tensor([600], dtype=torch.int32, device="cuda")
+    kv.kv_cache_append(cache, *x, table, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    q = rand(1, 1, 77, 256, seed=4).cuda()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, (M, L) = kv.paged_attn(q, cache, table, lens, causal=True)
+    for r in range(3):
+        q.copy_(rand(1, 1, 77, 256, seed=10 + r))
+        e, (Me, Le) = kv.paged_attn(q, cache, table, lens, causal=True)
+        torch.cuda.synchronize()
+        graph.replay()
+        assert torch.equal(o, e) and torch.equal(M, Me) and torch.equal(L, Le)
+
+
+def test_two_appends_and_reads_on_two_streams():
+    from lvar_amd import kv_cache_ops as kv
+    B, H, d, n = 2, 4, 128, 500
+    x = [rand(B, H, n, d, seed=i).cuda() for i in range(2)]
+    table, start = table_for(B, 8, 16, 1).cuda(), torch.zeros(B, dtype=torch.int32, device="cuda")
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            c = kv.PagedKVCache.alloc(16, H, d, 64, torch.float8_e4m3fn)
+            kv.kv_cache_append(c, *x, table, start)
+            got.append(kv.kv_cache_read(c, table, lens, n) + kv.paged_attn(x[0], c, table, lens)[:1])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_large_forms_of_the_norm():
+    """Calls large enough for four heads per workgroup, in both pair orders, with heads that do not fill the last chunk; the gradients of one."""
+    from lvar_amd import kv_cache_ops as kv
+    for d, H, Hkv, inter, norm in ((16, 14, 7, True, "l2"), (32, 6, 6, False, "rms"), (64, 10, 5, False, "l2"), (128, 7, 7, True, "rms"), (256, 5, 5, False, None)):
+        L = 4 * 1024 * 256 // 4 // d * 4 // (H + Hkv) * 2 + 1
+        q, k, _ = projection(1, H, Hkv, L, d, seed=d)
+        w = [weight("full", h, d, 7 + i) for i, h in enumerate((H, Hkv))]
+        cos, sin = tables(L, d // 2)
+        got = kv.qk_norm_rope(q.cuda(), k.cuda(), cos.cuda(), sin.cuda(), None, w[0].cuda(), w[1].cuda(), norm, None, inter)
+        at = ref.table_rows(1, L, L)
+        for x, y, wx in ((q, got[0], w[0]), (k, got[1], w[1])):
+            check_rows(y, ref.norm_rope(x, wx, cos, sin, at, norm, EPS[norm], inter), (d, norm))
+
+
 # ---- together ----
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
