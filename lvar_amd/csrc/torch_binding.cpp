@@ -655,11 +655,21 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     lvar_norm_rope_t h;
     const std::string how = ctx->saved_data["how"].toStringRef();
     std::memcpy(&h, how.data(), sizeof(h));
-    if (wq.defined()) h.q_weight.ptr = wq.data_ptr();
-    if (wk.defined()) h.k_weight.ptr = wk.data_ptr();
-    if (cos.defined()) { h.cos = cos.data_ptr<float>(); h.sin = sin.data_ptr<float>(); }
-    if (positions.defined()) h.positions = positions.data_ptr();
-    const int dev = q.get_device();
+    // (pointers and strides anew: hooks on saved tensors may return copies of another layout)
+    const int dev = q.get_device(), B = dim(q, 0), H = dim(q, 1), Hkv = dim(k, 1), L = dim(q, 2), d = dim(q, 3);
+    auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    auto there = [](const at::Tensor& t) { return t.defined() ? &t : nullptr; };
+    bool same = rows_ok(&q, dev) && rows_ok(&k, dev) && weight_ok(there(wq), H, d, dev, h.q_weight) && weight_ok(there(wk), Hkv, d, dev, h.k_weight);
+    if (cos.defined()) {
+      same = same && cos.is_cuda() && sin.is_cuda() && cos.get_device() == dev && sin.get_device() == dev && cos.stride(1) == 1 && sin.stride(1) == 1 && cos.stride(0) == sin.stride(0);
+      h.cos = cos.data_ptr<float>(); h.sin = sin.data_ptr<float>(); h.table_stride = cos.stride(0);
+    }
+    if (positions.defined()) {
+      same = same && positions.is_cuda() && positions.get_device() == dev;
+      h.positions = positions.data_ptr();
+      h.pos_stride_b = positions.dim() == 2 && B > 1 ? positions.stride(0) : 0; h.pos_stride_row = positions.stride(-1);
+    }
+    TORCH_CHECK(same, "qk_norm_rope: hooks on saved tensors returned tensors that the backward pass cannot read (device, alignment or strides)");
     const c10::DeviceGuard guard(q.device());
     auto rows = [](const at::Tensor& g) {
       at::Tensor c = g.contiguous();
@@ -669,13 +679,11 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     at::Tensor dq = rows_like(q), dk = rows_like(k), dwq, dwk, scratch;
     if (wq.defined() && wq.requires_grad()) dwq = at::empty(wq.sizes(), wq.options());
     if (wk.defined() && wk.requires_grad()) dwk = at::empty(wk.sizes(), wk.options());
-    const int B = dim(q, 0), H = dim(q, 1), Hkv = dim(k, 1), L = dim(q, 2), d = dim(q, 3);
     int64_t bytes = 0;
     if (dwq.defined() || dwk.defined()) {
       bytes = api.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d);
       if (bytes > 0) scratch = empty({bytes}, at::kByte, dev);
     }
-    auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
     const int st = api.lvar_qk_norm_rope_bwd(view(q), view(k), h, gq.data_ptr(), gk.data_ptr(), view(dq), view(dk), ptr(dwq), ptr(dwk), ptr(scratch), bytes, B, H,
                                              Hkv, L, d, c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream());
     TORCH_CHECK(st == LVAR_OK, "lvar_qk_norm_rope_bwd failed with status ", st);

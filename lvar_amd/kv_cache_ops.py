@@ -219,6 +219,10 @@ class _NormRope(torch.autograd.Function):
         norm, eps, interleaved = ctx.how
         B, H, L, d = q.shape
         Hkv = k.shape[1]
+        # (hooks on saved tensors may return copies of another layout, or on another device)
+        q, k = _prep(q, "q"), _prep(k, "k")
+        cos, sin = _table_arg(cos, sin, d, q.device)
+        _require(positions is None or positions.device == q.device, "positions must be on the device of q")
         dq, dk = _rows_like(q), _rows_like(k)
         dwq = torch.empty_like(wq, memory_format=torch.contiguous_format) if wq is not None and ctx.needs_input_grad[2] else None
         dwk = torch.empty_like(wk, memory_format=torch.contiguous_format) if wk is not None and ctx.needs_input_grad[3] else None

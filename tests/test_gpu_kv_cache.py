@@ -578,6 +578,29 @@ def test_step_in_a_graph(dtype):
             assert same(outs[i][0], o) and same(outs[i][1][0], M) and same(outs[i][1][1], L)
 
 
+@pytest.mark.parametrize("binding", [True, False])
+def test_gradients_with_hooks_on_saved_tensors(binding, monkeypatch):
+    """Saved tensors that come back as packed copies (as save_on_cpu does), where tables, weights and positions were slices of wider memory."""
+    from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
+    B, H, L, d = 2, 4, 37, 64
+    wide = [rand(B, H, L, 2 * d, seed=i).cuda() for i in range(2)]
+    cos, sin = (torch.cat([t, t], 1).cuda()[:, :d // 2] for t in tables(50, d // 2))
+    positions = torch.randint(0, 50, (1, L), generator=torch.Generator().manual_seed(1)).cuda().expand(B, L)
+    ws = [torch.cat([weight("full", H, d, 3 + i)] * 2, 1).cuda()[:, :d] for i in range(2)]
+    g = [rand(B, H, L, d, seed=7 + i).cuda() for i in range(2)]
+
+    def grads():
+        q, k = (t.detach()[..., :d].requires_grad_() for t in wide)
+        w = [t.detach().requires_grad_() for t in ws]
+        return torch.autograd.grad(kv.qk_norm_rope(q, k, cos, sin, positions, *w), (q, k, *w), g)
+    want = grads()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().cpu().contiguous(), lambda t: t.cuda()):
+        got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_gradients_in_a_graph():
     """Forward and backward captured on leaves of their own and replayed, beside eager work on other leaves."""
     from lvar_amd import kv_cache_ops as kv
@@ -735,7 +758,7 @@ def test_two_appends_and_reads_on_two_streams():
 
 
 def test_large_forms_of_the_norm():
-    """Calls large enough for four heads per workgroup, in both pair orders, with heads that do not fill the last chunk; the gradients of one."""
+    """Calls large enough for four heads per workgroup, in both pair orders, with heads that do not fill the last chunk."""
     from lvar_amd import kv_cache_ops as kv
     for d, H, Hkv, inter, norm in ((16, 14, 7, True, "l2"), (32, 6, 6, False, "rms"), (64, 10, 5, False, "l2"), (128, 7, 7, True, "rms"), (256, 5, 5, False, None)):
         L = 4 * 1024 * 256 // 4 // d * 4 // (H + Hkv) * 2 + 1
