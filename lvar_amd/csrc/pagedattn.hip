@@ -144,7 +144,7 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
   }
   // (the first 64 sequences are loaded once)
   const int len0 = lane < p.B ? length_of(p, lane) : 0, tiles0 = lane < p.B ? tiles_of(p, lane) : 0;
-  int len, st, tiles, n, pieces, share = 0x7fffffff;
+  int len, st, tiles, n, pieces, share = p.min_share;
   auto look = [&](int b0) {
     const int b = b0 + lane;
     len = b0 == 0 ? len0 : 0;
@@ -965,8 +965,9 @@ int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s) {
   p.whole = h.whole;
   p.slot_rows = h.rows;
   p.ws_head = ws_head_floats(p.B);
-  // without room for partial results every tile stays whole: a share longer than any sequence
-  p.min_share = p.ws ? PA_LEAST : 0x7fffffff;
+  // without room for partial results every tile stays whole: a share longer than any sequence (at most 2^23 stages), far enough from
+  // 2^31 that find_piece may still add to it
+  p.min_share = p.ws ? PA_LEAST : 1 << 28;
   if (head_dim == 128) return launch_d<128>(p, h, s);
   if (head_dim == 64) return launch_d<64>(p, h, s);
   if (head_dim == 256) return launch_d<256>(p, h, s);

@@ -637,6 +637,7 @@ PADDED_CASES = [
     (4, 8, 1, 64, [1500, 70, 40, 900], 64, 16, False, [1, 64, 64, 16]),
     (3, 4, 1, 50, [900, 2000, 10], 256, 32, True, [50, 1, 0]),
     (70, 4, 1, 40, [(i * 31) % 300 for i in range(70)], 64, 16, True, [(i * 7) % 45 - 2 for i in range(70)]),
+    (330, 4, 2, 66, [(i * 37) % 41 for i in range(330)], 64, 16, False, [(i * 11) % 69 - 1 for i in range(330)]),   # more uncut tiles than workgroups of a round
 ]
 
 
