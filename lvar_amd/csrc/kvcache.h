@@ -92,6 +92,11 @@ struct PagedAttnParams {
   int64_t ws_head;                // floats ahead of the partial results
 };
 
+constexpr int NB_HC = 2;   // heads of a workgroup of the norm's backward pass
+
+// A launch has at most 2^32 - 1 threads along x.
+inline bool grid_fits(int64_t workgroups, int threads) { return workgroups * threads <= 0xffffffffll; }
+
 int launch_norm_rope(NormRopeParams p, int head_dim, bool append, hipStream_t s);
 int norm_rope_bwd_blocks(int B, int H, int Hkv, int L, int head_dim);
 int launch_norm_rope_bwd(NormRopeParams p, int head_dim, hipStream_t s);

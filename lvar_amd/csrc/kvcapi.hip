@@ -17,10 +17,8 @@ bool rows_ok(const lvar_tensor_t& t) {
 
 int sizes_ok(int B, int H, int kv_heads, int L) {
   if (B <= 0 || L <= 0 || kv_heads <= 0 || H <= 0 || H % kv_heads != 0) return LVAR_EINVAL;
-  // grid axes: batch and heads on y and z
+  // grid axes: batch and heads on y and z (the x axis is checked where its workgroups are counted)
   if (B > 65535 || H > 16384 || (int64_t)B * L > kMostTokens) return LVAR_EINVAL;
-  // one axis for all rows, at least 8 of them to a workgroup
-  if (((int64_t)B * L / 8 + 1) * (H + 2ll * kv_heads) > 0x7fffffff) return LVAR_EINVAL;
   return LVAR_OK;
 }
 
@@ -84,7 +82,7 @@ int fill_cache(PagedView& v, const lvar_paged_cache_t& c) {
 }
 
 // partial rows of a weight gradient
-int grad_rows(const WeightView& w, int heads, int nblk) { return w.s_head == 0 ? nblk * ((heads + 1) / 2) : nblk; }
+int grad_rows(const WeightView& w, int heads, int nblk) { return w.s_head == 0 ? nblk * ((heads + NB_HC - 1) / NB_HC) : nblk; }
 int64_t grad_floats(int heads, int nblk, int d) { return (int64_t)nblk * heads * d; }   // (the larger of the two forms)
 
 }  // namespace

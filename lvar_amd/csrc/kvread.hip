@@ -37,19 +37,20 @@ __global__ __launch_bounds__(KR_T) void kv_read_kernel(const KvReadParams p) {
 }
 
 template <int D>
-static void launch_d(const KvReadParams& p, hipStream_t s) {
+static int launch_d(const KvReadParams& p, hipStream_t s) {
   constexpr int RPB = KR_T / (D / 8);
   const dim3 grid((p.Lmax + RPB - 1) / RPB, p.cache.kv_heads, p.B);
+  if (!grid_fits(grid.x, KR_T)) return LVAR_EINVAL;
   if (p.cache.k_exp) hipLaunchKernelGGL((kv_read_kernel<D, true>), grid, dim3(KR_T), 0, s, p);
   else hipLaunchKernelGGL((kv_read_kernel<D, false>), grid, dim3(KR_T), 0, s, p);
+  return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
 }
 
 int launch_kv_read(const KvReadParams& p, int head_dim, hipStream_t s) {
-  if (head_dim == 128) launch_d<128>(p, s);
-  else if (head_dim == 64) launch_d<64>(p, s);
-  else if (head_dim == 256) launch_d<256>(p, s);
-  else return LVAR_EUNSUPPORTED;
-  return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
+  if (head_dim == 128) return launch_d<128>(p, s);
+  if (head_dim == 64) return launch_d<64>(p, s);
+  if (head_dim == 256) return launch_d<256>(p, s);
+  return LVAR_EUNSUPPORTED;
 }
 
 }  // namespace lvar

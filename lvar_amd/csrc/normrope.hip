@@ -226,41 +226,42 @@ static void division_by(NormRopeParams& p) {
 }
 
 template <int D, int HC>
-static void launch_fwd(const NormRopeParams& p, bool append, hipStream_t s) {
+static bool launch_fwd(const NormRopeParams& p, bool append, hipStream_t s) {
   constexpr int RPB = NR_T / (D / 8);
-  const dim3 grid((uint32_t)chunks_of<HC>(p, append) * (uint32_t)((p.B * p.L + RPB - 1) / RPB));
-  if (append) hipLaunchKernelGGL((norm_rope_kernel<D, HC, true>), grid, dim3(NR_T), 0, s, p);
-  else hipLaunchKernelGGL((norm_rope_kernel<D, HC, false>), grid, dim3(NR_T), 0, s, p);
+  const int64_t groups = (int64_t)chunks_of<HC>(p, append) * ((p.B * p.L + RPB - 1) / RPB);
+  if (!grid_fits(groups, NR_T)) return false;
+  if (append) hipLaunchKernelGGL((norm_rope_kernel<D, HC, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+  else hipLaunchKernelGGL((norm_rope_kernel<D, HC, false>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+  return true;
 }
 
 template <int D>
-static void launch_fwd_d(const NormRopeParams& p, bool append, hipStream_t s) {
+static bool launch_fwd_d(const NormRopeParams& p, bool append, hipStream_t s) {
   // Four heads per workgroup once such workgroups are four per compute unit, one head before that (latency is the time there).
   constexpr int RPB = NR_T / (D / 8);
   const int64_t tiles = (int64_t)(p.B * p.L + RPB - 1) / RPB;
-  if (tiles * chunks_of<4>(p, append) >= 4ll * device_cus()) launch_fwd<D, 4>(p, append, s);
-  else launch_fwd<D, 1>(p, append, s);
+  return tiles * chunks_of<4>(p, append) >= 4ll * device_cus() ? launch_fwd<D, 4>(p, append, s) : launch_fwd<D, 1>(p, append, s);
 }
 
 int launch_norm_rope(NormRopeParams p, int head_dim, bool append, hipStream_t s) {
   division_by(p);
   p.inv_eps = 1.f / p.eps;
+  bool ok = true;
   switch (head_dim) {
-    case 16: if (append) return LVAR_EUNSUPPORTED; launch_fwd_d<16>(p, append, s); break;
-    case 32: if (append) return LVAR_EUNSUPPORTED; launch_fwd_d<32>(p, append, s); break;
-    case 64: launch_fwd_d<64>(p, append, s); break;
-    case 128: launch_fwd_d<128>(p, append, s); break;
-    case 256: launch_fwd_d<256>(p, append, s); break;
+    case 16: if (append) return LVAR_EUNSUPPORTED; ok = launch_fwd_d<16>(p, append, s); break;
+    case 32: if (append) return LVAR_EUNSUPPORTED; ok = launch_fwd_d<32>(p, append, s); break;
+    case 64: ok = launch_fwd_d<64>(p, append, s); break;
+    case 128: ok = launch_fwd_d<128>(p, append, s); break;
+    case 256: ok = launch_fwd_d<256>(p, append, s); break;
     default: return LVAR_EUNSUPPORTED;
   }
+  if (!ok) return LVAR_EINVAL;
   return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
 }
 
 // ---- backward ----
 
-constexpr int NB_HC = 2;   // heads of a workgroup
-
-// Workgroup (blk, chunk): tokens blk * RPB + g, + nblk * RPB, ... of up to 4 heads of q or of k.  The weight gradients of its
+// Workgroup (blk, chunk): tokens blk * RPB + g, + nblk * RPB, ... of up to NB_HC heads of q or of k.  The weight gradients of its
 // heads stay in registers over all its tokens and meet in LDS once, in a fixed order: row `blk` of the partial sums.
 template <int D, bool DW>
 __global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParams p) {

@@ -555,7 +555,6 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
       write_rows<D, NT, 1, CW>(p, w, fresh, t, c * CW, &so[0][0][0], LDO, sm, sl);
     }
   }
-  write_padding<D>(p, w);
 }
 
 // ---- many rows per key/value head ----
@@ -934,7 +933,7 @@ static void launch_join(const PagedAttnParams& p, hipStream_t s) {
 template <int D>
 static int launch_d(const PagedAttnParams& p, const Shape& h, hipStream_t s) {
   const int64_t items = (int64_t)p.B * p.cache.kv_heads * p.rt + (p.ws ? p.finer : 0);
-  if (items > 0x7ffffff0) return LVAR_EINVAL;
+  if (!grid_fits(items + 8, PA_T) || (p.ws && !grid_fits(((int64_t)p.G * p.Lq * D + 2047) / 2048, 512))) return LVAR_EINVAL;
   const int grid = (int)((items + 7) / 8 * 8);
   bool ok = true;
   if constexpr (D == 256) {

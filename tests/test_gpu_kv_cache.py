@@ -870,4 +870,9 @@ def test_refusals_on_the_device(binding, monkeypatch):
     refused(S, at, x[:, :1], c, table, i), refused(S, at, rand(2, 2, 3, 128).cuda(), c, table, i), refused(S, at, x[:1], c, table, i), refused(S, at, x, c, table, None)
     refused(T, at, x.half(), c, table, i), refused(T, at, x, c, table, i.long()), refused(S, at, x, c, table, i, max_len=-1)
     refused(RuntimeError, at, x.clone().requires_grad_(), c, table, i), refused(Exception, at, x, c, table, i, -1.0)
+    # more workgroups than a launch holds (the entry point says so before it launches anything)
+    from lvar_amd import _lib
+    many = kv._cache_arg(c, table, x.shape[0], x.device)
+    many.kv_heads = 16384
+    assert _lib.load().lvar_paged_attn_fwd(kv._view(x), many, i.data_ptr(), None, x.data_ptr(), x.data_ptr(), x.data_ptr(), None, 0, 4096, 16384, 1, 100, 0, 1.0, kv._stream(x)) == -1
     torch.cuda.synchronize()

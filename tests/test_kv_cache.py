@@ -143,7 +143,8 @@ def test_entry_points_refuse_bad_arguments(lib):
         assert lib.lvar_kv_cache_append(t, t, t, ctypes.byref(how(**kw)), one, good, one, None, 1, 4, 3, None) == status, kw
     fwd = lambda q, k, oq, ok, *dims: lib.lvar_qk_norm_rope_fwd(q, k, how(**H), oq, ok, *dims, None)  # noqa: E731
     for dims, status in (((0, 4, 2, 3, 128), -1), ((1, 4, 3, 3, 128), -1), ((1, 4, 0, 3, 128), -1), ((1, 4, 2, 0, 128), -1), ((1, 4, 2, 3, 96), -2),
-                         ((65536, 4, 2, 3, 128), -1), ((60000, 4, 2, 60000, 128), -1), ((1, 32768, 2, 3, 128), -1)):
+                         ((65536, 4, 2, 3, 128), -1), ((60000, 4, 2, 60000, 128), -1), ((1, 32768, 2, 3, 128), -1),
+                         ((1, 1, 1, 1 << 30, 16), -1)):   # (2^32 threads, more than a launch holds)
         assert fwd(t, t, one, one, *dims) == status, dims
     assert fwd(null, t, one, one, 1, 4, 2, 3, 128) == -1 and fwd(t, skew, one, one, 1, 4, 2, 3, 128) == -1
     assert fwd(t, t, None, one, 1, 4, 2, 3, 128) == -1 and fwd(t, t, one, odd, 1, 4, 2, 3, 128) == -1
@@ -160,7 +161,7 @@ def test_entry_points_refuse_bad_arguments(lib):
         assert app(*args) == -1
     # read
     for args in ((None, None, one, one, 1, 3), (None, one, None, one, 1, 3), (None, one, one, odd, 1, 3), (odd, one, one, one, 1, 3), (None, one, one, one, 0, 3),
-                 (None, one, one, one, 1, 0), (None, one, one, one, 1, -3)):
+                 (None, one, one, one, 1, 0), (None, one, one, one, 1, -3), (None, one, one, one, 1, 1 << 30)):
         assert lib.lvar_kv_cache_read(good, *args, None) == -1
     # attention
     att = lambda q=t, lengths=one, counts=None, o=one, M=one, L=one, B=1, H=4, Lq=3, n=100, scale=1.0: lib.lvar_paged_attn_fwd(  # noqa: E731
