@@ -629,7 +629,7 @@ int norm_rope_launch(const at::Tensor& q, const at::Tensor& k, const lvar_norm_r
 
 // memory for a gradient of t in t's own order of axes, if the kernels can write it
 at::Tensor rows_like(const at::Tensor& t) {
-  at::Tensor g = at::empty_like(t);
+  at::Tensor g = t.is_non_overlapping_and_dense() ? at::Tensor(at::detail::empty_strided_cuda(t.sizes(), t.strides(), at::kBFloat16, t.device())) : at::empty_like(t);
   const auto st = g.strides();
   return st[3] == 1 && ((st[0] | st[1] | st[2]) & 7) == 0 ? g : at::empty(t.sizes(), t.options());
 }
@@ -677,8 +677,8 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     };
     const at::Tensor gq = rows(grads[0]), gk = rows(grads[1]);
     at::Tensor dq = rows_like(q), dk = rows_like(k), dwq, dwk, scratch;
-    if (wq.defined() && wq.requires_grad()) dwq = at::empty(wq.sizes(), wq.options());
-    if (wk.defined() && wk.requires_grad()) dwk = at::empty(wk.sizes(), wk.options());
+    if (wq.defined() && wq.requires_grad()) dwq = empty(wq.sizes(), wq.scalar_type(), dev);
+    if (wk.defined() && wk.requires_grad()) dwk = empty(wk.sizes(), wk.scalar_type(), dev);
     int64_t bytes = 0;
     if (dwq.defined() || dwk.defined()) {
       bytes = api.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d);
