@@ -55,7 +55,8 @@ struct NormRopeParams {
   const bf16_t *gq, *gk;          // contiguous
   bf16_t *dq, *dk;
   int64_t dq_sb, dq_sh, dq_sr, dk_sb, dk_sh, dk_sr;
-  float *pq, *pk;                 // partial weight gradients, null: not wanted
+  float *pq, *pk;                 // partial weight gradients, null: not wanted, or
+  void *dqw, *dkw;                // ... written at once: there is one row of them
   int nblk;
 };
 
@@ -98,7 +99,7 @@ constexpr int NB_HC = 2;   // heads of a workgroup of the norm's backward pass
 inline bool grid_fits(int64_t workgroups, int threads) { return workgroups * threads <= 0xffffffffll; }
 
 int launch_norm_rope(NormRopeParams p, int head_dim, bool append, hipStream_t s);
-int norm_rope_bwd_blocks(int B, int H, int Hkv, int L, int head_dim);
+int norm_rope_bwd_blocks(int B, int H, int Hkv, int L, int head_dim, bool alone);
 int launch_norm_rope_bwd(NormRopeParams p, int head_dim, hipStream_t s);
 int launch_weight_grad(const WeightGradParams& w, hipStream_t s);
 int launch_kv_read(const KvReadParams& p, int head_dim, hipStream_t s);

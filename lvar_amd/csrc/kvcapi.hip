@@ -106,7 +106,7 @@ int64_t lvar_qk_norm_rope_bwd_scratch_bytes(int B, int H, int kv_heads, int L, i
   const int st = sizes_ok(B, H, kv_heads, L);
   if (st != LVAR_OK) return st;
   if (!norm_head_dim(head_dim)) return LVAR_EUNSUPPORTED;
-  const int nblk = norm_rope_bwd_blocks(B, H, kv_heads, L, head_dim);
+  const int nblk = norm_rope_bwd_blocks(B, H, kv_heads, L, head_dim, false);
   if (nblk <= 0) return LVAR_ELAUNCH;
   return 4 * grad_floats(H + kv_heads, nblk, head_dim);
 }
@@ -129,25 +129,33 @@ int lvar_qk_norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how
   if (dqw || dkw) {
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < lvar_qk_norm_rope_bwd_scratch_bytes(B, H, kv_heads, L, head_dim)) return LVAR_EINVAL;
   }
-  p.nblk = norm_rope_bwd_blocks(B, H, kv_heads, L, head_dim);
-  if (p.nblk <= 0) return LVAR_ELAUNCH;
-  float* part = (float*)scratch;
-  if (dqw) p.pq = part;
-  if (dkw) p.pk = part + grad_floats(H, p.nblk, head_dim);
-  if ((st = launch_norm_rope_bwd(p, head_dim, (hipStream_t)stream)) != LVAR_OK || (!dqw && !dkw)) return st;
-  WeightGradParams w{};
   const WeightView* wv[2] = {&p.wq, &p.wk};
   void* out[2] = {dqw, dkw};
-  const float* parts[2] = {p.pq, p.pk};
   const int heads[2] = {H, kv_heads};
+  bool alone = dqw || dkw;
+  for (int i = 0; i < 2; i++) alone = alone && !(out[i] && wv[i]->s_head == 0 && heads[i] > NB_HC);
+  p.nblk = norm_rope_bwd_blocks(B, H, kv_heads, L, head_dim, alone);
+  if (p.nblk <= 0) return LVAR_ELAUNCH;
+  float* parts[2] = {(float*)scratch, (float*)scratch + grad_floats(H, p.nblk, head_dim)};
+  WeightGradParams w{};
   w.D = head_dim;
+  bool rest = false;
   for (int i = 0; i < 2; i++) {
+    if (!out[i]) continue;
+    const int rows = grad_rows(*wv[i], heads[i], p.nblk);
+    if (rows == 1) {
+      (i ? p.dkw : p.dqw) = out[i];
+      continue;
+    }
+    rest = true;
+    (i ? p.pk : p.pq) = parts[i];
     w.out[i] = out[i]; w.part[i] = parts[i];
-    w.heads[i] = !out[i] ? 0 : wv[i]->s_head == 0 ? 1 : heads[i];
-    w.rows[i] = grad_rows(*wv[i], heads[i], p.nblk);
+    w.heads[i] = wv[i]->s_head == 0 ? 1 : heads[i];
+    w.rows[i] = rows;
     w.cols[i] = wv[i]->mode == W_COLUMN ? head_dim : 1;
     w.bf16[i] = wv[i]->bf16;
   }
+  if ((st = launch_norm_rope_bwd(p, head_dim, (hipStream_t)stream)) != LVAR_OK || !rest) return st;
   return launch_weight_grad(w, (hipStream_t)stream);
 }
 

@@ -134,6 +134,13 @@ def test_norm_rope_gradients(case, weights):
             assert bool((err <= tol).all()), f"dw{'qk'[i]}: {float((err - tol).max()):.3g} over"
 
 
+@pytest.mark.parametrize("kind", ["head", "full", "row", "dim", "one"])
+@pytest.mark.parametrize("H,Hkv,L,d", [(3, 1, 1, 128), (2, 2, 16, 128), (5, 5, 64, 128), (4, 2, 65, 128), (3, 3, 30, 256), (2, 1, 37, 64), (6, 3, 250, 32), (1, 1, 90, 32)])
+def test_norm_rope_gradients_of_few_tokens(kind, H, Hkv, L, d):
+    """Around the sizes up to which the gradient of a weight is written without partial sums (8 tiles of 2048 / d tokens)."""
+    test_norm_rope_gradients((2, H, Hkv, L, d, d, "rms" if L % 2 else "l2", kind, bool(L % 3), None), torch.float32 if H % 2 else torch.bfloat16)
+
+
 def test_norm_rope_gradient_against_differences():
     """The gradient of the operator against central differences of the 64-bit forward pass."""
     from lvar_amd import kv_cache_ops as kv
