@@ -88,7 +88,8 @@ struct PagedAttnParams {
   float c;                        // scale * log2(e)
   // set at launch
   int rt, tile_rows;              // row tiles per key/value head, rows of one
-  int target, finer, min_share, whole;   // pieces of one round, of several; fewest 128-key stages of one; tiles up to this many stay whole
+  int target, finer, whole;       // pieces of one round, of several; a call whose tiles have up to this many 128-key stages is not cut
+  uint32_t singles;               // up to this many stages in all, pieces may be of one
   int slot_rows;
   int64_t ws_head;                // floats ahead of the partial results
 };

@@ -102,15 +102,15 @@ __device__ __forceinline__ int tiles_of(const PagedAttnParams& p, int b) { retur
 // Length of sequence b within what the table can name.
 __device__ __forceinline__ int length_of(const PagedAttnParams& p, int b) { return max(0, min(p.lengths[b], p.max_len)); }
 
-// Stages of a piece: `total` stages spread over `target` pieces, but no less than min_share stages each.  (The launch has checked
-// that the stages of all tiles together fit 31 bits.)
+// Stages of a piece: `total` stages spread over `target` pieces, at least two each if there are more than `singles`.  (The launch has
+// checked that the stages of all tiles together fit 31 bits.)
 __device__ __forceinline__ int share_of(const PagedAttnParams& p, uint32_t total, uint32_t target) {
-  return max((int)((total - 1) / target) + 1, p.min_share);
+  return max((int)((total - 1) / target) + 1, total > p.singles ? 2 : 1);
 }
 
-// Pieces of a tile of `stages` > 0 stages; tiles of up to `whole` stages stay in one.
-__device__ __forceinline__ int pieces_of(const PagedAttnParams& p, int stages, int share) {
-  return stages <= p.whole ? 1 : (int)((uint32_t)(stages - 1) / (uint32_t)share) + 1;
+// Pieces of a tile of `stages` > 0 stages if tiles are cut at all; those of up to two stages stay in one.
+__device__ __forceinline__ int pieces_of(int stages, int share) {
+  return stages <= 2 ? 1 : (int)((uint32_t)(stages - 1) / (uint32_t)share) + 1;
 }
 
 // The piece of workgroup `wg`; false for the workgroups that are left over.  All lanes of a wave call it and get the same answer, in
@@ -144,7 +144,7 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
   }
   // (the first 64 sequences are loaded once)
   const int len0 = lane < p.B ? length_of(p, lane) : 0, tiles0 = lane < p.B ? tiles_of(p, lane) : 0;
-  int len, st, tiles, n, pieces, share = p.min_share;
+  int len, st, tiles, n, pieces, share = 0x7fffffff;
   auto look = [&](int b0) {
     const int b = b0 + lane;
     len = b0 == 0 ? len0 : 0;
@@ -154,12 +154,14 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
       tiles = tiles_of(p, b);
     }
     st = b < p.B ? stages_of(len) : 0;
-    n = b < p.B ? pieces_of(p, st, share) : 0;
+    n = b < p.B ? pieces_of(st, share) : 0;
   };
   uint32_t total = 0;
+  bool cut = false;     // nothing is, or everything may be: with the longest tile the call waits for the join
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     look(b0);
     total += last_lane(wave_scan(st * tiles));
+    cut = cut || __any(st > p.whole);
   }
   total *= (uint32_t)p.cache.kv_heads;
   auto count = [&]() {
@@ -170,15 +172,15 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
     }
     pieces *= p.cache.kv_heads;
   };
-  share = share_of(p, total, p.target);
+  if (cut) share = share_of(p, total, p.target);
   count();
   // One round of workgroups, with pieces up to 3 / 8 longer if that makes it one; otherwise fine pieces, whose last round is short.
   const int even = share;
-  for (int tries = 0; tries < 3 && pieces > p.target; tries++) {
+  for (int tries = 0; cut && tries < 3 && pieces > p.target; tries++) {
     share += max(1, even >> 3);
     count();
   }
-  if (pieces > p.target) {
+  if (cut && pieces > p.target) {
     share = share_of(p, total, p.finer);
     count();
   }
@@ -186,8 +188,8 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
   int before = 0, slots = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (b0 > 0) look(b0);
-    const int mine = n * tiles * p.cache.kv_heads, cut = n > 1 ? mine : 0;
-    const int upto = wave_scan(mine), cuts = wave_scan(cut);
+    const int mine = n * tiles * p.cache.kv_heads, slot = n > 1 ? mine : 0;
+    const int upto = wave_scan(mine), cuts = wave_scan(slot);
     const uint64_t hit = __ballot(before + upto > item);
     if (hit) {
       const int l = __builtin_ctzll(hit);
@@ -197,7 +199,7 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
       out.n = __builtin_amdgcn_readlane(n, l);
       out.rt = __builtin_amdgcn_readlane(tiles, l);
       const int rest = item - before - __builtin_amdgcn_readlane(upto - mine, l);
-      out.first_slot = slots + __builtin_amdgcn_readlane(cuts - cut, l);
+      out.first_slot = slots + __builtin_amdgcn_readlane(cuts - slot, l);
       out.slot = out.first_slot + rest;
       split(rest);
       return true;
@@ -860,8 +862,6 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p
 
 // ---- launch ----
 
-constexpr int PA_LEAST = 2;   // fewest stages of a share
-
 struct Shape { int nt, rw, rt, rows, whole, finer; bool staged; };
 
 // Rows per tile: 16 up to 16 rows of a key/value head, 32 up to 32 (each wave reads keys for itself), more with staged tiles: 64 up to
@@ -875,10 +875,16 @@ static Shape shape_of(int B, int H, int Hkv, int Lq, int head_dim) {
   const int tile = 16 * s.nt * s.rw;
   s.rt = (int)((rows + tile - 1) / tile);
   s.rows = (int)(rows < tile ? rows : tile);
-  // A workgroup on its own takes 1.2 us per stage, the join 4: tiles of up to 5 stages are not cut (512 tokens of one sequence 9.7 -> 8.2
-  // us), and where uncut tiles are half as many as compute units, none of up to 10 (16 x 768 tokens 15.5 -> 11.9, 32 x 1280 37.9
-  // -> 32.6; not of the staged tiles, whose stages take two to four times as long).
-  s.whole = !s.staged && (int64_t)B * Hkv * s.rt >= device_cus() / 2 ? 10 : 5;
+  // Calls whose tiles all have up to this many stages are not cut.  Cutting costs the join and the partial results, 4 to 6 us with few tiles and more with many;
+  // it saves the stages that a workgroup does not do: 0.65, 1.1 and 2.5 us each (head_dim 64, 128, 256), 1.5, 2.1 and 3.8 of staged
+  // tiles.  The limits are where both measured the same (uncut / cut at 4 stages, 16 heads of 64 rows: head_dim 64 11.7 / 12.1, 128 15.4 / 14.0,
+  // 256 22.2 / 17.8; of 1 row: head_dim 256 16.0 / 11.5), as measured with 1 / 16 to all of the compute units taken by uncut tiles: 128 tiles of
+  // 1 row at 8 stages 14.7 / 18.2, of 64 rows at 6 stages 20.3 / 20.5.  With a longer tile all are cut: 16 x 8 ragged tiles of 1 row and up to 19
+  // stages 16.1, with those of up to 6 whole 17.4, of up to 10 19.2 (head_dim 64).
+  const int cus = device_cus(), i = head_dim / 128;
+  const int64_t tiles = (int64_t)B * Hkv * s.rt;
+  static constexpr int kLimit[2][3] = {{8, 4, 2}, {4, 3, 2}}, kMore[2][3] = {{8, 8, 4}, {6, 6, 8}};
+  s.whole = kLimit[s.staged][i] + (cus > 0 ? (int)(kMore[s.staged][i] * (tiles < cus ? tiles : cus) / cus) : 0);
   s.finer = device_cus() * (s.staged ? 4 : 6);
   return s;
 }
@@ -896,13 +902,13 @@ static int round_of(const Shape& s, int head_dim, bool f8) {
 static int64_t ws_head_floats(int B) { return ((int64_t)2 * B + 63) / 64 * 64; }   // pieces and first slot of every sequence
 
 // Partial results are kept for tiles that are cut only; such a tile has n < 2 * stages / share pieces, and a share is at least the
-// `finer`-th part of all stages, so that there are fewer than 2 * finer of them in all; nor are there more than pieces of the shortest share.
+// `finer`-th part of all stages, so that there are fewer than 2 * finer of them in all; nor are there more than stages.
 int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim) {
   const Shape s = shape_of(B, H, Hkv, Lq, head_dim);
   if (s.finer <= 0) return LVAR_ELAUNCH;
   const int64_t stages = ((int64_t)max_len + PA_STAGE - 1) / PA_STAGE;
   if (stages <= s.whole) return 0;   // nothing can be cut
-  const int64_t most = (int64_t)B * Hkv * s.rt * ((stages + PA_LEAST - 1) / PA_LEAST), slots = most < 2ll * s.finer ? most : 2ll * s.finer;
+  const int64_t most = (int64_t)B * Hkv * s.rt * stages, slots = most < 2ll * s.finer ? most : 2ll * s.finer;
   return 4 * (ws_head_floats(B) + slots * s.rows * (head_dim + 2));
 }
 
@@ -961,12 +967,13 @@ int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s) {
   p.tile_rows = 16 * h.nt * h.rw;
   p.target = round_of(h, head_dim, p.cache.k_exp != nullptr);
   p.finer = h.finer;
-  p.whole = h.whole;
+  p.whole = p.ws ? h.whole : 0x7fffffff;   // (no room for partial results: nothing is cut)
   p.slot_rows = h.rows;
   p.ws_head = ws_head_floats(p.B);
-  // without room for partial results every tile stays whole: a share longer than any sequence (at most 2^23 stages), far enough from
-  // 2^31 that find_piece may still add to it
-  p.min_share = p.ws ? PA_LEAST : 1 << 28;
+  // Pieces of one stage, but of row tiles that are staged only while half of the compute units suffice for them (beyond that the join of the
+  // tiles costs more): one sequence of 1024 keys with one new token, 8 of 32 heads, 10.2 -> 8.9 us; 16 heads of 1000 keys with 64 new tokens
+  // 16.0 -> 15.3, of 2000 keys 17.6 -> 18.3, 2 x 4 heads of 3000 keys with 256 rows 27.2 -> 31.5.
+  p.singles = h.staged ? device_cus() / 2 : 0x7fffffff;
   if (head_dim == 128) return launch_d<128>(p, h, s);
   if (head_dim == 64) return launch_d<64>(p, h, s);
   if (head_dim == 256) return launch_d<256>(p, h, s);
