@@ -88,8 +88,9 @@ struct PagedAttnParams {
   float c;                        // scale * log2(e)
   // set at launch
   int rt, tile_rows;              // row tiles per key/value head, rows of one
-  int target, finer, whole;       // pieces of one round, of several; a call whose tiles have up to this many 128-key stages is not cut
+  int target, wide, wider, finer, whole;   // pieces of one round, of rounds of more, of several; a call whose tiles have up to this many 128-key stages is not cut
   uint32_t singles;               // up to this many stages in all, pieces may be of one
+  uint32_t some, many, most;      // stages in all from which on ragged lengths are cut for `wide`, `wider`, `target` again
   int slot_rows;
   int64_t ws_head;                // floats ahead of the partial results
 };

@@ -172,17 +172,24 @@ __device__ __forceinline__ bool find_piece(const PagedAttnParams& p, int wg, int
     }
     pieces *= p.cache.kv_heads;
   };
+  // One round of workgroups, with pieces up to 3 / 8 longer if that makes it one; otherwise fine pieces, whose last round is short.  Lengths
+  // that are alike give `target` equal pieces.  Of others some pieces are much longer than the rest, which a round of more workgroups per
+  // compute unit evens out if there is enough to do (16 x 8 tiles of up to 2500 keys in bf16, 23.6 -> 21.5 us; of up to 1300 keys with 64
+  // rows 22.6 -> 23.4), unless they are so long (32 stages) that their number hardly matters.
   if (cut) share = share_of(p, total, p.target);
   count();
-  // One round of workgroups, with pieces up to 3 / 8 longer if that makes it one; otherwise fine pieces, whose last round is short.
-  const int even = share;
-  for (int tries = 0; cut && tries < 3 && pieces > p.target; tries++) {
-    share += max(1, even >> 3);
-    count();
-  }
   if (cut && pieces > p.target) {
-    share = share_of(p, total, p.finer);
-    count();
+    const int round = total <= p.some || total > p.most ? p.target : total <= p.many ? p.wide : p.wider;
+    const int even = share_of(p, total, round);
+    int x = round == p.target ? 1 : 0;
+    do {
+      share = even + x * max(1, even >> 3);
+      count();
+    } while (pieces > round && ++x < 4);
+    if (pieces > round) {
+      share = share_of(p, total, p.finer);
+      count();
+    }
   }
   if (!take(pieces, item)) return false;
   int before = 0, slots = 0;
@@ -889,14 +896,15 @@ static Shape shape_of(int B, int H, int Hkv, int Lq, int head_dim) {
   return s;
 }
 
-// Pieces of one round, per compute unit.  A workgroup is bound by latency, about 1.2 us per stage, and as many are wanted as fill the
-// memory's bandwidth: more only add to what is joined.  That is one per compute unit with stages of 64 KiB or more (bf16, head_dim
-// 128), two with half of that, three with less; and two, all that fit, where row tiles share keys and the matrix units are the bound.
-// Two instead of one: 8 x 4096 keys in bf16 with 8 new tokens 30.6 -> 33.2 us, 131071 keys in e4m3 61.1 -> 57.5, 4 x 256 rows 50.0 -> 45.8.
-static int round_of(const Shape& s, int head_dim, bool f8) {
+// Workgroups per compute unit of a round of equal pieces.  A workgroup is bound by latency, and as many are wanted as fill the memory's
+// bandwidth: more only add to what is joined.  For tiles of up to 16 rows that is one with stages of 64 KiB or more (bf16, head_dim
+// 128), two with half of that, three with less; for more rows one, and two, all that fit, where row tiles share keys and the matrix units
+// are the bound.  Two instead of one: 8192 keys in bf16 13.8 -> 14.4 us, with head_dim 256 19.6 -> 22.7, 131071 keys in e4m3 61.3 -> 57.5;
+// 4 x 16 heads of 2521 keys with 32 rows 22.4 -> 24.0, with 256 rows 50.6 -> 44.6.
+static int per_cu(const Shape& s, int head_dim, bool f8) {
+  if (s.staged || s.nt == 2) return s.rt > 1 ? 2 : 1;
   const int stage = 2 * PA_STAGE * head_dim * (f8 ? 1 : 2);
-  const int per = stage >= 65536 ? 1 : stage >= 32768 ? 2 : s.staged ? 2 : 3;
-  return device_cus() * (s.staged && s.rt > 1 && head_dim < 256 ? 2 : per);
+  return stage >= 65536 ? 1 : stage >= 32768 ? 2 : 3;
 }
 
 static int64_t ws_head_floats(int B) { return ((int64_t)2 * B + 63) / 64 * 64; }   // pieces and first slot of every sequence
@@ -965,7 +973,15 @@ int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s) {
   if (h.finer <= 0) return LVAR_ELAUNCH;
   p.rt = h.rt;
   p.tile_rows = 16 * h.nt * h.rw;
-  p.target = round_of(h, head_dim, p.cache.k_exp != nullptr);
+  // Ragged lengths: two workgroups per compute unit from 4 stages on (tiles of 32 rows and head_dim 128, 16: 8 x 8 tiles of up to 4096 keys 23.7
+  // against 25.0 us, 32 x 8 of up to 8000 125 against 116), with head_dim 64 three, which fit, from 16 on (the latter in e4m3, 46 -> 38).
+  const int cus = device_cus(), per = per_cu(h, head_dim, p.cache.k_exp != nullptr);
+  p.target = per * cus;
+  p.wide = (per > 2 ? per : 2) * cus;
+  p.wider = !h.staged && head_dim == 64 ? 3 * cus : p.wide;
+  p.some = (!h.staged && h.nt == 2 && head_dim > 64 ? 16 : 4) * cus;
+  p.many = 16 * cus;
+  p.most = 64 * cus;
   p.finer = h.finer;
   p.whole = p.ws ? h.whole : 0x7fffffff;   // (no room for partial results: nothing is cut)
   p.slot_rows = h.rows;
@@ -973,7 +989,7 @@ int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s) {
   // Pieces of one stage, but of row tiles that are staged only while half of the compute units suffice for them (beyond that the join of the
   // tiles costs more): one sequence of 1024 keys with one new token, 8 of 32 heads, 10.2 -> 8.9 us; 16 heads of 1000 keys with 64 new tokens
   // 16.0 -> 15.3, of 2000 keys 17.6 -> 18.3, 2 x 4 heads of 3000 keys with 256 rows 27.2 -> 31.5.
-  p.singles = h.staged ? device_cus() / 2 : 0x7fffffff;
+  p.singles = h.staged ? cus / 2 : 0x7fffffff;
   if (head_dim == 128) return launch_d<128>(p, h, s);
   if (head_dim == 64) return launch_d<64>(p, h, s);
   if (head_dim == 256) return launch_d<256>(p, h, s);
