@@ -385,7 +385,7 @@ int lvar_window_key_scores(lvar_tensor_t q, lvar_tensor_t k, const int64_t* wind
  * ---- Norms, rotation and a paged key/value cache ----
  *
  * A paged cache: rows of head_dim keys or values in pages [num_pages, kv_heads, page_size, head_dim], either bf16 (k_exp and
- * v_exp NULL) or e4m3 codes with one power of two per row, value = code * 2^(byte - 127), bytes uint8
+ * v_exp NULL) or e4m3 codes with one power of two per row, value = code * 2^(byte - 127), bytes (1 to 254) uint8
  * [num_pages, kv_heads, page_size] with unit stride along the page.  k and v share the strides (in elements; rows 16-byte
  * aligned), k_exp and v_exp theirs (multiples of 4, 4-byte aligned bases).  page_size is a power of two from 16 to 1024, head_dim 64, 128 or 256.
  * page_table int32 [B, max_pages]: token n of sequence b is row n % page_size of page page_table[b, n / page_size].  Entries
@@ -447,7 +447,7 @@ int lvar_qk_norm_rope_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how
  * Gradients of lvar_qk_norm_rope_fwd: from q, k and the contiguous bf16 gradients gq, gk of its outputs, dq and dk (bf16 views) and
  * the weight gradients dqw, dkw (NULL: not wanted; contiguous, [heads or 1, head_dim or 1] as the weight's strides say, of its type).
  * scratch: lvar_qk_norm_rope_bwd_scratch_bytes() (16-byte aligned; needed for weight gradients only), written and read by this call.
- * Sums over tokens are formed in a fixed order.
+ * Sums over tokens are formed in a fixed order.  A weight whose stride_head is 0 gets one gradient for all heads.
  */
 int64_t lvar_qk_norm_rope_bwd_scratch_bytes(int B, int H, int kv_heads, int L, int head_dim);
 int lvar_qk_norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, const void* gq, const void* gk, lvar_tensor_t dq,
@@ -475,7 +475,8 @@ int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int
  * Attention of the newest Lq tokens q [B,H,Lq,d] (bf16 view) over the first lengths[b] tokens of the cache, which hold them already:
  * o = softmax(q k^T scale) v (contiguous bf16), M and L fp32 [B,H,Lq] as everywhere here.  causal: row i of sequence b sees tokens
  * j < lengths[b] - n + i + 1, n = counts[b] (NULL: Lq) its new tokens; rows i >= n, and rows that see no token, get o = 0, M = -inf, L = 1.
- * Query head h reads key/value head h / (H / kv_heads).  Lengths are clamped to max_len (at most max_pages * page_size).
+ * Query head h reads key/value head h / (H / kv_heads).  Lengths are clamped to max_len (at most max_pages * page_size).  What the cache holds
+ * behind them does not matter; a value that is not finite reaches the rows that see it and may reach rows up to 128 before them (0 * inf).
  * workspace: lvar_paged_attn_workspace_bytes() (16-byte aligned, its contents need no preparation; calls that overlap in time
  * need one each); without one, or with a smaller one, no sequence is cut and long ones are slow.  Results depend on the lengths of all
  * sequences of the call in the last bits (they decide where sequences are cut), not on timing.

@@ -13,7 +13,7 @@
 //     while it computes, and the four waves take turns at 32 keys.  32 sequences of up to 32768 tokens, 32 query heads over 8 of
 //     128: 2.2 GB of bf16 in 390 us (5.7 TB/s; a copy moves 5.2); 131071 tokens in e4m3: 0.27 GB in 55 us.
 //   paged_tile_kernel   more rows: keys and values staged in LDS, where the waves share them.  4 x 256 rows of 16 heads over 2521
-//     tokens: 45 .. 50 us, 420 .. 470 TFLOP/s.  (With 64 rows per wave and no LDS there is one wave per SIMD and nobody left to
+//     tokens: 44 .. 46 us, 460 .. 480 TFLOP/s.  (With 64 rows per wave and no LDS there is one wave per SIMD and nobody left to
 //     compute while it waits: 105 us where this takes 38, 8 sequences of up to 4001 tokens with up to 61 new ones.)
 //
 // The work is (sequence, key/value head, row tile) x stages of 128 keys.  It is cut into pieces of about equal length by the

@@ -29,7 +29,7 @@ _EPS = {None: 0.0, "l2": 1e-12, "rms": 1e-6}
 class PagedKVCache(NamedTuple):
     """Keys and values in pages: ``k`` and ``v`` ``[num_pages, kv_heads, page_size, head_dim]``, either bf16 or
     ``float8_e4m3fn`` codes with one power of two per row: ``k_exp`` and ``v_exp`` uint8 ``[num_pages, kv_heads, page_size]``,
-    value = code * 2^(byte - 127).  ``page_size`` is a power of two from 16 to 1024, ``head_dim`` 64, 128 or 256; ``k`` and ``v``
+    value = code * 2^(byte - 127) with bytes from 1 to 254.  ``page_size`` is a power of two from 16 to 1024, ``head_dim`` 64, 128 or 256; ``k`` and ``v``
     have the same strides, unit stride on the last axis, and rows that are 16-byte aligned.  The tuple only names
     the tensors: it holds no state.
 
@@ -252,7 +252,8 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
     ``q_weight`` / ``k_weight`` (fp32 or bf16; ``[d]``, ``[H,1]``, ``[1,d]`` or ``[H,d]``) multiply the result.  ``cos`` / ``sin``
     fp32 ``[rows, rot/2]`` rotate the first ``rot`` columns (a multiple of 16) in pairs ``(2i, 2i+1)``, or ``(i, i + rot/2)``
     with ``interleaved=False``; token i takes row i, or row ``positions[i]`` / ``positions[b,i]`` (clamped to the table).
-    ``head_dim`` 16, 32, 64, 128 or 256.  All in fp32, rounded once.  Differentiable in q, k and the weights (once); the
+    ``head_dim`` 16, 32, 64, 128 or 256.  All in fp32, rounded once.  Differentiable in q, k and the weights (once); a backward pass that
+    is captured in a graph wants leaves without a live eager graph, as always with autograd.  The
     reference's counterpart is models/sparvar/basic_sparvar.py:326-342, eager."""
     fast = _native()
     if fast is not None:
@@ -310,7 +311,7 @@ def kv_cache_append(cache: PagedKVCache, k, v, page_table, start, counts=None) -
 def qk_norm_rope_append(cache: PagedKVCache, q, k, v, page_table, start, cos=None, sin=None, counts=None, positions=None, q_weight=None,
                         k_weight=None, norm: Optional[str] = "l2", eps: Optional[float] = None, interleaved: bool = True) -> torch.Tensor:
     """:func:`qk_norm_rope` on q and k and :func:`kv_cache_append` of the keys and of ``v``, in one launch; returns the queries.
-    Without ``positions`` token i of sequence b takes row ``start[b] + i`` of the tables.  The keys are rounded once, from fp32 to
+    Without ``positions`` token i of sequence b takes row ``start[b] + i`` of the tables (clamped to them).  The keys are rounded once, from fp32 to
     the cache's type."""
     fast = _native()
     if fast is not None:
@@ -360,7 +361,8 @@ def paged_attn(q, cache: PagedKVCache, page_table, lengths, scale=None, causal: 
     ``(o, (M, L))`` as :func:`lvar_amd.sparse_attn_ops.dense_attn`.  One token, a small scale, or a chunk; query head h reads key/value
     head ``h // (H // Hkv)``.  ``causal``: row i of sequence b sees tokens ``j < lengths[b] - n + i + 1`` with ``n = counts[b]``
     (default Lq) new tokens; otherwise all ``lengths[b]``.  Rows ``i >= counts[b]`` of a padded batch and rows that see no token
-    get ``o = 0, M = -inf, L = 1``.  ``max_len`` bounds the lengths (longer ones are clamped to it; default: all that the page table
+    get ``o = 0, M = -inf, L = 1``.  What the cache holds behind ``lengths`` does not matter; a value that is not finite reaches the rows that
+    see it and may reach rows up to 128 before them (0 * inf).  ``max_len`` bounds the lengths (longer ones are clamped to it; default: all that the page table
     can name): a small bound lets the launch do without the pass that joins the parts of long sequences."""
     fast = _native()
     if fast is not None:
