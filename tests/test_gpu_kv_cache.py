@@ -179,6 +179,21 @@ def test_norm_rope_rows_below_eps_and_zero_rows():
         assert bool(((dx.double().cpu() - want).abs() <= BF16 * want.abs() + 4 * 80 * F32 * size).all())
 
 
+@pytest.mark.parametrize("norm", ["l2", "rms"])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_norm_rope_of_extreme_values(norm, interleaved):
+    """The largest bf16 values (whose squares are infinite in 32 bits: the factor is 0, as in eager fp32) and the smallest normal ones give finite results."""
+    from lvar_amd import kv_cache_ops as kv
+    cos, sin = (t.cuda() for t in tables(4, 32))
+    for v in (torch.finfo(torch.bfloat16).max, 1e25, 2e-38):
+        q = (torch.sign(rand(1, 2, 4, 64, seed=3)) * v).to(torch.bfloat16).cuda()
+        for w in (None, torch.full((64,), 2.0, device="cuda")):
+            got = kv.qk_norm_rope(q, q, cos, sin, q_weight=w, k_weight=w, norm=norm, interleaved=interleaved)
+            assert all(bool(torch.isfinite(t).all()) for t in got)
+            if v > 1:
+                assert all(bool((t == 0).all()) for t in got)
+
+
 def test_norm_rope_broadcast_inputs_and_one_output():
     """An expanded input gets the sum of its copies' gradients, an expanded weight a gradient per head; an output nobody used none."""
     from lvar_amd import kv_cache_ops as kv
