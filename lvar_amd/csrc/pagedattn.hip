@@ -331,6 +331,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
   constexpr int KS = D / 32;                  // steps of the contraction over the head dimension
   constexpr int CH = D < 128 ? 1 : D / 128;   // chunks of 128 (64) output columns
   constexpr int NE = D < 128 ? D / 16 : 8;    // columns of a chunk per lane and value row
+  constexpr bool TWO = D < 256 || F8;         // the exponentials as two bf16 terms
   constexpr int CW = 16 * NE;                 // columns of a chunk
   constexpr int LDO = CW + 4;
   __shared__ float so[PA_WAVES][16][LDO];
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
         for (int x = 0; x < KL; x++) ka[j][x] = kf[j][x];
       }
     }
-    u32x4 pf[NT];
+    u32x4 pf[NT], pl[TWO ? NT : 1];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       float s[8];
@@ -490,8 +491,16 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
             if (pg[j] < 0 || key + 16 * j + 4 * g + r >= limit[t]) s[4 * j + r] = -INFINITY;
       }
       softmax_step<8, CH * NE>(s, p.c, m[t], l[t], top[t], &o[t][0][0]);
-      // p is rounded to bf16 for the matrix instruction (its sum is not): 2^-9 per term, independent signs
+      // p goes into the matrix instruction as two bf16 terms, which leave 2^-17 of it out: the result is off by its own rounding only (rms 0.0017
+      // of it instead of 0.0023; a product more per value, 2 % of short calls).  256 columns of bf16 have no registers for the second: 2^-9 there.
       pf[t] = pack8u(s);
+      if constexpr (TWO) {
+        float back[8];
+        unpack8(pf[t], back);
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[e] -= back[e];
+        pl[t] = pack8u(s);
+      }
     }
     if (next < k_end) load_k(next, npg);
 
@@ -532,7 +541,10 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
         for (int x = 0; x < 4; x++)
           a[x] = __builtin_amdgcn_perm(row[2 * x + 1][e >> 1], row[2 * x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-        for (int t = 0; t < NT; t++) o[t][c][e] = mfma16(a, pf[t], o[t][c][e]);
+        for (int t = 0; t < NT; t++) {
+          o[t][c][e] = mfma16(a, pf[t], o[t][c][e]);
+          if constexpr (TWO) o[t][c][e] = mfma16(a, pl[t], o[t][c][e]);
+        }
       }
     }
     if (next < k_end) load_v(next, npg);
@@ -734,6 +746,8 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
           }
         }
         softmax_step<8, NB>(s, p.c, m[t], l[t], top[t], o[t]);
+        // (rounded to bf16, 2^-9 per term, independent signs, their sum is not: a second term would be half as many products again, and those
+        // are among the bounds here)
         pf[t] = pack8u(s);
       }
       u32x4 vx[2][4];
