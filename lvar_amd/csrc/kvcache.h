@@ -106,7 +106,7 @@ int launch_norm_rope_bwd(NormRopeParams p, int head_dim, hipStream_t s);
 int launch_weight_grad(const WeightGradParams& w, hipStream_t s);
 int launch_kv_read(const KvReadParams& p, int head_dim, hipStream_t s);
 int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim);
-int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s);
+int launch_paged_attn(PagedAttnParams p, void* workspace, int64_t workspace_bytes, int head_dim, hipStream_t s);
 
 template <int CTRL>
 __device__ __forceinline__ int dpp_mov(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }

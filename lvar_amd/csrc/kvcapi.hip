@@ -216,13 +216,7 @@ int lvar_paged_attn_fwd(lvar_tensor_t q, lvar_paged_cache_t cache, const int32_t
   p.lengths = lengths; p.counts = counts;
   p.B = B; p.H = H; p.Lq = Lq; p.G = H / cache.kv_heads; p.causal = causal ? 1 : 0; p.max_len = max_len;
   p.c = scale * kLog2e;
-  const int64_t need = paged_attn_ws_bytes(B, H, cache.kv_heads, Lq, max_len, cache.head_dim);
-  if (need < 0) return (int)need;
-  if (need > 0 && workspace && workspace_bytes >= need) {
-    if (!aligned(workspace, 16)) return LVAR_EINVAL;
-    p.ws = (float*)workspace;
-  }
-  return launch_paged_attn(p, cache.head_dim, (hipStream_t)stream);
+  return launch_paged_attn(p, workspace, workspace_bytes, cache.head_dim, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -883,12 +883,13 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedAttnParams p
 
 // ---- launch ----
 
-struct Shape { int nt, rw, rt, rows, whole, finer; bool staged; };
+struct Shape { int cus, nt, rw, rt, rows, whole, finer; bool staged; };
 
 // Rows per tile: 16 up to 16 rows of a key/value head, 32 up to 32 (each wave reads keys for itself), more with staged tiles: 64 up to
 // 64 rows, then 128 (head_dim 256: 64 from 17 rows on, its outputs take twice the registers).
 static Shape shape_of(int B, int H, int Hkv, int Lq, int head_dim) {
   Shape s;
+  s.cus = device_cus();
   const int64_t rows = (int64_t)(H / Hkv) * Lq;
   s.nt = rows <= 16 || head_dim == 256 ? 1 : 2;
   s.staged = rows > 16 * s.nt;
@@ -902,11 +903,11 @@ static Shape shape_of(int B, int H, int Hkv, int Lq, int head_dim) {
   // 256 22.2 / 17.8; of 1 row: head_dim 256 16.0 / 11.5), as measured with 1 / 16 to all of the compute units taken by uncut tiles: 128 tiles of
   // 1 row at 8 stages 14.7 / 18.2, of 64 rows at 6 stages 20.3 / 20.5.  With a longer tile all are cut: 16 x 8 ragged tiles of 1 row and up to 19
   // stages 16.1, with those of up to 6 whole 17.4, of up to 10 19.2 (head_dim 64).
-  const int cus = device_cus(), i = head_dim / 128;
+  const int cus = s.cus, i = head_dim / 128;
   const int64_t tiles = (int64_t)B * Hkv * s.rt;
   static constexpr int kLimit[2][3] = {{8, 4, 2}, {4, 3, 2}}, kMore[2][3] = {{8, 8, 4}, {6, 6, 8}};
   s.whole = kLimit[s.staged][i] + (cus > 0 ? (int)(kMore[s.staged][i] * (tiles < cus ? tiles : cus) / cus) : 0);
-  s.finer = device_cus() * (s.staged ? 4 : 6);
+  s.finer = cus * (s.staged ? 4 : 6);
   return s;
 }
 
@@ -925,13 +926,15 @@ static int64_t ws_head_floats(int B) { return ((int64_t)2 * B + 63) / 64 * 64; }
 
 // Partial results are kept for tiles that are cut only; such a tile has n < 2 * stages / share pieces, and a share is at least the
 // `finer`-th part of all stages, so that there are fewer than 2 * finer of them in all; nor are there more than stages.
-int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim) {
-  const Shape s = shape_of(B, H, Hkv, Lq, head_dim);
+static int64_t ws_bytes_of(const Shape& s, int B, int Hkv, int max_len, int head_dim) {
   if (s.finer <= 0) return LVAR_ELAUNCH;
   const int64_t stages = ((int64_t)max_len + PA_STAGE - 1) / PA_STAGE;
   if (stages <= s.whole) return 0;   // nothing can be cut
   const int64_t most = (int64_t)B * Hkv * s.rt * stages, slots = most < 2ll * s.finer ? most : 2ll * s.finer;
   return 4 * (ws_head_floats(B) + slots * s.rows * (head_dim + 2));
+}
+int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim) {
+  return ws_bytes_of(shape_of(B, H, Hkv, Lq, head_dim), B, Hkv, max_len, head_dim);
 }
 
 template <int D, int NT, int W>
@@ -975,21 +978,26 @@ static int launch_d(const PagedAttnParams& p, const Shape& h, hipStream_t s) {
   if (p.ws) {
     // few rows: all groups along the pieces of one row; many: a group per row
     constexpr int GR = 512 / (D / 4);
-    if ((int64_t)p.G * p.Lq * p.cache.kv_heads * p.B <= 4 * device_cus()) launch_join<D, 1>(p, s);
+    if ((int64_t)p.G * p.Lq * p.cache.kv_heads * p.B <= 4 * h.cus) launch_join<D, 1>(p, s);
     else launch_join<D, GR>(p, s);
     if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
   }
   return LVAR_OK;
 }
 
-int launch_paged_attn(PagedAttnParams p, int head_dim, hipStream_t s) {
+int launch_paged_attn(PagedAttnParams p, void* workspace, int64_t workspace_bytes, int head_dim, hipStream_t s) {
   const Shape h = shape_of(p.B, p.H, p.cache.kv_heads, p.Lq, head_dim);
-  if (h.finer <= 0) return LVAR_ELAUNCH;
+  const int64_t need = ws_bytes_of(h, p.B, p.cache.kv_heads, p.max_len, head_dim);
+  if (need < 0) return (int)need;
+  if (need > 0 && workspace && workspace_bytes >= need) {
+    if (((uintptr_t)workspace & 15) != 0) return LVAR_EINVAL;
+    p.ws = (float*)workspace;
+  }
   p.rt = h.rt;
   p.tile_rows = 16 * h.nt * h.rw;
   // Ragged lengths: two workgroups per compute unit from 4 stages on (tiles of 32 rows and head_dim 128, 16: 8 x 8 tiles of up to 4096 keys 23.7
   // against 25.0 us, 32 x 8 of up to 8000 125 against 116), with head_dim 64 three, which fit, from 16 on (the latter in e4m3, 46 -> 38).
-  const int cus = device_cus(), per = per_cu(h, head_dim, p.cache.k_exp != nullptr);
+  const int cus = h.cus, per = per_cu(h, head_dim, p.cache.k_exp != nullptr);
   p.target = per * cus;
   p.wide = (per > 2 ? per : 2) * cus;
   p.wider = !h.staged && head_dim == 64 ? 3 * cus : p.wide;

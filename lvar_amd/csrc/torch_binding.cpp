@@ -524,9 +524,11 @@ bool same_strides(const at::Tensor& a, const at::Tensor& b, int64_t dims) {
   return true;
 }
 
-// a[0..4]: k, v, k_exp, v_exp, page table (the entry points check alignments and limits)
-bool cache_ok(PyObject* const* a, int64_t B, int dev, lvar_paged_cache_t& c) {
-  const at::Tensor *k = tensor(a[0]), *v = tensor(a[1]), *table = tensor(a[4]), *ke, *ve;
+// cache: the tuple (k, v, k_exp, v_exp) (the entry points check alignments and limits)
+bool cache_ok(PyObject* cache, PyObject* page_table, int64_t B, int dev, lvar_paged_cache_t& c) {
+  if (!PyTuple_Check(cache) || PyTuple_GET_SIZE(cache) != 4) return false;
+  PyObject* const a[4] = {PyTuple_GET_ITEM(cache, 0), PyTuple_GET_ITEM(cache, 1), PyTuple_GET_ITEM(cache, 2), PyTuple_GET_ITEM(cache, 3)};
+  const at::Tensor *k = tensor(a[0]), *v = tensor(a[1]), *table = tensor(page_table), *ke, *ve;
   if (!k || !v || !table || !optional_tensor(a[2], ke) || !optional_tensor(a[3], ve)) return false;
   const bool f8 = k->scalar_type() == at::kFloat8_e4m3fn;
   if ((!f8 && k->scalar_type() != at::kBFloat16) || v->scalar_type() != k->scalar_type() || k->dim() != 4 || v->dim() != 4) return false;
@@ -717,20 +719,20 @@ LVAR_FAST(fast_qk_norm_rope) {
   END_HANDLE_TH_ERRORS
 }
 
-// (cache k, v, k_exp, v_exp, page table, start, counts, q | None, k, v[, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved]) -> q, or True
+// (cache, page table, start, counts, q | None, k, v[, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved]) -> q, or True
 LVAR_FAST(fast_kv_append) {
   HANDLE_TH_ERRORS
-  LVAR_NEED(n == 10 || n == 18);
-  const bool fused = n == 18;
-  const at::Tensor *q = fused ? tensor(a[7]) : tensor(a[8]), *k = tensor(a[8]), *v = tensor(a[9]), *start = tensor(a[5]), *counts, *wq = nullptr, *wk = nullptr;
+  LVAR_NEED(n == 7 || n == 15);
+  const bool fused = n == 15;
+  const at::Tensor *q = fused ? tensor(a[4]) : tensor(a[5]), *k = tensor(a[5]), *v = tensor(a[6]), *start = tensor(a[2]), *counts, *wq = nullptr, *wk = nullptr;
   int dev;
   void* stream;
-  LVAR_NEED(qk_ok(q, k, dev, stream) && rows_ok(v, dev) && v->sizes() == k->sizes() && start && optional_tensor(a[6], counts));
+  LVAR_NEED(qk_ok(q, k, dev, stream) && rows_ok(v, dev) && v->sizes() == k->sizes() && start && optional_tensor(a[3], counts));
   const int64_t B = k->size(0);
   lvar_paged_cache_t c;
-  LVAR_NEED(per_sequence(start, B, dev) && per_sequence(counts, B, dev) && cache_ok(a, B, dev, c) && c.kv_heads == k->size(1) && c.head_dim == k->size(3));
+  LVAR_NEED(per_sequence(start, B, dev) && per_sequence(counts, B, dev) && cache_ok(a[0], a[1], B, dev, c) && c.kv_heads == k->size(1) && c.head_dim == k->size(3));
   How w;
-  if (fused) LVAR_NEED(how_ok(a + 10, *q, *k, dev, false, w, wq, wk));
+  if (fused) LVAR_NEED(how_ok(a + 7, *q, *k, dev, false, w, wq, wk));
   LVAR_NEED(!wants_grad(q) && !wants_grad(k) && !wants_grad(v) && !wants_grad(wq) && !wants_grad(wk));
   at::Tensor oq;
   if (fused) oq = empty(q->sizes(), at::kBFloat16, dev);
@@ -750,18 +752,18 @@ bool as_bound(PyObject* o, const lvar_paged_cache_t& c, bool clamp, int64_t& v) 
   return v >= 0 && v <= INT32_MAX;
 }
 
-// (cache k, v, k_exp, v_exp, page table, lengths, max_len, start) -> (k, v)
+// (cache, page table, lengths, max_len, start) -> (k, v)
 LVAR_FAST(fast_kv_read) {
   HANDLE_TH_ERRORS
-  const at::Tensor *k = n == 8 ? tensor(a[0]) : nullptr, *table = n == 8 ? tensor(a[4]) : nullptr, *start;
-  LVAR_NEED(bound && k && table && k->is_cuda() && table->dim() == 2 && optional_tensor(a[7], start));
+  const at::Tensor *k = n == 5 && PyTuple_Check(a[0]) && PyTuple_GET_SIZE(a[0]) == 4 ? tensor(PyTuple_GET_ITEM(a[0], 0)) : nullptr, *table = n == 5 ? tensor(a[1]) : nullptr, *start;
+  LVAR_NEED(bound && k && table && k->is_cuda() && table->dim() == 2 && optional_tensor(a[4], start));
   const int dev = k->get_device();
   const int64_t B = table->size(0);
-  const at::Tensor* lengths = tensor(a[5]);
+  const at::Tensor* lengths = tensor(a[2]);
   lvar_paged_cache_t c;
   int64_t most;
-  LVAR_NEED(lengths && c10::hip::current_device() == dev && cache_ok(a, B, dev, c) && per_sequence(lengths, B, dev) && per_sequence(start, B, dev) &&
-            as_bound(a[6], c, false, most) && most > 0 && B > 0 && B <= 65535);
+  LVAR_NEED(lengths && c10::hip::current_device() == dev && cache_ok(a[0], a[1], B, dev, c) && per_sequence(lengths, B, dev) && per_sequence(start, B, dev) &&
+            as_bound(a[3], c, false, most) && most > 0 && B > 0 && B <= 65535);
   at::Tensor ko = empty({B, c.kv_heads, most, c.head_dim}, at::kBFloat16, dev), vo = empty({B, c.kv_heads, most, c.head_dim}, at::kBFloat16, dev);
   LVAR_NEED(api.lvar_kv_cache_read(c, ints(start), ints(lengths), ko.data_ptr(), vo.data_ptr(), static_cast<int>(B), static_cast<int>(most),
                                    c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream()) == LVAR_OK);
@@ -769,23 +771,23 @@ LVAR_FAST(fast_kv_read) {
   END_HANDLE_TH_ERRORS
 }
 
-// (q, cache k, v, k_exp, v_exp, page table, lengths, counts, scale, causal, max_len) -> (o, M, L)
+// (q, cache, page table, lengths, counts, scale, causal, max_len) -> (o, M, L)
 LVAR_FAST(fast_paged_attn) {
   HANDLE_TH_ERRORS
-  const at::Tensor *q = n == 11 ? tensor(a[0]) : nullptr, *counts;
+  const at::Tensor *q = n == 8 ? tensor(a[0]) : nullptr, *counts;
   LVAR_NEED(bound && q && q->is_cuda());
   Qkv x{};
   x.dev = q->get_device();
-  LVAR_NEED(rows_ok(q, x.dev) && q->numel() > 0 && c10::hip::current_device() == x.dev && !wants_grad(q) && optional_tensor(a[7], counts));
+  LVAR_NEED(rows_ok(q, x.dev) && q->numel() > 0 && c10::hip::current_device() == x.dev && !wants_grad(q) && optional_tensor(a[4], counts));
   for (int i = 0; i < 3; i++) LVAR_NEED(q->size(i) <= INT32_MAX);
   x.B = dim(*q, 0); x.H = dim(*q, 1); x.Lq = dim(*q, 2); x.d = dim(*q, 3);
-  const at::Tensor* lengths = tensor(a[6]);
+  const at::Tensor* lengths = tensor(a[3]);
   lvar_paged_cache_t c;
   float scale;
   bool causal;
   int64_t most;
-  LVAR_NEED(lengths && cache_ok(a + 1, x.B, x.dev, c) && c.head_dim == x.d && x.H % c.kv_heads == 0 && per_sequence(lengths, x.B, x.dev) &&
-            per_sequence(counts, x.B, x.dev) && as_scale(a[8], x.d, scale) && as_bool(a[9], causal) && as_bound(a[10], c, true, most));
+  LVAR_NEED(lengths && cache_ok(a[1], a[2], x.B, x.dev, c) && c.head_dim == x.d && x.H % c.kv_heads == 0 && per_sequence(lengths, x.B, x.dev) &&
+            per_sequence(counts, x.B, x.dev) && as_scale(a[5], x.d, scale) && as_bool(a[6], causal) && as_bound(a[7], c, true, most));
   const int64_t bytes = api.lvar_paged_attn_workspace_bytes(x.B, x.H, c.kv_heads, x.Lq, static_cast<int>(most), x.d);
   LVAR_NEED(bytes >= 0);
   at::Tensor o = empty_o(x), M, L, ws;

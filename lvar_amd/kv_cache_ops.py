@@ -299,7 +299,7 @@ def kv_cache_append(cache: PagedKVCache, k, v, page_table, start, counts=None) -
     head, the smallest power of two with ``max|x| <= 448 * 2^e`` and codes rounded to nearest even; infinities become NaN there.
     Positions outside the page table are dropped.  Two tokens of one call that go to the same row leave it undefined."""
     fast = _native()
-    if fast is not None and fast.fast_kv_append(cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, start, counts, None, k, v):
+    if fast is not None and fast.fast_kv_append(cache, page_table, start, counts, None, k, v):
         return
     _no_gradient("kv_cache_append", k, v)
     k, v = _prep(k, "k"), _prep(v, "v")
@@ -315,7 +315,7 @@ def qk_norm_rope_append(cache: PagedKVCache, q, k, v, page_table, start, cos=Non
     the cache's type."""
     fast = _native()
     if fast is not None:
-        r = fast.fast_kv_append(cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, start, counts, q, k, v, cos, sin, positions, q_weight, k_weight,
+        r = fast.fast_kv_append(cache, page_table, start, counts, q, k, v, cos, sin, positions, q_weight, k_weight,
                                 norm, eps, interleaved)
         if r is not None:
             return r
@@ -337,7 +337,7 @@ def kv_cache_read(cache: PagedKVCache, page_table, lengths, max_len: Optional[in
     table can name.  Exact: every cached value is a bf16 value."""
     fast = _native()
     if fast is not None:
-        r = fast.fast_kv_read(cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, lengths, max_len, start)
+        r = fast.fast_kv_read(cache, page_table, lengths, max_len, start)
         if r is not None:
             return r
     device = cache.k.device
@@ -366,7 +366,7 @@ def paged_attn(q, cache: PagedKVCache, page_table, lengths, scale=None, causal: 
     can name): a small bound lets the launch do without the pass that joins the parts of long sequences."""
     fast = _native()
     if fast is not None:
-        r = fast.fast_paged_attn(q, cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, lengths, counts, _plain_scale(scale), causal, max_len)
+        r = fast.fast_paged_attn(q, cache, page_table, lengths, counts, _plain_scale(scale), causal, max_len)
         if r is not None:
             return r[0], (r[1], r[2])
     _no_gradient("paged_attn", q)
