@@ -780,6 +780,33 @@ def test_two_appends_and_reads_on_two_streams():
     assert all(torch.equal(a, b) for a, b in zip(*got))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_cache_views_and_shared_pages(dtype):
+    """Keys and values as views of one buffer [pages, 2, heads, page, d]; two sequences whose first pages are the same, one page named twice in a row."""
+    from lvar_amd import kv_cache_ops as kv
+    P, H, page, d, n = 9, 3, 16, 64, 40
+    raw = torch.zeros(P, 2, H, page, d, dtype=torch.bfloat16 if dtype is torch.bfloat16 else torch.uint8, device="cuda")
+    exps = torch.full((P, 2, H, page), 127, dtype=torch.uint8, device="cuda")
+    buf = raw if dtype is torch.bfloat16 else raw.view(dtype)
+    cache = kv.PagedKVCache(buf[:, 0], buf[:, 1], *(() if dtype is torch.bfloat16 else (exps[:, 0], exps[:, 1])))
+    plain = kv.PagedKVCache.alloc(P, H, d, page, dtype)
+    x = [rand(1, H, n, d, seed=i).cuda() for i in range(2)]
+    first = torch.tensor([[4, 2, 7]], dtype=torch.int32, device="cuda")
+    start = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for c in (cache, plain):
+        kv.kv_cache_append(c, *x, first, start)
+    assert all(torch.equal(a.contiguous().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, plain) if a is not None)
+    table = torch.tensor([[4, 2, 7], [4, 2, 2]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([40, 48], dtype=torch.int32, device="cuda")
+    for Lq in (1, 40):
+        q = rand(2, 2 * H, Lq, d, seed=9).cuda()
+        got, want = (kv.paged_attn(q, c, table, lens, causal=True) for c in (cache, plain))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1][0], want[1][0]) and torch.equal(got[1][1], want[1][1])
+        k, v = (t.double().cpu() for t in kv.kv_cache_read(cache, table, lens))
+        assert torch.equal(k[0, :, :32], k[1, :, :32]) and torch.equal(k[1, :, 16:32], k[1, :, 32:])
+        check_attn(*[t for t in (got[0], *got[1])], *ref.paged_attn(q.cpu(), k, v, torch.arange(48)[None] < lens.cpu()[:, None], lens.cpu(), d ** -0.5, True), q.cpu(), k, d ** -0.5, 48)
+
+
 def test_large_forms_of_the_norm():
     """Calls large enough for four heads per workgroup, in both pair orders, with heads that do not fill the last chunk."""
     from lvar_amd import kv_cache_ops as kv
