@@ -11,7 +11,7 @@
 //     of a lane are regrouped by byte permutes into pairs of keys, and output columns come out as runs of 32 per lane.  No
 //     LDS and no barrier in the key loop: a wave waits for nothing but its own loads, the loads of its next 32 keys are in flight
 //     while it computes, and the four waves take turns at 32 keys.  32 sequences of up to 32768 tokens, 32 query heads over 8 of
-//     128: 2.2 GB of bf16 in 390 us (5.7 TB/s; a copy moves 5.2); 131071 tokens in e4m3: 0.27 GB in 55 us.
+//     128: 2.2 GB of bf16 in 395 us (5.6 TB/s; a copy moves 5.2); 131071 tokens in e4m3: 0.27 GB in 55 us.
 //   paged_tile_kernel   more rows: keys and values staged in LDS, where the waves share them.  4 x 256 rows of 16 heads over 2521
 //     tokens: 44 .. 46 us, 460 .. 480 TFLOP/s.  (With 64 rows per wave and no LDS there is one wave per SIMD and nobody left to
 //     compute while it waits: 105 us where this takes 38, 8 sequences of up to 4001 tokens with up to 61 new ones.)
