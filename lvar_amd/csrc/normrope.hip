@@ -246,8 +246,13 @@ static bool launch_fwd(const NormRopeParams& p, bool append, hipStream_t s) {
   constexpr int RPB = NR_T / (D / 8);
   const int64_t groups = (int64_t)chunks_of<HC>(p, append) * ((p.B * p.L + RPB - 1) / RPB);
   if (!grid_fits(groups, NR_T)) return false;
-  if (append) hipLaunchKernelGGL((norm_rope_kernel<D, HC, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
-  else hipLaunchKernelGGL((norm_rope_kernel<D, HC, false>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+  if constexpr (D >= 64) {   // (head dimensions of a cache)
+    if (append) {
+      hipLaunchKernelGGL((norm_rope_kernel<D, HC, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+      return true;
+    }
+  }
+  hipLaunchKernelGGL((norm_rope_kernel<D, HC, false>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
   return true;
 }
 
