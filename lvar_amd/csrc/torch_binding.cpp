@@ -513,6 +513,9 @@ bool optional_tensor(PyObject* o, const at::Tensor*& t) {
 }
 
 bool wants_grad(const at::Tensor* t) { return t && t->requires_grad() && at::GradMode::is_enabled(); }
+// a forward-mode derivative, which no operator here has (the Python path raises)
+bool has_tangent(const at::Tensor* t) { return t && t->_fw_grad(0).defined(); }
+bool wants_derivative(const at::Tensor* t) { return wants_grad(t) || has_tangent(t); }
 
 // int32 [B] on the device, or nothing
 bool per_sequence(const at::Tensor* t, int64_t B, int dev) { return !t || (packed(t, dev, at::kInt) && t->dim() == 1 && t->size(0) == B); }
@@ -592,7 +595,9 @@ bool how_ok(PyObject* const* a, const at::Tensor& q, const at::Tensor& k, int de
   if (!w.cos != !w.sin) return false;
   if (w.cos) {
     for (const at::Tensor* t : {w.cos, w.sin})
-      if (!t->is_cuda() || t->get_device() != dev || t->scalar_type() != at::kFloat || t->dim() != 2 || t->stride(1) != 1 || t->requires_grad()) return false;
+      if (!t->is_cuda() || t->get_device() != dev || t->scalar_type() != at::kFloat || t->dim() != 2 || t->stride(1) != 1 || t->requires_grad() ||
+          has_tangent(t))
+        return false;
     if (w.cos->sizes() != w.sin->sizes() || w.cos->stride(0) != w.sin->stride(0) || w.cos->size(0) <= 0 || w.cos->size(0) > INT32_MAX || 2 * w.cos->size(1) > d) return false;
     if (needs_rows && !w.positions && w.cos->size(0) < L) return false;
     w.h.cos = w.cos->data_ptr<float>(); w.h.sin = w.sin->data_ptr<float>(); w.h.table_stride = w.cos->stride(0);
@@ -652,6 +657,7 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope can be differentiated once: its gradients have no graph (create_graph)");
+    TORCH_CHECK(!has_tangent(&grads[0]) && !has_tangent(&grads[1]), "the gradient of qk_norm_rope has no forward-mode derivative: call it on tensors without a tangent");
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3], &cos = saved[4], &sin = saved[5], &positions = saved[6];
     lvar_norm_rope_t h;
@@ -701,6 +707,7 @@ LVAR_FAST(fast_qk_norm_rope) {
   void* stream;
   How w;
   LVAR_NEED(qk_ok(q, k, dev, stream) && how_ok(a + 2, *q, *k, dev, true, w, wq, wk));
+  LVAR_NEED(!has_tangent(q) && !has_tangent(k) && !has_tangent(wq) && !has_tangent(wk));
   at::Tensor oq, ok;
   if (wants_grad(q) || wants_grad(k) || wants_grad(wq) || wants_grad(wk)) {
     // (declined before a graph is built: what the entry point would refuse raises in the Python path)
@@ -733,7 +740,7 @@ LVAR_FAST(fast_kv_append) {
   LVAR_NEED(per_sequence(start, B, dev) && per_sequence(counts, B, dev) && cache_ok(a[0], a[1], B, dev, c) && c.kv_heads == k->size(1) && c.head_dim == k->size(3));
   How w;
   if (fused) LVAR_NEED(how_ok(a + 7, *q, *k, dev, false, w, wq, wk));
-  LVAR_NEED(!wants_grad(q) && !wants_grad(k) && !wants_grad(v) && !wants_grad(wq) && !wants_grad(wk));
+  LVAR_NEED(!wants_derivative(q) && !wants_derivative(k) && !wants_derivative(v) && !wants_derivative(wq) && !wants_derivative(wk));
   at::Tensor oq;
   if (fused) oq = empty(q->sizes(), at::kBFloat16, dev);
   LVAR_NEED(api.lvar_kv_cache_append(view(*q), view(*k), view(*v), fused ? &w.h : nullptr, fused ? oq.data_ptr() : nullptr, c, ints(start), ints(counts),
@@ -778,7 +785,7 @@ LVAR_FAST(fast_paged_attn) {
   LVAR_NEED(bound && q && q->is_cuda());
   Qkv x{};
   x.dev = q->get_device();
-  LVAR_NEED(rows_ok(q, x.dev) && q->numel() > 0 && c10::hip::current_device() == x.dev && !wants_grad(q) && optional_tensor(a[4], counts));
+  LVAR_NEED(rows_ok(q, x.dev) && q->numel() > 0 && c10::hip::current_device() == x.dev && !wants_derivative(q) && optional_tensor(a[4], counts));
   for (int i = 0; i < 3; i++) LVAR_NEED(q->size(i) <= INT32_MAX);
   x.B = dim(*q, 0); x.H = dim(*q, 1); x.Lq = dim(*q, 2); x.d = dim(*q, 3);
   const at::Tensor* lengths = tensor(a[3]);

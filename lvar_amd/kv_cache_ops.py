@@ -16,6 +16,7 @@ import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .sparse_attn_ops import ShapeError, _native, _on_device, _plain_scale, _prep, _ptr, _require, _scale, _stream, _view
@@ -177,7 +178,13 @@ def _norm_args(q, k, cos, sin, positions, norm, eps):
     return cos, sin, eps
 
 
+def _no_tangent(name: str, *tensors) -> None:
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative: call it on tensors without a tangent")
+
+
 def _no_gradient(name: str, *tensors) -> None:
+    _no_tangent(name, *tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
@@ -215,6 +222,7 @@ class _NormRope(torch.autograd.Function):
     def backward(ctx, gq, gk):
         if torch.is_grad_enabled():
             raise RuntimeError("qk_norm_rope can be differentiated once: its gradients have no graph (create_graph)")
+        _no_tangent("the gradient of qk_norm_rope", gq, gk)
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         norm, eps, interleaved = ctx.how
         B, H, L, d = q.shape
@@ -252,14 +260,16 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
     ``q_weight`` / ``k_weight`` (fp32 or bf16; ``[d]``, ``[H,1]``, ``[1,d]`` or ``[H,d]``) multiply the result.  ``cos`` / ``sin``
     fp32 ``[rows, rot/2]`` rotate the first ``rot`` columns (a multiple of 16) in pairs ``(2i, 2i+1)``, or ``(i, i + rot/2)``
     with ``interleaved=False``; token i takes row i, or row ``positions[i]`` / ``positions[b,i]`` (clamped to the table).
-    ``head_dim`` 16, 32, 64, 128 or 256.  All in fp32, rounded once.  Differentiable in q, k and the weights (once); a backward pass that
-    is captured in a graph wants leaves without a live eager graph, as always with autograd.  The
+    ``head_dim`` 16, 32, 64, 128 or 256.  All in fp32, rounded once.  Differentiable in q, k and the weights (once, in
+    reverse mode: inputs with a forward-mode tangent are refused); a backward pass that is captured in a graph wants leaves without a live eager
+    graph, as always with autograd.  The
     reference's counterpart is models/sparvar/basic_sparvar.py:326-342, eager."""
     fast = _native()
     if fast is not None:
         r = fast.fast_qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved)
         if r is not None:
             return r
+    _no_tangent("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
     q, k = _prep(q, "q"), _prep(k, "k")
     cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
     _require(q.shape[3] in (16, 32, 64, 128, 256), lambda: f"head_dim must be 16, 32, 64, 128 or 256, got {q.shape[3]}")
@@ -320,6 +330,7 @@ def qk_norm_rope_append(cache: PagedKVCache, q, k, v, page_table, start, cos=Non
         if r is not None:
             return r
     _no_gradient("qk_norm_rope_append", q, k, v, q_weight, k_weight)
+    _no_tangent("qk_norm_rope_append", cos, sin)
     q, k, v = _prep(q, "q"), _prep(k, "k"), _prep(v, "v")
     cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
     start, counts = _append_args(cache, k, v, page_table, start, counts)

@@ -925,3 +925,44 @@ def test_refusals_on_the_device(binding, monkeypatch):
     many.kv_heads = 16384
     assert _lib.load().lvar_paged_attn_fwd(kv._view(x), many, i.data_ptr(), None, x.data_ptr(), x.data_ptr(), x.data_ptr(), None, 0, 4096, 16384, 1, 100, 0, 1.0, kv._stream(x)) == -1
     torch.cuda.synchronize()
+
+
+# ---- derivatives, versions and values that are not there ----
+
+def small_call(dtype=torch.bfloat16):
+    """q, k, v, cache, table, start, lengths of a small step on the device"""
+    from lvar_amd import kv_cache_ops as kv
+    q, k, v = (t.cuda() for t in projection(2, 4, 2, 3, 64, seed=1))
+    cache = kv.PagedKVCache.alloc(4, 2, 64, 16, dtype)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda")
+    return q, k, v, cache, table, torch.zeros(2, dtype=torch.int32, device="cuda"), torch.full((2,), 3, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("binding", [True, False])
+def test_tangents_are_refused(binding, monkeypatch):
+    """Tensors with a forward-mode tangent: no operator may hand back outputs that have lost it."""
+    import torch.autograd.forward_ad as fw
+    from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
+    q, k, v, cache, table, start, lens = small_call()
+    w, (cos, sin) = torch.ones(64, device="cuda"), (t.cuda() for t in tables(3, 32))
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for f in (lambda: kv.qk_norm_rope(dual(q), k), lambda: kv.qk_norm_rope(q, dual(k)), lambda: kv.qk_norm_rope(q, k, q_weight=dual(w)),
+                  lambda: kv.qk_norm_rope(q, k, k_weight=dual(w)), lambda: kv.qk_norm_rope(q, k, dual(cos), sin), lambda: kv.qk_norm_rope(q, k, cos, dual(sin)),
+                  lambda: kv.qk_norm_rope(dual(q).transpose(0, 1), k.transpose(0, 1)),
+                  lambda: kv.kv_cache_append(cache, dual(k), v, table, start), lambda: kv.kv_cache_append(cache, k, dual(v), table, start),
+                  lambda: kv.qk_norm_rope_append(cache, dual(q), k, v, table, start), lambda: kv.qk_norm_rope_append(cache, q, k, v, table, start, k_weight=dual(w)),
+                  lambda: kv.qk_norm_rope_append(cache, q, k, v, table, start, cos, dual(sin)), lambda: kv.paged_attn(dual(q), cache, table, lens)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    f()
+        leaf = q.detach().clone().requires_grad_()
+        o, _ = kv.qk_norm_rope(leaf, k)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(o, leaf, dual(torch.ones_like(o)))
+        # plain tensors are taken as ever
+        assert torch.equal(kv.qk_norm_rope(leaf, k)[0], kv.qk_norm_rope(q, k)[0])
+        kv.kv_cache_append(cache, k, v, table, start)
+    assert torch.equal(kv.kv_cache_read(cache, table, lens, 3)[0], k)

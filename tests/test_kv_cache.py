@@ -178,3 +178,19 @@ def _fill(s, **kw):
     for n, v in kw.items():
         setattr(s, n, v)
     return s
+
+
+def test_operators_refuse_tangents():
+    """Ahead of everything else, so that it shows without a device too."""
+    import torch.autograd.forward_ad as fw
+    from lvar_amd import kv_cache_ops as kv
+    x, w = torch.zeros(1, 2, 3, 64, dtype=torch.bfloat16), torch.ones(64)
+    i, table, c = torch.zeros(1, dtype=torch.int32), torch.zeros(1, 4, dtype=torch.int32), _cache()
+    cos = torch.ones(3, 32)
+    with fw.dual_level():
+        y, wy, cy = (fw.make_dual(t, torch.ones_like(t)) for t in (x, w, cos))
+        for call in (lambda: kv.qk_norm_rope(y, x), lambda: kv.qk_norm_rope(x, y), lambda: kv.qk_norm_rope(x, x, k_weight=wy), lambda: kv.qk_norm_rope(x, x, cy, cos),
+                     lambda: kv.kv_cache_append(c, x, y, table, i), lambda: kv.qk_norm_rope_append(c, y, x, x, table, i),
+                     lambda: kv.qk_norm_rope_append(c, x, x, x, table, i, cos, cy), lambda: kv.paged_attn(y, c, table, i)):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
