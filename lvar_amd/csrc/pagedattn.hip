@@ -222,11 +222,12 @@ template <int D>
 __device__ __forceinline__ void write_padding(const PagedAttnParams& p, const Piece& w) {
   if (w.rt == p.rt || w.piece > 0 || w.tile != w.rt - 1) return;
   const int rows = p.G * p.Lq;
-  for (int x = w.rt * p.tile_rows * (D / 8) + threadIdx.x; x < rows * (D / 8); x += PA_T) {
-    const int r = x / (D / 8), i = r / p.G;
+  const int col = threadIdx.x % (D / 8) * 8;
+  for (int r = w.rt * p.tile_rows + threadIdx.x / (D / 8); r < rows; r += PA_T / (D / 8)) {   // (rows: their 16-byte pieces may be more than 31 bits)
+    const int i = r / p.G;
     const int64_t out = ((int64_t)w.b * p.H + w.head * p.G + (r - i * p.G)) * p.Lq + i;
-    *(u32x4*)(p.o + out * D + x % (D / 8) * 8) = u32x4{0u, 0u, 0u, 0u};
-    if (x % (D / 8) == 0) { p.M[out] = -INFINITY; p.L[out] = 1.f; }
+    *(u32x4*)(p.o + out * D + col) = u32x4{0u, 0u, 0u, 0u};
+    if (col == 0) { p.M[out] = -INFINITY; p.L[out] = 1.f; }
   }
 }
 

@@ -966,3 +966,31 @@ def test_tangents_are_refused(binding, monkeypatch):
         assert torch.equal(kv.qk_norm_rope(leaf, k)[0], kv.qk_norm_rope(q, k)[0])
         kv.kv_cache_append(cache, k, v, table, start)
     assert torch.equal(kv.kv_cache_read(cache, table, lens, 3)[0], k)
+
+
+@pytest.mark.parametrize("Lq,H", [((1 << 26) + 37, 1), ((1 << 25) + 1, 2)])
+def test_padding_of_more_than_31_bits_of_pieces(Lq, H):
+    """2^26 rows of head_dim 256 behind one new token: 2^31 pieces of 16 bytes, all of them written."""
+    from lvar_amd import _lib, kv_cache_ops as kv
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 36 GB")
+    d = 256
+    cache = kv.PagedKVCache.alloc(4, 1, d, 16)
+    x = [rand(1, 1, 40, d, seed=i).cuda() for i in range(2)]
+    table, zero = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4), torch.zeros(1, dtype=torch.int32, device="cuda")
+    kv.kv_cache_append(cache, *x, table, zero)
+    lens, counts = zero + 40, zero + 1
+    q = rand(1, 1, 1, d, seed=5).cuda()
+    o, M, L = torch.full((H * Lq, d), 7.0, dtype=torch.bfloat16, device="cuda"), torch.full((H * Lq,), 7.0, device="cuda"), torch.full((H * Lq,), 7.0, device="cuda")
+    rows = _lib.LvarTensor(q.data_ptr(), 0, 0, 0)           # (every query is the same row)
+    assert _lib.load().lvar_paged_attn_fwd(rows, kv._cache_arg(cache, table, 1, q.device), lens.data_ptr(), counts.data_ptr(), o.data_ptr(), M.data_ptr(), L.data_ptr(), None, 0,
+                                           1, H, Lq, 64, 1, d ** -0.5, kv._stream(q)) == 0
+    one, (M1, L1) = kv.paged_attn(q, cache, table, lens)
+    o, M, L = o.view(H, Lq, d), M.view(H, Lq), L.view(H, Lq)
+    for h in range(H):
+        # both are rounded, and the call of many rows rounds its probabilities
+        assert float((o[h, 0].float() - one[0, 0, 0].float()).abs().max()) <= 3 * BF16 * float(x[1].abs().max()) and float((M[h, 0] - M1.view(())).abs()) <= 2 * (d + 8) * F32 * float(M1.abs().max() + 10)
+        assert all(bool((c == 0).all()) for c in o[h, 1:].split(1 << 22))
+        assert bool((M[h, 1:] == -math.inf).all()) and bool((L[h, 1:] == 1).all())
+    del o, M, L
+    torch.cuda.empty_cache()
