@@ -535,6 +535,7 @@ bool cache_ok(PyObject* cache, PyObject* page_table, int64_t B, int dev, lvar_pa
   if (!k || !v || !table || !optional_tensor(a[2], ke) || !optional_tensor(a[3], ve)) return false;
   const bool f8 = k->scalar_type() == at::kFloat8_e4m3fn;
   if ((!f8 && k->scalar_type() != at::kBFloat16) || v->scalar_type() != k->scalar_type() || k->dim() != 4 || v->dim() != 4) return false;
+  if (wants_derivative(k) || wants_derivative(v)) return false;
   if (!k->is_cuda() || k->get_device() != dev || !v->is_cuda() || v->get_device() != dev || !same_strides(*k, *v, 4)) return false;
   if (k->stride(3) != 1 || v->stride(3) != 1 || k->numel() == 0) return false;
   for (int i = 0; i < 4; i++) if (k->size(i) > INT32_MAX) return false;

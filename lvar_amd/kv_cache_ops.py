@@ -311,7 +311,7 @@ def kv_cache_append(cache: PagedKVCache, k, v, page_table, start, counts=None) -
     fast = _native()
     if fast is not None and fast.fast_kv_append(cache, page_table, start, counts, None, k, v):
         return
-    _no_gradient("kv_cache_append", k, v)
+    _no_gradient("kv_cache_append", k, v, cache.k, cache.v)
     k, v = _prep(k, "k"), _prep(v, "v")
     start, counts = _append_args(cache, k, v, page_table, start, counts)
     if k.numel():
@@ -329,7 +329,7 @@ def qk_norm_rope_append(cache: PagedKVCache, q, k, v, page_table, start, cos=Non
                                 norm, eps, interleaved)
         if r is not None:
             return r
-    _no_gradient("qk_norm_rope_append", q, k, v, q_weight, k_weight)
+    _no_gradient("qk_norm_rope_append", q, k, v, q_weight, k_weight, cache.k, cache.v)
     _no_tangent("qk_norm_rope_append", cos, sin)
     q, k, v = _prep(q, "q"), _prep(k, "k"), _prep(v, "v")
     cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
@@ -351,6 +351,7 @@ def kv_cache_read(cache: PagedKVCache, page_table, lengths, max_len: Optional[in
         r = fast.fast_kv_read(cache, page_table, lengths, max_len, start)
         if r is not None:
             return r
+    _no_gradient("kv_cache_read", cache.k, cache.v)
     device = cache.k.device
     B = page_table.shape[0]
     arg = _cache_arg(cache, page_table, B, device)
@@ -380,7 +381,7 @@ def paged_attn(q, cache: PagedKVCache, page_table, lengths, scale=None, causal: 
         r = fast.fast_paged_attn(q, cache, page_table, lengths, counts, _plain_scale(scale), causal, max_len)
         if r is not None:
             return r[0], (r[1], r[2])
-    _no_gradient("paged_attn", q)
+    _no_gradient("paged_attn", q, cache.k, cache.v)
     q = _prep(q, "q")
     B, H, Lq, d = q.shape
     arg = _cache_arg(cache, page_table, B, q.device)

@@ -994,3 +994,29 @@ def test_padding_of_more_than_31_bits_of_pieces(Lq, H):
         assert bool((M[h, 1:] == -math.inf).all()) and bool((L[h, 1:] == 1).all())
     del o, M, L
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_caches_that_need_a_gradient_are_refused(dtype, binding, monkeypatch):
+    """Learned keys and values as pages: the operators have no gradient for them and say so, but take them where none is wanted."""
+    import torch.autograd.forward_ad as fw
+    from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
+    q, k, v, cache, table, start, lens = small_call(dtype)
+    calls = (lambda c: kv.kv_cache_append(c, k, v, table, start), lambda c: kv.qk_norm_rope_append(c, q, k, v, table, start), lambda c: kv.kv_cache_read(c, table, lens, 3),
+             lambda c: kv.paged_attn(q, c, table, lens))
+    for name in ("k", "v"):
+        learned = cache._replace(**{name: getattr(cache, name).detach().clone().requires_grad_()})
+        for f in calls:
+            with pytest.raises(RuntimeError, match="no backward"):
+                f(learned)
+            with torch.no_grad():
+                f(learned)
+        if dtype is torch.bfloat16:
+            with fw.dual_level():
+                dual = cache._replace(**{name: fw.make_dual(getattr(cache, name), torch.ones_like(cache.k))})
+                for f in calls:
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        f(dual)

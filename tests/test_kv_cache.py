@@ -194,3 +194,17 @@ def test_operators_refuse_tangents():
                      lambda: kv.qk_norm_rope_append(c, x, x, x, table, i, cos, cy), lambda: kv.paged_attn(y, c, table, i)):
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def test_operators_refuse_caches_that_need_a_gradient():
+    from lvar_amd import kv_cache_ops as kv
+    x, i, table = torch.zeros(1, 2, 3, 64, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 4, dtype=torch.int32)
+    for name in ("k", "v"):
+        c = _cache()
+        c = c._replace(**{name: getattr(c, name).clone().requires_grad_()})
+        for call in (lambda: kv.kv_cache_append(c, x, x, table, i), lambda: kv.qk_norm_rope_append(c, x, x, x, table, i), lambda: kv.kv_cache_read(c, table, i),
+                     lambda: kv.paged_attn(x, c, table, i)):
+            with pytest.raises(RuntimeError, match="no backward"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+                call()
