@@ -563,6 +563,14 @@ bool cache_ok(PyObject* cache, PyObject* page_table, int64_t B, int dev, lvar_pa
   return true;
 }
 
+// The tensors of a cache (as cache_ok takes it) have been written: autograd finds out where it has saved them; tensors of inference mode have no version.
+void count_write(PyObject* cache) {
+  for (int i = 0; i < 4; i++) {
+    const at::Tensor* t = tensor(PyTuple_GET_ITEM(cache, i));
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
+}
+
 bool weight_ok(const at::Tensor* w, int64_t heads, int64_t d, int dev, lvar_weight_t& v) {
   v = {};
   if (!w) return true;
@@ -746,6 +754,7 @@ LVAR_FAST(fast_kv_append) {
   if (fused) oq = empty(q->sizes(), at::kBFloat16, dev);
   LVAR_NEED(api.lvar_kv_cache_append(view(*q), view(*k), view(*v), fused ? &w.h : nullptr, fused ? oq.data_ptr() : nullptr, c, ints(start), ints(counts),
                                      static_cast<int>(B), dim(*q, 1), dim(*k, 2), stream) == LVAR_OK);
+  count_write(a[0]);
   if (!fused) Py_RETURN_TRUE;
   return THPVariable_Wrap(std::move(oq));
   END_HANDLE_TH_ERRORS

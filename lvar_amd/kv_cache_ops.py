@@ -290,6 +290,8 @@ def _append(cache, q, k, v, page_table, start, counts, how, oq):
                                              _cache_arg(cache, page_table, B, k.device), start.data_ptr(), _ptr(counts),
                                              B, Hkv if q is None else q.shape[1], L, _stream(k))
     _lib.check(st, "lvar_kv_cache_append")
+    # (autograd finds out where it has saved them; tensors of inference mode have no version)
+    torch.autograd.graph.increment_version([t for t in cache if t is not None and not t.is_inference()])
 
 
 def _append_args(cache, k, v, page_table, start, counts):

@@ -1020,3 +1020,32 @@ def test_caches_that_need_a_gradient_are_refused(dtype, binding, monkeypatch):
                 for f in calls:
                     with pytest.raises(RuntimeError, match="forward-mode"):
                         f(dual)
+
+
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_writing_a_cache_counts_as_a_change(dtype, binding, monkeypatch):
+    """Autograd finds out that a cache it has saved was written; a cache made in inference mode has no counter."""
+    from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
+    q, k, v, cache, table, start, lens = small_call(dtype)
+    for f in (lambda c: kv.kv_cache_append(c, k, v, table, start), lambda c: kv.qk_norm_rope_append(c, q, k, v, table, start)):
+        before = [t._version for t in cache if t is not None]
+        if dtype is torch.bfloat16:
+            x = torch.ones(64, dtype=dtype, device="cuda", requires_grad=True)
+            y = (cache.k * x).sum()
+        f(cache)
+        assert all(t._version > n for t, n in zip((t for t in cache if t is not None), before))
+        if dtype is torch.bfloat16:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+        before = [t._version for t in cache if t is not None]
+        kv.kv_cache_read(cache, table, lens, 3), kv.paged_attn(q, cache, table, lens)
+        assert [t._version for t in cache if t is not None] == before
+        with torch.inference_mode():
+            made = kv.PagedKVCache.alloc(4, 2, 64, 16, dtype)
+            f(made)
+        with torch.no_grad():
+            f(made)
+        assert torch.equal(made.k.view(torch.uint8), cache.k.view(torch.uint8))
