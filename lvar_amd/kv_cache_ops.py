@@ -163,8 +163,8 @@ def _how(cos, sin, positions, wq: "_lib.LvarWeight", wk: "_lib.LvarWeight", norm
 def _norm_args(q, k, cos, sin, positions, norm, eps):
     """Checks that the plain and the appending form share."""
     qs, ks = q.shape, k.shape
-    _require(qs[0] == ks[0] and qs[2] == ks[2] and qs[3] == ks[3] and ks[1] > 0 and qs[1] % ks[1] == 0,
-             lambda: f"q and k must be [B,H,L,d] and [B,Hkv,L,d] with H a multiple of Hkv, got {tuple(qs)}, {tuple(ks)}")
+    _require(qs[0] == ks[0] and qs[2] == ks[2] and qs[3] == ks[3] and ks[1] > 0 and qs[1] > 0 and qs[1] % ks[1] == 0,
+             lambda: f"q and k must be [B,H,L,d] and [B,Hkv,L,d] with H a positive multiple of Hkv, got {tuple(qs)}, {tuple(ks)}")
     _require(q.device == k.device, "q and k must be on the same device")
     _require(norm in _NORMS, lambda: f"norm must be 'l2', 'rms' or None, got {norm!r}")
     eps = _EPS[norm] if eps is None else float(eps)

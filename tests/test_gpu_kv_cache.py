@@ -1049,3 +1049,15 @@ def test_writing_a_cache_counts_as_a_change(dtype, binding, monkeypatch):
         with torch.no_grad():
             f(made)
         assert torch.equal(made.k.view(torch.uint8), cache.k.view(torch.uint8))
+
+
+@pytest.mark.parametrize("binding", [True, False])
+def test_no_query_heads_are_refused(binding, monkeypatch):
+    """0 is a multiple of the key heads, but a call without queries would hand back keys that nobody wrote."""
+    from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
+    q, k, v, cache, table, start, lens = small_call()
+    for f in (lambda: kv.qk_norm_rope(q[:, :0], k), lambda: kv.qk_norm_rope_append(cache, q[:, :0], k, v, table, start), lambda: kv.paged_attn(q[:, :0], cache, table, lens)):
+        with pytest.raises(kv.ShapeError):
+            f()

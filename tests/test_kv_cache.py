@@ -208,3 +208,12 @@ def test_operators_refuse_caches_that_need_a_gradient():
                 call()
             with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
                 call()
+
+
+def test_checks_refuse_no_heads():
+    from lvar_amd import kv_cache_ops as kv
+    x = torch.zeros(2, 2, 3, 64, dtype=torch.bfloat16)
+    for q, k in ((x[:, :0], x), (x, x[:, :0]), (x[:, :0], x[:, :0])):
+        with pytest.raises(kv.ShapeError):
+            kv._norm_args(q, k, None, None, None, "l2", None)
+    assert kv._norm_args(x[:0], x[:0], None, None, None, "l2", None) == (None, None, 1e-12)
