@@ -421,7 +421,7 @@ typedef struct {
  * (2i, 2i+1) if interleaved, else (i, i + rot_dim/2), by the angles whose cosines and sines are rows of cos and sin (fp32
  * [table_rows, rot_dim/2], row stride table_stride, 16-byte aligned rows; NULL: no rotation).  positions (int32, or int64 if
  * positions64; strides in elements, 0 broadcasts) gives the row of each token, clamped to the table; NULL: the token's number
- * in the call, plus start[b] where there is one.
+ * in the call, plus start[b] where there is one.  eps: 0 or a normal number, not negative.
  */
 typedef struct {
   int norm;

@@ -37,7 +37,7 @@ bool weight_ok(const lvar_weight_t& w, WeightView& v) {
 }
 
 int fill_how(NormRopeParams& p, const lvar_norm_rope_t& how, int head_dim) {
-  if (how.norm < LVAR_NORM_NONE || how.norm > LVAR_NORM_RMS || !std::isfinite(how.eps) || how.eps < 0.f) return LVAR_EINVAL;
+  if (how.norm < LVAR_NORM_NONE || how.norm > LVAR_NORM_RMS || !(how.eps == 0.f || std::isnormal(how.eps)) || how.eps < 0.f) return LVAR_EINVAL;
   if (!weight_ok(how.q_weight, p.wq) || !weight_ok(how.k_weight, p.wk)) return LVAR_EINVAL;
   p.norm = how.norm; p.eps = how.eps;
   if (!how.cos != !how.sin) return LVAR_EINVAL;

@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <limits>
 #include <memory>
 #include <optional>
 #include <string>
@@ -599,7 +600,7 @@ bool how_ok(PyObject* const* a, const at::Tensor& q, const at::Tensor& k, int de
   else return false;
   double eps;
   bool inter;
-  if (a[6] != Py_None) { if (!as_double(a[6], eps)) return false; w.h.eps = static_cast<float>(eps); }
+  if (a[6] != Py_None) { if (!as_double(a[6], eps) || (eps != 0.0 && !(eps >= std::numeric_limits<float>::min()))) return false; w.h.eps = static_cast<float>(eps); }
   if (!as_bool(a[7], inter)) return false;
   if (!w.cos != !w.sin) return false;
   if (w.cos) {

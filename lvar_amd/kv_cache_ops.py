@@ -25,6 +25,7 @@ __all__ = ["PagedKVCache", "qk_norm_rope", "qk_norm_rope_append", "kv_cache_appe
 
 _NORMS = {None: 0, "l2": 1, "rms": 2}
 _EPS = {None: 0.0, "l2": 1e-12, "rms": 1e-6}
+_LEAST, _MOST = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 class PagedKVCache(NamedTuple):
@@ -168,7 +169,8 @@ def _norm_args(q, k, cos, sin, positions, norm, eps):
     _require(q.device == k.device, "q and k must be on the same device")
     _require(norm in _NORMS, lambda: f"norm must be 'l2', 'rms' or None, got {norm!r}")
     eps = _EPS[norm] if eps is None else float(eps)
-    _require(0.0 <= eps < float("inf"), "eps must be finite and not negative")
+    # (the reciprocal of a smaller one is no fp32 number, and rows of zeros would come out as NaN)
+    _require(eps == 0.0 or _LEAST <= eps <= _MOST, "eps must be 0 or a normal fp32 number, and not negative")
     cos, sin = _table_arg(cos, sin, qs[3], q.device)
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
@@ -256,7 +258,8 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
                  eps: Optional[float] = None, interleaved: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """Queries ``[B,H,L,d]`` and keys ``[B,Hkv,L,d]`` normalised per head, scaled and rotated, in one pass: ``(q, k)`` contiguous bf16.
 
-    ``norm``: ``"l2"`` is ``x / max(|x|, eps)`` (eps 1e-12), ``"rms"`` ``x / sqrt(mean(x^2) + eps)`` (eps 1e-6), ``None`` leaves x.
+    ``norm``: ``"l2"`` is ``x / max(|x|, eps)`` (eps 1e-12), ``"rms"`` ``x / sqrt(mean(x^2) + eps)`` (eps 1e-6), ``None`` leaves x; an
+    eps of its own is 0 or a normal fp32 number.
     ``q_weight`` / ``k_weight`` (fp32 or bf16; ``[d]``, ``[H,1]``, ``[1,d]`` or ``[H,d]``) multiply the result.  ``cos`` / ``sin``
     fp32 ``[rows, rot/2]`` rotate the first ``rot`` columns (a multiple of 16) in pairs ``(2i, 2i+1)``, or ``(i, i + rot/2)``
     with ``interleaved=False``; token i takes row i, or row ``positions[i]`` / ``positions[b,i]`` (clamped to the table).

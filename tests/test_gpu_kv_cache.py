@@ -1061,3 +1061,24 @@ def test_no_query_heads_are_refused(binding, monkeypatch):
     for f in (lambda: kv.qk_norm_rope(q[:, :0], k), lambda: kv.qk_norm_rope_append(cache, q[:, :0], k, v, table, start), lambda: kv.paged_attn(q[:, :0], cache, table, lens)):
         with pytest.raises(kv.ShapeError):
             f()
+
+
+@pytest.mark.parametrize("binding", [True, False])
+def test_eps_below_the_normal_numbers_is_refused(binding, monkeypatch):
+    """Its reciprocal is no fp32 number (rows of zeros would come out as NaN); the least normal one is fine."""
+    from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
+    q, k, v, cache, table, start, _ = small_call()
+    q = q.clone()
+    q[:, :, 1] = 0
+    for norm in ("l2", "rms"):
+        for eps in (1e-39, 1e-60, 5e-324, 1e39):
+            for x in (q, q.detach().clone().requires_grad_()):
+                with pytest.raises(kv.ShapeError):
+                    kv.qk_norm_rope(x, k, norm=norm, eps=eps)
+            with pytest.raises(kv.ShapeError):
+                kv.qk_norm_rope_append(cache, q, k, v, table, start, norm=norm, eps=eps)
+        x = q.detach().clone().requires_grad_()
+        o, _ = kv.qk_norm_rope(x, k, norm=norm, eps=2.0 ** -126)
+        assert bool(torch.isfinite(o).all()) and float(o[:, :, 1].abs().sum()) == 0

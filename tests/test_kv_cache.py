@@ -217,3 +217,16 @@ def test_checks_refuse_no_heads():
         with pytest.raises(kv.ShapeError):
             kv._norm_args(q, k, None, None, None, "l2", None)
     assert kv._norm_args(x[:0], x[:0], None, None, None, "l2", None) == (None, None, 1e-12)
+
+
+def test_eps_is_zero_or_normal(lib):
+    from lvar_amd import kv_cache_ops as kv
+    _lib, t, _ = _structs()
+    x, one = torch.zeros(2, 2, 3, 64, dtype=torch.bfloat16), ctypes.c_void_p(0x5000)
+    for norm in ("l2", "rms", None):
+        for eps in (1e-39, 5e-324, 1e39, -0.1, float("nan"), float("inf")):
+            with pytest.raises(kv.ShapeError):
+                kv._norm_args(x, x, None, None, None, norm, eps)
+        assert kv._norm_args(x, x, None, None, None, norm, 2.0 ** -126)[2] == 2.0 ** -126 and kv._norm_args(x, x, None, None, None, norm, 0)[2] == 0.0
+    for eps in (1e-39, 1e-45, float("inf"), -1e-6):
+        assert lib.lvar_qk_norm_rope_fwd(t, t, _fill(_lib.LvarNormRope(), norm=1, eps=eps), one, one, 1, 4, 2, 3, 128, None) == -1
