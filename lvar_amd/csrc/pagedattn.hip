@@ -25,6 +25,9 @@ namespace lvar {
 
 constexpr int PA_T = 256, PA_WAVES = 4, PA_STAGE = 128;
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+
 // D(16x16) += A(16x32) B(32x16): lane l holds row (column) l % 16, k = 8 * (l / 16) .. + 7; D register r: row 4 * (l / 16) + r, column l % 16.
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -55,6 +58,49 @@ __device__ __forceinline__ u32x4 scaled8(u32x2 c, float scale) {
   for (int h = 0; h < 2; h++) {
     r[2 * h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[h], scale, false));
     r[2 * h + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[h], scale, true));
+  }
+  return r;
+}
+
+// A causal call has keys that some rows of a tile see and others do not.  Their probabilities are 0 for rows that do not, but 0 * inf and
+// 0 * NaN are NaN: at the causal border, values that are not finite go into the product as 0, and after the loop they are added one by one to the
+// rows that see them (a scan of the border's keys that happens only if there are such values).  The look at the border's values costs 0.2 to 0.5 us of a
+// causal call (16 x 8 heads of 32 keys with 8 new tokens 4.84 -> 5.10, 8 x 8 of 64 keys with 40 new tokens 7.87 -> 8.37), staged tiles elsewhere 0.2.
+template <class V>
+__device__ __forceinline__ void largest(const V& x, u16x2& top) {      // magnitudes of a vector of bf16 pairs, as bits
+#pragma unroll
+  for (int e = 0; e < (int)(sizeof(V) / 4); e++) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x[e] & 0x7fff7fffu));
+}
+__device__ __forceinline__ bool odd_pair(u16x2 top) { return top[0] >= 0x7f80 || top[1] >= 0x7f80; }
+template <int W, class V>
+__device__ __forceinline__ void drop_odd(V& x, uint32_t& any) {        // the infinities and NaN among 2 W bf16 become 0, and `any` not 0
+#pragma unroll
+  for (int e = 0; e < W; e++) {
+    const i16x2 room = i16x2{0x7f7f, 0x7f7f} - __builtin_bit_cast(i16x2, x[e] & 0x7fff7fffu);
+    const uint32_t odd = __builtin_bit_cast(uint32_t, room >> 15);     // 0xffff per half
+    x[e] &= ~odd;
+    any |= odd;
+  }
+}
+// a NaN among 8 codes, or a power of two that takes their largest beyond bf16
+__device__ __forceinline__ bool odd_codes(u32x2 c, uint32_t byte) {
+  return ((((c[0] & 0x7f7f7f7fu) + 0x01010101u) | ((c[1] & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u) != 0 || byte > 246u;
+}
+// columns col .. col + 3 of a value row where they are not finite, 0 elsewhere
+template <bool F8>
+__device__ __forceinline__ f32x4 odd_part(const uint8_t* row, float scale, int col) {
+  u32x2 x;
+  if constexpr (F8) {
+    const u32x4 y = scaled8(u32x2{*(const uint32_t*)(row + col), 0u}, scale);
+    x = u32x2{y[0], y[1]};
+  } else {
+    x = *(const u32x2*)(row + 2 * col);
+  }
+  f32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const uint32_t bits = e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16;
+    r[e] = __builtin_bit_cast(float, (bits & 0x7f800000u) == 0x7f800000u ? bits : 0u);
   }
   return r;
 }
@@ -391,7 +437,8 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
 
   constexpr int KL = F8 ? KS / 2 : KS;          // 16-byte loads per key row and lane
   u32x4 kf[2][KL];
-  u32x4 vr[F8 ? 1 : CH][F8 ? 1 : 8];            // bf16: NE elements of 8 value rows
+  using Row = std::conditional_t<NE == 8, u32x4, u32x2>;
+  Row vr[F8 ? 1 : CH][F8 ? 1 : 8];              // bf16: NE elements of 8 value rows
   u32x2 vc[F8 ? CH : 1][F8 ? 8 : 1];            // e4m3
   uint32_t ke[2], ve[2];
 
@@ -425,8 +472,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
             if constexpr (NE == 8) vc[c][4 * j + x] = *(const u32x2*)(base + off + c * 128);
             else vc[c][4 * j + x] = u32x2{*(const uint32_t*)(base + off), 0u};
           } else {
-            if constexpr (NE == 8) vr[c][4 * j + x] = *(const u32x4*)(base + off + c * 256);
-            else { const u32x2 y = *(const u32x2*)(base + off); vr[c][4 * j + x] = u32x4{y[0], y[1], 0u, 0u}; }
+            vr[c][4 * j + x] = *(const Row*)(base + off + c * 256);
           }
         }
       }
@@ -437,6 +483,7 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
   constexpr int STEP = 32 * PA_WAVES;
   int key = s0 * PA_STAGE + wave * 32;
   int pg[2] = {-1, -1}, entry[2] = {0, 0};   // entry: of the next 32 keys
+  uint64_t odd = 0;                          // lanes that dropped values
   if (key < k_end) {
     pg[0] = page_of(key, entry_of(key)); pg[1] = page_of(key + 16, entry_of(key + 16));
     load_k(key, pg);
@@ -514,9 +561,23 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
 #pragma unroll
         for (int c = 0; c < CH; c++) {
           if constexpr (F8) { if (dead) vc[c][x] = u32x2{0u, 0u}; }
-          else { if (dead) vr[c][x] = u32x4{0u, 0u, 0u, 0u}; }
+          else { if (dead) vr[c][x] = Row{}; }
         }
         if constexpr (F8) { if (dead) ve[j] &= ~(0xffu << (8 * (x & 3))); }   // (a leftover byte of 255 stands for infinity)
+      }
+    }
+    const bool border = least < k_end && key + 32 > least;   // some rows see these keys and others do not
+    if constexpr (!F8) {
+      if (border) {
+        uint32_t some = 0;
+#pragma unroll
+        for (int x = 0; x < 8; x++)
+#pragma unroll
+          for (int c = 0; c < CH; c++) {
+            drop_odd<NE / 2>(vr[c][x], some);
+            if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);   // (rows side by side take registers that the loop does not have)
+          }
+        odd |= __ballot(some != 0);
       }
     }
 #pragma unroll
@@ -532,7 +593,16 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
             row[x][2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vc[c][x][e], sc, true));
           }
         } else {
-          row[x] = vr[c][x];
+#pragma unroll
+          for (int e = 0; e < NE / 2; e++) row[x][e] = vr[c][x][e];
+        }
+      }
+      if constexpr (F8) {
+        if (border) {
+          uint32_t some = 0;
+#pragma unroll
+          for (int x = 0; x < 8; x++) drop_odd<NE / 2>(row[x], some);
+          odd |= __ballot(some != 0);
         }
       }
 #pragma unroll
@@ -551,6 +621,27 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
     if (next < k_end) load_v(next, npg);
     pg[0] = npg[0]; pg[1] = npg[1];
     key = next;
+  }
+  if (__builtin_expect(odd != 0, false)) {
+#pragma unroll 1
+    for (int at = max(s0 * PA_STAGE, least & ~31); at < k_end; at++) {
+      const int page = page_of(at, entry_of(at)), slot = at & mask;
+      if (page < 0 || ((at >> 5) & (PA_WAVES - 1)) != wave) continue;
+      const uint8_t* from = vb + page * p.cache.s_page + slot * p.cache.s_row;
+      const float sc = F8 ? exp_value((veb + page * p.cache.e_page)[slot]) : 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int e = 0; e < NE; e += 4) {
+            const f32x4 y = odd_part<F8>(from, sc, c * CW + (4 * g + r) * NE + e);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) o[t][c][e + i][r] += at < limit[t] ? y[i] : 0.f;
+          }
+    }
   }
 
   // the waves' results become one
@@ -600,7 +691,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
   constexpr int LDO = D + 4;
   extern __shared__ __align__(16) char smem[];              // [2 buffers][keys, values][BUF]; then the outputs
   __shared__ float sm[PA_WAVES][NT * 16], sl[PA_WAVES][NT * 16];
-  __shared__ __align__(4) uint8_t missing[2][4];             // quarters of a tile without a page (or behind the last key)
+  __shared__ __align__(4) uint8_t missing[2][4];             // quarters of a tile: 1 without a page (or behind the last key), 2 with values that were dropped
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave % RW, kw = wave / RW;
@@ -615,6 +706,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
   // limits do not fall from row to row: the last row of the tile, and of the wave, has the largest
   const int k_end = min(s1 * PA_STAGE, limit_of(p, w, fresh, min(tile0 + NT * RW * 16, rows) - 1));
   const int least = limit_of(p, w, fresh, row0);
+  const int lowest = p.causal ? max(0, w.len - fresh) : 0x7fffffff;   // keys that all rows see (new tokens aside)
   const int mine = row0 < fresh * p.G ? limit_of(p, w, fresh, row0 + NT * 16 - 1) : 0;   // a wave without new rows only fills
 
   u32x4 qf[NT][KS];
@@ -676,24 +768,46 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
   auto deposit = [&](const Fill& f, int key, int buf) {
     const int first = quarter_of(key);
     const bool ragged = first + KT / 4 > k_end || f.page < 0;
-#pragma unroll
-    for (int x = 0; x < NI; x++) {
-      const int row = wave * (KT / 4) + x * RPI + fr;
-      const int kc = fc ^ (D == 64 ? (row >> 1) & 7 : row & 15), vc = fc ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1);
-      u32x4 kx, vx;
-      if constexpr (F8) {
-        kx = scaled8(f.code[0][x], exp_value(f.byte[0][x]));
-        vx = scaled8(f.code[1][x], exp_value(f.byte[1][x]));
-      } else {
-        kx = f.row[0][x];
-        vx = f.row[1][x];
-      }
+    auto value_of = [&](int x) {
+      u32x4 vx;
+      if constexpr (F8) vx = scaled8(f.code[1][x], exp_value(f.byte[1][x]));
+      else vx = f.row[1][x];
       // rows of keys nobody may see hold anything, NaN too, and 0 * NaN is not 0
       if (ragged && (f.page < 0 || first + x * RPI + fr >= k_end)) vx = u32x4{0u, 0u, 0u, 0u};
-      *(u32x4*)(smem + (2 * buf) * BUF + row * RB + kc * 16) = kx;
-      *(u32x4*)(smem + (2 * buf + 1) * BUF + row * RB + vc * 16) = vx;
+      return vx;
+    };
+    auto place_of = [&](int x, bool values) {
+      const int row = wave * (KT / 4) + x * RPI + fr;
+      const int kc = fc ^ (D == 64 ? (row >> 1) & 7 : row & 15), vc = fc ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1);
+      return (u32x4*)(smem + (2 * buf + (values ? 1 : 0)) * BUF + row * RB + (values ? vc : kc) * 16);
+    };
+#pragma unroll
+    for (int x = 0; x < NI; x++) {
+      if constexpr (F8) *place_of(x, false) = scaled8(f.code[0][x], exp_value(f.byte[0][x]));
+      else *place_of(x, false) = f.row[0][x];
+      *place_of(x, true) = value_of(x);
     }
-    if (lane == 0) missing[buf][wave] = f.page < 0;
+    uint32_t flags = f.page < 0 ? 1u : 0u;
+    if (__builtin_expect(first + KT / 4 > lowest, false)) {
+      bool odd = false;
+      u16x2 top = {0, 0};
+#pragma unroll
+      for (int x = 0; x < NI; x++) {
+        if constexpr (F8) odd = odd || odd_codes(f.code[1][x], f.byte[1][x]);
+        else largest(f.row[1][x], top);
+      }
+      if (__builtin_expect(__any(odd || odd_pair(top)), false)) {   // once more, without them
+        uint32_t some = 0;
+#pragma unroll
+        for (int x = 0; x < NI; x++) {
+          u32x4 vx = value_of(x);
+          drop_odd<4>(vx, some);
+          *place_of(x, true) = vx;
+        }
+        if (__any(some != 0)) flags |= 2u;
+      }
+    }
+    if (lane == 0) missing[buf][wave] = (uint8_t)flags;
   };
 
   // addresses of the reads: constants of a product's steps are exclusive-ored in, rows added
@@ -706,6 +820,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
 #pragma unroll
   for (int n = 0; n < NB; n++) vp[n] = lds + (va ^ (n * 32)) + kw * HALVES * 32 * RB;
 
+  uint32_t dropped = 0;                                     // values of the causal border
   auto compute = [&](int key, int buf) {
     const uint32_t gone = *(const uint32_t*)missing[buf];
 #pragma unroll
@@ -773,6 +888,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
       }
       __builtin_amdgcn_s_setprio(0);
     }
+    dropped |= __builtin_amdgcn_readfirstlane(gone) & 0x02020202u;
   };
 
   // (the table entry that the next request needs is loaded ahead of a barrier: scalar loads and LDS reads share a counter)
@@ -792,6 +908,21 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
     deposit(f, key + 2 * KT, 0);
     entry = entry_of(quarter_of(key + 3 * KT));
     __syncthreads();
+  }
+  if (__builtin_expect(dropped != 0, false)) {
+#pragma unroll 1
+    for (int at = max(k0, lowest & ~31); at < k_end; at++) {
+      const int page = page_of(at, entry_of(at)), slot = at & mask;
+      if (page < 0 || at / 32 % (KT / 32) / HALVES != kw) continue;
+      const uint8_t* from = vb + page * p.cache.s_page + slot * p.cache.s_row;
+      const float sc = F8 ? exp_value((veb + page * p.cache.e_page)[slot]) : 0.f;
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        const f32x4 y = odd_part<F8>(from, sc, n * 16 + 4 * g);
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[t][n] += at < limit[t] ? y : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
   }
 
 #pragma unroll

@@ -379,7 +379,7 @@ def paged_attn(q, cache: PagedKVCache, page_table, lengths, scale=None, causal: 
     head ``h // (H // Hkv)``.  ``causal``: row i of sequence b sees tokens ``j < lengths[b] - n + i + 1`` with ``n = counts[b]``
     (default Lq) new tokens; otherwise all ``lengths[b]``.  Rows ``i >= counts[b]`` of a padded batch and rows that see no token
     get ``o = 0, M = -inf, L = 1``.  What the cache holds behind ``lengths`` does not matter; a value that is not finite reaches the rows that
-    see it and may reach rows up to 128 before them (0 * inf).  ``max_len`` bounds the lengths (longer ones are clamped to it; default: all that the page table
+    see it and no others.  ``max_len`` bounds the lengths (longer ones are clamped to it; default: all that the page table
     can name): a small bound lets the launch do without the pass that joins the parts of long sequences."""
     fast = _native()
     if fast is not None:

@@ -1082,3 +1082,93 @@ def test_eps_below_the_normal_numbers_is_refused(binding, monkeypatch):
         x = q.detach().clone().requires_grad_()
         o, _ = kv.qk_norm_rope(x, k, norm=norm, eps=2.0 ** -126)
         assert bool(torch.isfinite(o).all()) and float(o[:, :, 1].abs().sum()) == 0
+
+
+def leak_case(Lq, H, Hkv, d, lengths, dtype, page=16, counts=None):
+    """Causal calls whose newest values hold infinities and NaN: column by column, rows that see one are not finite, all others are what they are without it."""
+    from lvar_amd import kv_cache_ops as kv
+    B, n = len(lengths), max(lengths)
+    per = -(-n // page)
+    table = table_for(B, per, B * per + 1, 3)
+    x = [rand(B, Hkv, n, d, seed=20 + i) for i in range(2)]
+    lens, zero = torch.tensor(lengths, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)
+    new = [Lq] * B if counts is None else counts
+    g = torch.Generator().manual_seed(Lq + d)
+    bad = torch.zeros(B, Hkv, n, d, dtype=torch.bool)
+    for b in range(B):
+        first = max(0, lengths[b] - new[b])
+        for j in {lengths[b] - 1, first + (lengths[b] - first) // 2, min(first + 1, lengths[b] - 1), max(0, lengths[b] - 33)}:
+            for h in range(Hkv):
+                bad[b, h, j, torch.randint(0, d, (3,), generator=g)] = True
+    kinds = torch.tensor([math.inf, -math.inf, math.nan]).to(torch.bfloat16)
+    spoiled = torch.where(bad, kinds[torch.randint(0, 3, bad.shape, generator=g)], x[1])
+    caches = []
+    for v in (torch.where(bad, torch.zeros((), dtype=torch.bfloat16), x[1]), spoiled):
+        c = to_gpu(make_cache(B * per + 1, Hkv, page, d, dtype, 6))
+        kv.kv_cache_append(c, x[0].cuda(), v.cuda(), table.cuda(), zero.cuda(), lens.cuda())
+        caches.append(c)
+    q = rand(B, H, Lq, d, seed=9)
+    c = None if counts is None else torch.tensor(counts, dtype=torch.int32)
+    (o, (M, L)), (want, (Mw, Lw)) = (kv.paged_attn(q.cuda(), x, table.cuda(), lens.cuda(), causal=True, counts=cu(c)) for x in (caches[1], caches[0]))
+    assert torch.equal(M, Mw) and torch.equal(L, Lw)
+    # which (row, column) sees which value
+    i = torch.arange(Lq)
+    limit = torch.stack([torch.where(i < new[b], lengths[b] - new[b] + i + 1, 0) for b in range(B)])      # [B, Lq]
+    sees = (torch.arange(n) < limit[..., None]).double()                                                  # [B, Lq, n]
+    hit = torch.matmul(sees[:, None], bad.double()) > 0                                                   # [B, Hkv, Lq, d]
+    hit = hit.repeat_interleave(H // Hkv, 1)
+    assert bool(hit.any()) and not bool(hit.all())
+    o, want = o.cpu(), want.cpu()
+    assert bool(torch.isfinite(want).all())
+    assert not bool(torch.isfinite(o[hit]).any()), "a row that sees a value which is not finite"
+    assert torch.equal(o[~hit], want[~hit]), f"{int((~(o == want))[~hit].sum())} results of rows that do not see one"
+
+
+LEAK_CASES = [
+    # Lq, H, Hkv, d, lengths, counts
+    (4, 2, 2, 64, [40, 4], None), (4, 2, 2, 128, [130, 70], None), (3, 2, 1, 256, [33, 300], None),          # up to 16 rows
+    (29, 2, 2, 64, [64, 200], None), (13, 4, 2, 128, [13, 77], [13, 5]),                                     # up to 32
+    (50, 2, 2, 64, [50, 190], None), (60, 2, 2, 128, [129, 61], [60, 31]),                                   # staged, 64 rows
+    (70, 4, 2, 64, [500, 70], None), (200, 2, 1, 128, [200, 1300], None), (70, 1, 1, 256, [75, 600], None),  # several row tiles, cut
+    (5, 2, 2, 128, [2500, 700], None), (5, 2, 2, 256, [1500, 64], None),                                     # cut and joined
+]
+
+
+@pytest.mark.parametrize("case", LEAK_CASES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_values_that_are_not_finite_stay_behind_the_causal_border(case, dtype):
+    Lq, H, Hkv, d, lengths, counts = case
+    leak_case(Lq, H, Hkv, d, lengths, dtype, counts=counts)
+
+
+@pytest.mark.parametrize("Lq,d", [(1, 128), (2, 64), (9, 256), (40, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_values_that_are_not_finite_reach_who_sees_them(Lq, d, dtype):
+    """Anywhere in the cache, beside pages that are missing and behind the causal border or not."""
+    from lvar_amd import kv_cache_ops as kv
+    n, page = 331, 16
+    table = torch.arange(21, dtype=torch.int32).view(1, 21)
+    k, v = (rand(1, 1, n, d, seed=i) for i in (1, 2))
+    for spot in (0, 5, 40, 200, 319, 320, n - Lq, n - 1):
+        for x in (math.inf, math.nan):
+            w = v.clone()
+            w[0, 0, spot, d // 3] = x
+            c = to_gpu(make_cache(22, 1, page, d, dtype, 6))
+            kv.kv_cache_append(c, k.cuda(), w.cuda(), table.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda"))
+            holes = table.clone()
+            holes[0, 1] = holes[0, min(spot // 16 ^ 1, 19)] = -1          # (of 16 keys beside it)
+            seen = int(holes[0, spot // 16]) >= 0
+            for causal in (False, True):
+                o, _ = kv.paged_attn(rand(1, 2, Lq, d, seed=3).cuda(), c, holes.cuda(), torch.full((1,), n, dtype=torch.int32, device="cuda"), causal=causal)
+                rows = torch.arange(n - Lq, n) >= spot if causal else torch.ones(Lq, dtype=torch.bool)
+                want = torch.ones(Lq, d, dtype=torch.bool)
+                want[:, d // 3] = ~(rows & seen)
+                assert torch.equal(torch.isfinite(o[0]).cpu(), want.expand(2, Lq, d)), (spot, x, causal)
+        # a key: whole rows
+        w = k.clone()
+        w[0, 0, spot, d // 3] = math.nan
+        c = to_gpu(make_cache(22, 1, page, d, dtype, 6))
+        kv.kv_cache_append(c, w.cuda(), v.cuda(), table.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda"))
+        o, _ = kv.paged_attn(rand(1, 2, Lq, d, seed=3).cuda(), c, table.cuda(), torch.full((1,), n, dtype=torch.int32, device="cuda"), causal=True)
+        rows = torch.arange(n - Lq, n) < spot
+        assert torch.equal(torch.isfinite(o[0]).cpu(), rows[:, None].expand(2, Lq, d)), (spot, "key")
