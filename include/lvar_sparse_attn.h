@@ -476,7 +476,8 @@ int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int
  * o = softmax(q k^T scale) v (contiguous bf16), M and L fp32 [B,H,Lq] as everywhere here.  causal: row i of sequence b sees tokens
  * j < lengths[b] - n + i + 1, n = counts[b] (NULL: Lq) its new tokens; rows i >= n, and rows that see no token, get o = 0, M = -inf, L = 1.
  * Query head h reads key/value head h / (H / kv_heads).  Lengths are clamped to max_len (at most max_pages * page_size).  What the cache holds
- * behind them does not matter; a value that is not finite reaches the rows that see it and no others.
+ * behind them does not matter; a value that is not finite reaches the rows that see it and no others.  Scores, M, L and sums are fp32; probabilities
+ * enter the second product as two bf16 terms (2^-16) for up to 32 rows H / kv_heads * Lq (head_dim 256: 16, e4m3 only), as one (2^-8) otherwise.
  * workspace: lvar_paged_attn_workspace_bytes() (16-byte aligned, its contents need no preparation; calls that overlap in time
  * need one each); without one, or with a smaller one, no sequence is cut and long ones are slow.  Results depend on the lengths of all
  * sequences of the call in the last bits (they decide where sequences are cut), not on timing.

@@ -4,7 +4,9 @@
 // e4m3 codes with one power of two per row: value = code * 2^(byte - 127), byte the smallest one >= 1 with max|x| <= 448 * 2^(byte - 127).
 // A power of two instead of max / 448: scaling and its inverse are exact, a code has 4 significant bits and so every value
 // is exact in bf16 -- reading back or feeding the matrix instructions rounds nothing, and the only rounding of a cached
-// element is the one to its code.  It costs at most one of e4m3's 15 normal binades at the small end.
+// element is the one to its code.  It costs at most one of e4m3's 15 normal binades at the small end.  (But at the ends of bf16's range: bytes 1 and 2 have
+// values below its smallest number's steps, and with byte 247 codes of 256 and more, the code of elements from 1.9375 * 2^127 on, stand for 2^128, an
+// infinity there.)
 #pragma once
 #include "launch.h"
 

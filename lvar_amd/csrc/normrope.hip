@@ -14,8 +14,9 @@ namespace lvar {
 
 constexpr int NR_T = 256;
 
-// Results of large launches go past the L2s, whoever reads them next mostly sits on another XCD: 2 x 16 x 4096 rows of q and of k
-// 28.3 -> 26.4 us, their gradients over 10521 tokens 240 -> 220.
+// Results of large forward launches go past the L2s, whoever reads them next mostly sits on another XCD: 2 x 16 x 4096 rows of q and of k
+// 28.3 -> 26.4 us.  Gradients do so at every size (with a reader of each behind them, through the L2s / past them: 2 x 8 x 20 tokens 7.1 / 7.3 us,
+// 2 x 16 x 256 9.7 / 9.3, 4096 58.3 / 60.6, 4 x 16 x 10521 342 / 340; the kernel alone over 10521 tokens 240 / 220).
 template <bool STREAM>
 __device__ __forceinline__ void put(bf16_t* to, u32x4 x) {
   if constexpr (STREAM) __builtin_nontemporal_store(x, (u32x4*)to);
@@ -99,8 +100,8 @@ __device__ __forceinline__ void load_weight(const WeightView& w, int head, int l
 
 // r of a row with this sum of squares; `flat`: |x| <= eps, where the l2 norm is a division by eps.  The reciprocal root is the
 // hardware's (sums below its normal range scaled into it), off by up to one step of fp32, and one Newton step for the rest: with a root
-// and a quotient rounded to nearest, a quarter of the instructions of a row went into these lines, and without the step the codes of e4m3
-// rows are a quarter further off (12 x 3.8 M elements against 64 bits: 0.103, 0.074 with it, 0.093 by root and quotient).
+// and a quotient rounded to nearest, a quarter of the instructions of a row went into these lines (append of 2 x 16 x 4096 tokens in e4m3
+// 39.1 us, 37.7 with the step, 37.3 without it).  Of 6 x 16.8 M keys in e4m3, 95, 92 and 92 then have another code than in 64 bits.
 template <int D>
 __device__ __forceinline__ float norm_factor(const NormRopeParams& p, float ss, bool& flat) {
   flat = false;
@@ -173,7 +174,8 @@ __global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p)
   a.on = false;
   if (!plain && p.cos) load_angles<LPR>(p, table_row(p, b, i, base), lane, a);
   // One factor for all columns commutes with the rotation and comes last: the rotation of bf16 values costs two roundings instead of three
-  // or four (of 10^7 elements of e4m3 rows 7 have another code than in 64 bits, not 11).  Halved angles, so that the largest values do not overflow.
+  // or four (of 6 x 16.8 M keys in e4m3, 92 have another code than in 64 bits, 135 with the factor first).  Halved angles, so that the largest
+  // values do not overflow.
   const float both = a.on ? 2.f : 1.f;
   if (a.on) {
 #pragma unroll

@@ -13,7 +13,7 @@
 //     while it computes, and the four waves take turns at 32 keys.  32 sequences of up to 32768 tokens, 32 query heads over 8 of
 //     128: 2.2 GB of bf16 in 395 us (5.6 TB/s; a copy moves 5.2); 131071 tokens in e4m3: 0.27 GB in 55 us.
 //   paged_tile_kernel   more rows: keys and values staged in LDS, where the waves share them.  4 x 256 rows of 16 heads over 2521
-//     tokens: 44 .. 46 us, 460 .. 480 TFLOP/s.  (With 64 rows per wave and no LDS there is one wave per SIMD and nobody left to
+//     tokens: 45 .. 48 us, 440 .. 470 TFLOP/s.  (With 64 rows per wave and no LDS there is one wave per SIMD and nobody left to
 //     compute while it waits: 105 us where this takes 38, 8 sequences of up to 4001 tokens with up to 61 new ones.)
 //
 // The work is (sequence, key/value head, row tile) x stages of 128 keys.  It is cut into pieces of about equal length by the
@@ -539,8 +539,8 @@ __global__ __launch_bounds__(PA_T, WAVES_PER_SIMD) void paged_attn_kernel(const 
             if (pg[j] < 0 || key + 16 * j + 4 * g + r >= limit[t]) s[4 * j + r] = -INFINITY;
       }
       softmax_step<8, CH * NE>(s, p.c, m[t], l[t], top[t], &o[t][0][0]);
-      // p goes into the matrix instruction as two bf16 terms, which leave 2^-17 of it out: the result is off by its own rounding only (rms 0.0017
-      // of it instead of 0.0023; a product more per value, 2 % of short calls).  256 columns of bf16 have no registers for the second: 2^-9 there.
+      // p goes into the matrix instruction as two bf16 terms, which leave at most 2^-16 of it out: the result is off by its own rounding only (rms 0.0017
+      // of it instead of 0.0023; a product more per value, 2 % of short calls).  256 columns of bf16 have no registers for the second: up to 2^-8 there.
       pf[t] = pack8u(s);
       if constexpr (TWO) {
         float back[8];
@@ -862,8 +862,8 @@ __global__ __launch_bounds__(PA_T, 2) void paged_tile_kernel(const PagedAttnPara
           }
         }
         softmax_step<8, NB>(s, p.c, m[t], l[t], top[t], o[t]);
-        // (rounded to bf16, 2^-9 per term, independent signs, their sum is not: a second term would be half as many products again, and those
-        // are among the bounds here)
+        // (one bf16 term: off by up to 2^-8 each, with independent signs; their sum is not rounded.  A second term is half as many products again, and those
+        // are among the bounds here: 8 x 8 ragged tiles of 61 new tokens 51.2 -> 59.8 us, 4 x 16 heads of 2521 keys with 256 rows 46.9 -> 53.9)
         pf[t] = pack8u(s);
       }
       u32x4 vx[2][4];

@@ -350,7 +350,8 @@ def qk_norm_rope_append(cache: PagedKVCache, q, k, v, page_table, start, cos=Non
 def kv_cache_read(cache: PagedKVCache, page_table, lengths, max_len: Optional[int] = None, start=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Tokens ``start[b] ..`` (default 0) of every sequence as contiguous bf16 ``(k, v)`` ``[B,Hkv,max_len,d]``, the form that the
     dense and sparse attention operators take; zeros from position ``lengths[b]`` on.  ``max_len`` defaults to all that the page
-    table can name.  Exact: every cached value is a bf16 value."""
+    table can name.  Every value that an append has written is a bf16 value and comes back exactly, but at the ends of the range: rounded below
+    2^-130, and infinite from 2^128 on, to which an 8-bit cache rounds elements of 1.9375 * 2^127 and more."""
     fast = _native()
     if fast is not None:
         r = fast.fast_kv_read(cache, page_table, lengths, max_len, start)
@@ -379,7 +380,8 @@ def paged_attn(q, cache: PagedKVCache, page_table, lengths, scale=None, causal: 
     head ``h // (H // Hkv)``.  ``causal``: row i of sequence b sees tokens ``j < lengths[b] - n + i + 1`` with ``n = counts[b]``
     (default Lq) new tokens; otherwise all ``lengths[b]``.  Rows ``i >= counts[b]`` of a padded batch and rows that see no token
     get ``o = 0, M = -inf, L = 1``.  What the cache holds behind ``lengths`` does not matter; a value that is not finite reaches the rows that
-    see it and no others.  ``max_len`` bounds the lengths (longer ones are clamped to it; default: all that the page table
+    see it and no others.  Scores, statistics and sums are fp32; the probabilities enter the second product as two bf16 terms (2^-16) up to 32 rows
+    (query heads per key/value head times Lq; up to 16 for 8-bit caches of head_dim 256), as one (2^-8) beyond, and for bf16 caches of head_dim 256.  ``max_len`` bounds the lengths (longer ones are clamped to it; default: all that the page table
     can name): a small bound lets the launch do without the pass that joins the parts of long sequences."""
     fast = _native()
     if fast is not None:
