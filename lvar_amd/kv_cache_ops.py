@@ -60,6 +60,12 @@ class PagedKVCache(NamedTuple):
         return self.k.shape[2]
 
 
+def _rows(t, name: str):
+    """``t`` as the kernels read it.  (A tensor whose base is misaligned, or with odd strides on axes of one element, may count as contiguous: it is copied.)"""
+    t = _prep(t, name)
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]) else t
+
+
 def _same_strides(a, b) -> bool:
     return all(n <= 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
 
@@ -230,7 +236,7 @@ class _NormRope(torch.autograd.Function):
         B, H, L, d = q.shape
         Hkv = k.shape[1]
         # (hooks on saved tensors may return copies of another layout, or on another device)
-        q, k = _prep(q, "q"), _prep(k, "k")
+        q, k = _rows(q, "q"), _rows(k, "k")
         cos, sin = _table_arg(cos, sin, d, q.device)
         _require(positions is None or positions.device == q.device, "positions must be on the device of q")
         dq, dk = _rows_like(q), _rows_like(k)
@@ -241,7 +247,7 @@ class _NormRope(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
             return dq, dk, dwq, dwk, None, None, None, None, None, None
-        gq, gk = _prep(gq.contiguous(), "gradient"), _prep(gk.contiguous(), "gradient")
+        gq, gk = _rows(gq.contiguous(), "gradient"), _rows(gk.contiguous(), "gradient")
         (wq, aq), (wk, ak) = _weight_arg(wq, H, d, "q_weight", q.device), _weight_arg(wk, Hkv, d, "k_weight", q.device)
         lib = _lib.load()
         with _on_device(q):
@@ -273,7 +279,7 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
         if r is not None:
             return r
     _no_tangent("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
-    q, k = _prep(q, "q"), _prep(k, "k")
+    q, k = _rows(q, "q"), _rows(k, "k")
     cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
     _require(q.shape[3] in (16, 32, 64, 128, 256), lambda: f"head_dim must be 16, 32, 64, 128 or 256, got {q.shape[3]}")
     _require(cos is None or positions is not None or cos.shape[0] >= q.shape[2],
@@ -317,7 +323,7 @@ def kv_cache_append(cache: PagedKVCache, k, v, page_table, start, counts=None) -
     if fast is not None and fast.fast_kv_append(cache, page_table, start, counts, None, k, v):
         return
     _no_gradient("kv_cache_append", k, v, cache.k, cache.v)
-    k, v = _prep(k, "k"), _prep(v, "v")
+    k, v = _rows(k, "k"), _rows(v, "v")
     start, counts = _append_args(cache, k, v, page_table, start, counts)
     if k.numel():
         _append(cache, None, k, v, page_table, start, counts, None, None)
@@ -336,7 +342,7 @@ def qk_norm_rope_append(cache: PagedKVCache, q, k, v, page_table, start, cos=Non
             return r
     _no_gradient("qk_norm_rope_append", q, k, v, q_weight, k_weight, cache.k, cache.v)
     _no_tangent("qk_norm_rope_append", cos, sin)
-    q, k, v = _prep(q, "q"), _prep(k, "k"), _prep(v, "v")
+    q, k, v = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
     cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
     start, counts = _append_args(cache, k, v, page_table, start, counts)
     B, H, L, d = q.shape
@@ -389,7 +395,7 @@ def paged_attn(q, cache: PagedKVCache, page_table, lengths, scale=None, causal: 
         if r is not None:
             return r[0], (r[1], r[2])
     _no_gradient("paged_attn", q, cache.k, cache.v)
-    q = _prep(q, "q")
+    q = _rows(q, "q")
     B, H, Lq, d = q.shape
     arg = _cache_arg(cache, page_table, B, q.device)
     Hkv = cache.k.shape[1]

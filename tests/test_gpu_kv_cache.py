@@ -1172,3 +1172,33 @@ def test_values_that_are_not_finite_reach_who_sees_them(Lq, d, dtype):
         o, _ = kv.paged_attn(rand(1, 2, Lq, d, seed=3).cuda(), c, table.cuda(), torch.full((1,), n, dtype=torch.int32, device="cuda"), causal=True)
         rows = torch.arange(n - Lq, n) < spot
         assert torch.equal(torch.isfinite(o[0]).cpu(), rows[:, None].expand(2, Lq, d)), (spot, "key")
+
+
+@pytest.mark.parametrize("binding", [True, False])
+def test_rows_at_odd_places(binding, monkeypatch):
+    """Unit stride on d is all that a tensor needs: bases between 16-byte borders, and odd strides of axes of one element, which count as contiguous."""
+    from lvar_amd import kv_cache_ops as kv
+    if not binding:
+        monkeypatch.setattr(kv, "_native", lambda: None)
+    d = 64
+    table, zero = torch.arange(2, dtype=torch.int32, device="cuda").view(1, 2), torch.zeros(1, dtype=torch.int32, device="cuda")
+    flat = rand(4 * 300, seed=1).cuda()
+    places = [lambda i: flat[i * 300 + 1:i * 300 + 1 + d].view(1, 1, 1, d),                                  # contiguous, 2 bytes behind a border
+              lambda i: flat.as_strided((1, 1, 1, d), (131, 67, 3, 1), i * 304),                              # aligned, odd strides
+              lambda i: flat.as_strided((1, 1, 3, d), (131, 67, 72, 1), i * 304)]
+    for place in places:
+        x = [place(i) for i in range(4)]
+        y = [t.clone(memory_format=torch.contiguous_format) for t in x]
+        got, want = [], []
+        for ts, out in ((x, got), (y, want)):
+            q, k, v, g = ts
+            cache = kv.PagedKVCache.alloc(2, 1, d, 16)
+            out += kv.qk_norm_rope(q, k)
+            out.append(kv.qk_norm_rope_append(cache, q, k, v, table, zero))
+            kv.kv_cache_append(cache, k, v, table, zero + 5)
+            lens = zero + 5 + k.shape[2]
+            out += [cache.k, cache.v, kv.paged_attn(q, cache, table, lens)[0]]
+            a, b = (t.detach().requires_grad_() for t in (q, k))
+            o = kv.qk_norm_rope(a, b)
+            out += torch.autograd.grad(o, (a, b), (g, v))
+        assert all(torch.equal(s, t) for s, t in zip(got, want))
