@@ -487,6 +487,30 @@ int lvar_paged_attn_fwd(lvar_tensor_t q, lvar_paged_cache_t cache, const int32_t
                         float* L, void* workspace, int64_t workspace_bytes, int B, int H, int Lq, int max_len, int causal,
                         float scale, void* stream);
 
+/*
+ * Attention over packed sequences.  Sequence b of `batch` has queries offsets[b] .. offsets[b+1]-1 of q [H,tokens,d] and keys
+ * k_offsets[b] .. k_offsets[b+1]-1 of k, v [kv_heads,k_tokens,d] (bf16 views; stride_b is not used; int32 [batch+1] on the device,
+ * ascending, the same array where queries and keys are of the same tokens).  Row i of n queries over m keys sees keys j < m - n + i + 1
+ * (causal) or all m.  o = softmax(q k^T scale) v (bf16 view [H,tokens,d]), M and L fp32 [H,tokens] as everywhere here.  Rows that see no key,
+ * and rows of no sequence (ahead of the first offset, behind the last), get o = 0, M = -inf, L = 1.  Query head h reads key/value head
+ * h / (H / kv_heads).  head_dim 64, 128 or 256; rows 16-byte aligned; a head's rows span less than 2^31 bytes.  A value that is not finite reaches
+ * the rows that see it and no others.  Scores, M, L and sums are fp32; probabilities enter the second product as bf16 (2^-9).
+ */
+int lvar_packed_attn_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar_tensor_t o, const int32_t* offsets, const int32_t* k_offsets,
+                         float* M, float* L, int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal, float scale,
+                         void* stream);
+
+/*
+ * Its gradients: from what the forward call took and gave, and the gradient go of o (bf16 view), dq, dk and dv (bf16 views; ptr NULL: not
+ * wanted), summed over the query heads that share a key/value head; zeros where a row is of no sequence, or nobody sees a key.  The order of
+ * every sum is fixed.  workspace: lvar_packed_attn_bwd_workspace_bytes() (16-byte aligned, written and read by this call).
+ */
+int64_t lvar_packed_attn_bwd_workspace_bytes(int tokens, int H);
+int lvar_packed_attn_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar_tensor_t o, lvar_tensor_t go, const int32_t* offsets,
+                         const int32_t* k_offsets, const float* M, const float* L, lvar_tensor_t dq, lvar_tensor_t dk, lvar_tensor_t dv,
+                         void* workspace, int64_t workspace_bytes, int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim,
+                         int causal, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@ EXPORTED_SYMBOLS = (
     "lvar_window_key_scores",
     "lvar_qk_norm_rope_fwd", "lvar_qk_norm_rope_bwd_scratch_bytes", "lvar_qk_norm_rope_bwd", "lvar_kv_cache_append", "lvar_kv_cache_read",
     "lvar_paged_attn_workspace_bytes", "lvar_paged_attn_fwd",
+    "lvar_packed_attn_fwd", "lvar_packed_attn_bwd_workspace_bytes", "lvar_packed_attn_bwd",
 )
 
 
@@ -142,6 +143,12 @@ def load() -> C.CDLL:
     lib.lvar_paged_attn_workspace_bytes.argtypes = [I, I, I, I, I, I]
     lib.lvar_paged_attn_fwd.restype = I
     lib.lvar_paged_attn_fwd.argtypes = [T, G, P, P, P, P, P, P, I64, I, I, I, I, I, F, P]
+    lib.lvar_packed_attn_fwd.restype = I
+    lib.lvar_packed_attn_fwd.argtypes = [T, T, T, T, P, P, P, P, I, I, I, I, I, I, I, F, P]
+    lib.lvar_packed_attn_bwd_workspace_bytes.restype = I64
+    lib.lvar_packed_attn_bwd_workspace_bytes.argtypes = [I, I]
+    lib.lvar_packed_attn_bwd.restype = I
+    lib.lvar_packed_attn_bwd.argtypes = [T, T, T, T, T, P, P, P, P, T, T, T, P, I64, I, I, I, I, I, I, I, F, P]
     _lib = lib
     return lib
 

@@ -1,0 +1,180 @@
+// What the kernels of the attention over packed sequences share: launch parameters, which tile a workgroup takes, filling a tile into LDS.
+//
+// Sequence b of a batch has queries offsets[b] .. offsets[b+1]-1 and keys k_offsets[b] .. k_offsets[b+1]-1 of the packed tensors
+// [heads, tokens, d].  Row i of n queries over m keys sees keys j < m - n + i + 1 (causal) or j < m.
+#pragma once
+#include "attn_tile.h"
+#include "launch.h"
+
+namespace lvar {
+
+struct PackedParams {
+  const bf16_t *q, *k, *v;
+  int64_t q_sh, q_sr, k_sh, k_sr, v_sh, v_sr;
+  bf16_t* o;                        // [H,T,d], strides o_sh, o_sr
+  int64_t o_sh, o_sr;
+  float *M, *L;                     // [H,T]
+  const int32_t *q_off, *k_off;     // [B+1]
+  int B, T, Tk, H, Hkv, G, causal;
+  float c, scale;                   // c = scale * log2(e)
+  // backward
+  const bf16_t* g;                  // gradient of o
+  int64_t g_sh, g_sr;
+  bf16_t *dq, *dk, *dv;             // null: not wanted
+  int64_t dq_sh, dq_sr, dk_sh, dk_sr, dv_sh, dv_sr;
+  float *nl, *nd;                   // [H,T]: -(M + log2 L) / c (-inf: the row sees nothing), -sum(do * o)
+  int slots;                        // set at launch: places for tiles, see find_tile
+};
+
+int launch_packed_fwd(PackedParams p, int head_dim, hipStream_t s);
+int launch_packed_bwd(PackedParams p, int head_dim, hipStream_t s);
+
+// Tiles of R rows of T packed rows in B sequences: the ranges between sequence borders, one ahead of the first sequence and one
+// behind the last included, have at most these many.
+inline int64_t packed_slots(int T, int B, int R) { return (int64_t)T / R + B + 2; }
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+struct PackedTile {
+  int b;         // sequence, or -1: rows of no sequence
+  int first, n;  // its first row and how many it has
+  int row0;      // first row of the tile within it
+};
+
+// Border v of the B + 3 borders of T rows: 0, the offsets, T.  (Offsets out of range, a caller's mistake, stay in it.)
+__device__ __forceinline__ int packed_border(const int32_t* off, int B, int T, int v) {
+  if (v <= 0) return 0;
+  return v > B + 1 ? T : max(0, min(off[v - 1], T));
+}
+
+// The range and tile of place `slot`.  Range v takes the places from floor(border(v) / R) + v on: a range of n rows starting anywhere
+// has at most floor((border + n) / R) - floor(border / R) + 1 tiles, so its places suffice, and which range a place belongs to
+// is found among the borders without knowing the lengths in between: 64 candidates per step.  False: a place without a tile.
+template <int R>
+__device__ __forceinline__ bool find_tile(const int32_t* off, int B, int T, int slot, PackedTile& t) {
+  const int lane = __builtin_amdgcn_workitem_id_x() & 63;
+  int v = 0, n = B + 2;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, at = v + lane * step;
+    const bool in = lane * step < n;
+    const int e = packed_border(off, B, T, in ? at : 0);
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(in && e / R + at <= slot);
+    const int k = mine ? 63 - __builtin_clzll(mine) : 0;
+    v += k * step;
+    n = min(step, n - k * step);
+  }
+  v = __builtin_amdgcn_readfirstlane(v);
+  t.first = __builtin_amdgcn_readfirstlane(packed_border(off, B, T, v));
+  t.n = __builtin_amdgcn_readfirstlane(packed_border(off, B, T, v + 1)) - t.first;
+  t.row0 = (slot - (t.first / R + v)) * R;
+  t.b = v >= 1 && v <= B ? v - 1 : -1;
+  return t.row0 >= 0 && t.row0 < t.n;
+}
+
+// Rows of a sequence on the other side (keys of a query tile, queries of a key tile); none for rows of no sequence.
+__device__ __forceinline__ void packed_range(const int32_t* off, int b, int T, int& first, int& n) {
+  first = n = 0;
+  if (b < 0) return;
+  first = __builtin_amdgcn_readfirstlane(max(0, min(off[b], T)));
+  n = max(0, __builtin_amdgcn_readfirstlane(max(0, min(off[b + 1], T))) - first);
+}
+
+// Rows of D bf16 in LDS, unpadded (an LDS fill writes 1 KiB of consecutive bytes), the 16-byte chunks of a row moved by an XOR that suits both
+// ways of reading: 16 consecutive rows, one chunk each (ds_read_b128), lie on all banks, since the XOR is another one for every
+// row of 16 (of 8 pairs of rows at D = 64); and 4 consecutive rows, one 64-byte segment each (transposing reads), too, since its upper
+// bits, which move segments, are the lower bits of the row.
+template <int D>
+struct PackedLds {
+  static constexpr int ROWB = D * 2, CPR = ROWB / 16, RPI = 1024 / ROWB, NI = 64 / RPI, TILE = 64 * ROWB;
+  __device__ static __forceinline__ int swz(int row) {
+    return D >= 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  }
+  int row_at, tr_at;   // byte offsets of this lane's reads
+  __device__ __forceinline__ PackedLds(int lane) {
+    const int hh = lane >> 5, r = lane & 31, sq = (lane & 15) >> 2, sm = lane & 3;
+    row_at = r * ROWB + ((hh ^ swz(r)) << 4);
+    tr_at = (4 * hh + sq) * ROWB + (((((lane >> 4) & 1) << 1 | (sm >> 1)) ^ swz(4 * hh + sq)) << 4) + (sm & 1) * 8;
+  }
+  // A operand of rows 32 sub .. +31, columns 16 ks .. +15
+  __device__ __forceinline__ bf16x8 rows(const char* buf, int sub, int ks) const {
+    return *(const bf16x8*)(buf + (row_at ^ (ks << 5)) + sub * 32 * ROWB);
+  }
+  // A operand of columns 32 m .. +31 (as rows) over rows 16 kb .. +15, in the order in which accumulators hold them
+  __device__ __forceinline__ bf16x8 columns(const char* buf, int kb, int m) const {
+    const char* a = buf + kb * 16 * ROWB;
+    const int at = tr_at ^ (m << 6);
+    const bf16x4 lo = lds_read_tr(a + at), hi = lds_read_tr(a + (at ^ 32) + 8 * ROWB);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+// Raw buffer descriptor of n rows (bytes below 2^31, checked on the host): what lies beyond reads as zeros.
+__device__ __forceinline__ i32x4 packed_rsrc(const bf16_t* base, int n, int row_bytes, int stride_bytes) {
+  const uint64_t a = (uint64_t)base;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(uint32_t)((a >> 32) & 0xffffu)),
+               __builtin_amdgcn_readfirstlane(n > 0 ? (n - 1) * stride_bytes + row_bytes : 0), 0x00020000};
+}
+
+// One of the fills of rows row0 .. row0 + 63 into LDS at byte address dst: the s-th of the NI / NW that a wave issues.  Inline assembly, so that
+// the compiler does not make LDS reads of other buffers wait for it; wait_fills() before the barrier does.
+template <int D, int NW>
+__device__ __forceinline__ void fill_slot(const i32x4& rsrc, int srb, int row0, uint32_t dst, int wave, int lane, int s) {
+  using S = PackedLds<D>;
+  static_assert(S::NI % NW == 0, "every wave issues as many fills");
+  // the XOR has a period of 16 rows: fills whose rows are whole periods apart share the lane's offset
+  constexpr int PER = NW * S::RPI >= 16 ? 1 : 16 / (NW * S::RPI);
+  const int lrow = lane / S::CPR, lcs = lane % S::CPR;
+  const int trow = (wave + (s % PER) * NW) * S::RPI + lrow;
+  const int voff = trow * srb + ((lcs ^ S::swz(trow)) << 4);
+  const int soff = (row0 + (s / PER) * PER * NW * S::RPI) * srb;
+  const uint32_t m0v = dst + (wave + s * NW) * 1024;
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(m0v), "v"(voff), "s"(rsrc), "s"(soff)
+      : "memory");
+}
+template <int D, int NW>
+__device__ __forceinline__ void fill_tile(const i32x4& rsrc, int srb, int row0, uint32_t dst, int wave, int lane) {
+#pragma unroll
+  for (int s = 0; s < PackedLds<D>::NI / NW; s++) fill_slot<D, NW>(rsrc, srb, row0, dst, wave, lane, s);
+}
+
+// Head of place j of H: with a multiple of 8 heads, those of an XCD (workgroups are dealt to the 8 in turn) are neighbours, which share keys and values.
+__device__ __forceinline__ int packed_head(int j, int H) { return (H & 7) == 0 ? (j & 7) * (H >> 3) + (j >> 3) : j; }
+
+// Is x infinite or NaN?  (On the bits: float comparisons may assume that there are none.)
+__device__ __forceinline__ bool not_finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) == 0x7f800000u; }
+
+// The transposed accumulators of a wave, 32 rows of D columns, as bf16 rows: through LDS (32 * (2 D + 16) bytes at `buf`, this wave's
+// own), so that rows are stored in 16-byte pieces.  rows < n are stored.
+template <int D, int MT>
+__device__ __forceinline__ void store_rows(char* buf, const f32x16 (&acc)[MT], float factor, bf16_t* to, int64_t stride, int n, int lane) {
+  static_assert(MT * 32 == D, "all columns");
+  constexpr int STR = D * 2 + 16, CPR = D / 8;
+  const int hh = lane >> 5, r = lane & 31;
+#pragma unroll
+  for (int m = 0; m < MT; m++)
+#pragma unroll
+    for (int a = 0; a < 4; a++) {
+      const u32x2 pk = {pack_bf16(acc[m][4 * a] * factor, acc[m][4 * a + 1] * factor), pack_bf16(acc[m][4 * a + 2] * factor, acc[m][4 * a + 3] * factor)};
+      *(u32x2*)(buf + r * STR + (m * 32 + 8 * a + 4 * hh) * 2) = pk;
+    }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < 32 * CPR / 64; i++) {
+    const int at = lane + i * 64, row = at / CPR, chunk = at - row * CPR;
+    const u32x4 x = *(const u32x4*)(buf + row * STR + chunk * 16);
+    if (row < n) *(u32x4*)(to + row * stride + chunk * 8) = x;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+#endif  // __HIP_DEVICE_COMPILE__
+
+}  // namespace lvar

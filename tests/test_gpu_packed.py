@@ -1,0 +1,109 @@
+"""Attention over packed sequences and its gradients on the GPU, against the 64-bit oracle, whose tolerances count roundings: half a step of
+bf16 (2^-8 of the value) for each result, each probability and each of their gradients, 2^-24 for each term of a sum in 32 bits."""
+import math
+
+import pytest
+import torch
+
+from oracle import packed_oracle as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(*shape, seed=0, amp=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * amp).to(torch.bfloat16)
+
+
+def starts(lengths, first=0):
+    at = [first]
+    for n in lengths:
+        at.append(at[-1] + n)
+    return at
+
+
+def inputs(lens, klens, H, Hkv, d, lead=0, tail=0, seed=0, amp=1.0):
+    """q, k, v as views on one fused projection (or q, and k and v, on one each), and the offsets."""
+    off = starts(lens, lead)
+    T = off[-1] + tail
+    if klens is None:
+        x = rand(1, T, H + 2 * Hkv, d, seed=seed, amp=amp).transpose(1, 2)
+        return x[:, :H], x[:, H:H + Hkv], x[:, H + Hkv:], off, None
+    koff = starts(klens, lead)
+    kv = rand(1, koff[-1] + tail, 2 * Hkv, d, seed=seed + 1, amp=amp).transpose(1, 2)
+    return rand(1, T, H, d, seed=seed, amp=amp).transpose(1, 2), kv[:, :Hkv], kv[:, Hkv:], off, koff
+
+
+def i32(x):
+    return None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def near(got, want, tol, what):
+    err = (got.detach().double().cpu() - want).abs()
+    bad = ~(err <= tol) & ~((got.detach().double().cpu() == want))
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} off, at {bad.nonzero()[0].tolist()} by {float(err[bad][0]):.3g} of {float(tol[bad][0]):.3g}"
+
+
+CASES = [
+    # lengths, key lengths (None: the same), H, Hkv, d, causal, rows ahead and behind
+    ([1], None, 1, 1, 64, True, 0, 0),
+    ([77], None, 3, 3, 64, True, 0, 0),
+    ([64], None, 2, 1, 128, False, 0, 0),
+    ([128, 1, 63], None, 4, 2, 128, True, 0, 0),
+    ([0, 5, 0, 0, 130, 3], None, 8, 8, 64, True, 3, 7),
+    ([257, 66], None, 6, 2, 128, True, 0, 1),
+    ([300], None, 8, 1, 128, True, 0, 0),
+    ([33, 190], None, 4, 4, 256, True, 2, 2),
+    ([129], None, 4, 2, 256, False, 0, 0),
+    ([40, 200, 1], [300, 7, 65], 4, 4, 128, False, 0, 0),
+    ([40, 200, 1, 9], [300, 7, 65, 0], 4, 2, 64, True, 1, 5),       # rows that see no key, in the middle of a tile and everywhere
+    ([5, 0, 100], [0, 50, 333], 2, 2, 256, True, 0, 0),
+    ([17] * 70, None, 2, 1, 64, True, 0, 0),                          # more borders than a wave has lanes
+    ([700], None, 2, 2, 64, False, 0, 0),
+    ([520, 260], None, 2, 1, 128, True, 0, 0),
+    ([10, 90], [20, 70], 3, 1, 16, True, 0, 0),
+    ([70], None, 2, 2, 32, False, 0, 0),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: str(c).replace(" ", "")[:60])
+def test_forward(case):
+    from lvar_amd.packed_ops import packed_attn
+    lens, klens, H, Hkv, d, causal, lead, tail = case
+    q, k, v, off, koff = inputs(lens, klens, H, Hkv, d, lead, tail, seed=sum(lens))
+    o, (M, L) = packed_attn(q.cuda(), k.cuda(), v.cuda(), i32(off), i32(koff), causal=causal)
+    r = ref.packed_attn(q, k, v, off, koff, causal=causal)
+    assert o.dtype == torch.bfloat16 and o.shape == q.shape and M.shape == L.shape == (1, H, q.shape[2], 1)
+    for name, x in (("o", o), ("M", M), ("L", L)):
+        near(x, r[name], r["t_" + name], name)
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: str(c).replace(" ", "")[:60])
+def test_gradients(case):
+    from lvar_amd.packed_ops import packed_attn
+    lens, klens, H, Hkv, d, causal, lead, tail = case
+    q, k, v, off, koff = inputs(lens, klens, H, Hkv, d, lead, tail, seed=sum(lens) + 1)
+    go = rand(1, q.shape[2], H, d, seed=5).transpose(1, 2)
+    leaves = [x.cuda().detach().requires_grad_() for x in (q, k, v)]
+    o, (M, L) = packed_attn(*leaves, i32(off), i32(koff), scale=0.9 / math.sqrt(d), causal=causal)
+    assert o.requires_grad and not M.requires_grad and not L.requires_grad
+    grads = torch.autograd.grad(o, leaves, go.cuda())
+    r = ref.packed_attn(q, k, v, off, koff, scale=0.9 / math.sqrt(d), causal=causal, go=go)
+    near(o, r["o"], r["t_o"], "o")
+    for name, x, leaf in zip(("dq", "dk", "dv"), grads, leaves):
+        assert x.dtype == torch.bfloat16 and x.shape == leaf.shape
+        near(x, r[name], r["t_" + name], name)
+
+
+@pytest.mark.parametrize("amp", [1e-3, 6.0])
+def test_flat_and_peaked_rows(amp):
+    """Scores around 0, and of hundreds (probabilities of 0 and 1, a maximum that keeps rising)."""
+    from lvar_amd.packed_ops import packed_attn
+    q, k, v, off, _ = inputs([150, 400], None, 4, 2, 128, seed=3, amp=amp)
+    k = k * torch.linspace(0.1, 3, k.shape[2])[None, None, :, None].to(torch.bfloat16)
+    go = rand(*q.shape, seed=8)
+    leaves = [x.cuda().detach().requires_grad_() for x in (q, k, v)]
+    o, (M, L) = packed_attn(*leaves, i32(off))
+    grads = torch.autograd.grad(o, leaves, go.cuda())
+    r = ref.packed_attn(q, k, v, off, go=go)
+    for name, x in (("o", o), ("M", M), ("L", L), ("dq", grads[0]), ("dk", grads[1]), ("dv", grads[2])):
+        near(x, r[name], r["t_" + name], name)
