@@ -465,11 +465,64 @@ int lvar_kv_cache_append(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, cons
                          const int32_t* start, const int32_t* counts, int B, int H, int L, void* stream);
 
 /*
+ * Rotation by angles that come from several position axes (rows and columns of an image, time of a video): pair i of token t is turned by
+ * sum over a < axes of positions[a, t] * freqs[a, i] radians, the sum formed in 64 bits.  freqs [axes, rot_dim/2] fp64 (freq_type 0) or
+ * fp32 (1), 16-byte aligned rows; positions int32, int64 or fp32 (position_type), strides in elements, 0 broadcasts.  1 to 8 axes.
+ * The eager counterpart: the two-dimensional grid of models/sparvar/basic_sparvar.py:326-342, whose positions are fractions at small scales.
+ */
+#define LVAR_POSITIONS_I32 0
+#define LVAR_POSITIONS_I64 1
+#define LVAR_POSITIONS_F32 2
+typedef struct {
+  const void* freqs;
+  int64_t freq_stride;
+  int freq_type, axes, rot_dim, interleaved;
+  const void* positions;
+  int64_t pos_stride_b, pos_stride_axis, pos_stride_row;
+  int position_type;
+} lvar_rope_axes_t;
+
+/* lvar_qk_norm_rope_fwd, lvar_qk_norm_rope_bwd (its scratch too) and lvar_kv_cache_append with such a rotation; how.cos and how.sin NULL. */
+int lvar_qk_norm_axes_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, lvar_rope_axes_t axes, void* oq, void* ok, int B, int H,
+                          int kv_heads, int L, int head_dim, void* stream);
+int lvar_qk_norm_axes_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, lvar_rope_axes_t axes, const void* gq, const void* gk,
+                          lvar_tensor_t dq, lvar_tensor_t dk, void* dqw, void* dkw, void* scratch, int64_t scratch_bytes, int B, int H,
+                          int kv_heads, int L, int head_dim, void* stream);
+int lvar_kv_cache_append_axes(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar_norm_rope_t how, lvar_rope_axes_t axes, void* oq,
+                              lvar_paged_cache_t cache, const int32_t* start, const int32_t* counts, int B, int H, int L, void* stream);
+
+/*
  * Tokens start[b] .. start[b] + max_len - 1 of the cache (start NULL: 0) as contiguous bf16 k, v [B,kv_heads,max_len,d]; zeros from
  * lengths[b] on.
  */
 int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int32_t* lengths, void* k, void* v, int B, int max_len,
                        void* stream);
+
+/*
+ * The life of pages.  page_table [rows, max_pages] (row stride table_stride, at least max_pages) names pages of a pool of num_pages, refs
+ * [num_pages] counts how many of its entries name each page; a page is free where that is not positive.  Entries outside the pool
+ * name no page.  All of it is read and written on the device, in place; at most 65535 rows and forks.
+ *   lvar_kv_pages_alloc   entries first[r] .. last[r]-1 (clamped to the row) of every row r get the lowest free pages in order of rows and
+ *                         entries, counted once; -1 where there are no more.  What the entries named before is not looked at.
+ *   lvar_kv_pages_free    entries from keep[r] on (NULL: all) become -1, their pages are counted down.
+ *   lvar_kv_cache_fork    row target[i] gets the first lengths[source[i]] tokens of row source[i] (lengths [rows]): its whole pages by name,
+ *                         counted up, the tokens of the page that is not whole in the lowest free page; -1 behind it.  What the row
+ *                         named before is not looked at (free it first).  Pairs outside the table, and of a row with itself, are left out.
+ *                         Two forks with one target, or a target that is a source, leave these rows undefined.
+ * scratch: lvar_kv_pages_scratch_bytes(rows or forks, num_pages) (4-byte aligned, needs no preparation; may be 0).
+ *   lvar_kv_cache_compact token i < n (counts[b], NULL: all n) of head h of the pages of out_table's row b gets the bytes of token
+ *                         keep[b, h, i] (int32, or int64 if keep64; strides in elements) of page_table's row b; zeros where that names no token.
+ *                         A page that both tables name is undefined.
+ */
+int64_t lvar_kv_pages_scratch_bytes(int rows, int num_pages);
+int lvar_kv_pages_alloc(int32_t* refs, int num_pages, int32_t* page_table, int64_t table_stride, int rows, int max_pages, const int32_t* first,
+                        const int32_t* last, void* scratch, int64_t scratch_bytes, void* stream);
+int lvar_kv_pages_free(int32_t* refs, int num_pages, int32_t* page_table, int64_t table_stride, int rows, int max_pages, const int32_t* keep,
+                       void* stream);
+int lvar_kv_cache_fork(lvar_paged_cache_t cache, int32_t* refs, int32_t* page_table, int rows, const int32_t* source, const int32_t* target,
+                       const int32_t* lengths, int forks, void* scratch, int64_t scratch_bytes, void* stream);
+int lvar_kv_cache_compact(lvar_paged_cache_t cache, const int32_t* out_table, int64_t out_stride, int out_pages, const void* keep, int keep64,
+                          int64_t keep_stride_b, int64_t keep_stride_head, int64_t keep_stride, const int32_t* counts, int B, int n, void* stream);
 
 /*
  * Attention of the newest Lq tokens q [B,H,Lq,d] (bf16 view) over the first lengths[b] tokens of the cache, which hold them already:

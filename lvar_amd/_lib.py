@@ -22,6 +22,8 @@ EXPORTED_SYMBOLS = (
     "lvar_window_key_scores",
     "lvar_qk_norm_rope_fwd", "lvar_qk_norm_rope_bwd_scratch_bytes", "lvar_qk_norm_rope_bwd", "lvar_kv_cache_append", "lvar_kv_cache_read",
     "lvar_paged_attn_workspace_bytes", "lvar_paged_attn_fwd",
+    "lvar_qk_norm_axes_fwd", "lvar_qk_norm_axes_bwd", "lvar_kv_cache_append_axes",
+    "lvar_kv_pages_scratch_bytes", "lvar_kv_pages_alloc", "lvar_kv_pages_free", "lvar_kv_cache_fork", "lvar_kv_cache_compact",
     "lvar_packed_attn_fwd", "lvar_packed_attn_bwd_workspace_bytes", "lvar_packed_attn_bwd",
 )
 
@@ -49,6 +51,11 @@ class LvarNormRope(C.Structure):
     _fields_ = [("norm", C.c_int), ("eps", C.c_float), ("q_weight", LvarWeight), ("k_weight", LvarWeight), ("cos", C.c_void_p), ("sin", C.c_void_p),
                 ("table_stride", C.c_int64), ("table_rows", C.c_int), ("rot_dim", C.c_int), ("interleaved", C.c_int), ("positions", C.c_void_p),
                 ("pos_stride_b", C.c_int64), ("pos_stride_row", C.c_int64), ("positions64", C.c_int)]
+
+
+class LvarRopeAxes(C.Structure):
+    _fields_ = [("freqs", C.c_void_p), ("freq_stride", C.c_int64), ("freq_type", C.c_int), ("axes", C.c_int), ("rot_dim", C.c_int), ("interleaved", C.c_int),
+                ("positions", C.c_void_p), ("pos_stride_b", C.c_int64), ("pos_stride_axis", C.c_int64), ("pos_stride_row", C.c_int64), ("position_type", C.c_int)]
 
 
 class LvarError(RuntimeError):
@@ -137,12 +144,29 @@ def load() -> C.CDLL:
     lib.lvar_qk_norm_rope_bwd.argtypes = [T, T, N, P, P, T, T, P, P, P, I64, I, I, I, I, I, P]
     lib.lvar_kv_cache_append.restype = I
     lib.lvar_kv_cache_append.argtypes = [T, T, T, P, P, G, P, P, I, I, I, P]
+    X = LvarRopeAxes
+    lib.lvar_qk_norm_axes_fwd.restype = I
+    lib.lvar_qk_norm_axes_fwd.argtypes = [T, T, N, X, P, P, I, I, I, I, I, P]
+    lib.lvar_qk_norm_axes_bwd.restype = I
+    lib.lvar_qk_norm_axes_bwd.argtypes = [T, T, N, X, P, P, T, T, P, P, P, I64, I, I, I, I, I, P]
+    lib.lvar_kv_cache_append_axes.restype = I
+    lib.lvar_kv_cache_append_axes.argtypes = [T, T, T, N, X, P, G, P, P, I, I, I, P]
     lib.lvar_kv_cache_read.restype = I
     lib.lvar_kv_cache_read.argtypes = [G, P, P, P, P, I, I, P]
     lib.lvar_paged_attn_workspace_bytes.restype = I64
     lib.lvar_paged_attn_workspace_bytes.argtypes = [I, I, I, I, I, I]
     lib.lvar_paged_attn_fwd.restype = I
     lib.lvar_paged_attn_fwd.argtypes = [T, G, P, P, P, P, P, P, I64, I, I, I, I, I, F, P]
+    lib.lvar_kv_pages_scratch_bytes.restype = I64
+    lib.lvar_kv_pages_scratch_bytes.argtypes = [I, I]
+    lib.lvar_kv_pages_alloc.restype = I
+    lib.lvar_kv_pages_alloc.argtypes = [P, I, P, I64, I, I, P, P, P, I64, P]
+    lib.lvar_kv_pages_free.restype = I
+    lib.lvar_kv_pages_free.argtypes = [P, I, P, I64, I, I, P, P]
+    lib.lvar_kv_cache_fork.restype = I
+    lib.lvar_kv_cache_fork.argtypes = [G, P, P, I, P, P, P, I, P, I64, P]
+    lib.lvar_kv_cache_compact.restype = I
+    lib.lvar_kv_cache_compact.argtypes = [G, P, I64, I, P, I, I64, I64, I64, P, I, I, P]
     lib.lvar_packed_attn_fwd.restype = I
     lib.lvar_packed_attn_fwd.argtypes = [T, T, T, T, P, P, P, P, I, I, I, I, I, I, I, F, P]
     lib.lvar_packed_attn_bwd_workspace_bytes.restype = I64

@@ -19,7 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "liblvar_sparse_attn.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["attn_fwd.hip", "colsum.hip", "rowlse.hip", "blockscore.hip", "masklist.hip", "listbuild.hip", "windowscore.hip", "capi.hip",
-           "normrope.hip", "kvread.hip", "pagedattn.hip", "kvcapi.hip",
+           "normrope.hip", "kvread.hip", "pagedattn.hip", "pages.hip", "kvcapi.hip",
            "packedattn.hip", "packedbwd.hip", "packedapi.hip"]
 ARCH = "gfx950"
 # -packed-fp32-ops is switched off: hipcc must not form v_pk_{add,mul,fma}_f32 from float code
@@ -27,7 +27,7 @@ ARCH = "gfx950"
 HIPCC_FLAGS = ["-O3", f"--offload-arch={ARCH}", "-fPIC", "-std=c++17", "-fno-honor-nans", "-mno-amdgpu-ieee",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # these keep NaN as NaN (a cache may hold some in places that nobody reads, and what is read has to show them)
-HONOR_NANS = ("normrope.hip", "kvread.hip", "pagedattn.hip", "kvcapi.hip", "packedapi.hip")
+HONOR_NANS = ("normrope.hip", "kvread.hip", "pagedattn.hip", "pages.hip", "kvcapi.hip", "packedapi.hip")
 
 
 def _hipcc() -> str:

@@ -46,6 +46,9 @@ struct NormRopeParams {
   const void* positions;         // int32 or int64, strides in elements; null: the row's own number (plus start[b])
   int64_t pos_sb, pos_sl;
   int pos64;
+  const void* freqs;             // [axes, rot/2] radians per unit of position, fp64 or fp32 (freq32); null: cos and sin, or no rotation
+  int64_t freq_sa, pos_sa;       // then positions are [B or 1, axes, L]: int32, int64 or (pos64 = 2) fp32
+  int axes, freq32;
   int B, H, Hkv, L;
   uint32_t div_mul;              // division by L, set at launch
   int div_s1, div_s2;
@@ -97,6 +100,24 @@ struct PagedAttnParams {
   int64_t ws_head;                // floats ahead of the partial results
 };
 
+// pages of a table, and how many of its entries name each
+struct PagesParams {
+  int32_t *table, *refs, *scratch;
+  int64_t table_stride;
+  int rows, max_pages, num_pages, shift;    // rows of the table, entries of one
+  const int32_t *first, *last;              // alloc: entries of each row; free: first is where a row is cut (null: 0)
+  const int32_t *source, *target, *lengths; // fork
+  int n;                                    // rows (alloc), forks (fork)
+};
+
+struct CompactParams {
+  PagedView cache, out;                     // the same pages under two tables
+  const void* keep;                         // [B, heads, n], strides in elements
+  int64_t keep_sb, keep_sh, keep_si;
+  int keep64, n;
+  const int32_t* counts;
+};
+
 constexpr int NB_HC = 2;   // heads of a workgroup of the norm's backward pass
 
 // A launch has at most 2^32 - 1 threads along x.
@@ -108,6 +129,11 @@ int launch_norm_rope_bwd(NormRopeParams p, int head_dim, hipStream_t s);
 int launch_weight_grad(const WeightGradParams& w, hipStream_t s);
 int launch_kv_read(const KvReadParams& p, int head_dim, hipStream_t s);
 int64_t paged_attn_ws_bytes(int B, int H, int Hkv, int Lq, int max_len, int head_dim);
+int64_t pages_scratch_ints(int rows, int num_pages);
+int launch_pages_alloc(const PagesParams& p, hipStream_t s);
+int launch_pages_free(const PagesParams& p, hipStream_t s);
+int launch_pages_fork(const PagesParams& p, const PagedView& c, int row_bytes, hipStream_t s);
+int launch_pages_compact(const CompactParams& p, int B, int row_bytes, hipStream_t s);
 int launch_paged_attn(PagedAttnParams p, void* workspace, int64_t workspace_bytes, int head_dim, hipStream_t s);
 
 template <int CTRL>

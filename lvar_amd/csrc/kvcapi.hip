@@ -53,6 +53,18 @@ int fill_how(NormRopeParams& p, const lvar_norm_rope_t& how, int head_dim) {
   return LVAR_OK;
 }
 
+int fill_axes(NormRopeParams& p, const lvar_rope_axes_t* ax, int B, int head_dim) {
+  if (!ax) return LVAR_OK;
+  if (p.cos || !ax->freqs || !ax->positions || ax->axes <= 0 || ax->axes > 8 || ax->rot_dim <= 0 || ax->rot_dim > head_dim) return LVAR_EINVAL;
+  if (ax->rot_dim % 16 != 0) return LVAR_EUNSUPPORTED;
+  if (ax->position_type < LVAR_POSITIONS_I32 || ax->position_type > LVAR_POSITIONS_F32 || (ax->freq_type != 0 && ax->freq_type != 1)) return LVAR_EINVAL;
+  if (!aligned(ax->freqs, 16) || ax->freq_stride % (ax->freq_type ? 4 : 2) != 0) return LVAR_EINVAL;
+  if (!aligned(ax->positions, ax->position_type == LVAR_POSITIONS_I64 ? 8 : 4)) return LVAR_EINVAL;
+  p.freqs = ax->freqs; p.freq_sa = ax->freq_stride; p.freq32 = ax->freq_type; p.axes = ax->axes; p.rot = ax->rot_dim; p.interleaved = ax->interleaved ? 1 : 0;
+  p.positions = ax->positions; p.pos64 = ax->position_type; p.pos_sb = B > 1 ? ax->pos_stride_b : 0; p.pos_sa = ax->pos_stride_axis; p.pos_sl = ax->pos_stride_row;
+  return LVAR_OK;
+}
+
 void fill_qk(NormRopeParams& p, const lvar_tensor_t& q, const lvar_tensor_t& k, int B, int H, int kv_heads, int L) {
   p.q = (const bf16_t*)q.ptr; p.q_sb = q.stride_b; p.q_sh = q.stride_h; p.q_sr = q.stride_row;
   p.k = (const bf16_t*)k.ptr; p.k_sb = k.stride_b; p.k_sh = k.stride_h; p.k_sr = k.stride_row;
@@ -85,24 +97,20 @@ int fill_cache(PagedView& v, const lvar_paged_cache_t& c) {
 int grad_rows(const WeightView& w, int heads, int nblk) { return w.s_head == 0 ? nblk * ((heads + NB_HC - 1) / NB_HC) : nblk; }
 int64_t grad_floats(int heads, int nblk, int d) { return (int64_t)nblk * heads * d; }   // (the larger of the two forms)
 
-}  // namespace
-
-extern "C" {
-
-int lvar_qk_norm_rope_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, void* oq, void* ok, int B, int H, int kv_heads,
-                          int L, int head_dim, void* stream) {
+int norm_rope_fwd(lvar_tensor_t q, lvar_tensor_t k, const lvar_norm_rope_t& how, const lvar_rope_axes_t* ax, void* oq, void* ok, int B, int H, int kv_heads, int L,
+                  int head_dim, void* stream) {
   int st = sizes_ok(B, H, kv_heads, L);
   if (st != LVAR_OK) return st;
   if (!rows_ok(q) || !rows_ok(k) || !oq || !ok || !aligned(oq, 16) || !aligned(ok, 16)) return LVAR_EINVAL;
   if (!norm_head_dim(head_dim)) return LVAR_EUNSUPPORTED;
   NormRopeParams p{};
   fill_qk(p, q, k, B, H, kv_heads, L);
-  if ((st = fill_how(p, how, head_dim)) != LVAR_OK) return st;
+  if ((st = fill_how(p, how, head_dim)) != LVAR_OK || (st = fill_axes(p, ax, B, head_dim)) != LVAR_OK) return st;
   p.oq = (bf16_t*)oq; p.ok = (bf16_t*)ok;
   return launch_norm_rope(p, head_dim, false, (hipStream_t)stream);
 }
 
-int64_t lvar_qk_norm_rope_bwd_scratch_bytes(int B, int H, int kv_heads, int L, int head_dim) {
+int64_t scratch_bytes(int B, int H, int kv_heads, int L, int head_dim) {
   const int st = sizes_ok(B, H, kv_heads, L);
   if (st != LVAR_OK) return st;
   if (!norm_head_dim(head_dim)) return LVAR_EUNSUPPORTED;
@@ -111,8 +119,8 @@ int64_t lvar_qk_norm_rope_bwd_scratch_bytes(int B, int H, int kv_heads, int L, i
   return 4 * grad_floats(H + kv_heads, nblk, head_dim);
 }
 
-int lvar_qk_norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, const void* gq, const void* gk, lvar_tensor_t dq,
-                          lvar_tensor_t dk, void* dqw, void* dkw, void* scratch, int64_t scratch_bytes, int B, int H,
+int norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, const lvar_norm_rope_t& how, const lvar_rope_axes_t* ax, const void* gq, const void* gk, lvar_tensor_t dq,
+                          lvar_tensor_t dk, void* dqw, void* dkw, void* scratch, int64_t bytes, int B, int H,
                           int kv_heads, int L, int head_dim, void* stream) {
   int st = sizes_ok(B, H, kv_heads, L);
   if (st != LVAR_OK) return st;
@@ -121,13 +129,13 @@ int lvar_qk_norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how
   if (!norm_head_dim(head_dim)) return LVAR_EUNSUPPORTED;
   NormRopeParams p{};
   fill_qk(p, q, k, B, H, kv_heads, L);
-  if ((st = fill_how(p, how, head_dim)) != LVAR_OK) return st;
+  if ((st = fill_how(p, how, head_dim)) != LVAR_OK || (st = fill_axes(p, ax, B, head_dim)) != LVAR_OK) return st;
   p.gq = (const bf16_t*)gq; p.gk = (const bf16_t*)gk;
   p.dq = (bf16_t*)dq.ptr; p.dq_sb = dq.stride_b; p.dq_sh = dq.stride_h; p.dq_sr = dq.stride_row;
   p.dk = (bf16_t*)dk.ptr; p.dk_sb = dk.stride_b; p.dk_sh = dk.stride_h; p.dk_sr = dk.stride_row;
   // (a weight whose heads do not differ in memory gets one gradient for all of them)
   if (dqw || dkw) {
-    if (!scratch || !aligned(scratch, 16) || scratch_bytes < lvar_qk_norm_rope_bwd_scratch_bytes(B, H, kv_heads, L, head_dim)) return LVAR_EINVAL;
+    if (!scratch || !aligned(scratch, 16) || bytes < scratch_bytes(B, H, kv_heads, L, head_dim)) return LVAR_EINVAL;
   }
   const WeightView* wv[2] = {&p.wq, &p.wk};
   void* out[2] = {dqw, dkw};
@@ -159,7 +167,7 @@ int lvar_qk_norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how
   return launch_weight_grad(w, (hipStream_t)stream);
 }
 
-int lvar_kv_cache_append(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, const lvar_norm_rope_t* how, void* oq, lvar_paged_cache_t cache,
+int append(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, const lvar_norm_rope_t* how, const lvar_rope_axes_t* ax, void* oq, lvar_paged_cache_t cache,
                          const int32_t* start, const int32_t* counts, int B, int H, int L, void* stream) {
   NormRopeParams p{};
   int st = fill_cache(p.cache, cache);
@@ -170,11 +178,65 @@ int lvar_kv_cache_append(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, cons
   if (how && (!rows_ok(q) || !aligned(oq, 16))) return LVAR_EINVAL;
   fill_qk(p, q, k, B, H, cache.kv_heads, L);
   p.v = (const bf16_t*)v.ptr; p.v_sb = v.stride_b; p.v_sh = v.stride_h; p.v_sr = v.stride_row;
-  if (how && (st = fill_how(p, *how, cache.head_dim)) != LVAR_OK) return st;
+  if (how && ((st = fill_how(p, *how, cache.head_dim)) != LVAR_OK || (st = fill_axes(p, ax, B, cache.head_dim)) != LVAR_OK)) return st;
   p.ready = how ? 0 : 1;
   p.oq = (bf16_t*)oq;
   p.start = start; p.counts = counts;
   return launch_norm_rope(p, cache.head_dim, true, (hipStream_t)stream);
+}
+
+// a table whose pages are counted
+int fill_pages(PagesParams& p, int32_t* refs, int num_pages, int32_t* table, int64_t table_stride, int rows, int max_pages) {
+  if (!refs || !table || !aligned(refs, 4) || !aligned(table, 4) || num_pages <= 0 || num_pages > kMostTokens || rows <= 0 || rows > 65535 || max_pages <= 0 ||
+      max_pages > kMostTokens || table_stride < 0 || (rows > 1 && table_stride < max_pages))
+    return LVAR_EINVAL;
+  p.refs = refs; p.num_pages = num_pages; p.table = table; p.table_stride = table_stride; p.rows = rows; p.max_pages = max_pages;
+  return LVAR_OK;
+}
+
+int fill_scratch(PagesParams& p, void* scratch, int64_t bytes) {
+  const int64_t ints = pages_scratch_ints(p.n, p.num_pages);
+  if (ints > 0 && (!scratch || !aligned(scratch, 4) || bytes < 4 * ints)) return LVAR_EINVAL;
+  p.scratch = (int32_t*)scratch;
+  return LVAR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lvar_qk_norm_rope_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, void* oq, void* ok, int B, int H, int kv_heads,
+                          int L, int head_dim, void* stream) {
+  return norm_rope_fwd(q, k, how, nullptr, oq, ok, B, H, kv_heads, L, head_dim, stream);
+}
+
+int lvar_qk_norm_axes_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, lvar_rope_axes_t axes, void* oq, void* ok, int B, int H, int kv_heads,
+                          int L, int head_dim, void* stream) {
+  return norm_rope_fwd(q, k, how, &axes, oq, ok, B, H, kv_heads, L, head_dim, stream);
+}
+
+int64_t lvar_qk_norm_rope_bwd_scratch_bytes(int B, int H, int kv_heads, int L, int head_dim) { return scratch_bytes(B, H, kv_heads, L, head_dim); }
+
+int lvar_qk_norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, const void* gq, const void* gk, lvar_tensor_t dq,
+                          lvar_tensor_t dk, void* dqw, void* dkw, void* scratch, int64_t scratch_bytes, int B, int H,
+                          int kv_heads, int L, int head_dim, void* stream) {
+  return norm_rope_bwd(q, k, how, nullptr, gq, gk, dq, dk, dqw, dkw, scratch, scratch_bytes, B, H, kv_heads, L, head_dim, stream);
+}
+
+int lvar_qk_norm_axes_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, lvar_rope_axes_t axes, const void* gq, const void* gk, lvar_tensor_t dq,
+                          lvar_tensor_t dk, void* dqw, void* dkw, void* scratch, int64_t scratch_bytes, int B, int H,
+                          int kv_heads, int L, int head_dim, void* stream) {
+  return norm_rope_bwd(q, k, how, &axes, gq, gk, dq, dk, dqw, dkw, scratch, scratch_bytes, B, H, kv_heads, L, head_dim, stream);
+}
+
+int lvar_kv_cache_append(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, const lvar_norm_rope_t* how, void* oq, lvar_paged_cache_t cache,
+                         const int32_t* start, const int32_t* counts, int B, int H, int L, void* stream) {
+  return append(q, k, v, how, nullptr, oq, cache, start, counts, B, H, L, stream);
+}
+
+int lvar_kv_cache_append_axes(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar_norm_rope_t how, lvar_rope_axes_t axes, void* oq,
+                              lvar_paged_cache_t cache, const int32_t* start, const int32_t* counts, int B, int H, int L, void* stream) {
+  return append(q, k, v, &how, &axes, oq, cache, start, counts, B, H, L, stream);
 }
 
 int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int32_t* lengths, void* k, void* v, int B, int max_len,
@@ -186,6 +248,58 @@ int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int
   if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || !lengths || !aligned(lengths, 4) || !aligned(start, 4)) return LVAR_EINVAL;
   p.k = (bf16_t*)k; p.v = (bf16_t*)v; p.start = start; p.lengths = lengths; p.B = B; p.Lmax = max_len;
   return launch_kv_read(p, cache.head_dim, (hipStream_t)stream);
+}
+
+int64_t lvar_kv_pages_scratch_bytes(int rows, int num_pages) {
+  if (rows < 0 || num_pages <= 0) return LVAR_EINVAL;
+  return 4 * pages_scratch_ints(rows, num_pages);
+}
+
+int lvar_kv_pages_alloc(int32_t* refs, int num_pages, int32_t* page_table, int64_t table_stride, int rows, int max_pages, const int32_t* first,
+                        const int32_t* last, void* scratch, int64_t scratch_bytes, void* stream) {
+  PagesParams p{};
+  int st = fill_pages(p, refs, num_pages, page_table, table_stride, rows, max_pages);
+  if (st != LVAR_OK) return st;
+  if (!first || !last || !aligned(first, 4) || !aligned(last, 4)) return LVAR_EINVAL;
+  p.first = first; p.last = last; p.n = rows;
+  if ((st = fill_scratch(p, scratch, scratch_bytes)) != LVAR_OK) return st;
+  return launch_pages_alloc(p, (hipStream_t)stream);
+}
+
+int lvar_kv_pages_free(int32_t* refs, int num_pages, int32_t* page_table, int64_t table_stride, int rows, int max_pages, const int32_t* keep,
+                       void* stream) {
+  PagesParams p{};
+  const int st = fill_pages(p, refs, num_pages, page_table, table_stride, rows, max_pages);
+  if (st != LVAR_OK) return st;
+  if (!aligned(keep, 4)) return LVAR_EINVAL;
+  p.first = keep;
+  return launch_pages_free(p, (hipStream_t)stream);
+}
+
+int lvar_kv_cache_fork(lvar_paged_cache_t cache, int32_t* refs, int32_t* page_table, int rows, const int32_t* source, const int32_t* target,
+                       const int32_t* lengths, int forks, void* scratch, int64_t scratch_bytes, void* stream) {
+  PagesParams p{};
+  PagedView c{};
+  int st = fill_cache(c, cache);
+  if (st != LVAR_OK || (st = fill_pages(p, refs, cache.num_pages, page_table, cache.table_stride, rows, cache.max_pages)) != LVAR_OK) return st;
+  if (!source || !target || !lengths || !aligned(source, 4) || !aligned(target, 4) || !aligned(lengths, 4) || forks <= 0 || forks > 65535) return LVAR_EINVAL;
+  p.source = source; p.target = target; p.lengths = lengths; p.n = forks; p.shift = c.shift;
+  if ((st = fill_scratch(p, scratch, scratch_bytes)) != LVAR_OK) return st;
+  return launch_pages_fork(p, c, cache.head_dim * (cache.k_exp ? 1 : 2), (hipStream_t)stream);
+}
+
+int lvar_kv_cache_compact(lvar_paged_cache_t cache, const int32_t* out_table, int64_t out_stride, int out_pages, const void* keep, int keep64,
+                          int64_t keep_stride_b, int64_t keep_stride_head, int64_t keep_stride, const int32_t* counts, int B, int n, void* stream) {
+  CompactParams p{};
+  int st = fill_cache(p.cache, cache);
+  if (st != LVAR_OK) return st;
+  if ((st = sizes_ok(B, cache.kv_heads, cache.kv_heads, n)) != LVAR_OK) return st;
+  cache.page_table = out_table; cache.table_stride = out_stride; cache.max_pages = out_pages;
+  if ((st = fill_cache(p.out, cache)) != LVAR_OK) return st;
+  if (!keep || !aligned(keep, keep64 ? 8 : 4) || !aligned(counts, 4)) return LVAR_EINVAL;
+  p.keep = keep; p.keep64 = keep64 ? 1 : 0; p.keep_sb = keep_stride_b; p.keep_sh = keep_stride_head; p.keep_si = keep_stride;
+  p.counts = counts; p.n = n;
+  return launch_pages_compact(p, B, cache.head_dim * (cache.k_exp ? 1 : 2), (hipStream_t)stream);
 }
 
 int64_t lvar_paged_attn_workspace_bytes(int B, int H, int kv_heads, int Lq, int max_len, int head_dim) {

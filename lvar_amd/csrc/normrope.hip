@@ -13,6 +13,7 @@
 namespace lvar {
 
 constexpr int NR_T = 256;
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 
 // Results of large forward launches go past the L2s, whoever reads them next mostly sits on another XCD: 2 x 16 x 4096 rows of q and of k
 // 28.3 -> 26.4 us.  Gradients do so at every size (with a reader of each behind them, through the L2s / past them: 2 x 8 x 20 tokens 7.1 / 7.3 us,
@@ -30,10 +31,13 @@ struct Angles {
   bool second;        // halves: this lane holds the second elements
 };
 
-template <int LPR>
-__device__ __forceinline__ void load_angles(const NormRopeParams& p, int64_t row, int lane, Angles& a) {
+// Cosines and sines of the lane's pairs: of a row of the tables, or (AXES) of the sum over the axes of position times frequency, of token i of
+// sequence b.  That sum is formed in 64 bits, as turns of which only the fraction is kept: a position of 2^20 times a frequency of 1 is known to
+// 2^-4 of a radian in 32 bits.  Sine and cosine of the fraction are 32-bit functions (off by about one step).
+template <int LPR, bool AXES>
+__device__ __forceinline__ void load_angles(const NormRopeParams& p, int64_t row, int b, int i, int lane, Angles& a) {
   const int col = lane * 8, half = p.rot >> 1;
-  a.on = p.cos && col < p.rot;
+  a.on = (AXES || p.cos) && col < p.rot;
   a.second = false;
   a.partner = lane;
   int pair = col >> 1;
@@ -43,6 +47,40 @@ __device__ __forceinline__ void load_angles(const NormRopeParams& p, int64_t row
     a.partner = a.second ? lane - (half >> 3) : lane + (half >> 3);
   }
   if (!a.on) { a.partner = lane; return; }
+  if constexpr (AXES) {
+    double turn[8] = {};
+    for (int x = 0; x < p.axes; x++) {
+      const int64_t at = b * p.pos_sb + x * p.pos_sa + i * p.pos_sl;
+      const double pos = (p.pos64 == 2 ? (double)((const float*)p.positions)[at]
+                          : p.pos64    ? (double)((const int64_t*)p.positions)[at]
+                                       : (double)((const int32_t*)p.positions)[at]) * 0.15915494309189533577;   // 1 / (2 pi)
+      const int64_t f = x * p.freq_sa + pair;
+      if (p.freq32) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          if (e == 0 || !p.interleaved) {
+            const f32x4 v = *(const f32x4*)((const float*)p.freqs + f + e);
+#pragma unroll
+            for (int j = 0; j < 4; j++) turn[e + j] = __builtin_fma(pos, (double)v[j], turn[e + j]);
+          }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+          if (e < 4 || !p.interleaved) {
+            const f64x2 v = *(const f64x2*)((const double*)p.freqs + f + e);
+            turn[e] = __builtin_fma(pos, v[0], turn[e]);
+            turn[e + 1] = __builtin_fma(pos, v[1], turn[e + 1]);
+          }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (e < 4 || !p.interleaved) {
+        const float part = (float)(turn[e] - __builtin_rint(turn[e]));
+        sincospif(2.f * part, &a.s[e], &a.c[e]);
+      }
+    return;
+  }
   const float *cp = p.cos + row * p.cs_row + pair, *sp = p.sin + row * p.cs_row + pair;
   const f32x4 c0 = *(const f32x4*)cp, s0 = *(const f32x4*)sp;
 #pragma unroll
@@ -55,9 +93,9 @@ __device__ __forceinline__ void load_angles(const NormRopeParams& p, int64_t row
 }
 
 // f <- R f (BACK: R^T f).  Every lane takes part (the exchange of the halves).
-template <int LPR, bool BACK>
+template <int LPR, bool BACK, bool AXES>
 __device__ __forceinline__ void rotate(const NormRopeParams& p, const Angles& a, float* f) {
-  if (!p.cos) return;
+  if (!AXES && !p.cos) return;
   if (p.interleaved) {
     if (!a.on) return;
 #pragma unroll
@@ -142,8 +180,8 @@ __host__ __device__ __forceinline__ int chunks_of(const NormRopeParams& p, bool 
   return (append && p.ready ? 0 : (p.H + HC - 1) / HC) + (append ? 2 * nk : nk);
 }
 
-template <int D, int HC, bool APPEND>
-__global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p) {
+template <int D, int HC, bool APPEND, bool AXES>
+__device__ __forceinline__ void norm_rope_item(const NormRopeParams& p) {
   constexpr int LPR = D / 8, RPB = NR_T / LPR;
   const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
   // heads fastest: the rows of a token lie next to each other in a fused projection (heads slowest, so that workgroups in flight
@@ -172,7 +210,7 @@ __global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p)
   const bool plain = APPEND && (which == 2 || p.ready);   // written as it is
   Angles a;
   a.on = false;
-  if (!plain && p.cos) load_angles<LPR>(p, table_row(p, b, i, base), lane, a);
+  if (!plain && (AXES || p.cos)) load_angles<LPR, AXES>(p, AXES ? 0 : table_row(p, b, i, base), b, i, lane, a);
   // One factor for all columns commutes with the rotation and comes last: the rotation of bf16 values costs two roundings instead of three
   // or four (of 6 x 16.8 M keys in e4m3, 92 have another code than in 64 bits, 135 with the factor first).  Halved angles, so that the largest
   // values do not overflow.
@@ -206,7 +244,7 @@ __global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p)
       const float last = (columns ? 1.f : r * wf[0]) * both;
 #pragma unroll
       for (int e = 0; e < 8; e++) f[e] *= columns ? r * wf[e] : 1.f;
-      rotate<LPR, false>(p, a, f);
+      rotate<LPR, false, AXES>(p, a, f);
 #pragma unroll
       for (int e = 0; e < 8; e++) f[e] *= last;
     }
@@ -233,6 +271,13 @@ __global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p)
   }
 }
 
+template <int D, int HC, bool APPEND>
+__global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p) { norm_rope_item<D, HC, APPEND, false>(p); }
+
+// the same with angles from several position axes
+template <int D, int HC, bool APPEND>
+__global__ __launch_bounds__(NR_T) void norm_axes_kernel(const NormRopeParams p) { norm_rope_item<D, HC, APPEND, true>(p); }
+
 // Constants of the division of 32-bit numbers by L (rounded-up reciprocal, Granlund and Montgomery 1994, figure 4.1).
 static void division_by(NormRopeParams& p) {
   const uint32_t L = (uint32_t)p.L;
@@ -250,11 +295,13 @@ static bool launch_fwd(const NormRopeParams& p, bool append, hipStream_t s) {
   if (!grid_fits(groups, NR_T)) return false;
   if constexpr (D >= 64) {   // (head dimensions of a cache)
     if (append) {
-      hipLaunchKernelGGL((norm_rope_kernel<D, HC, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+      if (p.freqs) hipLaunchKernelGGL((norm_axes_kernel<D, HC, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+      else hipLaunchKernelGGL((norm_rope_kernel<D, HC, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
       return true;
     }
   }
-  hipLaunchKernelGGL((norm_rope_kernel<D, HC, false>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+  if (p.freqs) hipLaunchKernelGGL((norm_axes_kernel<D, HC, false>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+  else hipLaunchKernelGGL((norm_rope_kernel<D, HC, false>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
   return true;
 }
 
@@ -286,10 +333,9 @@ int launch_norm_rope(NormRopeParams p, int head_dim, bool append, hipStream_t s)
 
 // Workgroup (blk, chunk): tokens blk * RPB + g, + nblk * RPB, ... of up to NB_HC heads of q or of k.  The weight gradients of its
 // heads stay in registers over all its tokens and meet in LDS once, in a fixed order: row `blk` of the partial sums.
-template <int D, bool DW>
-__global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParams p) {
+template <int D, bool DW, bool AXES>
+__device__ __forceinline__ void norm_rope_bwd_item(const NormRopeParams& p, float* red) {
   constexpr int LPR = D / 8, RPB = NR_T / LPR, HC = NB_HC;
-  __shared__ float red[DW ? RPB * D : 1];
   const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
   const int T = p.B * p.L;
   const int nq = (p.H + HC - 1) / HC, nc = chunks_of<HC>(p, false);
@@ -319,7 +365,7 @@ __global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParam
     }
     Angles a;
     a.on = false;
-    if (p.cos) load_angles<LPR>(p, table_row(p, b, i, 0), lane, a);
+    if (AXES || p.cos) load_angles<LPR, AXES>(p, AXES ? 0 : table_row(p, b, i, 0), b, i, lane, a);
 #pragma unroll
     for (int j = 0; j < HC; j++) {
       const int head = h0 + j;
@@ -333,7 +379,7 @@ __global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParam
       ss = row_sum<LPR>(ss);
       bool flat;
       const float r = norm_factor<D>(p, ss, flat);
-      rotate<LPR, true>(p, a, gu);
+      rotate<LPR, true, AXES>(p, a, gu);
       load_weight(w, head, lane, wf);
       float dot = 0.f;
 #pragma unroll
@@ -394,6 +440,18 @@ __global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParam
       }
     }
   }
+}
+
+template <int D, bool DW>
+__global__ __launch_bounds__(NR_T) void norm_rope_bwd_kernel(const NormRopeParams p) {
+  __shared__ float red[DW ? NR_T * 8 : 1];
+  norm_rope_bwd_item<D, DW, false>(p, red);
+}
+
+template <int D, bool DW>
+__global__ __launch_bounds__(NR_T) void norm_axes_bwd_kernel(const NormRopeParams p) {
+  __shared__ float red[DW ? NR_T * 8 : 1];
+  norm_rope_bwd_item<D, DW, true>(p, red);
 }
 
 // A workgroup per (head, 32 columns) of a gradient with columns, per head of one without; a gradient shared by the heads has one
@@ -465,8 +523,15 @@ int norm_rope_bwd_blocks(int B, int H, int Hkv, int L, int head_dim, bool alone)
 template <int D>
 static void launch_bwd(const NormRopeParams& p, hipStream_t s) {
   const dim3 grid((uint32_t)chunks_of<NB_HC>(p, false) * (uint32_t)p.nblk);
-  if (p.pq || p.pk || p.dqw || p.dkw) hipLaunchKernelGGL((norm_rope_bwd_kernel<D, true>), grid, dim3(NR_T), 0, s, p);
-  else hipLaunchKernelGGL((norm_rope_bwd_kernel<D, false>), grid, dim3(NR_T), 0, s, p);
+  const bool weights = p.pq || p.pk || p.dqw || p.dkw;
+  if (p.freqs) {
+    if (weights) hipLaunchKernelGGL((norm_axes_bwd_kernel<D, true>), grid, dim3(NR_T), 0, s, p);
+    else hipLaunchKernelGGL((norm_axes_bwd_kernel<D, false>), grid, dim3(NR_T), 0, s, p);
+  } else if (weights) {
+    hipLaunchKernelGGL((norm_rope_bwd_kernel<D, true>), grid, dim3(NR_T), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((norm_rope_bwd_kernel<D, false>), grid, dim3(NR_T), 0, s, p);
+  }
 }
 
 int launch_norm_rope_bwd(NormRopeParams p, int head_dim, hipStream_t s) {

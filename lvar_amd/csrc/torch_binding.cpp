@@ -45,7 +45,9 @@ namespace {
   X(lvar_block_sparse_attn_fwd) X(lvar_block_topk_lists) X(lvar_topk_token_lists) X(lvar_topk_union_lists)                \
   X(lvar_remap_concat_lists) X(lvar_mask_to_lists) X(lvar_window_key_scores)                                              \
   X(lvar_qk_norm_rope_fwd) X(lvar_qk_norm_rope_bwd_scratch_bytes) X(lvar_qk_norm_rope_bwd) X(lvar_kv_cache_append)        \
-  X(lvar_kv_cache_read) X(lvar_paged_attn_workspace_bytes) X(lvar_paged_attn_fwd)
+  X(lvar_kv_cache_read) X(lvar_paged_attn_workspace_bytes) X(lvar_paged_attn_fwd)                                         \
+  X(lvar_qk_norm_axes_fwd) X(lvar_qk_norm_axes_bwd) X(lvar_kv_cache_append_axes)                                          \
+  X(lvar_kv_pages_scratch_bytes) X(lvar_kv_pages_alloc) X(lvar_kv_pages_free) X(lvar_kv_cache_fork) X(lvar_kv_cache_compact)
 struct Api {
 #define LVAR_FIELD(name) decltype(&::name) name = nullptr;
   LVAR_ENTRIES(LVAR_FIELD)
@@ -586,14 +588,32 @@ bool weight_ok(const at::Tensor* w, int64_t heads, int64_t d, int dev, lvar_weig
 // what a call says about the norm and the rotation, apart from the weights
 struct How {
   lvar_norm_rope_t h;
-  const at::Tensor *cos, *sin, *positions;
+  const at::Tensor *cos, *sin, *positions, *freqs;
+  lvar_rope_axes_t ax;   // freqs: angles from several position axes
 };
 
-// a: cos, sin, positions, q_weight, k_weight, norm, eps, interleaved
+// strides and pointers of a rotation with several axes (types and limits too)
+bool axes_ok(const at::Tensor& f, const at::Tensor& p, int64_t B, int64_t L, int64_t d, int dev, lvar_rope_axes_t& x) {
+  const bool f32 = f.scalar_type() == at::kFloat;
+  if ((!f32 && f.scalar_type() != at::kDouble) || f.dim() != 2 || f.size(0) < 1 || f.size(0) > 8 || f.requires_grad() || p.requires_grad()) return false;
+  if (!f.is_cuda() || f.get_device() != dev || !p.is_cuda() || p.get_device() != dev || has_tangent(&f) || has_tangent(&p)) return false;
+  const int64_t rot = 2 * f.size(1), n = p.dim();
+  if (rot <= 0 || rot > d || rot % 16 != 0 || f.stride(1) != 1 || f.stride(0) % (f32 ? 4 : 2) != 0 || (reinterpret_cast<uintptr_t>(f.data_ptr()) & 15u)) return false;
+  const auto ty = p.scalar_type();
+  if ((n != 2 && n != 3) || p.size(n - 1) != L || p.size(n - 2) != f.size(0) || (n == 3 && p.size(0) != B)) return false;
+  if (ty != at::kInt && ty != at::kLong && ty != at::kFloat) return false;
+  x.freqs = f.data_ptr(); x.freq_stride = f.stride(0); x.freq_type = f32; x.axes = static_cast<int>(f.size(0)); x.rot_dim = static_cast<int>(rot);
+  x.positions = p.data_ptr(); x.pos_stride_b = n == 3 && B > 1 ? p.stride(0) : 0; x.pos_stride_axis = p.stride(n - 2); x.pos_stride_row = p.stride(n - 1);
+  x.position_type = ty == at::kInt ? LVAR_POSITIONS_I32 : ty == at::kLong ? LVAR_POSITIONS_I64 : LVAR_POSITIONS_F32;
+  return true;
+}
+
+// a: cos, sin, positions, q_weight, k_weight, norm, eps, interleaved, freqs
 bool how_ok(PyObject* const* a, const at::Tensor& q, const at::Tensor& k, int dev, bool needs_rows, How& w, const at::Tensor*& wq, const at::Tensor*& wk) {
   const int64_t B = q.size(0), L = q.size(2), d = q.size(3);
   w.h = {};
-  if (!optional_tensor(a[0], w.cos) || !optional_tensor(a[1], w.sin) || !optional_tensor(a[2], w.positions) || !optional_tensor(a[3], wq) || !optional_tensor(a[4], wk)) return false;
+  w.ax = {};
+  if (!optional_tensor(a[8], w.freqs) || !optional_tensor(a[0], w.cos) || !optional_tensor(a[1], w.sin) || !optional_tensor(a[2], w.positions) || !optional_tensor(a[3], wq) || !optional_tensor(a[4], wk)) return false;
   if (a[5] == Py_None) { w.h.norm = LVAR_NORM_NONE; w.h.eps = 0.f; }
   else if (PyUnicode_Check(a[5]) && PyUnicode_CompareWithASCIIString(a[5], "l2") == 0) { w.h.norm = LVAR_NORM_L2; w.h.eps = 1e-12f; }
   else if (PyUnicode_Check(a[5]) && PyUnicode_CompareWithASCIIString(a[5], "rms") == 0) { w.h.norm = LVAR_NORM_RMS; w.h.eps = 1e-6f; }
@@ -613,7 +633,10 @@ bool how_ok(PyObject* const* a, const at::Tensor& q, const at::Tensor& k, int de
     w.h.cos = w.cos->data_ptr<float>(); w.h.sin = w.sin->data_ptr<float>(); w.h.table_stride = w.cos->stride(0);
     w.h.table_rows = static_cast<int>(w.cos->size(0)); w.h.rot_dim = static_cast<int>(2 * w.cos->size(1)); w.h.interleaved = inter;
   }
-  if (w.positions) {
+  if (w.freqs) {
+    w.ax.interleaved = inter;
+    if (w.cos || !w.positions || !axes_ok(*w.freqs, *w.positions, B, L, d, dev, w.ax)) return false;
+  } else if (w.positions) {
     const at::Tensor& p = *w.positions;
     const int64_t n = p.dim();
     if (!p.is_cuda() || p.get_device() != dev || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong)) return false;
@@ -638,9 +661,10 @@ bool qk_ok(const at::Tensor* q, const at::Tensor* k, int& dev, void*& stream) {
 
 int dim(const at::Tensor& t, int i) { return static_cast<int>(t.size(i)); }
 
-int norm_rope_launch(const at::Tensor& q, const at::Tensor& k, const lvar_norm_rope_t& h, at::Tensor& oq, at::Tensor& ok, int dev, void* stream) {
+int norm_rope_launch(const at::Tensor& q, const at::Tensor& k, const lvar_norm_rope_t& h, const lvar_rope_axes_t* ax, at::Tensor& oq, at::Tensor& ok, int dev, void* stream) {
   oq = empty(q.sizes(), at::kBFloat16, dev);
   ok = empty(k.sizes(), at::kBFloat16, dev);
+  if (ax) return api.lvar_qk_norm_axes_fwd(view(q), view(k), h, *ax, oq.data_ptr(), ok.data_ptr(), dim(q, 0), dim(q, 1), dim(k, 1), dim(q, 2), dim(q, 3), stream);
   return api.lvar_qk_norm_rope_fwd(view(q), view(k), h, oq.data_ptr(), ok.data_ptr(), dim(q, 0), dim(q, 1), dim(k, 1), dim(q, 2), dim(q, 3), stream);
 }
 
@@ -655,13 +679,14 @@ at::Tensor rows_like(const at::Tensor& t) {
 struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
   using Maybe = std::optional<at::Tensor>;   // (undefined tensors are no inputs)
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const Maybe& wq,
-                                                const Maybe& wk, const Maybe& cos, const Maybe& sin, const Maybe& positions, const lvar_norm_rope_t* h,
-                                                int64_t stream) {
+                                                const Maybe& wk, const Maybe& cos, const Maybe& sin, const Maybe& positions, const Maybe& freqs,
+                                                const lvar_norm_rope_t* h, const lvar_rope_axes_t* ax, int64_t stream) {
     auto some = [](const Maybe& t) { return t.value_or(at::Tensor()); };
-    ctx->save_for_backward({q, k, some(wq), some(wk), some(cos), some(sin), some(positions)});
+    ctx->save_for_backward({q, k, some(wq), some(wk), some(cos), some(sin), some(positions), some(freqs)});
     ctx->saved_data["how"] = std::string(reinterpret_cast<const char*>(h), sizeof(*h));
+    ctx->saved_data["interleaved"] = ax && ax->interleaved;
     at::Tensor oq, ok;
-    const int st = norm_rope_launch(q, k, *h, oq, ok, q.get_device(), reinterpret_cast<void*>(stream));
+    const int st = norm_rope_launch(q, k, *h, ax, oq, ok, q.get_device(), reinterpret_cast<void*>(stream));
     TORCH_CHECK(st == LVAR_OK, "lvar_qk_norm_rope_fwd failed with status ", st);
     return {oq, ok};
   }
@@ -669,7 +694,7 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope can be differentiated once: its gradients have no graph (create_graph)");
     TORCH_CHECK(!has_tangent(&grads[0]) && !has_tangent(&grads[1]), "the gradient of qk_norm_rope has no forward-mode derivative: call it on tensors without a tangent");
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3], &cos = saved[4], &sin = saved[5], &positions = saved[6];
+    const at::Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3], &cos = saved[4], &sin = saved[5], &positions = saved[6], &freqs = saved[7];
     lvar_norm_rope_t h;
     const std::string how = ctx->saved_data["how"].toStringRef();
     std::memcpy(&h, how.data(), sizeof(h));
@@ -682,7 +707,11 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
       same = same && cos.is_cuda() && sin.is_cuda() && cos.get_device() == dev && sin.get_device() == dev && cos.stride(1) == 1 && sin.stride(1) == 1 && cos.stride(0) == sin.stride(0);
       h.cos = cos.data_ptr<float>(); h.sin = sin.data_ptr<float>(); h.table_stride = cos.stride(0);
     }
-    if (positions.defined()) {
+    lvar_rope_axes_t ax{};
+    if (freqs.defined()) {
+      ax.interleaved = ctx->saved_data["interleaved"].toBool();
+      same = same && axes_ok(freqs, positions, B, L, d, dev, ax);
+    } else if (positions.defined()) {
       same = same && positions.is_cuda() && positions.get_device() == dev;
       h.positions = positions.data_ptr();
       h.pos_stride_b = positions.dim() == 2 && B > 1 ? positions.stride(0) : 0; h.pos_stride_row = positions.stride(-1);
@@ -702,17 +731,19 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
       bytes = api.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d);
       if (bytes > 0) scratch = empty({bytes}, at::kByte, dev);
     }
-    const int st = api.lvar_qk_norm_rope_bwd(view(q), view(k), h, gq.data_ptr(), gk.data_ptr(), view(dq), view(dk), ptr(dwq), ptr(dwk), ptr(scratch), bytes, B, H,
-                                             Hkv, L, d, c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream());
+    void* const stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+    const int st = freqs.defined()
+        ? api.lvar_qk_norm_axes_bwd(view(q), view(k), h, ax, gq.data_ptr(), gk.data_ptr(), view(dq), view(dk), ptr(dwq), ptr(dwk), ptr(scratch), bytes, B, H, Hkv, L, d, stream)
+        : api.lvar_qk_norm_rope_bwd(view(q), view(k), h, gq.data_ptr(), gk.data_ptr(), view(dq), view(dk), ptr(dwq), ptr(dwk), ptr(scratch), bytes, B, H, Hkv, L, d, stream);
     TORCH_CHECK(st == LVAR_OK, "lvar_qk_norm_rope_bwd failed with status ", st);
-    return {dq, dk, dwq, dwk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    return {dq, dk, dwq, dwk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
-// (q, k, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved) -> (q, k)
+// (q, k, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved, freqs) -> (q, k)
 LVAR_FAST(fast_qk_norm_rope) {
   HANDLE_TH_ERRORS
-  const at::Tensor *q = n == 10 ? tensor(a[0]) : nullptr, *k = n == 10 ? tensor(a[1]) : nullptr, *wq, *wk;
+  const at::Tensor *q = n == 11 ? tensor(a[0]) : nullptr, *k = n == 11 ? tensor(a[1]) : nullptr, *wq, *wk;
   int dev;
   void* stream;
   How w;
@@ -728,19 +759,20 @@ LVAR_FAST(fast_qk_norm_rope) {
     const int64_t d = q->size(3);
     LVAR_NEED((d == 16 || d == 32 || d == 64 || d == 128 || d == 256) && q->size(0) <= 65535 && q->size(1) <= 16384 && q->size(0) * q->size(2) <= (1ll << 30));
     auto some = [](const at::Tensor* t) { return t ? std::optional<at::Tensor>(*t) : std::nullopt; };
-    auto r = NormRopeFunction::apply(*q, *k, some(wq), some(wk), some(w.cos), some(w.sin), some(w.positions), &w.h, reinterpret_cast<int64_t>(stream));
+    auto r = NormRopeFunction::apply(*q, *k, some(wq), some(wk), some(w.cos), some(w.sin), some(w.positions), some(w.freqs), &w.h, w.freqs ? &w.ax : nullptr,
+                                    reinterpret_cast<int64_t>(stream));
     return tuple(std::move(r[0]), std::move(r[1]));
   }
-  LVAR_NEED(norm_rope_launch(*q, *k, w.h, oq, ok, dev, stream) == LVAR_OK);
+  LVAR_NEED(norm_rope_launch(*q, *k, w.h, w.freqs ? &w.ax : nullptr, oq, ok, dev, stream) == LVAR_OK);
   return tuple(std::move(oq), std::move(ok));
   END_HANDLE_TH_ERRORS
 }
 
-// (cache, page table, start, counts, q | None, k, v[, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved]) -> q, or True
+// (cache, page table, start, counts, q | None, k, v[, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved, freqs]) -> q, or True
 LVAR_FAST(fast_kv_append) {
   HANDLE_TH_ERRORS
-  LVAR_NEED(n == 7 || n == 15);
-  const bool fused = n == 15;
+  LVAR_NEED(n == 7 || n == 16);
+  const bool fused = n == 16;
   const at::Tensor *q = fused ? tensor(a[4]) : tensor(a[5]), *k = tensor(a[5]), *v = tensor(a[6]), *start = tensor(a[2]), *counts, *wq = nullptr, *wk = nullptr;
   int dev;
   void* stream;
@@ -753,8 +785,11 @@ LVAR_FAST(fast_kv_append) {
   LVAR_NEED(!wants_derivative(q) && !wants_derivative(k) && !wants_derivative(v) && !wants_derivative(wq) && !wants_derivative(wk));
   at::Tensor oq;
   if (fused) oq = empty(q->sizes(), at::kBFloat16, dev);
-  LVAR_NEED(api.lvar_kv_cache_append(view(*q), view(*k), view(*v), fused ? &w.h : nullptr, fused ? oq.data_ptr() : nullptr, c, ints(start), ints(counts),
-                                     static_cast<int>(B), dim(*q, 1), dim(*k, 2), stream) == LVAR_OK);
+  const int st = fused && w.freqs
+      ? api.lvar_kv_cache_append_axes(view(*q), view(*k), view(*v), w.h, w.ax, oq.data_ptr(), c, ints(start), ints(counts), static_cast<int>(B), dim(*q, 1), dim(*k, 2), stream)
+      : api.lvar_kv_cache_append(view(*q), view(*k), view(*v), fused ? &w.h : nullptr, fused ? oq.data_ptr() : nullptr, c, ints(start), ints(counts), static_cast<int>(B),
+                                 dim(*q, 1), dim(*k, 2), stream);
+  LVAR_NEED(st == LVAR_OK);
   count_write(a[0]);
   if (!fused) Py_RETURN_TRUE;
   return THPVariable_Wrap(std::move(oq));
@@ -786,6 +821,105 @@ LVAR_FAST(fast_kv_read) {
   LVAR_NEED(api.lvar_kv_cache_read(c, ints(start), ints(lengths), ko.data_ptr(), vo.data_ptr(), static_cast<int>(B), static_cast<int>(most),
                                    c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream()) == LVAR_OK);
   return tuple(std::move(ko), std::move(vo));
+  END_HANDLE_TH_ERRORS
+}
+
+// a table of counted pages on the current device
+bool counted(const at::Tensor* refs, const at::Tensor* table, int& dev, void*& stream) {
+  if (!bound || !refs || !table || !refs->is_cuda()) return false;
+  dev = refs->get_device();
+  if (c10::hip::current_device() != dev || !packed(refs, dev, at::kInt) || refs->dim() != 1 || refs->numel() == 0 || refs->numel() > INT32_MAX) return false;
+  if (!table->is_cuda() || table->get_device() != dev || table->scalar_type() != at::kInt || table->dim() != 2 || table->numel() == 0 ||
+      table->size(0) > INT32_MAX || table->size(1) > INT32_MAX || (table->size(1) > 1 && table->stride(1) != 1) || (table->size(0) > 1 && table->stride(0) < table->size(1)))
+    return false;
+  stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  return true;
+}
+int64_t table_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+void count_writes(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts) if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+at::Tensor pages_scratch(int64_t rows, int64_t pages, int dev, int64_t& bytes) {
+  bytes = std::max<int64_t>(0, api.lvar_kv_pages_scratch_bytes(static_cast<int>(rows), static_cast<int>(pages)));
+  return bytes > 0 ? empty({bytes}, at::kByte, dev) : at::Tensor();
+}
+
+// (refs, page table, first, last) -> True
+LVAR_FAST(fast_pages_alloc) {
+  HANDLE_TH_ERRORS
+  LVAR_NEED(n == 4);
+  const at::Tensor *refs = tensor(a[0]), *table = tensor(a[1]), *first = tensor(a[2]), *last = tensor(a[3]);
+  int dev;
+  void* stream;
+  LVAR_NEED(counted(refs, table, dev, stream) && first && last);
+  const int64_t B = table->size(0);
+  LVAR_NEED(per_sequence(first, B, dev) && per_sequence(last, B, dev));
+  int64_t bytes;
+  const at::Tensor ws = pages_scratch(B, refs->numel(), dev, bytes);
+  LVAR_NEED(api.lvar_kv_pages_alloc(refs->data_ptr<int32_t>(), static_cast<int>(refs->numel()), table->data_ptr<int32_t>(), table_stride(*table), dim(*table, 0), dim(*table, 1),
+                                    ints(first), ints(last), bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream) == LVAR_OK);
+  count_writes({refs, table});
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (refs, page table, keep) -> True
+LVAR_FAST(fast_pages_free) {
+  HANDLE_TH_ERRORS
+  LVAR_NEED(n == 3);
+  const at::Tensor *refs = tensor(a[0]), *table = tensor(a[1]), *keep;
+  int dev;
+  void* stream;
+  LVAR_NEED(counted(refs, table, dev, stream) && optional_tensor(a[2], keep) && per_sequence(keep, table->size(0), dev));
+  LVAR_NEED(api.lvar_kv_pages_free(refs->data_ptr<int32_t>(), static_cast<int>(refs->numel()), table->data_ptr<int32_t>(), table_stride(*table), dim(*table, 0), dim(*table, 1),
+                                   ints(keep), stream) == LVAR_OK);
+  count_writes({refs, table});
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (cache, refs, page table, source, target, lengths) -> True
+LVAR_FAST(fast_cache_fork) {
+  HANDLE_TH_ERRORS
+  LVAR_NEED(n == 6);
+  const at::Tensor *refs = tensor(a[1]), *table = tensor(a[2]), *source = tensor(a[3]), *target = tensor(a[4]), *lengths = tensor(a[5]);
+  int dev;
+  void* stream;
+  LVAR_NEED(counted(refs, table, dev, stream) && source && target && lengths && source->dim() == 1 && source->numel() > 0 && source->numel() <= 65535);
+  const int64_t B = table->size(0), forks = source->numel();
+  lvar_paged_cache_t c;
+  LVAR_NEED(cache_ok(a[0], a[2], B, dev, c) && c.num_pages == refs->numel() && per_sequence(source, forks, dev) && per_sequence(target, forks, dev) && per_sequence(lengths, B, dev));
+  c.table_stride = table_stride(*table);
+  int64_t bytes;
+  const at::Tensor ws = pages_scratch(forks, refs->numel(), dev, bytes);
+  LVAR_NEED(api.lvar_kv_cache_fork(c, refs->data_ptr<int32_t>(), table->data_ptr<int32_t>(), static_cast<int>(B), ints(source), ints(target), ints(lengths), static_cast<int>(forks),
+                                   bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream) == LVAR_OK);
+  count_write(a[0]);
+  count_writes({refs, table});
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (cache, page table, keep, out table, counts) -> True
+LVAR_FAST(fast_cache_compact) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *k = n == 5 && PyTuple_Check(a[0]) && PyTuple_GET_SIZE(a[0]) == 4 ? tensor(PyTuple_GET_ITEM(a[0], 0)) : nullptr;
+  LVAR_NEED(bound && k && k->is_cuda());
+  const at::Tensor *table = tensor(a[1]), *keep = tensor(a[2]), *out = tensor(a[3]), *counts;
+  const int dev = k->get_device();
+  LVAR_NEED(table && keep && out && table->dim() == 2 && c10::hip::current_device() == dev && optional_tensor(a[4], counts));
+  const int64_t B = table->size(0);
+  lvar_paged_cache_t c, o;
+  LVAR_NEED(B > 0 && B <= 65535 && cache_ok(a[0], a[1], B, dev, c) && cache_ok(a[0], a[3], B, dev, o) && per_sequence(counts, B, dev));
+  LVAR_NEED(keep->is_cuda() && keep->get_device() == dev && (keep->scalar_type() == at::kInt || keep->scalar_type() == at::kLong) && keep->dim() == 3 &&
+            keep->size(0) == B && keep->size(1) == c.kv_heads && keep->size(2) > 0 && keep->size(2) <= INT32_MAX);
+  LVAR_NEED(api.lvar_kv_cache_compact(c, o.page_table, o.table_stride, o.max_pages, keep->data_ptr(), keep->scalar_type() == at::kLong, keep->stride(0), keep->stride(1),
+                                      keep->stride(2), ints(counts), static_cast<int>(B), dim(*keep, 2),
+                                      c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream()) == LVAR_OK);
+  count_write(a[0]);
+  Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
 
@@ -869,6 +1003,7 @@ PyMethodDef fast_methods[] = {
     LVAR_METHOD(fast_full_step), LVAR_METHOD(fast_sparse_step), LVAR_METHOD(fast_block_sparse_attn), LVAR_METHOD(fast_block_topk_lists),
     LVAR_METHOD(fast_topk_token_lists), LVAR_METHOD(fast_remap_concat_lists), LVAR_METHOD(fast_mask_to_lists), LVAR_METHOD(fast_window_keys),
     LVAR_METHOD(fast_qk_norm_rope), LVAR_METHOD(fast_kv_append), LVAR_METHOD(fast_kv_read), LVAR_METHOD(fast_paged_attn),
+    LVAR_METHOD(fast_pages_alloc), LVAR_METHOD(fast_pages_free), LVAR_METHOD(fast_cache_fork), LVAR_METHOD(fast_cache_compact),
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

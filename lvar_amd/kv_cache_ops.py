@@ -21,7 +21,8 @@ from torch.autograd import forward_ad
 from . import _lib
 from .sparse_attn_ops import ShapeError, _native, _on_device, _plain_scale, _prep, _ptr, _require, _scale, _stream, _view
 
-__all__ = ["PagedKVCache", "qk_norm_rope", "qk_norm_rope_append", "kv_cache_append", "kv_cache_read", "paged_attn", "ShapeError"]
+__all__ = ["PagedKVCache", "axis_freqs", "qk_norm_rope", "qk_norm_rope_append", "kv_cache_append", "kv_cache_read", "kv_pages_alloc",
+           "kv_pages_free", "kv_cache_fork", "kv_cache_compact", "paged_attn", "ShapeError"]
 
 _NORMS = {None: 0, "l2": 1, "rms": 2}
 _EPS = {None: 0.0, "l2": 1e-12, "rms": 1e-6}
@@ -167,7 +168,32 @@ def _how(cos, sin, positions, wq: "_lib.LvarWeight", wk: "_lib.LvarWeight", norm
     return h
 
 
-def _norm_args(q, k, cos, sin, positions, norm, eps):
+_POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _axes_arg(freqs, positions, interleaved: bool, B: int, L: int, d: int, device):
+    """Frequencies and positions as the kernels read them."""
+    if freqs.dtype not in (torch.float64, torch.float32):
+        raise TypeError(f"freqs must be float64 or float32, got {freqs.dtype}")
+    _require(freqs.dim() == 2 and 1 <= freqs.shape[0] <= 8, lambda: f"freqs must be [axes, rot/2] with 1 to 8 axes, got {tuple(freqs.shape)}")
+    rot = 2 * freqs.shape[1]
+    _require(0 < rot <= d and rot % 16 == 0, lambda: f"the rotated columns (2 * {freqs.shape[1]}) must be a multiple of 16 up to head_dim = {d}")
+    _require(positions is not None, "freqs need positions")
+    if positions.dtype not in _POSITIONS:
+        raise TypeError(f"positions must be int32, int64 or float32 with freqs, got {positions.dtype}")
+    A = freqs.shape[0]
+    _require(tuple(positions.shape) in ((A, L), (B, A, L)), lambda: f"positions must be [axes, L] or [B, axes, L] = {(B, A, L)} with freqs, got {tuple(positions.shape)}")
+    _require(freqs.device == device and positions.device == device, "freqs and positions must be on the device of q")
+    if freqs.requires_grad or positions.requires_grad:
+        raise RuntimeError("freqs and positions take no gradient: detach them")
+    if freqs.stride(1) != 1 or freqs.stride(0) * freqs.element_size() % 16 or freqs.data_ptr() % 16:
+        freqs = freqs.clone(memory_format=torch.contiguous_format)
+    x = _lib.LvarRopeAxes(freqs.data_ptr(), freqs.stride(0), 0 if freqs.dtype == torch.float64 else 1, A, rot, 1 if interleaved else 0, positions.data_ptr(),
+                          positions.stride(0) if positions.dim() == 3 and B > 1 else 0, positions.stride(-2), positions.stride(-1), _POSITIONS[positions.dtype])
+    return freqs, positions, x
+
+
+def _norm_args(q, k, cos, sin, positions, norm, eps, freqs=None):
     """Checks that the plain and the appending form share."""
     qs, ks = q.shape, k.shape
     _require(qs[0] == ks[0] and qs[2] == ks[2] and qs[3] == ks[3] and ks[1] > 0 and qs[1] > 0 and qs[1] % ks[1] == 0,
@@ -178,7 +204,9 @@ def _norm_args(q, k, cos, sin, positions, norm, eps):
     # (the reciprocal of a smaller one is no fp32 number, and rows of zeros would come out as NaN)
     _require(eps == 0.0 or _LEAST <= eps <= _MOST, "eps must be 0 or a normal fp32 number, and not negative")
     cos, sin = _table_arg(cos, sin, qs[3], q.device)
-    if positions is not None:
+    if freqs is not None:
+        _require(cos is None, "a rotation has cos and sin, or freqs")
+    elif positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError("positions must be int32 or int64")
         _require(tuple(positions.shape) in ((qs[2],), (qs[0], qs[2])), lambda: f"positions must be [L] or [B,L], got {tuple(positions.shape)}")
@@ -197,7 +225,7 @@ def _no_gradient(name: str, *tensors) -> None:
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
-def _norm_rope_launch(q, k, wq, wk, cos, sin, positions, norm, eps, interleaved):
+def _norm_rope_launch(q, k, wq, wk, cos, sin, positions, norm, eps, interleaved, freqs=None):
     B, H, L, d = q.shape
     Hkv = k.shape[1]
     oq = torch.empty((B, H, L, d), dtype=q.dtype, device=q.device)
@@ -205,9 +233,15 @@ def _norm_rope_launch(q, k, wq, wk, cos, sin, positions, norm, eps, interleaved)
     if oq.numel() == 0:
         return oq, ok
     (wq, dq), (wk, dk) = _weight_arg(wq, H, d, "q_weight", q.device), _weight_arg(wk, Hkv, d, "k_weight", q.device)
+    how = _how(cos, sin, positions, dq, dk, norm, eps, interleaved, B, L, q.device)
+    if freqs is not None:
+        freqs, positions, axes = _axes_arg(freqs, positions, interleaved, B, L, d, q.device)
+        with _on_device(q):
+            st = _lib.load().lvar_qk_norm_axes_fwd(_view(q), _view(k), how, axes, oq.data_ptr(), ok.data_ptr(), B, H, Hkv, L, d, _stream(q))
+        _lib.check(st, "lvar_qk_norm_axes_fwd")
+        return oq, ok
     with _on_device(q):
-        st = _lib.load().lvar_qk_norm_rope_fwd(_view(q), _view(k), _how(cos, sin, positions, dq, dk, norm, eps, interleaved, B, L, q.device),
-                                              oq.data_ptr(), ok.data_ptr(), B, H, Hkv, L, d, _stream(q))
+        st = _lib.load().lvar_qk_norm_rope_fwd(_view(q), _view(k), how, oq.data_ptr(), ok.data_ptr(), B, H, Hkv, L, d, _stream(q))
     _lib.check(st, "lvar_qk_norm_rope_fwd")
     return oq, ok
 
@@ -221,17 +255,17 @@ def _rows_like(t):
 
 class _NormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, positions, norm, eps, interleaved):
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, norm, eps, interleaved, freqs=None):
         ctx.how = (norm, eps, interleaved)
-        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
-        return _norm_rope_launch(q, k, wq, wk, cos, sin, positions, norm, eps, interleaved)
+        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions, freqs)
+        return _norm_rope_launch(q, k, wq, wk, cos, sin, positions, norm, eps, interleaved, freqs)
 
     @staticmethod
     def backward(ctx, gq, gk):
         if torch.is_grad_enabled():
             raise RuntimeError("qk_norm_rope can be differentiated once: its gradients have no graph (create_graph)")
         _no_tangent("the gradient of qk_norm_rope", gq, gk)
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        q, k, wq, wk, cos, sin, positions, freqs = ctx.saved_tensors
         norm, eps, interleaved = ctx.how
         B, H, L, d = q.shape
         Hkv = k.shape[1]
@@ -246,22 +280,39 @@ class _NormRope(torch.autograd.Function):
             for t in (dwq, dwk):
                 if t is not None:
                     t.zero_()
-            return dq, dk, dwq, dwk, None, None, None, None, None, None
+            return dq, dk, dwq, dwk, None, None, None, None, None, None, None
         gq, gk = _rows(gq.contiguous(), "gradient"), _rows(gk.contiguous(), "gradient")
         (wq, aq), (wk, ak) = _weight_arg(wq, H, d, "q_weight", q.device), _weight_arg(wk, Hkv, d, "k_weight", q.device)
         lib = _lib.load()
         with _on_device(q):
             nbytes = int(lib.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d)) if dwq is not None or dwk is not None else 0
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-            st = lib.lvar_qk_norm_rope_bwd(_view(q), _view(k), _how(cos, sin, positions, aq, ak, norm, eps, interleaved, B, L, q.device),
-                                           gq.data_ptr(), gk.data_ptr(), _view(dq), _view(dk), _ptr(dwq), _ptr(dwk), _ptr(scratch), nbytes,
-                                           B, H, Hkv, L, d, _stream(q))
+            how = _how(cos, sin, positions, aq, ak, norm, eps, interleaved, B, L, q.device)
+            rest = (gq.data_ptr(), gk.data_ptr(), _view(dq), _view(dk), _ptr(dwq), _ptr(dwk), _ptr(scratch), nbytes, B, H, Hkv, L, d, _stream(q))
+            if freqs is not None:
+                freqs, positions, axes = _axes_arg(freqs, positions, interleaved, B, L, d, q.device)
+                st = lib.lvar_qk_norm_axes_bwd(_view(q), _view(k), how, axes, *rest)
+            else:
+                st = lib.lvar_qk_norm_rope_bwd(_view(q), _view(k), how, *rest)
         _lib.check(st, "lvar_qk_norm_rope_bwd")
-        return dq, dk, dwq, dwk, None, None, None, None, None, None
+        return dq, dk, dwq, dwk, None, None, None, None, None, None, None
+
+
+def axis_freqs(columns, theta: float = 10000.0, device="cuda") -> torch.Tensor:
+    """Frequencies of a rotation in which every axis has columns of its own: fp64 ``[axes, sum(columns) / 2]`` for :func:`qk_norm_rope`, from the (even)
+    numbers of columns of each axis, one behind the other; pair i of an axis with c columns turns by ``theta ** (-2 i / c)`` radians per unit of
+    position.  ``axis_freqs((64, 64))`` is the grid of rows and columns of the reference (models/sparvar/basic_sparvar.py:326-342)."""
+    _require(len(columns) > 0 and all(c >= 0 and c % 2 == 0 for c in columns), lambda: f"columns must be even numbers, got {tuple(columns)}")
+    f = torch.zeros((len(columns), sum(columns) // 2), dtype=torch.float64)
+    at = 0
+    for a, c in enumerate(columns):
+        f[a, at:at + c // 2] = float(theta) ** (-2.0 * torch.arange(c // 2, dtype=torch.float64) / max(1, c))
+        at += c // 2
+    return f.to(device)
 
 
 def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weight=None, norm: Optional[str] = "l2",
-                 eps: Optional[float] = None, interleaved: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+                 eps: Optional[float] = None, interleaved: bool = True, freqs=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Queries ``[B,H,L,d]`` and keys ``[B,Hkv,L,d]`` normalised per head, scaled and rotated, in one pass: ``(q, k)`` contiguous bf16.
 
     ``norm``: ``"l2"`` is ``x / max(|x|, eps)`` (eps 1e-12), ``"rms"`` ``x / sqrt(mean(x^2) + eps)`` (eps 1e-6), ``None`` leaves x; an
@@ -269,35 +320,44 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
     ``q_weight`` / ``k_weight`` (fp32 or bf16; ``[d]``, ``[H,1]``, ``[1,d]`` or ``[H,d]``) multiply the result.  ``cos`` / ``sin``
     fp32 ``[rows, rot/2]`` rotate the first ``rot`` columns (a multiple of 16) in pairs ``(2i, 2i+1)``, or ``(i, i + rot/2)``
     with ``interleaved=False``; token i takes row i, or row ``positions[i]`` / ``positions[b,i]`` (clamped to the table).
+    Instead of tables, ``freqs`` (fp64 or fp32, ``[axes, rot/2]``, up to 8 axes) and ``positions`` (int32, int64 or fp32, ``[axes, L]`` or ``[B, axes, L]``)
+    give the angles of images and videos: pair i of token t turns by ``sum over axes a of positions[a, t] * freqs[a, i]``, summed in 64 bits
+    (:func:`axis_freqs` gives every axis its own columns; a dense ``freqs`` mixes them).
     ``head_dim`` 16, 32, 64, 128 or 256.  All in fp32, rounded once.  Differentiable in q, k and the weights (once, in
     reverse mode: inputs with a forward-mode tangent are refused); a backward pass that is captured in a graph wants leaves without a live eager
     graph, as always with autograd.  The
     reference's counterpart is models/sparvar/basic_sparvar.py:326-342, eager."""
     fast = _native()
     if fast is not None:
-        r = fast.fast_qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved)
+        r = fast.fast_qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, norm, eps, interleaved, freqs)
         if r is not None:
             return r
-    _no_tangent("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
+    _no_tangent("qk_norm_rope", q, k, cos, sin, q_weight, k_weight, freqs, positions)
     q, k = _rows(q, "q"), _rows(k, "k")
-    cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
+    cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps, freqs)
     _require(q.shape[3] in (16, 32, 64, 128, 256), lambda: f"head_dim must be 16, 32, 64, 128 or 256, got {q.shape[3]}")
     _require(cos is None or positions is not None or cos.shape[0] >= q.shape[2],
              lambda: f"cos and sin have {cos.shape[0]} rows for {q.shape[2]} tokens: give positions, or a longer table")
+    if freqs is not None:
+        _axes_arg(freqs, positions, bool(interleaved), q.shape[0], q.shape[2], q.shape[3], q.device)
     for w, heads, name in ((q_weight, q.shape[1], "q_weight"), (k_weight, k.shape[1], "k_weight")):
         _weight_arg(w, heads, q.shape[3], name, q.device)
-    args = (q, k, q_weight, k_weight, cos, sin, positions, norm, eps, bool(interleaved))
+    args = (q, k, q_weight, k_weight, cos, sin, positions, norm, eps, bool(interleaved), freqs)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _NormRope.apply(*args)
     return _norm_rope_launch(*args)
 
 
-def _append(cache, q, k, v, page_table, start, counts, how, oq):
+def _append(cache, q, k, v, page_table, start, counts, how, oq, axes=None):
     B, Hkv, L, d = k.shape
     with _on_device(k):
-        st = _lib.load().lvar_kv_cache_append(_view(q), _view(k), _view(v), None if how is None else C.byref(how), _ptr(oq),
-                                             _cache_arg(cache, page_table, B, k.device), start.data_ptr(), _ptr(counts),
-                                             B, Hkv if q is None else q.shape[1], L, _stream(k))
+        if axes is not None:
+            st = _lib.load().lvar_kv_cache_append_axes(_view(q), _view(k), _view(v), how, axes, _ptr(oq), _cache_arg(cache, page_table, B, k.device), start.data_ptr(),
+                                                      _ptr(counts), B, q.shape[1], L, _stream(k))
+        else:
+            st = _lib.load().lvar_kv_cache_append(_view(q), _view(k), _view(v), None if how is None else C.byref(how), _ptr(oq),
+                                                 _cache_arg(cache, page_table, B, k.device), start.data_ptr(), _ptr(counts),
+                                                 B, Hkv if q is None else q.shape[1], L, _stream(k))
     _lib.check(st, "lvar_kv_cache_append")
     # (autograd finds out where it has saved them; tensors of inference mode have no version)
     torch.autograd.graph.increment_version([t for t in cache if t is not None and not t.is_inference()])
@@ -330,26 +390,29 @@ def kv_cache_append(cache: PagedKVCache, k, v, page_table, start, counts=None) -
 
 
 def qk_norm_rope_append(cache: PagedKVCache, q, k, v, page_table, start, cos=None, sin=None, counts=None, positions=None, q_weight=None,
-                        k_weight=None, norm: Optional[str] = "l2", eps: Optional[float] = None, interleaved: bool = True) -> torch.Tensor:
+                        k_weight=None, norm: Optional[str] = "l2", eps: Optional[float] = None, interleaved: bool = True, freqs=None) -> torch.Tensor:
     """:func:`qk_norm_rope` on q and k and :func:`kv_cache_append` of the keys and of ``v``, in one launch; returns the queries.
-    Without ``positions`` token i of sequence b takes row ``start[b] + i`` of the tables (clamped to them).  The keys are rounded once, from fp32 to
+    With ``freqs``, ``positions`` are those of the call's tokens, as there.  Without ``positions`` token i of sequence b takes row ``start[b] + i`` of the tables (clamped to them).  The keys are rounded once, from fp32 to
     the cache's type."""
     fast = _native()
     if fast is not None:
         r = fast.fast_kv_append(cache, page_table, start, counts, q, k, v, cos, sin, positions, q_weight, k_weight,
-                                norm, eps, interleaved)
+                                norm, eps, interleaved, freqs)
         if r is not None:
             return r
     _no_gradient("qk_norm_rope_append", q, k, v, q_weight, k_weight, cache.k, cache.v)
-    _no_tangent("qk_norm_rope_append", cos, sin)
+    _no_tangent("qk_norm_rope_append", cos, sin, freqs, positions)
     q, k, v = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
-    cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps)
+    cos, sin, eps = _norm_args(q, k, cos, sin, positions, norm, eps, freqs)
     start, counts = _append_args(cache, k, v, page_table, start, counts)
     B, H, L, d = q.shape
+    axes = None
+    if freqs is not None:
+        freqs, positions, axes = _axes_arg(freqs, positions, bool(interleaved), B, L, d, q.device)
     oq = torch.empty((B, H, L, d), dtype=q.dtype, device=q.device)
     (wq, aq), (wk, ak) = _weight_arg(q_weight, H, d, "q_weight", q.device), _weight_arg(k_weight, k.shape[1], d, "k_weight", q.device)
     if oq.numel():
-        _append(cache, q, k, v, page_table, start, counts, _how(cos, sin, positions, aq, ak, norm, eps, bool(interleaved), B, L, q.device), oq)
+        _append(cache, q, k, v, page_table, start, counts, _how(cos, sin, positions, aq, ak, norm, eps, bool(interleaved), B, L, q.device), oq, axes)
     return oq
 
 
@@ -378,6 +441,126 @@ def kv_cache_read(cache: PagedKVCache, page_table, lengths, max_len: Optional[in
             st = _lib.load().lvar_kv_cache_read(arg, _ptr(start), lengths.data_ptr(), k.data_ptr(), v.data_ptr(), B, max_len, _stream(k))
         _lib.check(st, "lvar_kv_cache_read")
     return k, v
+
+
+def _counted(refs, page_table, name: str = "page_table"):
+    """A table whose pages are counted, as the kernels write it: (rows, entries of a row)."""
+    for t, n in ((refs, "refs"), (page_table, name)):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{n} must be int32")
+        if not t.is_cuda:
+            raise RuntimeError(f"{n} must live on a HIP device; lvar_amd has no CPU path")
+    _require(refs.dim() == 1 and refs.shape[0] > 0 and refs.is_contiguous(), lambda: f"refs must be [num_pages], contiguous, got {tuple(refs.shape)}")
+    _require(page_table.dim() == 2 and page_table.shape[0] > 0 and page_table.shape[1] > 0, lambda: f"{name} must be [B, max_pages], got {tuple(page_table.shape)}")
+    B, n = page_table.shape
+    _require((n == 1 or page_table.stride(1) == 1) and (B == 1 or page_table.stride(0) >= n), lambda: f"rows of {name} must be apart from each other, with unit stride along the pages")
+    _require(refs.device == page_table.device, lambda: f"refs and {name} must be on the same device")
+    return B, n
+
+
+def _table_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _written(*tensors) -> None:
+    """(autograd finds out where it has saved them; tensors of inference mode have no version)"""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None and not t.is_inference()])
+
+
+def _scratch(rows: int, num_pages: int, device):
+    nbytes = int(_lib.load().lvar_kv_pages_scratch_bytes(rows, num_pages))
+    return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None), max(0, nbytes)
+
+
+def kv_pages_alloc(refs, page_table, first, last) -> None:
+    """Opens pages: entries ``first[b] .. last[b]-1`` (int32 ``[B]``, clamped to the row) of every row of ``page_table`` int32 ``[B, max_pages]`` get
+    free pages, in place.  ``refs`` int32 ``[num_pages]`` counts how many entries name each page; a page is free where that is not positive.
+    The lowest free pages are given, in the order of rows and entries, and counted once; entries for which there is none get -1.  What the
+    entries named before is not looked at: give it back first (:func:`kv_pages_free`)."""
+    fast = _native()
+    if fast is not None and fast.fast_pages_alloc(refs, page_table, first, last):
+        return
+    B, n = _counted(refs, page_table)
+    first, last = _per_sequence(first, "first", B, refs.device), _per_sequence(last, "last", B, refs.device)
+    _require(first is not None and last is not None, "first and last must be given")
+    with _on_device(refs):
+        ws, nbytes = _scratch(B, refs.shape[0], refs.device)
+        st = _lib.load().lvar_kv_pages_alloc(refs.data_ptr(), refs.shape[0], page_table.data_ptr(), _table_stride(page_table), B, n, first.data_ptr(), last.data_ptr(),
+                                            _ptr(ws), nbytes, _stream(refs))
+    _lib.check(st, "lvar_kv_pages_alloc")
+    _written(refs, page_table)
+
+
+def kv_pages_free(refs, page_table, keep=None) -> None:
+    """Gives pages back: entries from ``keep[b]`` on (int32 ``[B]``; default: all) of every row become -1, and their pages are counted down in
+    ``refs``; a page that no entry names any more is free.  In place."""
+    fast = _native()
+    if fast is not None and fast.fast_pages_free(refs, page_table, keep):
+        return
+    B, n = _counted(refs, page_table)
+    keep = _per_sequence(keep, "keep", B, refs.device)
+    with _on_device(refs):
+        st = _lib.load().lvar_kv_pages_free(refs.data_ptr(), refs.shape[0], page_table.data_ptr(), _table_stride(page_table), B, n, _ptr(keep), _stream(refs))
+    _lib.check(st, "lvar_kv_pages_free")
+    _written(refs, page_table)
+
+
+def kv_cache_fork(cache: PagedKVCache, refs, page_table, source, target, lengths) -> None:
+    """Row ``target[i]`` of ``page_table`` becomes a copy of the sequence in row ``source[i]`` (int32 ``[n]``, on the device), of its first
+    ``lengths[source[i]]`` tokens (int32 ``[B]``): whole pages are shared, by name, and counted up in ``refs``; the tokens of the page that is not whole are
+    copied to the lowest free page, so that both sequences can go on; entries behind it become -1.  In place.
+
+    What the target's row named before is not looked at: give it back first (:func:`kv_pages_free`).  Where there is no free page the entry gets
+    -1.  Pairs with a row outside the table, and of a row with itself, are left out.  Two forks with the same target, or a target that is
+    the source of another, leave these rows undefined."""
+    fast = _native()
+    if fast is not None and fast.fast_cache_fork(cache, refs, page_table, source, target, lengths):
+        return
+    _no_gradient("kv_cache_fork", cache.k, cache.v)
+    B, _ = _counted(refs, page_table)
+    arg = _cache_arg(cache, page_table, B, refs.device)
+    arg.table_stride = _table_stride(page_table)
+    _require(refs.shape[0] == cache.k.shape[0], lambda: f"refs must be [num_pages = {cache.k.shape[0]}], got {tuple(refs.shape)}")
+    _require(source is not None and target is not None and lengths is not None, "source, target and lengths must be given")
+    n = source.shape[0] if source.dim() == 1 else -1
+    source, target = _per_sequence(source, "source", n, refs.device), _per_sequence(target, "target", n, refs.device)
+    lengths = _per_sequence(lengths, "lengths", B, refs.device)
+    if n == 0:
+        return
+    with _on_device(refs):
+        ws, nbytes = _scratch(n, refs.shape[0], refs.device)
+        st = _lib.load().lvar_kv_cache_fork(arg, refs.data_ptr(), page_table.data_ptr(), B, source.data_ptr(), target.data_ptr(), lengths.data_ptr(), n,
+                                           _ptr(ws), nbytes, _stream(refs))
+    _lib.check(st, "lvar_kv_cache_fork")
+    _written(refs, page_table, *cache)
+
+
+def kv_cache_compact(cache: PagedKVCache, page_table, keep, out_table, counts=None) -> None:
+    """Keeps a part of each sequence: token i of head h in the pages of ``out_table`` becomes token ``keep[b, h, i]`` of those of ``page_table`` (both
+    int32 ``[B, max_pages]``), as its bytes are, for the first ``counts[b]`` (int32 ``[B]``; default: all) of the n that ``keep`` (int32 or
+    int64 ``[B, kv_heads, n]``; a broadcast one is read in place) lists: what :func:`lvar_amd.sparse_attn_ops.scalekv_keep_indices` selects, every
+    head other tokens.  Tokens that ``page_table`` does not name become zeros; places that ``out_table`` does not name are not written.  A page
+    that both tables name is left undefined: open new pages (:func:`kv_pages_alloc`) and give the old ones back afterwards."""
+    fast = _native()
+    if fast is not None and fast.fast_cache_compact(cache, page_table, keep, out_table, counts):
+        return
+    _no_gradient("kv_cache_compact", cache.k, cache.v)
+    device, B = cache.k.device, page_table.shape[0]
+    arg = _cache_arg(cache, page_table, B, device)
+    out = _cache_arg(cache, out_table, B, device)
+    if keep.dtype not in (torch.int32, torch.int64):
+        raise TypeError("keep must be int32 or int64")
+    Hkv = cache.k.shape[1]
+    _require(keep.dim() == 3 and tuple(keep.shape[:2]) == (B, Hkv), lambda: f"keep must be [B, kv_heads, n] = [{B}, {Hkv}, n], got {tuple(keep.shape)}")
+    _require(keep.device == device, "keep must be on the device of the cache")
+    counts = _per_sequence(counts, "counts", B, device)
+    if keep.shape[2] == 0 or B == 0:
+        return
+    with _on_device(cache.k):
+        st = _lib.load().lvar_kv_cache_compact(arg, out.page_table, out.table_stride, out.max_pages, keep.data_ptr(), 1 if keep.dtype == torch.int64 else 0,
+                                              keep.stride(0), keep.stride(1), keep.stride(2), _ptr(counts), B, keep.shape[2], _stream(cache.k))
+    _lib.check(st, "lvar_kv_cache_compact")
+    _written(*cache)
 
 
 def paged_attn(q, cache: PagedKVCache, page_table, lengths, scale=None, causal: bool = False, counts=None, max_len: Optional[int] = None):

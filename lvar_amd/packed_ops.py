@@ -68,12 +68,15 @@ class _PackedAttn(torch.autograd.Function):
         ctx.how = (causal, scale)
         ctx.save_for_backward(q, k, v, o, M, L, offsets, k_offsets)
         ctx.mark_non_differentiable(M, L)
+        ctx.set_materialize_grads(False)
         return o, M, L
 
     @staticmethod
     def backward(ctx, go, *_):
         if torch.is_grad_enabled():
             raise RuntimeError("packed_attn can be differentiated once: its gradients have no graph (create_graph)")
+        if go is None:
+            return (None,) * 7
         _no_tangent("the gradient of packed_attn", go)
         q, k, v, o, M, L, offsets, k_offsets = ctx.saved_tensors
         causal, scale = ctx.how
