@@ -482,9 +482,15 @@ typedef struct {
   int position_type;
 } lvar_rope_axes_t;
 
-/* lvar_qk_norm_rope_fwd, lvar_qk_norm_rope_bwd (its scratch too) and lvar_kv_cache_append with such a rotation; how.cos and how.sin NULL. */
+/*
+ * lvar_qk_norm_rope_fwd, lvar_qk_norm_rope_bwd and lvar_kv_cache_append with such a rotation; how.cos and how.sin NULL.
+ * scratch of the backward pass: lvar_qk_norm_axes_bwd_scratch_bytes() (16-byte aligned, needs no preparation; per_sequence: pos_stride_b is not 0,
+ * the positions differ between sequences), for the weight gradients and for tables of the angles of large calls; without room for the tables
+ * angles are formed where they are used, with the same results.
+ */
 int lvar_qk_norm_axes_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, lvar_rope_axes_t axes, void* oq, void* ok, int B, int H,
                           int kv_heads, int L, int head_dim, void* stream);
+int64_t lvar_qk_norm_axes_bwd_scratch_bytes(int B, int H, int kv_heads, int L, int head_dim, int rot_dim, int per_sequence);
 int lvar_qk_norm_axes_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, lvar_rope_axes_t axes, const void* gq, const void* gk,
                           lvar_tensor_t dq, lvar_tensor_t dk, void* dqw, void* dkw, void* scratch, int64_t scratch_bytes, int B, int H,
                           int kv_heads, int L, int head_dim, void* stream);

@@ -22,7 +22,7 @@ EXPORTED_SYMBOLS = (
     "lvar_window_key_scores",
     "lvar_qk_norm_rope_fwd", "lvar_qk_norm_rope_bwd_scratch_bytes", "lvar_qk_norm_rope_bwd", "lvar_kv_cache_append", "lvar_kv_cache_read",
     "lvar_paged_attn_workspace_bytes", "lvar_paged_attn_fwd",
-    "lvar_qk_norm_axes_fwd", "lvar_qk_norm_axes_bwd", "lvar_kv_cache_append_axes",
+    "lvar_qk_norm_axes_fwd", "lvar_qk_norm_axes_bwd_scratch_bytes", "lvar_qk_norm_axes_bwd", "lvar_kv_cache_append_axes",
     "lvar_kv_pages_scratch_bytes", "lvar_kv_pages_alloc", "lvar_kv_pages_free", "lvar_kv_cache_fork", "lvar_kv_cache_compact",
     "lvar_packed_attn_fwd", "lvar_packed_attn_bwd_workspace_bytes", "lvar_packed_attn_bwd",
 )
@@ -147,6 +147,8 @@ def load() -> C.CDLL:
     X = LvarRopeAxes
     lib.lvar_qk_norm_axes_fwd.restype = I
     lib.lvar_qk_norm_axes_fwd.argtypes = [T, T, N, X, P, P, I, I, I, I, I, P]
+    lib.lvar_qk_norm_axes_bwd_scratch_bytes.restype = I64
+    lib.lvar_qk_norm_axes_bwd_scratch_bytes.argtypes = [I] * 7
     lib.lvar_qk_norm_axes_bwd.restype = I
     lib.lvar_qk_norm_axes_bwd.argtypes = [T, T, N, X, P, P, T, T, P, P, P, I64, I, I, I, I, I, P]
     lib.lvar_kv_cache_append_axes.restype = I

@@ -125,6 +125,8 @@ inline bool grid_fits(int64_t workgroups, int threads) { return workgroups * thr
 
 int launch_norm_rope(NormRopeParams p, int head_dim, bool append, hipStream_t s);
 int norm_rope_bwd_blocks(int B, int H, int Hkv, int L, int head_dim, bool alone);
+int64_t axis_table_bytes(const NormRopeParams& p);
+int launch_axis_tables(NormRopeParams& p, void* scratch, hipStream_t s);
 int launch_norm_rope_bwd(NormRopeParams p, int head_dim, hipStream_t s);
 int launch_weight_grad(const WeightGradParams& w, hipStream_t s);
 int launch_kv_read(const KvReadParams& p, int head_dim, hipStream_t s);

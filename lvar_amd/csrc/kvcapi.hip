@@ -65,6 +65,13 @@ int fill_axes(NormRopeParams& p, const lvar_rope_axes_t* ax, int B, int head_dim
   return LVAR_OK;
 }
 
+// tables of the angles, where the call is large and there is room for them
+int make_tables(NormRopeParams& p, void* scratch, int64_t bytes, hipStream_t s) {
+  const int64_t want = p.freqs ? axis_table_bytes(p) : 0;
+  if (want == 0 || !scratch || bytes < want) return LVAR_OK;
+  return aligned(scratch, 16) ? launch_axis_tables(p, scratch, s) : LVAR_EINVAL;
+}
+
 void fill_qk(NormRopeParams& p, const lvar_tensor_t& q, const lvar_tensor_t& k, int B, int H, int kv_heads, int L) {
   p.q = (const bf16_t*)q.ptr; p.q_sb = q.stride_b; p.q_sh = q.stride_h; p.q_sr = q.stride_row;
   p.k = (const bf16_t*)k.ptr; p.k_sb = k.stride_b; p.k_sh = k.stride_h; p.k_sr = k.stride_row;
@@ -163,12 +170,14 @@ int norm_rope_bwd(lvar_tensor_t q, lvar_tensor_t k, const lvar_norm_rope_t& how,
     w.cols[i] = wv[i]->mode == W_COLUMN ? head_dim : 1;
     w.bf16[i] = wv[i]->bf16;
   }
+  const int64_t weights = (scratch_bytes(B, H, kv_heads, L, head_dim) + 15) / 16 * 16;
+  if (ax && (st = make_tables(p, scratch ? (char*)scratch + weights : nullptr, bytes - weights, (hipStream_t)stream)) != LVAR_OK) return st;
   if ((st = launch_norm_rope_bwd(p, head_dim, (hipStream_t)stream)) != LVAR_OK || !rest) return st;
   return launch_weight_grad(w, (hipStream_t)stream);
 }
 
 int append(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, const lvar_norm_rope_t* how, const lvar_rope_axes_t* ax, void* oq, lvar_paged_cache_t cache,
-                         const int32_t* start, const int32_t* counts, int B, int H, int L, void* stream) {
+           const int32_t* start, const int32_t* counts, int B, int H, int L, void* stream) {
   NormRopeParams p{};
   int st = fill_cache(p.cache, cache);
   if (st != LVAR_OK) return st;
@@ -213,6 +222,15 @@ int lvar_qk_norm_rope_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how
 int lvar_qk_norm_axes_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_norm_rope_t how, lvar_rope_axes_t axes, void* oq, void* ok, int B, int H, int kv_heads,
                           int L, int head_dim, void* stream) {
   return norm_rope_fwd(q, k, how, &axes, oq, ok, B, H, kv_heads, L, head_dim, stream);
+}
+
+int64_t lvar_qk_norm_axes_bwd_scratch_bytes(int B, int H, int kv_heads, int L, int head_dim, int rot_dim, int per_sequence) {
+  const int64_t weights = scratch_bytes(B, H, kv_heads, L, head_dim);   // (checks the sizes)
+  if (weights < 0) return weights;
+  if (rot_dim <= 0 || rot_dim > head_dim) return LVAR_EINVAL;
+  NormRopeParams p{};
+  p.B = B; p.H = H; p.Hkv = kv_heads; p.L = L; p.rot = rot_dim; p.pos_sb = per_sequence ? L : 0;
+  return (weights + 15) / 16 * 16 + axis_table_bytes(p);
 }
 
 int64_t lvar_qk_norm_rope_bwd_scratch_bytes(int B, int H, int kv_heads, int L, int head_dim) { return scratch_bytes(B, H, kv_heads, L, head_dim); }

@@ -13,6 +13,7 @@
 namespace lvar {
 
 constexpr int NR_T = 256;
+constexpr int64_t AXIS_TABLE_ROWS = 1 << 18;   // rows (tokens x heads) from which on a backward pass makes tables of its angles
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 
 // Results of large forward launches go past the L2s, whoever reads them next mostly sits on another XCD: 2 x 16 x 4096 rows of q and of k
@@ -31,9 +32,48 @@ struct Angles {
   bool second;        // halves: this lane holds the second elements
 };
 
+// Sine and cosine of a number of turns in -1/2 .. 1/2, off by about a step of 32 bits: the nearest quarter turn is taken off in 64 bits, and what is
+// left, at most pi / 4, goes into the power series of both up to x^9 and x^8 (their next terms are below 2^-28 and 2^-25 there).
+__device__ __forceinline__ void sincos_of_turns(double t, float& s, float& c) {
+  const float n = __builtin_rintf(4.f * (float)t);
+  const float x = 6.28318530717958647692f * (float)__builtin_fma((double)n, -0.25, t), z = x * x;
+  const float a = x * __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), 1.f);
+  const float b = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 1.f / 40320, -1.f / 720), 1.f / 24), -0.5f), 1.f);
+  const int q = (int)n & 3;   // (of NaN: 0, and a and b are NaN)
+  const float u = q & 1 ? b : a, v = q & 1 ? a : b;
+  s = q & 2 ? -u : u;
+  c = (q + 1) & 2 ? -v : v;
+}
+
+// Sines and cosines of pairs pair .. pair + 3 of token i of sequence b.
+__device__ __forceinline__ void four_angles(const NormRopeParams& p, int b, int i, int pair, float* s, float* c) {
+  double turn[4] = {};
+  for (int x = 0; x < p.axes; x++) {
+    const int64_t at = b * p.pos_sb + x * p.pos_sa + i * p.pos_sl;
+    const double pos = (p.pos64 == 2 ? (double)((const float*)p.positions)[at]
+                        : p.pos64    ? (double)((const int64_t*)p.positions)[at]
+                                     : (double)((const int32_t*)p.positions)[at]) * 0.15915494309189533577;   // 1 / (2 pi)
+    const int64_t f = x * p.freq_sa + pair;
+    if (p.freq32) {
+      const f32x4 v = *(const f32x4*)((const float*)p.freqs + f);
+#pragma unroll
+      for (int e = 0; e < 4; e++) turn[e] = __builtin_fma(pos, (double)v[e], turn[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const f64x2 v = *(const f64x2*)((const double*)p.freqs + f + e);
+        turn[e] = __builtin_fma(pos, v[0], turn[e]);
+        turn[e + 1] = __builtin_fma(pos, v[1], turn[e + 1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) sincos_of_turns(turn[e] - __builtin_rint(turn[e]), s[e], c[e]);
+}
+
 // Cosines and sines of the lane's pairs: of a row of the tables, or (AXES) of the sum over the axes of position times frequency, of token i of
 // sequence b.  That sum is formed in 64 bits, as turns of which only the fraction is kept: a position of 2^20 times a frequency of 1 is known to
-// 2^-4 of a radian in 32 bits.  Sine and cosine of the fraction are 32-bit functions (off by about one step).
+// 2^-4 of a radian in 32 bits.
 template <int LPR, bool AXES>
 __device__ __forceinline__ void load_angles(const NormRopeParams& p, int64_t row, int b, int i, int lane, Angles& a) {
   const int col = lane * 8, half = p.rot >> 1;
@@ -48,37 +88,19 @@ __device__ __forceinline__ void load_angles(const NormRopeParams& p, int64_t row
   }
   if (!a.on) { a.partner = lane; return; }
   if constexpr (AXES) {
-    double turn[8] = {};
-    for (int x = 0; x < p.axes; x++) {
-      const int64_t at = b * p.pos_sb + x * p.pos_sa + i * p.pos_sl;
-      const double pos = (p.pos64 == 2 ? (double)((const float*)p.positions)[at]
-                          : p.pos64    ? (double)((const int64_t*)p.positions)[at]
-                                       : (double)((const int32_t*)p.positions)[at]) * 0.15915494309189533577;   // 1 / (2 pi)
-      const int64_t f = x * p.freq_sa + pair;
-      if (p.freq32) {
+    // Four pairs per lane: those of two neighbouring columns are its own; of the halves, whose pairs two lanes share, each forms one half and they swap.
+    if (!p.interleaved) pair += a.second ? 4 : 0;
+    four_angles(p, b, i, pair, a.s, a.c);
+    if (!p.interleaved) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 4)
-          if (e == 0 || !p.interleaved) {
-            const f32x4 v = *(const f32x4*)((const float*)p.freqs + f + e);
-#pragma unroll
-            for (int j = 0; j < 4; j++) turn[e + j] = __builtin_fma(pos, (double)v[j], turn[e + j]);
-          }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2)
-          if (e < 4 || !p.interleaved) {
-            const f64x2 v = *(const f64x2*)((const double*)p.freqs + f + e);
-            turn[e] = __builtin_fma(pos, v[0], turn[e]);
-            turn[e + 1] = __builtin_fma(pos, v[1], turn[e + 1]);
-          }
+      for (int e = 0; e < 4; e++) {
+        const float so = __shfl(a.s[e], a.partner, LPR), co = __shfl(a.c[e], a.partner, LPR);
+        a.s[4 + e] = a.second ? a.s[e] : so;
+        a.c[4 + e] = a.second ? a.c[e] : co;
+        a.s[e] = a.second ? so : a.s[e];
+        a.c[e] = a.second ? co : a.c[e];
       }
     }
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (e < 4 || !p.interleaved) {
-        const float part = (float)(turn[e] - __builtin_rint(turn[e]));
-        sincospif(2.f * part, &a.s[e], &a.c[e]);
-      }
     return;
   }
   const float *cp = p.cos + row * p.cs_row + pair, *sp = p.sin + row * p.cs_row + pair;
@@ -180,8 +202,9 @@ __host__ __device__ __forceinline__ int chunks_of(const NormRopeParams& p, bool 
   return (append && p.ready ? 0 : (p.H + HC - 1) / HC) + (append ? 2 * nk : nk);
 }
 
-template <int D, int HC, bool APPEND, bool AXES>
-__device__ __forceinline__ void norm_rope_item(const NormRopeParams& p) {
+// AXES: angles from several position axes
+template <int D, int HC, bool APPEND, bool AXES = false>
+__global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p) {
   constexpr int LPR = D / 8, RPB = NR_T / LPR;
   const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
   // heads fastest: the rows of a token lie next to each other in a fused projection (heads slowest, so that workgroups in flight
@@ -271,13 +294,6 @@ __device__ __forceinline__ void norm_rope_item(const NormRopeParams& p) {
   }
 }
 
-template <int D, int HC, bool APPEND>
-__global__ __launch_bounds__(NR_T) void norm_rope_kernel(const NormRopeParams p) { norm_rope_item<D, HC, APPEND, false>(p); }
-
-// the same with angles from several position axes
-template <int D, int HC, bool APPEND>
-__global__ __launch_bounds__(NR_T) void norm_axes_kernel(const NormRopeParams p) { norm_rope_item<D, HC, APPEND, true>(p); }
-
 // Constants of the division of 32-bit numbers by L (rounded-up reciprocal, Granlund and Montgomery 1994, figure 4.1).
 static void division_by(NormRopeParams& p) {
   const uint32_t L = (uint32_t)p.L;
@@ -295,12 +311,12 @@ static bool launch_fwd(const NormRopeParams& p, bool append, hipStream_t s) {
   if (!grid_fits(groups, NR_T)) return false;
   if constexpr (D >= 64) {   // (head dimensions of a cache)
     if (append) {
-      if (p.freqs) hipLaunchKernelGGL((norm_axes_kernel<D, HC, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+      if (p.freqs) hipLaunchKernelGGL((norm_rope_kernel<D, HC, true, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
       else hipLaunchKernelGGL((norm_rope_kernel<D, HC, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
       return true;
     }
   }
-  if (p.freqs) hipLaunchKernelGGL((norm_axes_kernel<D, HC, false>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
+  if (p.freqs) hipLaunchKernelGGL((norm_rope_kernel<D, HC, false, true>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
   else hipLaunchKernelGGL((norm_rope_kernel<D, HC, false>), dim3((uint32_t)groups), dim3(NR_T), 0, s, p);
   return true;
 }
@@ -507,6 +523,46 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const WeightGradParam
       else ((float*)w.out[k])[at] = s;
     }
   }
+}
+
+// ---- tables of the angles of a call ----
+
+// A large backward pass reads cosines and sines from tables that a launch ahead of it writes to scratch memory, with the row of every token: the
+// angles are formed once, not once per pair of heads.  Formed in place / from tables, both launches, 32 + 8 heads of 128 with three axes, pairs of
+// neighbours: 410 tokens 12.2 / 14.7 us, 3280 34.5 / 36.0, 8192 65.5 / 64.2, 32768 285 / 266; of halves 12.3 / 14.9, 35.3 / 35.3, 68.1 / 65.0, 308 / 277.
+// The forward launches, whose workgroups form them for four heads and do not loop, gain nothing (2 x 32 heads of 4096 into a cache 39.7 / 41.1).
+__global__ __launch_bounds__(NR_T) void axis_tables_kernel(const NormRopeParams p, float* cos, float* sin, int32_t* row_of, int rows) {
+  const int quads = p.rot >> 3;                                  // of pairs
+  const int64_t at = (int64_t)blockIdx.x * NR_T + threadIdx.x;
+  const int64_t r = at / quads;
+  if (at < (int64_t)p.B * p.L) row_of[at] = rows == p.L ? (int)(at % p.L) : (int)at;
+  if (r >= rows) return;
+  const int q = (int)(at - r * quads), b = (int)(r / p.L), i = (int)(r - (int64_t)b * p.L);
+  float s[4], c[4];
+  four_angles(p, b, i, 4 * q, s, c);
+  *(f32x4*)(cos + r * (p.rot >> 1) + 4 * q) = f32x4{c[0], c[1], c[2], c[3]};
+  *(f32x4*)(sin + r * (p.rot >> 1) + 4 * q) = f32x4{s[0], s[1], s[2], s[3]};
+}
+
+static int64_t axis_rows(const NormRopeParams& p) { return p.pos_sb ? (int64_t)p.B * p.L : p.L; }
+
+int64_t axis_table_bytes(const NormRopeParams& p) {
+  if ((int64_t)p.B * p.L * (p.H + p.Hkv) < AXIS_TABLE_ROWS) return 0;
+  return axis_rows(p) * p.rot * 4 + (int64_t)p.B * p.L * 4;
+}
+
+// Writes the tables and turns p into a call that reads them.
+int launch_axis_tables(NormRopeParams& p, void* scratch, hipStream_t s) {
+  const int64_t rows = axis_rows(p), half = p.rot >> 1, tokens = (int64_t)p.B * p.L;
+  float *cos = (float*)scratch, *sin = cos + rows * half;
+  int32_t* row_of = (int32_t*)(sin + rows * half);
+  const int64_t threads = rows * (half >> 2) > tokens ? rows * (half >> 2) : tokens, groups = (threads + NR_T - 1) / NR_T;
+  if (!grid_fits(groups, NR_T)) return LVAR_EINVAL;
+  hipLaunchKernelGGL(axis_tables_kernel, dim3((uint32_t)groups), dim3(NR_T), 0, s, p, cos, sin, row_of, (int)rows);
+  p.cos = cos; p.sin = sin; p.cs_row = half; p.table_rows = (int)rows;
+  p.positions = row_of; p.pos64 = 0; p.pos_sb = p.L; p.pos_sl = 1;
+  p.freqs = nullptr;
+  return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
 }
 
 // Rows of partial weight gradients: as many workgroups along the tokens as give every compute unit about eight, but no more than there are tiles.

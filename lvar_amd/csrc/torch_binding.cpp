@@ -46,7 +46,7 @@ namespace {
   X(lvar_remap_concat_lists) X(lvar_mask_to_lists) X(lvar_window_key_scores)                                              \
   X(lvar_qk_norm_rope_fwd) X(lvar_qk_norm_rope_bwd_scratch_bytes) X(lvar_qk_norm_rope_bwd) X(lvar_kv_cache_append)        \
   X(lvar_kv_cache_read) X(lvar_paged_attn_workspace_bytes) X(lvar_paged_attn_fwd)                                         \
-  X(lvar_qk_norm_axes_fwd) X(lvar_qk_norm_axes_bwd) X(lvar_kv_cache_append_axes)                                          \
+  X(lvar_qk_norm_axes_fwd) X(lvar_qk_norm_axes_bwd_scratch_bytes) X(lvar_qk_norm_axes_bwd) X(lvar_kv_cache_append_axes)   \
   X(lvar_kv_pages_scratch_bytes) X(lvar_kv_pages_alloc) X(lvar_kv_pages_free) X(lvar_kv_cache_fork) X(lvar_kv_cache_compact)
 struct Api {
 #define LVAR_FIELD(name) decltype(&::name) name = nullptr;
@@ -727,10 +727,9 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     if (wq.defined() && wq.requires_grad()) dwq = empty(wq.sizes(), wq.scalar_type(), dev);
     if (wk.defined() && wk.requires_grad()) dwk = empty(wk.sizes(), wk.scalar_type(), dev);
     int64_t bytes = 0;
-    if (dwq.defined() || dwk.defined()) {
-      bytes = api.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d);
-      if (bytes > 0) scratch = empty({bytes}, at::kByte, dev);
-    }
+    if (freqs.defined()) bytes = api.lvar_qk_norm_axes_bwd_scratch_bytes(B, H, Hkv, L, d, ax.rot_dim, ax.pos_stride_b != 0);
+    else if (dwq.defined() || dwk.defined()) bytes = api.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d);
+    if (bytes > 0) scratch = empty({bytes}, at::kByte, dev);
     void* const stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
     const int st = freqs.defined()
         ? api.lvar_qk_norm_axes_bwd(view(q), view(k), h, ax, gq.data_ptr(), gk.data_ptr(), view(dq), view(dk), ptr(dwq), ptr(dwk), ptr(scratch), bytes, B, H, Hkv, L, d, stream)

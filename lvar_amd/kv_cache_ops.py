@@ -285,12 +285,16 @@ class _NormRope(torch.autograd.Function):
         (wq, aq), (wk, ak) = _weight_arg(wq, H, d, "q_weight", q.device), _weight_arg(wk, Hkv, d, "k_weight", q.device)
         lib = _lib.load()
         with _on_device(q):
-            nbytes = int(lib.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d)) if dwq is not None or dwk is not None else 0
+            axes = None
+            if freqs is not None:
+                freqs, positions, axes = _axes_arg(freqs, positions, interleaved, B, L, d, q.device)
+                nbytes = int(lib.lvar_qk_norm_axes_bwd_scratch_bytes(B, H, Hkv, L, d, axes.rot_dim, 1 if axes.pos_stride_b else 0))
+            else:
+                nbytes = int(lib.lvar_qk_norm_rope_bwd_scratch_bytes(B, H, Hkv, L, d)) if dwq is not None or dwk is not None else 0
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
             how = _how(cos, sin, positions, aq, ak, norm, eps, interleaved, B, L, q.device)
             rest = (gq.data_ptr(), gk.data_ptr(), _view(dq), _view(dk), _ptr(dwq), _ptr(dwk), _ptr(scratch), nbytes, B, H, Hkv, L, d, _stream(q))
-            if freqs is not None:
-                freqs, positions, axes = _axes_arg(freqs, positions, interleaved, B, L, d, q.device)
+            if axes is not None:
                 st = lib.lvar_qk_norm_axes_bwd(_view(q), _view(k), how, axes, *rest)
             else:
                 st = lib.lvar_qk_norm_rope_bwd(_view(q), _view(k), how, *rest)
