@@ -28,6 +28,8 @@ HIPCC_FLAGS = ["-O3", f"--offload-arch={ARCH}", "-fPIC", "-std=c++17", "-fno-hon
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # these keep NaN as NaN (a cache may hold some in places that nobody reads, and what is read has to show them)
 HONOR_NANS = ("normrope.hip", "kvread.hip", "pagedattn.hip", "pages.hip", "kvcapi.hip", "packedapi.hip")
+def _flags(src: str):
+    return [f for f in HIPCC_FLAGS if src not in HONOR_NANS or f not in ("-fno-honor-nans", "-mno-amdgpu-ieee")]
 
 
 def _hipcc() -> str:
@@ -54,8 +56,7 @@ def build_library(verbose: bool = False) -> str:
 
     def compile_one(pair):
         src, obj = pair
-        flags = [f for f in HIPCC_FLAGS if src not in HONOR_NANS or f not in ("-fno-honor-nans", "-mno-amdgpu-ieee")]
-        return _run([hipcc, *flags, "-c", os.path.join(CSRC, src), "-o", obj])
+        return _run([hipcc, *_flags(src), "-c", os.path.join(CSRC, src), "-o", obj])
 
     with ThreadPoolExecutor(max_workers=min(4, len(SOURCES))) as ex:
         outs = list(ex.map(compile_one, zip(SOURCES, objs)))

@@ -22,8 +22,8 @@ struct PackedParams {
   int64_t g_sh, g_sr;
   bf16_t *dq, *dk, *dv;             // null: not wanted
   int64_t dq_sh, dq_sr, dk_sh, dk_sr, dv_sh, dv_sr;
-  float *nl, *nd;                   // [H,T]: -(M + log2 L) / c (-inf: the row sees nothing), -sum(do * o)
-  int slots;                        // set at launch: places for tiles, see find_tile
+  int slots;                        // set at launch: places for query tiles, see find_tile
+  float* stats;                     // [H,2,T]: -(M + log2 L) / c (-inf: the row sees nothing), and -sum(do * o)
 };
 
 int launch_packed_fwd(PackedParams p, int head_dim, hipStream_t s);
@@ -35,10 +35,20 @@ inline int64_t packed_slots(int T, int B, int R) { return (int64_t)T / R + B + 2
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
+// Sum over the 64 lanes, the same in all of them
+__device__ __forceinline__ int wave_sum(int x) {
+  auto add = [](int v, auto ctrl) { return v + __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, 0xf, 0xf, true); };
+  x = add(x, std::integral_constant<int, 0xB1>{});    // quad_perm [1,0,3,2]
+  x = add(x, std::integral_constant<int, 0x4E>{});    // quad_perm [2,3,0,1]
+  x = add(x, std::integral_constant<int, 0x141>{});   // row_half_mirror
+  x = add(x, std::integral_constant<int, 0x140>{});   // row_mirror
+  return __builtin_amdgcn_readlane(x, 0) + __builtin_amdgcn_readlane(x, 16) + __builtin_amdgcn_readlane(x, 32) + __builtin_amdgcn_readlane(x, 48);
+}
+
 struct PackedTile {
-  int b;         // sequence, or -1: rows of no sequence
-  int first, n;  // its first row and how many it has
-  int row0;      // first row of the tile within it
+  int first, n;               // the sequence's first row and how many it has
+  int row0;                   // first row of the tile within it
+  int other_first, other_n;   // its rows on the other side (keys of a query tile, queries of a key tile); none for rows of no sequence
 };
 
 // Border v of the B + 3 borders of T rows: 0, the offsets, T.  (Offsets out of range, a caller's mistake, stay in it.)
@@ -47,36 +57,69 @@ __device__ __forceinline__ int packed_border(const int32_t* off, int B, int T, i
   return v > B + 1 ? T : max(0, min(off[v - 1], T));
 }
 
-// The range and tile of place `slot`.  Range v takes the places from floor(border(v) / R) + v on: a range of n rows starting anywhere
-// has at most floor((border + n) / R) - floor(border / R) + 1 tiles, so its places suffice, and which range a place belongs to
-// is found among the borders without knowing the lengths in between: 64 candidates per step.  False: a place without a tile.
+// The range and tile of place `slot`, and the sequence's rows on the other side.  Range v takes the places from floor(border(v) / R) + v on: a range of
+// n rows starting anywhere has at most floor((border + n) / R) - floor(border / R) + 1 tiles, so its places suffice, and which range a
+// place belongs to is found among the borders without knowing the lengths in between: 64 candidates per step, and with up to 62 sequences in
+// one round trip to memory.  False: a place without a tile.
+//
+// `levels` (up to 62 sequences, a lane each): of a causal launch over key tiles those of a range differ in work, the first having the most
+// rows behind it, and the launch would end on whichever long one comes late: place by place the tiles with the most behind
+// them, of all ranges.  (12 sequences of up to 2047 tokens, 8 x 4 heads: 492 -> 404 us.  Query tiles, four times as many and each shorter, gain nothing.)
 template <int R>
-__device__ __forceinline__ bool find_tile(const int32_t* off, int B, int T, int slot, PackedTile& t) {
+__device__ __forceinline__ bool find_tile(const int32_t* off, int T, const int32_t* other, int other_T, int B, int slot, bool levels, PackedTile& t) {
   const int lane = __builtin_amdgcn_workitem_id_x() & 63;
-  int v = 0, n = B + 2;
-  while (n > 1) {
-    const int step = (n + 63) >> 6, at = v + lane * step;
-    const bool in = lane * step < n;
-    const int e = packed_border(off, B, T, in ? at : 0);
-    const uint64_t mine = __builtin_amdgcn_ballot_w64(in && e / R + at <= slot);
-    const int k = mine ? 63 - __builtin_clzll(mine) : 0;
-    v += k * step;
-    n = min(step, n - k * step);
+  int v;
+  if (B + 2 <= 64) {
+    const int first = packed_border(off, B, T, lane), next = packed_border(off, B, T, lane + 1);
+    const int o_first = packed_border(other, B, other_T, lane), o_next = packed_border(other, B, other_T, lane + 1);
+    const bool range = lane < B + 2;
+    if (levels) {
+      const int tiles = range ? (max(0, next - first) + R - 1) / R : 0;
+      auto tiles_from = [&](int level) { return wave_sum(max(0, tiles - level)); };   // on levels level + 1 and up
+      if (slot >= tiles_from(0)) return false;
+      int lo = 0, hi = (T + R - 1) / R;                                               // tiles_from(hi) <= slot < tiles_from(lo)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tiles_from(mid) <= slot) hi = mid; else lo = mid;
+      }
+      const int rank = slot - tiles_from(hi);   // among the ranges with a tile on level hi
+      const uint64_t mine = __builtin_amdgcn_ballot_w64(tiles >= hi);
+      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(mine >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mine, 0));
+      v = __builtin_ctzll(__builtin_amdgcn_ballot_w64(tiles >= hi && before == rank));
+      t.row0 = (__builtin_amdgcn_readlane(tiles, v) - hi) * R;
+    } else {
+      const uint64_t mine = __builtin_amdgcn_ballot_w64(range && first / R + lane <= slot);
+      v = mine ? 63 - __builtin_clzll(mine) : 0;
+      t.row0 = (slot - (__builtin_amdgcn_readlane(first, v) / R + v)) * R;
+    }
+    t.first = __builtin_amdgcn_readlane(first, v);
+    t.n = __builtin_amdgcn_readlane(next, v) - t.first;
+    t.other_first = __builtin_amdgcn_readlane(o_first, v);
+    t.other_n = __builtin_amdgcn_readlane(o_next, v) - t.other_first;
+  } else {
+    v = 0;
+    int n = B + 2;
+    while (n > 1) {
+      const int step = (n + 63) >> 6, at = v + lane * step;
+      const bool in = lane * step < n;
+      const int e = packed_border(off, B, T, in ? at : 0);
+      const uint64_t mine = __builtin_amdgcn_ballot_w64(in && e / R + at <= slot);
+      const int k = mine ? 63 - __builtin_clzll(mine) : 0;
+      v += k * step;
+      n = min(step, n - k * step);
+    }
+    v = __builtin_amdgcn_readfirstlane(v);
+    const int two = v + (lane & 1);
+    const int e = packed_border(off, B, T, two), o = packed_border(other, B, other_T, two);
+    t.first = __builtin_amdgcn_readlane(e, 0);
+    t.n = __builtin_amdgcn_readlane(e, 1) - t.first;
+    t.row0 = (slot - (t.first / R + v)) * R;
+    t.other_first = __builtin_amdgcn_readlane(o, 0);
+    t.other_n = __builtin_amdgcn_readlane(o, 1) - t.other_first;
   }
-  v = __builtin_amdgcn_readfirstlane(v);
-  t.first = __builtin_amdgcn_readfirstlane(packed_border(off, B, T, v));
-  t.n = __builtin_amdgcn_readfirstlane(packed_border(off, B, T, v + 1)) - t.first;
-  t.row0 = (slot - (t.first / R + v)) * R;
-  t.b = v >= 1 && v <= B ? v - 1 : -1;
+  if (v == 0 || v > B) t.other_n = 0;
+  t.other_n = max(0, t.other_n);
   return t.row0 >= 0 && t.row0 < t.n;
-}
-
-// Rows of a sequence on the other side (keys of a query tile, queries of a key tile); none for rows of no sequence.
-__device__ __forceinline__ void packed_range(const int32_t* off, int b, int T, int& first, int& n) {
-  first = n = 0;
-  if (b < 0) return;
-  first = __builtin_amdgcn_readfirstlane(max(0, min(off[b], T)));
-  n = max(0, __builtin_amdgcn_readfirstlane(max(0, min(off[b + 1], T))) - first);
 }
 
 // Rows of D bf16 in LDS, unpadded (an LDS fill writes 1 KiB of consecutive bytes), the 16-byte chunks of a row moved by an XOR that suits both
@@ -108,11 +151,28 @@ struct PackedLds {
   }
 };
 
-// Raw buffer descriptor of n rows (bytes below 2^31, checked on the host): what lies beyond reads as zeros.
-__device__ __forceinline__ i32x4 packed_rsrc(const bf16_t* base, int n, int row_bytes, int stride_bytes) {
+// The same operands from LDS byte addresses that hold the lane's own offset (row_at, tr_at) already, on buffers aligned to 512 bytes: what differs per
+// operand is an XOR or part of the instruction, and nothing is kept in registers for it.
+template <int D>
+struct PackedOperands {
+  static __device__ __forceinline__ bf16x8 rows(uint32_t at, int ks) { return *(LVAR_LDS const bf16x8*)(uintptr_t)(at ^ (ks << 5)); }
+  static __device__ __forceinline__ bf16x8 columns(uint32_t at, int kb, int m) {
+    const uint32_t lo = at ^ (m << 6), hi = at ^ (m << 6) ^ 32;
+    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LVAR_LDS bf16x4*)(uintptr_t)(lo + kb * 32 * D));
+    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LVAR_LDS bf16x4*)(uintptr_t)(hi + kb * 32 * D + 16 * D));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+// Raw buffer descriptor of `bytes` from base on (below 2^31, checked on the host): what lies beyond reads as zeros.
+__device__ __forceinline__ i32x4 packed_rsrc(const void* base, int bytes) {
   const uint64_t a = (uint64_t)base;
   return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(uint32_t)((a >> 32) & 0xffffu)),
-               __builtin_amdgcn_readfirstlane(n > 0 ? (n - 1) * stride_bytes + row_bytes : 0), 0x00020000};
+               __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+// ... of n rows
+__device__ __forceinline__ i32x4 packed_rsrc(const bf16_t* base, int n, int row_bytes, int stride_bytes) {
+  return packed_rsrc(base, n > 0 ? (n - 1) * stride_bytes + row_bytes : 0);
 }
 
 // One of the fills of rows row0 .. row0 + 63 into LDS at byte address dst: the s-th of the NI / NW that a wave issues.  Inline assembly, so that
@@ -135,6 +195,13 @@ __device__ __forceinline__ void fill_slot(const i32x4& rsrc, int srb, int row0, 
       :
       : "s"(m0v), "v"(voff), "s"(rsrc), "s"(soff)
       : "memory");
+}
+// The NR / RPI / NW fills of a wave for NR rows
+template <int D, int NW, int NR>
+__device__ __forceinline__ void fill_rows(const i32x4& rsrc, int srb, int row0, uint32_t dst, int wave, int lane) {
+  static_assert(NR / PackedLds<D>::RPI % NW == 0, "every wave issues as many fills");
+#pragma unroll
+  for (int s = 0; s < NR / PackedLds<D>::RPI / NW; s++) fill_slot<D, NW>(rsrc, srb, row0, dst, wave, lane, s);
 }
 template <int D, int NW>
 __device__ __forceinline__ void fill_tile(const i32x4& rsrc, int srb, int row0, uint32_t dst, int wave, int lane) {

@@ -69,7 +69,7 @@ int lvar_packed_attn_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar
   p.dq = (bf16_t*)dq.ptr; p.dq_sh = dq.stride_h; p.dq_sr = dq.stride_row;
   p.dk = (bf16_t*)dk.ptr; p.dk_sh = dk.stride_h; p.dk_sr = dk.stride_row;
   p.dv = (bf16_t*)dv.ptr; p.dv_sh = dv.stride_h; p.dv_sr = dv.stride_row;
-  p.nl = (float*)workspace; p.nd = p.nl + (int64_t)tokens * H;
+  p.stats = (float*)workspace;
   return launch_packed_bwd(p, head_dim, (hipStream_t)stream);
 }
 

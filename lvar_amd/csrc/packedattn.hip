@@ -46,8 +46,7 @@ __device__ __forceinline__ void packed_fwd_item(const PackedParams& p, char* sme
   const int wave = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_workitem_id_x() >> 6);
   const int hh = lane >> 5, r = lane & 31;
   const S at(lane);
-  int k_first, m;
-  packed_range(p.k_off, w.b, p.Tk, k_first, m);
+  const int k_first = w.other_first, m = w.other_n;
   const int hk = h / p.G, q0 = w.row0 + wave * 32;   // first row of the wave
   const int shift = p.causal ? m - w.n : m;          // row i sees keys below i + shift + 1 (causal), below m
   auto seen_by = [&](int row) { return max(0, p.causal ? min(m, row + shift + 1) : m); };
@@ -302,7 +301,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_fwd_kernel(c
   const int id = __builtin_amdgcn_workgroup_id_x(), place = id / p.H;
   PackedTile w;
   // the places from the last one on: of a causal sequence the tiles with the most keys come first
-  if (!find_tile<NW * 32>(p.q_off, p.B, p.T, p.slots - 1 - place, w)) return;
+  if (!find_tile<NW * 32>(p.q_off, p.T, p.k_off, p.Tk, p.B, p.slots - 1 - place, false, w)) return;
   packed_fwd_item<D, NW>(p, smem, w, packed_head(id - place * p.H, p.H));
 #endif
 }

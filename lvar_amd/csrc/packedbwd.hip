@@ -45,12 +45,10 @@ struct CarefulRow {
       }
     }
   }
-  // columns lo .. hi-1
-  __device__ __forceinline__ void store(const float* a, float factor, bf16_t* to, int lo, int hi) const {
+  __device__ __forceinline__ void store(const float* a, float factor, bf16_t* to) const {
     const int lane = __builtin_amdgcn_workitem_id_x() & 63;
 #pragma unroll
-    for (int e = 0; e < D / 64; e++)
-      if (e * 64 >= lo && e * 64 < hi) to[e * 64 + lane] = (bf16_t)(a[e] * factor);
+    for (int e = 0; e < D / 64; e++) to[e * 64 + lane] = (bf16_t)(a[e] * factor);
   }
 };
 
@@ -79,9 +77,9 @@ __device__ __forceinline__ bf16x8 pack_half(const f32x16& x, int kb) {
 #endif
 
 template <int D>
-constexpr int bwd_lds(int waves, int extra) {
+constexpr int dq_lds(int waves) {
   const int bufs = 4 * 64 * D * 2, out = waves * 32 * (D * 2 + 16);
-  return (bufs > out ? bufs : out) + extra;
+  return bufs > out ? bufs : out;
 }
 
 // ---- dq: 32 query rows per wave, tiles of 64 keys.  S^T and dP^T = V do^T with the rows of q and do as B operands in registers, so a lane
@@ -95,14 +93,13 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
   constexpr int KS = D / 16, MTD = D / 32, TILE = S::TILE;
   const int id = __builtin_amdgcn_workgroup_id_x(), place = id / p.H;
   PackedTile w;
-  if (!find_tile<NW * 32>(p.q_off, p.B, p.T, p.slots - 1 - place, w)) return;
+  if (!find_tile<NW * 32>(p.q_off, p.T, p.k_off, p.Tk, p.B, p.slots - 1 - place, false, w)) return;
   const int h = packed_head(id - place * p.H, p.H), hk = h / p.G;
   const int lane = __builtin_amdgcn_workitem_id_x() & 63;
   const int wave = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_workitem_id_x() >> 6);
   const int hh = lane >> 5, r = lane & 31;
   const S at(lane);
-  int k_first, m;
-  packed_range(p.k_off, w.b, p.Tk, k_first, m);
+  const int k_first = w.other_first, m = w.other_n;
   const int q0 = w.row0 + wave * 32, shift = p.causal ? m - w.n : m;
   auto seen_by = [&](int row) { return max(0, p.causal ? min(m, row + shift + 1) : m); };
   const int T = (seen_by(min(w.row0 + NW * 32, w.n) - 1) + 63) >> 6;
@@ -131,7 +128,11 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
   const float M = p.M[stat], L = p.L[stat];
   const bool sees = seen > 0;
   const float nl = sees ? -(M + __builtin_amdgcn_logf(L)) / c : -INFINITY, nd = sees ? -delta : 0.f;
-  if (hh == 0 && live) { p.nl[stat] = nl; p.nd[stat] = nd; }
+  if (hh == 0 && live) {
+    float* to = p.stats + (int64_t)h * 2 * p.T + trow;
+    to[0] = nl;
+    to[p.T] = nd;
+  }
 
   f32x16 acc[MTD];
   clear(acc);
@@ -197,139 +198,252 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
       CarefulRow<D, false> a;
       a.clear();
       a.add(p.q + h * p.q_sh + x * p.q_sr, p.g + h * p.g_sh + x * p.g_sr, kp, p.k_sr, vp, p.v_sr, 0, __shfl(seen, i, 64), &nli, &ndi, c);
-      a.store(a.a0, p.scale, to + i * p.dq_sr, 0, D);
+      a.store(a.a0, p.scale, to + i * p.dq_sr);
     }
   }
 #endif
 }
 
-// ---- dk and dv: 32 keys per wave, tiles of 64 query rows of every query head that shares the key head.  S and dP with the rows of k and v as
-// B operands in registers, so a lane owns a key column, and P and dS are in the B operand's layout of dv^T += do^T P and
-// dk^T += q^T dS.  The accumulators of S and dP start at -(M + log2 L) / c and -delta of their rows: P is one exp2 of c times the
-// sum, dS one product.  SPLIT (head_dim 256): a workgroup accumulates half of the columns of dk and dv, for whole ones take all registers. ----
+// ---- dk and dv: tiles of 128 keys and of 64 query rows (head_dim 256: 64 and 32) of every query head that shares the key head.
+//
+// Two waves share 32 keys.  One forms S = q k^T and P and adds do^T P to dv^T; the other forms dP = do v^T, takes P from the first through LDS,
+// and adds q^T dS to dk^T.  Each has one operand (k or v) and one sum in registers, which leaves room for what hides latency: it forms S or dP
+// of the coming tile on the matrix cores while the vector ALU turns those of the present one into P or dS, and then adds the present one to its
+// sum.  (One wave with both sums: 2500 cycles per 32 products if it has its SIMD to itself, for it issues an instruction every four cycles at most;
+// as two per SIMD without a tile in hand 2000; of these the matrix cores need 1024.)  The second wave is a tile behind the
+// first, so that P passes behind the barrier that a tile has anyway.  A lane owns a key column: P and dS are in the B operand's layout
+// of the second product as they leave the vector ALU.  S and dP start at -(M + log2 L) / c and -delta of their rows: P is one exp2 of c
+// times the sum, dS one product.
+//
+// Tiles come from the last rows to the first, all heads of a tile behind each other: the workgroups of a sequence, which all end at
+// its last rows, read the same tile at about the same time, from the L2 (from the first rows on, 71 % of the reads missed it); half of the reads
+// still come from further away, so tiles are requested LEAD rounds ahead. ----
 
-constexpr int DKV_STAT = 2 * 2 * 64 * 4;   // bytes of the row statistics of two stages
+template <int D>
+struct Dkv {
+  static constexpr int KW = D == 256 ? 2 : 4, WAVES = 2 * KW, KEYS = 32 * KW;     // pairs of waves; head_dim 256: one wave per SIMD
+  static constexpr int SUB = D == 256 ? 1 : 2, R = 32 * SUB, TILE = R * D * 2;    // 32-row blocks and rows of a tile, its bytes
+  // tiles of q: t-1 .. t+1 are in use, of do: t
+  static constexpr int LEAD = D == 128 ? 1 : 2, Q_RING = LEAD + 3, G_RING = LEAD + 1;
+  static constexpr int G_AT = Q_RING * TILE, P_AT = G_AT + G_RING * TILE, P_WAVE = R * 32 * 2;   // P: [parity][pair]
+  static constexpr int STAT_AT = P_AT + 2 * KW * P_WAVE, STAT_WAVE = Q_RING * 256;               // statistics: [wave][place in the ring]
+  static constexpr int OUT = WAVES * 32 * (D * 2 + 16);
+  static constexpr int bytes() { return STAT_AT + WAVES * STAT_WAVE > OUT ? STAT_AT + WAVES * STAT_WAVE : OUT; }
+};
 
-template <int D, int NW, int SPLIT>
-__global__ __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) void packed_dkv_kernel(const PackedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
-  using S = PackedLds<D>;
-  constexpr int KS = D / 16, MTD = D / 32 / SPLIT, TILE = S::TILE;
-  const int per = p.Hkv * SPLIT;
-  const int id = __builtin_amdgcn_workgroup_id_x(), place = id / per, j = id - place * per;
-  PackedTile w;
-  if (!find_tile<NW * 32>(p.k_off, p.B, p.Tk, place, w)) return;
-  const int hk = j / SPLIT, m0 = (j - hk * SPLIT) * MTD;
-  const int tid = __builtin_amdgcn_workitem_id_x(), lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hh = lane >> 5, r = lane & 31;
-  const S at(lane);
-  int q_first, n;
-  packed_range(p.q_off, w.b, p.T, q_first, n);
-  const int k0 = w.row0 + wave * 32, key = min(k0 + r, w.n - 1);
-  // rows from `from` on see the lane's key; those of the workgroup's first key come first
-  const int shift = w.n - n;
-  const int from = p.causal ? max(0, key - shift) : 0;
-  const int t0 = p.causal ? min(max(0, w.row0 - shift), n) >> 6 : 0, nT = (n + 63) >> 6, per_head = max(0, nT - t0), steps = per_head * p.G;
-  const float c = p.c;
 
-  bf16x8 kf[KS], vf[KS];
-  {
-    const bf16_t *kp = p.k + hk * p.k_sh + (int64_t)(w.first + key) * p.k_sr + hh * 8, *vp = p.v + hk * p.v_sh + (int64_t)(w.first + key) * p.v_sr + hh * 8;
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-      kf[ks] = *(const bf16x8*)(kp + ks * 16);
-      vf[ks] = *(const bf16x8*)(vp + ks * 16);
-    }
+// the first of N elements in slot g: three quarters over the NS steps of the first product, the others over the first HB of the second
+template <int N, int NS, int HB>
+struct DkvSlots {
+  static constexpr int lo(int g) {
+    constexpr int early = N * 3 / 4;
+    return g <= 0 ? 0 : g < NS ? g * early / NS : g < NS + HB ? early + (g - NS) * (N - early) / HB : N;
   }
-  f32x16 dk[MTD], dv[MTD];
-  clear(dk);
-  clear(dv);
-  if (steps > 0) {
-    const int q_srb = (int)p.q_sr * 2, g_srb = (int)p.g_sr * 2;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(LVAR_LDS char*)smem;
-    float* const stats = (float*)(smem + 4 * TILE);   // [stage parity][-(M + log2 L) / c, -delta][64]
-    // stage x: tile t0 + x % per_head of head x / per_head; this thread's statistic of it
-    auto stage = [&](int head, int t, int par) -> float {
-      const int hq = hk * p.G + head;
-      const bf16_t *qp = p.q + hq * p.q_sh + (int64_t)q_first * p.q_sr, *gp = p.g + hq * p.g_sh + (int64_t)q_first * p.g_sr;
-      fill_tile<D, NW>(packed_rsrc(qp, n, S::ROWB, q_srb), q_srb, 64 * t, lds0 + par * TILE, wave, lane);
-      fill_tile<D, NW>(packed_rsrc(gp, n, S::ROWB, g_srb), g_srb, 64 * t, lds0 + (2 + par) * TILE, wave, lane);
-      const int i = 64 * t + (tid & 63);
-      const float* from_stat = tid < 64 ? p.nl : p.nd;
-      return tid < 128 && i < n ? from_stat[(int64_t)hq * p.T + q_first + i] : tid < 64 ? -INFINITY : 0.f;
+};
+
+template <int D, int ROLE>   // ROLE 0: dv, 1: dk
+__device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, const PackedTile& w, const int hk, const int all_waves) {
+  using S = PackedLds<D>;
+  using Q = Dkv<D>;
+  using P = PackedOperands<D>;
+  constexpr int KS = D / 16, MTD = D / 32, TILE = Q::TILE, SUB = Q::SUB, NE = 16 * SUB;
+  const int lane = __builtin_amdgcn_workitem_id_x() & 63, hh = lane >> 5, r = lane & 31;
+  const int wave = all_waves & (Q::KW - 1);
+  const S at(lane);
+  const int q_first = w.other_first, n = w.other_n;
+  const int k0 = w.row0 + wave * 32, key = min(k0 + r, w.n - 1);
+  const int shift = w.n - n;
+  const int from = p.causal ? max(0, key - shift) : 0;   // the first row that sees the lane's key
+  const int b0 = p.causal ? min(max(0, w.row0 - shift), n) / Q::R : 0, last = (n + Q::R - 1) / Q::R - 1, T = max(0, last + 1 - b0) * p.G;
+  const int whole0 = p.causal ? max(0, k0 + 31 - shift) : 0;   // rows from here on see all keys of the wave
+  const float c = p.c;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(LVAR_LDS char*)smem;
+
+  f32x16 acc[MTD];
+  clear(acc);
+  if (T > 0) {
+    // The first waves of the pairs request q, the others do, each with its own copy of the statistic that its sums start at.
+    constexpr int RING = ROLE ? Q::G_RING : Q::Q_RING, FILLS = Q::R / S::RPI / Q::KW + 1;
+    const int srb = (int)(ROLE ? p.g_sr : p.q_sr) * 2, bytes = __builtin_amdgcn_readfirstlane((n - 1) * srb + S::ROWB);
+    const int64_t head_stride = ROLE ? p.g_sh : p.q_sh;
+    const bf16_t* const x0 = (ROLE ? p.g + hk * p.G * p.g_sh : p.q + hk * p.G * p.q_sh) + (int64_t)q_first * (ROLE ? p.g_sr : p.q_sr);
+    const float* const s0 = p.stats + ((int64_t)hk * p.G * 2 + ROLE) * p.T + q_first;
+    const uint32_t fill0 = lds0 + (ROLE ? Q::G_AT : 0), stat0 = lds0 + Q::STAT_AT + all_waves * Q::STAT_WAVE;
+    auto after = [](int pl, int ring) { return pl + TILE == ring * TILE ? 0 : pl + TILE; };   // the next place of a ring
+    int f_t = 0, f_blk = last, f_head = 0, f_pl = 0;   // the tile that is requested next
+    const bf16_t* xp = x0;
+    const float* sp = s0;
+    auto request = [&]() {
+      const bool there = f_t < T;                    // behind the last tile: as many fills, of nothing
+      const int row = there ? f_blk * Q::R : 0;
+      fill_rows<D, Q::KW, Q::R>(packed_rsrc(xp, there ? bytes : 0), srb, row, fill0 + f_pl, wave, lane);
+      const i32x4 rsrc = packed_rsrc(sp, there ? n * 4 : 0);
+      const int voff = lane * 4, soff = row * 4;
+      const uint32_t m0v = stat0 + f_pl / (TILE / 256);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(m0v), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+      f_t++;
+      f_pl = after(f_pl, RING);
+      const bool wrap = ++f_head == p.G;
+      f_head = wrap ? 0 : f_head;
+      f_blk -= wrap ? 1 : 0;
+      xp = wrap ? x0 : xp + head_stride;
+      sp = wrap ? s0 : sp + 2 * (int64_t)p.T;
     };
-    float st = stage(0, t0, 0);
-    if (tid < 128) stats[tid] = st;
-    wait_fills<0>();
-    __syncthreads();
-    int head = 0, t = t0;
-    for (int x = 0; x < steps; x++) {
-      const int par = x & 1;
-      int head_n = head, t_n = t + 1;
-      if (t_n == nT) { t_n = t0; head_n++; }
-      const bool more = x + 1 < steps;
-      if (more) st = stage(head_n, t_n, 1 - par);
-      const char *qbuf = smem + par * TILE, *gbuf = smem + (2 + par) * TILE;
-      const float* sp = stats + par * 128;
+    // Rows behind the last one, in the first tile of every head, have read zeros as their statistics: they see nothing.
+    auto patch = [&](int t, int pl) {
+      if (t < p.G && last * Q::R + lane >= n) *(LVAR_LDS float*)(uintptr_t)(stat0 + pl / (TILE / 256) + lane * 4) = ROLE ? 0.f : -INFINITY;
+    };
+
+    constexpr int AHEAD_T = Q::LEAD + (ROLE ? 0 : 1);   // tiles requested ahead of the first round
+    for (int x = 0; x < AHEAD_T; x++) request();
+    bf16x8 xf[KS];   // rows of k or of v
+    {
+      const bf16_t* kv = ROLE ? p.v + hk * p.v_sh + (int64_t)(w.first + key) * p.v_sr : p.k + hk * p.k_sh + (int64_t)(w.first + key) * p.k_sr;
 #pragma unroll
-      for (int sub = 0; sub < 2; sub++) {
-        const int i0 = 64 * t + 32 * sub;
-        // no row of these sees a key of the wave (its first key is the first to be seen)
-        if (i0 >= n || (p.causal && i0 + 31 < k0 - shift)) continue;
-        f32x16 s, dp;
+      for (int ks = 0; ks < KS; ks++) xf[ks] = *(const bf16x8*)(kv + hh * 8 + ks * 16);
+    }
+    const uint32_t row_at = fill0 + at.row_at, col_at = lds0 + (ROLE ? 0 : Q::G_AT) + at.tr_at;
+    const uint32_t p_at = lds0 + Q::P_AT + wave * Q::P_WAVE + lane * 16;
+    constexpr int NS = SUB * KS, NP = 2 * SUB * MTD, NT = NS + NP, AHEAD = READ_AHEAD;
+    // places of the tile whose S or dP is formed (rows) and of the one that is added (columns)
+    int r_pl = 0, c_pl = 0, r_blk = last, r_head = 0;
+    // starting values of S or dP of the tile at r_pl; -infinity where a row does not see the lane's key
+    auto starts = [&](f32x16 (&s)[SUB]) {
+      LVAR_LDS const float* st = (LVAR_LDS const float*)(uintptr_t)(stat0 + r_pl / (TILE / 256));
+#pragma unroll
+      for (int b = 0; b < SUB; b++)
 #pragma unroll
         for (int a = 0; a < 4; a++) {
-          const f32x4 x0 = *(const f32x4*)(sp + 32 * sub + 8 * a + 4 * hh), x1 = *(const f32x4*)(sp + 64 + 32 * sub + 8 * a + 4 * hh);
+          const f32x4 v = *(LVAR_LDS const f32x4*)(st + 32 * b + 8 * a + 4 * hh);
 #pragma unroll
-          for (int e = 0; e < 4; e++) { s[4 * a + e] = x0[e]; dp[4 * a + e] = x1[e]; }
+          for (int e = 0; e < 4; e++) s[b][4 * a + e] = v[e];
         }
+      if constexpr (ROLE == 0) {
+        if (r_blk * Q::R < whole0) {
+          const int lo = from - r_blk * Q::R - 4 * hh;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-          s = mfma32(at.rows(qbuf, sub, ks), kf[ks], s);
-          dp = mfma32(at.rows(gbuf, sub, ks), vf[ks], dp);
-        }
-        if (p.causal && i0 < k0 + 31 - shift) {
-          const int lim = from - i0 - 4 * hh;
+          for (int b = 0; b < SUB; b++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const bool sees = 8 * (i >> 2) + (i & 3) >= lim;
-            s[i] = sees ? fast_exp2(s[i] * c) : 0.f;
-            dp[i] = sees ? s[i] * dp[i] : 0.f;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            s[i] = fast_exp2(s[i] * c);
-            dp[i] = s[i] * dp[i];
-          }
-        }
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-          const bf16x8 pb = pack_half(s, kb), db = pack_half(dp, kb);
-#pragma unroll
-          for (int i = 0; i < MTD; i++) {
-            dv[i] = mfma32(at.columns(gbuf, 2 * sub + kb, m0 + i), pb, dv[i]);
-            dk[i] = mfma32(at.columns(qbuf, 2 * sub + kb, m0 + i), db, dk[i]);
-          }
+            for (int e = 0; e < 16; e++) s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) >= lo ? s[b][e] : -INFINITY;
         }
       }
-      if (more && tid < 128) stats[(1 - par) * 128 + tid] = st;
-      head = head_n; t = t_n;
-      wait_fills<0>();
+    };
+    auto next_rows = [&]() {
+      r_pl = after(r_pl, RING);
+      const bool wrap = ++r_head == p.G;
+      r_head = wrap ? 0 : r_head;
+      r_blk -= wrap ? 1 : 0;
+    };
+    int landed = 0, l_pl = 0;   // tiles that have landed
+    auto settle = [&](auto rounds) {   // all but the last `rounds` requested tiles have
+      wait_fills<decltype(rounds)::value * FILLS>();
+      patch(landed, l_pl);
+      landed++;
+      l_pl = after(l_pl, RING);
       __syncthreads();
+    };
+    // A round.  Tile t of this wave: its S or dP is in s.  FIRST: that of the coming tile is formed, in nx; SECOND: tile t is added to the sum.
+    auto round = [&](int t, auto first, auto second, f32x16 (&s)[SUB], f32x16 (&nx)[SUB]) {
+      constexpr bool FIRST = decltype(first)::value, SECOND = decltype(second)::value;
+      const uint32_t rows = row_at + r_pl, cols = col_at + c_pl, pt = p_at + (t & 1) * Q::KW * Q::P_WAVE;
+      bf16x8 frag[NT];
+      uint32_t pw[8 * SUB];   // P or dS, packed
+      u32x4 pin[2 * SUB];     // P from the other wave
+      auto operand = [&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (i < NS) { if constexpr (FIRST) frag[i] = P::rows(rows + i % SUB * 32 * S::ROWB, i / SUB); }
+        else if constexpr (i < NT) { if constexpr (SECOND) frag[i] = P::columns(cols, (i - NS) / MTD, (i - NS) % MTD); }
+      };
+      using Sch = DkvSlots<NE, NS, SUB == 1 ? NP / 4 : NP / 2>;
+      // (what a product takes is finished two slots ahead of it)
+      static_assert(Sch::lo(NS - 2) >= 8 && Sch::lo(NS + MTD - 2) >= 16 && (SUB == 1 || (Sch::lo(NS + 2 * MTD - 2) >= 24 && Sch::lo(NS + 3 * MTD - 2) >= 32)));
+      auto finish = [&](auto ec) {
+        constexpr int e = decltype(ec)::value;
+        if constexpr (ROLE == 1) s[e / 16][e % 16] *= (e & 1) ? bf16_hi(pin[e / 8][e % 8 / 2]) : bf16_lo(pin[e / 8][e % 8 / 2]);
+        if constexpr (e & 1) pw[e >> 1] = pack_bf16(s[e / 16][e % 16 - 1], s[e / 16][e % 16]);
+        if constexpr (ROLE == 0 && e % 8 == 7) *(LVAR_LDS u32x4*)(uintptr_t)(pt + e / 8 * 1024) = u32x4{pw[e / 2 - 3], pw[e / 2 - 2], pw[e / 2 - 1], pw[e / 2]};
+      };
+      auto slot = [&](auto gc) {
+        constexpr int g = decltype(gc)::value;
+        if constexpr (SECOND) {
+          static_for<Sch::lo(g - 2), Sch::lo(g - 1)>(finish);
+          if constexpr (ROLE == 0) {
+            static_for<Sch::lo(g - 1), Sch::lo(g)>([&](auto ec) { constexpr int e = decltype(ec)::value; s[e / 16][e % 16] = fast_exp2(s[e / 16][e % 16]); });
+            static_for<Sch::lo(g), Sch::lo(g + 1)>([&](auto ec) { constexpr int e = decltype(ec)::value; s[e / 16][e % 16] *= c; });
+          }
+        }
+      };
+      if constexpr (ROLE == 1 && SECOND) {
+#pragma unroll
+        for (int i = 0; i < 2 * SUB; i++) pin[i] = *(LVAR_LDS const u32x4*)(uintptr_t)(pt + i * 1024);
+      }
+      if constexpr (FIRST) starts(nx);
+      static_for<FIRST ? 0 : NS, (FIRST ? 0 : NS) + AHEAD>(operand);
+      request();
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<0, NS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (FIRST) {
+          operand(std::integral_constant<int, i + AHEAD>{});
+          nx[i % SUB] = mfma32(frag[i], xf[i / SUB], nx[i % SUB]);
+        }
+        slot(ic);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (SECOND) {
+        static_for<NS, NT>([&](auto ic) {
+          constexpr int i = decltype(ic)::value, kb = (i - NS) / MTD, m = (i - NS) % MTD;
+          operand(std::integral_constant<int, i + AHEAD>{});
+          acc[m] = mfma32(frag[i], __builtin_bit_cast(bf16x8, u32x4{pw[4 * kb], pw[4 * kb + 1], pw[4 * kb + 2], pw[4 * kb + 3]}), acc[m]);
+          slot(ic);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        c_pl = after(c_pl, ROLE ? Q::Q_RING : Q::G_RING);
+      }
+      if constexpr (FIRST) next_rows();
+      settle(std::integral_constant<int, Q::LEAD - 1>{});
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    f32x16 sa[SUB], sb[SUB];
+    // ahead of the first round: S(0) by the first waves
+    settle(std::integral_constant<int, AHEAD_T - 1>{});
+    if constexpr (ROLE == 0) {
+      starts(sa);
+      static_for<0, NS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        sa[i % SUB] = mfma32(P::rows(row_at + i % SUB * 32 * S::ROWB, i / SUB), xf[i / SUB], sa[i % SUB]);
+      });
+      next_rows();
+      settle(std::integral_constant<int, Q::LEAD - 1>{});
+    } else {
+      __syncthreads();
+      round(-1, Yes{}, No{}, sb, sa);   // the first round forms dP(0)
     }
+    int t = 0;
+    for (; t + 2 < T; t += 2) {
+      round(t, Yes{}, Yes{}, sa, sb);
+      round(t + 1, Yes{}, Yes{}, sb, sa);
+    }
+    if (t + 1 < T) {
+      round(t, Yes{}, Yes{}, sa, sb);
+      round(t + 1, No{}, Yes{}, sb, sa);
+    } else {
+      round(t, No{}, Yes{}, sa, sb);
+    }
+    if constexpr (ROLE == 0) __syncthreads();   // the others' last round
+    wait_fills<0>();
+    __syncthreads();
   }
-  constexpr int DW = MTD * 32;   // columns of this workgroup
-  char* buf = smem + wave * (32 * (DW * 2 + 16));
-  bf16_t* dk_to = p.dk + hk * p.dk_sh + (int64_t)(w.first + k0) * p.dk_sr;
-  bf16_t* dv_to = p.dv + hk * p.dv_sh + (int64_t)(w.first + k0) * p.dv_sr;
-  if (p.dk) store_rows<DW>(buf, dk, p.scale, dk_to + m0 * 32, p.dk_sr, w.n - k0, lane);
-  if (p.dv) store_rows<DW>(buf, dv, 1.f, dv_to + m0 * 32, p.dv_sr, w.n - k0, lane);
+  bf16_t* out = ROLE ? p.dk : p.dv;
+  if (!out) return;
+  const int64_t out_sr = ROLE ? p.dk_sr : p.dv_sr;
+  bf16_t* to = out + hk * (ROLE ? p.dk_sh : p.dv_sh) + (int64_t)(w.first + k0) * out_sr;
+  const float factor = ROLE ? p.scale : 1.f;
+  store_rows<D>(smem + all_waves * (32 * (D * 2 + 16)), acc, factor, to, out_sr, w.n - k0, lane);
   if (p.causal) {
-    const bool bad = any_not_finite(dk) | any_not_finite(dv);
-    uint64_t keys = __builtin_amdgcn_ballot_w64(bad && k0 + r < w.n);
+    uint64_t keys = __builtin_amdgcn_ballot_w64(any_not_finite(acc) && k0 + r < w.n);
     keys = (keys | keys >> 32) & 0xffffffffu;
     if (keys) wait_fills<0>();   // the rows as stored above are written again
     while (keys) {
@@ -340,34 +454,44 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) void packed_dkv_kernel(co
       a.clear();
       for (int head = 0; head < p.G; head++) {
         const int hq = hk * p.G + head;
-        const int64_t stat = (int64_t)hq * p.T + q_first;
+        const float* st = p.stats + (int64_t)hq * 2 * p.T + q_first;
         a.add(p.k + hk * p.k_sh + x * p.k_sr, p.v + hk * p.v_sh + x * p.v_sr, p.q + hq * p.q_sh + (int64_t)q_first * p.q_sr, p.q_sr,
-              p.g + hq * p.g_sh + (int64_t)q_first * p.g_sr, p.g_sr, min(__shfl(from, i, 64), n), n, p.nl + stat, p.nd + stat, c);
+              p.g + hq * p.g_sh + (int64_t)q_first * p.g_sr, p.g_sr, min(__shfl(from, i, 64), n), n, st, st + p.T, c);
       }
-      if (p.dk) a.store(a.a0, p.scale, dk_to + i * p.dk_sr, m0 * 32, m0 * 32 + DW);
-      if (p.dv) a.store(a.a1, 1.f, dv_to + i * p.dv_sr, m0 * 32, m0 * 32 + DW);
+      a.store(ROLE ? a.a0 : a.a1, factor, to + i * out_sr);
     }
   }
+}
+
+#endif
+
+template <int D>
+__global__ __launch_bounds__(Dkv<D>::WAVES * 64, D <= 128 ? 2 : 1) void packed_dkv_kernel(const PackedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int id = __builtin_amdgcn_workgroup_id_x(), place = id / p.Hkv;
+  PackedTile w;
+  if (!find_tile<Dkv<D>::KEYS>(p.k_off, p.Tk, p.q_off, p.T, p.B, place, p.causal, w)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_workitem_id_x() >> 6);
+  if (wave < Dkv<D>::KW) dkv_wave<D, 0>(p, smem, w, id - place * p.Hkv, wave);
+  else dkv_wave<D, 1>(p, smem, w, id - place * p.Hkv, wave);
 #endif
 }
 
 template <int D>
 static int launch_bwd(PackedParams p, hipStream_t s) {
-  constexpr int NW = 4, SPLIT = D > 128 ? 2 : 1;
-  constexpr int DQ_LDS = bwd_lds<D>(NW, 0), DKV_LDS = bwd_lds<D>(NW, DKV_STAT);
-  const int64_t q_slots = packed_slots(p.T, p.B, NW * 32), k_slots = packed_slots(p.Tk, p.B, NW * 32);
-  const int64_t q_groups = q_slots * p.H, k_groups = k_slots * p.Hkv * SPLIT;
-  if (q_groups * (NW * 64) > 0xffffffffll || k_groups * (NW * 64) > 0xffffffffll) return LVAR_EINVAL;
+  constexpr int NW = 4, DQ_LDS = dq_lds<D>(NW), DKV_LDS = Dkv<D>::bytes();
+  p.slots = (int)packed_slots(p.T, p.B, NW * 32);
+  const int64_t q_groups = (int64_t)p.slots * p.H, k_groups = packed_slots(p.Tk, p.B, Dkv<D>::KEYS) * p.Hkv;
+  if (q_groups * (NW * 64) > 0xffffffffll || k_groups * (Dkv<D>::WAVES * 64) > 0xffffffffll) return LVAR_EINVAL;
   auto dq = packed_dq_kernel<D, NW>;
-  auto dkv = packed_dkv_kernel<D, NW, SPLIT>;
+  auto dkv = packed_dkv_kernel<D>;
   static std::atomic<uint64_t> ready_q{0}, ready_k{0};
   if (!ensure_lds_limit((const void*)dq, DQ_LDS, ready_q) || !ensure_lds_limit((const void*)dkv, DKV_LDS, ready_k)) return LVAR_ELAUNCH;
-  p.slots = (int)q_slots;
   hipLaunchKernelGGL(dq, dim3((uint32_t)q_groups), dim3(NW * 64), DQ_LDS, s, p);
   if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
   if (!p.dk && !p.dv) return LVAR_OK;
-  p.slots = (int)k_slots;
-  hipLaunchKernelGGL(dkv, dim3((uint32_t)k_groups), dim3(NW * 64), DKV_LDS, s, p);
+  hipLaunchKernelGGL(dkv, dim3((uint32_t)k_groups), dim3(Dkv<D>::WAVES * 64), DKV_LDS, s, p);
   return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
 }
 
