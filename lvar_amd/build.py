@@ -28,6 +28,8 @@ HIPCC_FLAGS = ["-O3", f"--offload-arch={ARCH}", "-fPIC", "-std=c++17", "-fno-hon
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # these keep NaN as NaN (a cache may hold some in places that nobody reads, and what is read has to show them)
 HONOR_NANS = ("normrope.hip", "kvread.hip", "pagedattn.hip", "pages.hip", "kvcapi.hip", "packedapi.hip")
+
+
 def _flags(src: str):
     return [f for f in HIPCC_FLAGS if src not in HONOR_NANS or f not in ("-fno-honor-nans", "-mno-amdgpu-ieee")]
 

@@ -47,7 +47,8 @@ namespace {
   X(lvar_qk_norm_rope_fwd) X(lvar_qk_norm_rope_bwd_scratch_bytes) X(lvar_qk_norm_rope_bwd) X(lvar_kv_cache_append)        \
   X(lvar_kv_cache_read) X(lvar_paged_attn_workspace_bytes) X(lvar_paged_attn_fwd)                                         \
   X(lvar_qk_norm_axes_fwd) X(lvar_qk_norm_axes_bwd_scratch_bytes) X(lvar_qk_norm_axes_bwd) X(lvar_kv_cache_append_axes)   \
-  X(lvar_kv_pages_scratch_bytes) X(lvar_kv_pages_alloc) X(lvar_kv_pages_free) X(lvar_kv_cache_fork) X(lvar_kv_cache_compact)
+  X(lvar_kv_pages_scratch_bytes) X(lvar_kv_pages_alloc) X(lvar_kv_pages_free) X(lvar_kv_cache_fork) X(lvar_kv_cache_compact) \
+  X(lvar_packed_attn_fwd) X(lvar_packed_attn_bwd_workspace_bytes) X(lvar_packed_attn_bwd)
 struct Api {
 #define LVAR_FIELD(name) decltype(&::name) name = nullptr;
   LVAR_ENTRIES(LVAR_FIELD)
@@ -952,6 +953,117 @@ LVAR_FAST(fast_paged_attn) {
 }
 
 // rows are read with 16-byte accesses: anything else is copied into a plain tensor first
+// ---- attention over packed sequences (lvar_amd.packed_ops) ----
+
+// rows that the kernels address with 31 bits (axes of one element may have any stride)
+bool packed_rows(const at::Tensor* t, int dev) {
+  return rows_ok(t, dev) && t->size(0) == 1 && t->size(1) <= INT32_MAX && t->size(2) <= INT32_MAX &&
+         (t->size(2) <= 1 || (t->size(2) - 1) * t->stride(2) * 2 + t->size(3) * 2 < INT32_MAX);
+}
+lvar_tensor_t packed_view(const at::Tensor& t) {
+  if (!t.defined()) return lvar_tensor_t{nullptr, 0, 0, 0};
+  return lvar_tensor_t{t.data_ptr(), 0, t.size(1) > 1 ? t.stride(1) : 0, t.size(2) > 1 ? t.stride(2) : t.size(3)};
+}
+bool offsets_ok(const at::Tensor* t, int dev) { return t && packed(t, dev, at::kInt) && t->dim() == 1 && t->size(0) > 1 && t->size(0) <= INT32_MAX; }
+
+// memory for a tensor [1,H,T,d] in t's own order of axes
+at::Tensor packed_like(const at::Tensor& t) {
+  const int64_t H = t.size(1), T = t.size(2), d = t.size(3);
+  const bool tokens_first = H > 1 && T > 1 && t.stride(1) < t.stride(2);
+  return at::Tensor(at::detail::empty_strided_cuda(t.sizes(), {H * T * d, tokens_first ? d : T * d, tokens_first ? H * d : d, 1}, at::kBFloat16, t.device()));
+}
+
+struct PackedCall {
+  const at::Tensor *q, *k, *v, *off, *k_off;
+  bool causal;
+  float scale;
+};
+
+int packed_forward(const PackedCall& x, at::Tensor& o, at::Tensor& M, at::Tensor& L) {
+  const int dev = x.q->get_device(), H = dim(*x.q, 1), T = dim(*x.q, 2);
+  o = packed_like(*x.q);
+  Qkv sizes{};
+  sizes.B = 1; sizes.H = H; sizes.Lq = T; sizes.dev = dev;
+  empty_stats(sizes, M, L);
+  return api.lvar_packed_attn_fwd(packed_view(*x.q), packed_view(*x.k), packed_view(*x.v), packed_view(o), x.off->data_ptr<int32_t>(), x.k_off->data_ptr<int32_t>(),
+                                  M.data_ptr<float>(), L.data_ptr<float>(), dim(*x.off, 0) - 1, T, dim(*x.k, 2), H, dim(*x.k, 1), dim(*x.q, 3), x.causal, x.scale,
+                                  c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream());
+}
+
+struct PackedAttnFunction : torch::autograd::Function<PackedAttnFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                const at::Tensor& off, const at::Tensor& k_off, bool causal, double scale) {
+    at::Tensor o, M, L;
+    const int st = packed_forward({&q, &k, &v, &off, &k_off, causal, static_cast<float>(scale)}, o, M, L);
+    TORCH_CHECK(st == LVAR_OK, "lvar_packed_attn_fwd failed with status ", st);
+    ctx->save_for_backward({q, k, v, o, M, L, off, k_off});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({M, L});
+    ctx->set_materialize_grads(false);
+    return {o, M, L};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "packed_attn can be differentiated once: its gradients have no graph (create_graph)");
+    if (!grads[0].defined()) return torch::autograd::variable_list(7);
+    TORCH_CHECK(!has_tangent(&grads[0]), "the gradient of packed_attn has no forward-mode derivative: call it on tensors without a tangent");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &M = saved[4], &L = saved[5], &off = saved[6], &k_off = saved[7];
+    const int dev = q.get_device(), H = dim(q, 1), Hkv = dim(k, 1), T = dim(q, 2), Tk = dim(k, 2), d = dim(q, 3);
+    // (hooks on saved tensors may return copies of another layout, or on another device)
+    bool same = true;
+    for (const at::Tensor* t : {&q, &k, &v, &o}) same = same && packed_rows(t, dev);
+    for (const at::Tensor* t : {&M, &L}) same = same && packed(t, dev, at::kFloat);
+    TORCH_CHECK(same && offsets_ok(&off, dev) && offsets_ok(&k_off, dev),
+                "packed_attn: hooks on saved tensors returned tensors that the backward pass cannot read (device, alignment or strides)");
+    const c10::DeviceGuard guard(q.device());
+    at::Tensor go = grads[0];
+    if (!packed_rows(&go, dev)) {
+      go = go.contiguous();
+      if (!packed_rows(&go, dev)) go = go.clone(at::MemoryFormat::Contiguous);
+    }
+    at::Tensor d3[3];
+    const at::Tensor* leaves[3] = {&q, &k, &v};
+    for (int i = 0; i < 3; i++) if (ctx->needs_input_grad(i)) d3[i] = packed_like(*leaves[i]);
+    const int64_t bytes = api.lvar_packed_attn_bwd_workspace_bytes(T, H);
+    const at::Tensor ws = empty({std::max<int64_t>(bytes, 16)}, at::kByte, dev);
+    const int st = api.lvar_packed_attn_bwd(packed_view(q), packed_view(k), packed_view(v), packed_view(o), packed_view(go), off.data_ptr<int32_t>(), k_off.data_ptr<int32_t>(),
+                                            M.data_ptr<float>(), L.data_ptr<float>(), packed_view(d3[0]), packed_view(d3[1]), packed_view(d3[2]), ws.data_ptr(), bytes,
+                                            dim(off, 0) - 1, T, Tk, H, Hkv, d, ctx->saved_data["causal"].toBool(), static_cast<float>(ctx->saved_data["scale"].toDouble()),
+                                            c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream());
+    TORCH_CHECK(st == LVAR_OK, "lvar_packed_attn_bwd failed with status ", st);
+    return {d3[0], d3[1], d3[2], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// (q, k, v, offsets, k_offsets, scale, causal) -> (o, M, L)
+LVAR_FAST(fast_packed_attn) {
+  HANDLE_TH_ERRORS
+  LVAR_NEED(bound && n == 7);
+  PackedCall x{tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), nullptr, true, 0.f};
+  LVAR_NEED(x.q && x.k && x.v && x.q->is_cuda() && optional_tensor(a[4], x.k_off));
+  const int dev = x.q->get_device();
+  LVAR_NEED(c10::hip::current_device() == dev);
+  for (const at::Tensor* t : {x.q, x.k, x.v}) LVAR_NEED(packed_rows(t, dev) && t->numel() > 0 && !has_tangent(t));
+  const int64_t d = x.q->size(3);
+  LVAR_NEED(x.k->sizes() == x.v->sizes() && x.k->size(3) == d && x.q->size(1) % x.k->size(1) == 0 && (d == 64 || d == 128 || d == 256) && x.q->size(1) <= 16384);
+  LVAR_NEED(offsets_ok(x.off, dev) && x.off->size(0) <= (1 << 24));
+  if (!x.k_off) {
+    LVAR_NEED(x.q->size(2) == x.k->size(2));
+    x.k_off = x.off;
+  }
+  LVAR_NEED(offsets_ok(x.k_off, dev) && x.k_off->size(0) == x.off->size(0) && as_scale(a[5], d, x.scale) && as_bool(a[6], x.causal));
+  LVAR_NEED(x.scale > 1e-30f && x.scale < 1e30f);   // (what the entry point would refuse raises in the Python path)
+  at::Tensor o, M, L;
+  if (wants_grad(x.q) || wants_grad(x.k) || wants_grad(x.v)) {
+    auto r = PackedAttnFunction::apply(*x.q, *x.k, *x.v, *x.off, *x.k_off, x.causal, static_cast<double>(x.scale));
+    return tuple(std::move(r[0]), std::move(r[1]), std::move(r[2]));
+  }
+  LVAR_NEED(packed_forward(x, o, M, L) == LVAR_OK);
+  return tuple(std::move(o), std::move(M), std::move(L));
+  END_HANDLE_TH_ERRORS
+}
+
 at::Tensor as_plain(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.dim() == 4, name, " must be [B,H,L,d], got ", t.sizes());
   TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16, got ", t.scalar_type());
@@ -1003,6 +1115,7 @@ PyMethodDef fast_methods[] = {
     LVAR_METHOD(fast_topk_token_lists), LVAR_METHOD(fast_remap_concat_lists), LVAR_METHOD(fast_mask_to_lists), LVAR_METHOD(fast_window_keys),
     LVAR_METHOD(fast_qk_norm_rope), LVAR_METHOD(fast_kv_append), LVAR_METHOD(fast_kv_read), LVAR_METHOD(fast_paged_attn),
     LVAR_METHOD(fast_pages_alloc), LVAR_METHOD(fast_pages_free), LVAR_METHOD(fast_cache_fork), LVAR_METHOD(fast_cache_compact),
+    LVAR_METHOD(fast_packed_attn),
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .kv_cache_ops import _no_tangent, _rows, _rows_like
-from .sparse_attn_ops import ShapeError, _on_device, _pad_head_dim, _ptr, _require, _scale_for, _stream
+from .sparse_attn_ops import ShapeError, _native, _on_device, _pad_head_dim, _plain_scale, _ptr, _require, _scale_for, _stream
 
 __all__ = ["packed_attn", "ShapeError"]
 
@@ -115,6 +115,11 @@ def packed_attn(q, k, v, offsets, k_offsets=None, scale=None, causal: bool = Tru
     bf16 where they enter a product.  The order of all sums is fixed: the same call gives the same bits.  A value that is not finite reaches the
     rows that see it, and through them the gradients, and nothing else.  ``o`` and the gradients have the order of axes of their inputs.  Once
     differentiable, in reverse mode."""
+    fast = _native()
+    if fast is not None:
+        r = fast.fast_packed_attn(q, k, v, offsets, k_offsets, _plain_scale(scale), causal)
+        if r is not None:
+            return r[0], (r[1], r[2])
     _no_tangent("packed_attn", q, k, v)
     d = q.shape[-1] if q.dim() else 0
     q, k, v, small = _pad_head_dim(q, k, v)
