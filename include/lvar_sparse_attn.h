@@ -564,7 +564,7 @@ int lvar_packed_attn_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar
  * wanted), summed over the query heads that share a key/value head; zeros where a row is of no sequence, or nobody sees a key.  The order of
  * every sum is fixed.  workspace: lvar_packed_attn_bwd_workspace_bytes() (16-byte aligned, written and read by this call).
  */
-int64_t lvar_packed_attn_bwd_workspace_bytes(int tokens, int H);
+int64_t lvar_packed_attn_bwd_workspace_bytes(int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal);
 int lvar_packed_attn_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar_tensor_t o, lvar_tensor_t go, const int32_t* offsets,
                          const int32_t* k_offsets, const float* M, const float* L, lvar_tensor_t dq, lvar_tensor_t dk, lvar_tensor_t dv,
                          void* workspace, int64_t workspace_bytes, int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim,

@@ -172,7 +172,7 @@ def load() -> C.CDLL:
     lib.lvar_packed_attn_fwd.restype = I
     lib.lvar_packed_attn_fwd.argtypes = [T, T, T, T, P, P, P, P, I, I, I, I, I, I, I, F, P]
     lib.lvar_packed_attn_bwd_workspace_bytes.restype = I64
-    lib.lvar_packed_attn_bwd_workspace_bytes.argtypes = [I, I]
+    lib.lvar_packed_attn_bwd_workspace_bytes.argtypes = [I] * 7
     lib.lvar_packed_attn_bwd.restype = I
     lib.lvar_packed_attn_bwd.argtypes = [T, T, T, T, T, P, P, P, P, T, T, T, P, I64, I, I, I, I, I, I, I, F, P]
     _lib = lib

@@ -23,11 +23,14 @@ struct PackedParams {
   bf16_t *dq, *dk, *dv;             // null: not wanted
   int64_t dq_sh, dq_sr, dk_sh, dk_sr, dv_sh, dv_sr;
   int slots;                        // set at launch: places for query tiles, see find_tile
+  int shares;                       // set at launch: workgroups that share the query rows of a key tile
+  float* parts;                     // their sums, [shares][dk, dv][Hkv][Tk][D]
   float* stats;                     // [H,2,T]: -(M + log2 L) / c (-inf: the row sees nothing), and -sum(do * o)
 };
 
 int launch_packed_fwd(PackedParams p, int head_dim, hipStream_t s);
-int launch_packed_bwd(PackedParams p, int head_dim, hipStream_t s);
+int64_t packed_bwd_bytes(const PackedParams& p, int head_dim);
+int launch_packed_bwd(PackedParams p, void* workspace, int head_dim, hipStream_t s);
 
 // Tiles of R rows of T packed rows in B sequences: the ranges between sequence borders, one ahead of the first sequence and one
 // behind the last included, have at most these many.
@@ -120,6 +123,26 @@ __device__ __forceinline__ bool find_tile(const int32_t* off, int T, const int32
   if (v == 0 || v > B) t.other_n = 0;
   t.other_n = max(0, t.other_n);
   return t.row0 >= 0 && t.row0 < t.n;
+}
+
+// The sequence of row `row` and its rows on both sides; none on the other side for rows of no sequence.
+__device__ __forceinline__ void find_row(const int32_t* off, int T, const int32_t* other, int other_T, int B, int row, PackedTile& t) {
+  const int lane = __builtin_amdgcn_workitem_id_x() & 63;
+  int v = 0, n = B + 2;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, at = v + lane * step;
+    const bool in = lane * step < n;
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(in && packed_border(off, B, T, in ? at : 0) <= row);
+    const int k = mine ? 63 - __builtin_clzll(mine) : 0;
+    v += k * step;
+    n = min(step, n - k * step);
+  }
+  v = __builtin_amdgcn_readfirstlane(v);
+  t.first = packed_border(off, B, T, v);
+  t.n = packed_border(off, B, T, v + 1) - t.first;
+  t.row0 = row - t.first;
+  t.other_first = packed_border(other, B, other_T, v);
+  t.other_n = v == 0 || v > B ? 0 : max(0, packed_border(other, B, other_T, v + 1) - t.other_first);
 }
 
 // Rows of D bf16 in LDS, unpadded (an LDS fill writes 1 KiB of consecutive bytes), the 16-byte chunks of a row moved by an XOR that suits both

@@ -17,9 +17,13 @@ bool rows_ok(const lvar_tensor_t& t, int tokens, int head_dim) {
          t.stride_row < (1 << 29) && (int64_t)(tokens - 1) * t.stride_row * 2 + 2 * head_dim < 0x7fffffffll;
 }
 
+bool sizes_ok(int batch, int tokens, int k_tokens, int H, int kv_heads) {
+  return batch > 0 && batch <= (1 << 24) && tokens >= 0 && k_tokens >= 0 && kv_heads > 0 && H > 0 && H % kv_heads == 0 && H <= 16384;
+}
+
 int fill(PackedParams& p, const lvar_tensor_t& q, const lvar_tensor_t& k, const lvar_tensor_t& v, const lvar_tensor_t& o, const int32_t* offsets,
          const int32_t* k_offsets, float* M, float* L, int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal, float scale) {
-  if (batch <= 0 || batch > (1 << 24) || tokens < 0 || k_tokens < 0 || kv_heads <= 0 || H <= 0 || H % kv_heads != 0 || H > 16384) return LVAR_EINVAL;
+  if (!sizes_ok(batch, tokens, k_tokens, H, kv_heads)) return LVAR_EINVAL;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return LVAR_EUNSUPPORTED;
   if (!offsets || !k_offsets || !aligned(offsets, 4) || !aligned(k_offsets, 4) || !std::isfinite(scale) || scale <= 0.f) return LVAR_EINVAL;
   // c and its reciprocal are used
@@ -48,9 +52,12 @@ int lvar_packed_attn_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar
   return launch_packed_fwd(p, head_dim, (hipStream_t)stream);
 }
 
-int64_t lvar_packed_attn_bwd_workspace_bytes(int tokens, int H) {
-  if (tokens < 0 || H <= 0) return LVAR_EINVAL;
-  return 8ll * tokens * H;
+int64_t lvar_packed_attn_bwd_workspace_bytes(int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal) {
+  if (!sizes_ok(batch, tokens, k_tokens, H, kv_heads)) return LVAR_EINVAL;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return LVAR_EUNSUPPORTED;
+  PackedParams p{};
+  p.B = batch; p.T = tokens; p.Tk = k_tokens; p.H = H; p.Hkv = kv_heads; p.G = H / kv_heads; p.causal = causal ? 1 : 0;
+  return packed_bwd_bytes(p, head_dim);
 }
 
 int lvar_packed_attn_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar_tensor_t o, lvar_tensor_t go, const int32_t* offsets,
@@ -63,14 +70,13 @@ int lvar_packed_attn_bwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar
   if (!rows_ok(go, tokens, head_dim) || (dq.ptr && !rows_ok(dq, tokens, head_dim)) || (dk.ptr && !rows_ok(dk, k_tokens, head_dim)) ||
       (dv.ptr && !rows_ok(dv, k_tokens, head_dim)))
     return LVAR_EINVAL;
-  const int64_t bytes = lvar_packed_attn_bwd_workspace_bytes(tokens, H);
+  const int64_t bytes = packed_bwd_bytes(p, head_dim);
   if (bytes > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < bytes)) return LVAR_EINVAL;
   p.g = (const bf16_t*)go.ptr; p.g_sh = go.stride_h; p.g_sr = go.stride_row;
   p.dq = (bf16_t*)dq.ptr; p.dq_sh = dq.stride_h; p.dq_sr = dq.stride_row;
   p.dk = (bf16_t*)dk.ptr; p.dk_sh = dk.stride_h; p.dk_sr = dk.stride_row;
   p.dv = (bf16_t*)dv.ptr; p.dv_sh = dv.stride_h; p.dv_sr = dv.stride_row;
-  p.stats = (float*)workspace;
-  return launch_packed_bwd(p, head_dim, (hipStream_t)stream);
+  return launch_packed_bwd(p, workspace, head_dim, (hipStream_t)stream);
 }
 
 }  // extern "C"

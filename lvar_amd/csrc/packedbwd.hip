@@ -204,7 +204,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
 #endif
 }
 
-// ---- dk and dv: tiles of 128 keys and of 64 query rows (head_dim 256: 64 and 32) of every query head that shares the key head.
+// ---- dk and dv: tiles of 128 keys (head_dim 64 and 256: 64) and of 64 query rows (256: 32) of every query head that shares the key head.
 //
 // Two waves share 32 keys.  One forms S = q k^T and P and adds do^T P to dv^T; the other forms dP = do v^T, takes P from the first through LDS,
 // and adds q^T dS to dk^T.  Each has one operand (k or v) and one sum in registers, which leaves room for what hides latency: it forms S or dP
@@ -221,10 +221,12 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
 
 template <int D>
 struct Dkv {
-  static constexpr int KW = D == 256 ? 2 : 4, WAVES = 2 * KW, KEYS = 32 * KW;     // pairs of waves; head_dim 256: one wave per SIMD
+  // Pairs of waves.  head_dim 64: two, so that two workgroups share a compute unit and wait at barriers of their own (16384 rows of 16 heads over 725
+  // keys 72 -> 54 us); 128: four, half of the reads for the same time (12 sequences of 32 over 8 heads 263 / 254 us); 256: one wave per SIMD.
+  static constexpr int KW = D == 128 ? 4 : 2, WAVES = 2 * KW, KEYS = 32 * KW;
   static constexpr int SUB = D == 256 ? 1 : 2, R = 32 * SUB, TILE = R * D * 2;    // 32-row blocks and rows of a tile, its bytes
   // tiles of q: t-1 .. t+1 are in use, of do: t
-  static constexpr int LEAD = D == 128 ? 1 : 2, Q_RING = LEAD + 3, G_RING = LEAD + 1;
+  static constexpr int LEAD = D == 256 ? 2 : 1, Q_RING = LEAD + 3, G_RING = LEAD + 1;
   static constexpr int G_AT = Q_RING * TILE, P_AT = G_AT + G_RING * TILE, P_WAVE = R * 32 * 2;   // P: [parity][pair]
   static constexpr int STAT_AT = P_AT + 2 * KW * P_WAVE, STAT_WAVE = Q_RING * 256;               // statistics: [wave][place in the ring]
   static constexpr int OUT = WAVES * 32 * (D * 2 + 16);
@@ -242,8 +244,24 @@ struct DkvSlots {
   }
 };
 
+// dk or dv of one key, see CarefulRow; rows from `from` on see it
+template <int D, int ROLE>
+__device__ __forceinline__ void careful_key(const PackedParams& p, const PackedTile& w, int hk, int key, int from) {
+  const int64_t x = w.first + key;
+  CarefulRow<D, true> a;
+  a.clear();
+  for (int head = 0; head < p.G; head++) {
+    const int hq = hk * p.G + head;
+    const float* st = p.stats + (int64_t)hq * 2 * p.T + w.other_first;
+    a.add(p.k + hk * p.k_sh + x * p.k_sr, p.v + hk * p.v_sh + x * p.v_sr, p.q + hq * p.q_sh + (int64_t)w.other_first * p.q_sr, p.q_sr,
+          p.g + hq * p.g_sh + (int64_t)w.other_first * p.g_sr, p.g_sr, min(from, w.other_n), w.other_n, st, st + p.T, p.c);
+  }
+  if constexpr (ROLE == 0) a.store(a.a1, 1.f, p.dv + hk * p.dv_sh + x * p.dv_sr);
+  else a.store(a.a0, p.scale, p.dk + hk * p.dk_sh + x * p.dk_sr);
+}
+
 template <int D, int ROLE>   // ROLE 0: dv, 1: dk
-__device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, const PackedTile& w, const int hk, const int all_waves) {
+__device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, const PackedTile& w, const int hk, const int share, const int all_waves) {
   using S = PackedLds<D>;
   using Q = Dkv<D>;
   using P = PackedOperands<D>;
@@ -255,7 +273,11 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
   const int k0 = w.row0 + wave * 32, key = min(k0 + r, w.n - 1);
   const int shift = w.n - n;
   const int from = p.causal ? max(0, key - shift) : 0;   // the first row that sees the lane's key
-  const int b0 = p.causal ? min(max(0, w.row0 - shift), n) / Q::R : 0, last = (n + Q::R - 1) / Q::R - 1, T = max(0, last + 1 - b0) * p.G;
+  const int b0 = p.causal ? min(max(0, w.row0 - shift), n) / Q::R : 0, last = (n + Q::R - 1) / Q::R - 1;
+  // tiles of this workgroup's share: T_all * share / shares ..
+  const int64_t T_all = (int64_t)max(0, last + 1 - b0) * p.G;
+  const int t_first = (int)(T_all * share / p.shares), T = (int)(T_all * (share + 1) / p.shares) - t_first;
+  const int blk_first = last - t_first / p.G, head_first = t_first % p.G;
   const int whole0 = p.causal ? max(0, k0 + 31 - shift) : 0;   // rows from here on see all keys of the wave
   const float c = p.c;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LVAR_LDS char*)smem;
@@ -271,9 +293,9 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
     const float* const s0 = p.stats + ((int64_t)hk * p.G * 2 + ROLE) * p.T + q_first;
     const uint32_t fill0 = lds0 + (ROLE ? Q::G_AT : 0), stat0 = lds0 + Q::STAT_AT + all_waves * Q::STAT_WAVE;
     auto after = [](int pl, int ring) { return pl + TILE == ring * TILE ? 0 : pl + TILE; };   // the next place of a ring
-    int f_t = 0, f_blk = last, f_head = 0, f_pl = 0;   // the tile that is requested next
-    const bf16_t* xp = x0;
-    const float* sp = s0;
+    int f_t = 0, f_blk = blk_first, f_head = head_first, f_pl = 0;   // the tile that is requested next
+    const bf16_t* xp = x0 + head_first * head_stride;
+    const float* sp = s0 + 2 * (int64_t)head_first * p.T;
     auto request = [&]() {
       const bool there = f_t < T;                    // behind the last tile: as many fills, of nothing
       const int row = there ? f_blk * Q::R : 0;
@@ -292,7 +314,7 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
     };
     // Rows behind the last one, in the first tile of every head, have read zeros as their statistics: they see nothing.
     auto patch = [&](int t, int pl) {
-      if (t < p.G && last * Q::R + lane >= n) *(LVAR_LDS float*)(uintptr_t)(stat0 + pl / (TILE / 256) + lane * 4) = ROLE ? 0.f : -INFINITY;
+      if (t_first + t < p.G && last * Q::R + lane >= n) *(LVAR_LDS float*)(uintptr_t)(stat0 + pl / (TILE / 256) + lane * 4) = ROLE ? 0.f : -INFINITY;
     };
 
     constexpr int AHEAD_T = Q::LEAD + (ROLE ? 0 : 1);   // tiles requested ahead of the first round
@@ -307,7 +329,7 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
     const uint32_t p_at = lds0 + Q::P_AT + wave * Q::P_WAVE + lane * 16;
     constexpr int NS = SUB * KS, NP = 2 * SUB * MTD, NT = NS + NP, AHEAD = READ_AHEAD;
     // places of the tile whose S or dP is formed (rows) and of the one that is added (columns)
-    int r_pl = 0, c_pl = 0, r_blk = last, r_head = 0;
+    int r_pl = 0, c_pl = 0, r_blk = blk_first, r_head = head_first;
     // starting values of S or dP of the tile at r_pl; -infinity where a row does not see the lane's key
     auto starts = [&](f32x16 (&s)[SUB]) {
       LVAR_LDS const float* st = (LVAR_LDS const float*)(uintptr_t)(stat0 + r_pl / (TILE / 256));
@@ -438,10 +460,19 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
   }
   bf16_t* out = ROLE ? p.dk : p.dv;
   if (!out) return;
+  if (p.shares > 1) {   // as it is, transposed: packed_dkv_join_kernel does the rest
+    float* part = p.parts + (((int64_t)share * 2 + ROLE) * p.Hkv + hk) * p.Tk * D + (int64_t)(w.first + k0 + r) * D + 4 * hh;
+    if (k0 + r < w.n) {
+#pragma unroll
+      for (int m = 0; m < MTD; m++)
+#pragma unroll
+        for (int a = 0; a < 4; a++) *(f32x4*)(part + 32 * m + 8 * a) = f32x4{acc[m][4 * a], acc[m][4 * a + 1], acc[m][4 * a + 2], acc[m][4 * a + 3]};
+    }
+    return;
+  }
   const int64_t out_sr = ROLE ? p.dk_sr : p.dv_sr;
   bf16_t* to = out + hk * (ROLE ? p.dk_sh : p.dv_sh) + (int64_t)(w.first + k0) * out_sr;
-  const float factor = ROLE ? p.scale : 1.f;
-  store_rows<D>(smem + all_waves * (32 * (D * 2 + 16)), acc, factor, to, out_sr, w.n - k0, lane);
+  store_rows<D>(smem + all_waves * (32 * (D * 2 + 16)), acc, ROLE ? p.scale : 1.f, to, out_sr, w.n - k0, lane);
   if (p.causal) {
     uint64_t keys = __builtin_amdgcn_ballot_w64(any_not_finite(acc) && k0 + r < w.n);
     keys = (keys | keys >> 32) & 0xffffffffu;
@@ -449,16 +480,7 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
     while (keys) {
       const int i = __builtin_ctzll(keys);
       keys &= keys - 1;
-      const int64_t x = w.first + k0 + i;
-      CarefulRow<D, true> a;
-      a.clear();
-      for (int head = 0; head < p.G; head++) {
-        const int hq = hk * p.G + head;
-        const float* st = p.stats + (int64_t)hq * 2 * p.T + q_first;
-        a.add(p.k + hk * p.k_sh + x * p.k_sr, p.v + hk * p.v_sh + x * p.v_sr, p.q + hq * p.q_sh + (int64_t)q_first * p.q_sr, p.q_sr,
-              p.g + hq * p.g_sh + (int64_t)q_first * p.g_sr, p.g_sr, min(__shfl(from, i, 64), n), n, st, st + p.T, c);
-      }
-      a.store(ROLE ? a.a0 : a.a1, factor, to + i * out_sr);
+      careful_key<D, ROLE>(p, w, hk, k0 + i, __shfl(from, i, 64));
     }
   }
 }
@@ -469,21 +491,75 @@ template <int D>
 __global__ __launch_bounds__(Dkv<D>::WAVES * 64, D <= 128 ? 2 : 1) void packed_dkv_kernel(const PackedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const int id = __builtin_amdgcn_workgroup_id_x(), place = id / p.Hkv;
+  const int id = __builtin_amdgcn_workgroup_id_x(), place = id / (p.Hkv * p.shares), j = id - place * p.Hkv * p.shares, hk = j % p.Hkv, share = j / p.Hkv;
   PackedTile w;
   if (!find_tile<Dkv<D>::KEYS>(p.k_off, p.Tk, p.q_off, p.T, p.B, place, p.causal, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_workitem_id_x() >> 6);
-  if (wave < Dkv<D>::KW) dkv_wave<D, 0>(p, smem, w, id - place * p.Hkv, wave);
-  else dkv_wave<D, 1>(p, smem, w, id - place * p.Hkv, wave);
+  if (wave < Dkv<D>::KW) dkv_wave<D, 0>(p, smem, w, hk, share, wave);
+  else dkv_wave<D, 1>(p, smem, w, hk, share, wave);
 #endif
 }
 
+// dk and dv from the sums of the shares of a launch, in their order: a wave per key and head.
 template <int D>
-static int launch_bwd(PackedParams p, hipStream_t s) {
+__global__ __launch_bounds__(256) void packed_dkv_join_kernel(const PackedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int E = D / 64;
+  const int tid = __builtin_amdgcn_workitem_id_x(), lane = tid & 63;
+  const int64_t x = (int64_t)__builtin_amdgcn_workgroup_id_x() * 4 + __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (x >= (int64_t)p.Hkv * p.Tk) return;
+  const int hk = (int)(x / p.Tk), row = (int)(x - (int64_t)hk * p.Tk);
+  const int64_t plane = (int64_t)p.Hkv * p.Tk * D;
+#pragma unroll
+  for (int role = 0; role < 2; role++) {
+    bf16_t* out = role ? p.dk : p.dv;
+    if (!out) continue;
+    const float* part = p.parts + role * plane + x * D + lane * E;
+    float sum[E] = {};
+    for (int s = 0; s < p.shares; s++)
+#pragma unroll
+      for (int e = 0; e < E; e++) sum[e] += part[2 * s * plane + e];
+    bf16_t* to = out + hk * (role ? p.dk_sh : p.dv_sh) + (int64_t)row * (role ? p.dk_sr : p.dv_sr) + lane * E;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      bad |= not_finite(sum[e]);
+      to[e] = (bf16_t)(sum[e] * (role ? p.scale : 1.f));
+    }
+    if (p.causal && __builtin_amdgcn_ballot_w64(bad)) {
+      wait_fills<0>();   // the row as stored above is written again
+      PackedTile w;
+      find_row(p.k_off, p.Tk, p.q_off, p.T, p.B, row, w);
+      const int from = max(0, w.row0 - (w.n - w.other_n));
+      if (role) careful_key<D, 1>(p, w, hk, w.row0, from); else careful_key<D, 0>(p, w, hk, w.row0, from);
+    }
+  }
+#endif
+}
+
+// Workgroups that share the query rows of a key tile, where the key tiles alone leave compute units idle (few keys under many rows, or one key
+// head under many query heads): as many as give each unit one, twice that if causal, where the first tile has twice the work of the mean one;
+// none gets fewer than SHARE_TILES tiles of an average sequence.  Against one workgroup per tile, the sum of the parts included: 4096 rows of
+// 8 heads over one key head of 128, causal 697 -> 102 us (half as many shares 133); of 256 976 -> 192 us; two of 2048 of 8 over 2 heads of 64
+// 90 -> 48 us; 16384 rows of 16 heads of 128 over 77 keys 353 -> 52 us.
+template <int D>
+static int dkv_shares(const PackedParams& p) {
+  constexpr int SHARE_TILES = 8;
+  const int64_t groups = ((int64_t)p.Tk / Dkv<D>::KEYS + p.B) * p.Hkv, cus = device_cus(), tiles = (int64_t)p.T / p.B * p.G / Dkv<D>::R / (p.causal ? 2 : 1);
+  const int64_t most = tiles / SHARE_TILES, want = (p.causal ? 2 : 1) * cus / (groups > 0 ? groups : 1);
+  const int64_t n = want < most ? want : most;
+  return n < 2 ? 1 : n > 64 ? 64 : (int)n;
+}
+
+template <int D>
+static int launch_bwd(PackedParams p, void* workspace, hipStream_t s) {
   constexpr int NW = 4, DQ_LDS = dq_lds<D>(NW), DKV_LDS = Dkv<D>::bytes();
   p.slots = (int)packed_slots(p.T, p.B, NW * 32);
-  const int64_t q_groups = (int64_t)p.slots * p.H, k_groups = packed_slots(p.Tk, p.B, Dkv<D>::KEYS) * p.Hkv;
-  if (q_groups * (NW * 64) > 0xffffffffll || k_groups * (Dkv<D>::WAVES * 64) > 0xffffffffll) return LVAR_EINVAL;
+  p.shares = dkv_shares<D>(p);
+  p.stats = (float*)workspace;
+  p.parts = p.stats + ((int64_t)p.H * 2 * p.T + 3) / 4 * 4;
+  const int64_t q_groups = (int64_t)p.slots * p.H, k_groups = packed_slots(p.Tk, p.B, Dkv<D>::KEYS) * p.Hkv * p.shares, joins = ((int64_t)p.Hkv * p.Tk + 3) / 4;
+  if (q_groups * (NW * 64) > 0xffffffffll || k_groups * (Dkv<D>::WAVES * 64) > 0xffffffffll || joins * 256 > 0xffffffffll) return LVAR_EINVAL;
   auto dq = packed_dq_kernel<D, NW>;
   auto dkv = packed_dkv_kernel<D>;
   static std::atomic<uint64_t> ready_q{0}, ready_k{0};
@@ -492,13 +568,21 @@ static int launch_bwd(PackedParams p, hipStream_t s) {
   if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
   if (!p.dk && !p.dv) return LVAR_OK;
   hipLaunchKernelGGL(dkv, dim3((uint32_t)k_groups), dim3(Dkv<D>::WAVES * 64), DKV_LDS, s, p);
+  if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
+  if (p.shares > 1 && joins > 0) hipLaunchKernelGGL(packed_dkv_join_kernel<D>, dim3((uint32_t)joins), dim3(256), 0, s, p);
   return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
 }
 
-int launch_packed_bwd(PackedParams p, int head_dim, hipStream_t s) {
-  if (head_dim == 128) return launch_bwd<128>(p, s);
-  if (head_dim == 64) return launch_bwd<64>(p, s);
-  if (head_dim == 256) return launch_bwd<256>(p, s);
+// statistics of the rows, and the sums of shares
+int64_t packed_bwd_bytes(const PackedParams& p, int head_dim) {
+  const int shares = head_dim == 64 ? dkv_shares<64>(p) : head_dim == 128 ? dkv_shares<128>(p) : dkv_shares<256>(p);
+  return 4 * (((int64_t)p.H * 2 * p.T + 3) / 4 * 4 + (shares > 1 ? (int64_t)shares * 2 * p.Hkv * p.Tk * head_dim : 0));
+}
+
+int launch_packed_bwd(PackedParams p, void* workspace, int head_dim, hipStream_t s) {
+  if (head_dim == 128) return launch_bwd<128>(p, workspace, s);
+  if (head_dim == 64) return launch_bwd<64>(p, workspace, s);
+  if (head_dim == 256) return launch_bwd<256>(p, workspace, s);
   return LVAR_EUNSUPPORTED;
 }
 

@@ -1025,11 +1025,12 @@ struct PackedAttnFunction : torch::autograd::Function<PackedAttnFunction> {
     at::Tensor d3[3];
     const at::Tensor* leaves[3] = {&q, &k, &v};
     for (int i = 0; i < 3; i++) if (ctx->needs_input_grad(i)) d3[i] = packed_like(*leaves[i]);
-    const int64_t bytes = api.lvar_packed_attn_bwd_workspace_bytes(T, H);
+    const bool causal = ctx->saved_data["causal"].toBool();
+    const int64_t bytes = api.lvar_packed_attn_bwd_workspace_bytes(dim(off, 0) - 1, T, Tk, H, Hkv, d, causal);
     const at::Tensor ws = empty({std::max<int64_t>(bytes, 16)}, at::kByte, dev);
     const int st = api.lvar_packed_attn_bwd(packed_view(q), packed_view(k), packed_view(v), packed_view(o), packed_view(go), off.data_ptr<int32_t>(), k_off.data_ptr<int32_t>(),
                                             M.data_ptr<float>(), L.data_ptr<float>(), packed_view(d3[0]), packed_view(d3[1]), packed_view(d3[2]), ws.data_ptr(), bytes,
-                                            dim(off, 0) - 1, T, Tk, H, Hkv, d, ctx->saved_data["causal"].toBool(), static_cast<float>(ctx->saved_data["scale"].toDouble()),
+                                            dim(off, 0) - 1, T, Tk, H, Hkv, d, causal, static_cast<float>(ctx->saved_data["scale"].toDouble()),
                                             c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream());
     TORCH_CHECK(st == LVAR_OK, "lvar_packed_attn_bwd failed with status ", st);
     return {d3[0], d3[1], d3[2], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};

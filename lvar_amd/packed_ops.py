@@ -91,7 +91,7 @@ class _PackedAttn(torch.autograd.Function):
         dq, dk, dv = (_rows_like(t) if need else None for t, need in zip((q, k, v), ctx.needs_input_grad))
         lib = _lib.load()
         with _on_device(q):
-            nbytes = int(lib.lvar_packed_attn_bwd_workspace_bytes(T, H))
+            nbytes = int(lib.lvar_packed_attn_bwd_workspace_bytes(offsets.shape[0] - 1, T, Tk, H, Hkv, d, 1 if causal else 0))
             ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
             st = lib.lvar_packed_attn_bwd(_view(q), _view(k), _view(v), _view(o), _view(go), offsets.data_ptr(), k_offsets.data_ptr(), M.data_ptr(), L.data_ptr(),
                                           _view(dq), _view(dk), _view(dv), _ptr(ws), nbytes, offsets.shape[0] - 1, T, Tk, H, Hkv, d,

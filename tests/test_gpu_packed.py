@@ -61,6 +61,9 @@ CASES = [
     ([700], None, 2, 2, 64, False, 0, 0),
     ([520, 260], None, 2, 1, 128, True, 0, 0),
     ([10, 90], [20, 70], 3, 1, 16, True, 0, 0),
+    ([1500, 3, 900], [70, 130, 0], 2, 1, 64, False, 0, 2),           # few keys under many rows: several workgroups share them
+    ([700, 40], None, 8, 1, 128, True, 1, 0),
+    ([310], None, 8, 1, 256, True, 0, 0),
     ([70], None, 2, 2, 32, False, 0, 0),
 ]
 

@@ -115,6 +115,10 @@ def test_backward_entry_point_refuses(lib, change):
 
 
 def test_workspace(lib):
-    assert lib.lvar_packed_attn_bwd_workspace_bytes(8, 4) == 256
-    assert lib.lvar_packed_attn_bwd_workspace_bytes(1 << 30, 16384) == 8 << 44
-    assert lib.lvar_packed_attn_bwd_workspace_bytes(-1, 4) < 0 and lib.lvar_packed_attn_bwd_workspace_bytes(8, 0) < 0
+    size = lambda batch=2, tokens=8, k_tokens=8, H=4, kv_heads=2, head_dim=128, causal=1: lib.lvar_packed_attn_bwd_workspace_bytes(  # noqa: E731
+        batch, tokens, k_tokens, H, kv_heads, head_dim, causal)
+    assert size() == 256                        # two statistics per row and head
+    assert size(tokens=1 << 30, k_tokens=0, H=16384) == 8 << 44
+    for bad in (dict(batch=0), dict(tokens=-1), dict(k_tokens=-1), dict(H=3), dict(kv_heads=0)):
+        assert size(**bad) == -1
+    assert size(head_dim=80) == -2
