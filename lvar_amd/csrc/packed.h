@@ -235,8 +235,12 @@ __device__ __forceinline__ void fill_tile(const i32x4& rsrc, int srb, int row0, 
 // Head of place j of H: with a multiple of 8 heads, those of an XCD (workgroups are dealt to the 8 in turn) are neighbours, which share keys and values.
 __device__ __forceinline__ int packed_head(int j, int H) { return (H & 7) == 0 ? (j & 7) * (H >> 3) + (j >> 3) : j; }
 
-// Is x infinite or NaN?  (On the bits: float comparisons may assume that there are none.)
-__device__ __forceinline__ bool not_finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) == 0x7f800000u; }
+// Is x infinite or NaN?  On bits that the compiler cannot trace back to a float: with -fno-honor-nans it turns the test into one for infinity.
+__device__ __forceinline__ bool not_finite(float x) {
+  uint32_t u = __builtin_bit_cast(uint32_t, x);
+  asm("" : "+v"(u));
+  return (u & 0x7f800000u) == 0x7f800000u;
+}
 
 // The transposed accumulators of a wave, 32 rows of D columns, as bf16 rows: through LDS (32 * (2 D + 16) bytes at `buf`, this wave's
 // own), so that rows are stored in 16-byte pieces.  rows < n are stored.

@@ -10,11 +10,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// rows that the kernels read (in 31 bits of byte offsets) or write
+// rows that the kernels read (with 31 bits of byte offsets, and 32 for tiles that end behind them, which reach less than 512 rows further) or write
 bool rows_ok(const lvar_tensor_t& t, int tokens, int head_dim) {
   if (tokens == 0) return true;
   return t.ptr && aligned(t.ptr, 16) && t.stride_h % 8 == 0 && t.stride_row % 8 == 0 && t.stride_row >= 0 &&
-         t.stride_row < (1 << 29) && (int64_t)(tokens - 1) * t.stride_row * 2 + 2 * head_dim < 0x7fffffffll;
+         (tokens == 1 || t.stride_row <= (1 << 20)) && (int64_t)(tokens - 1) * t.stride_row * 2 + 2 * head_dim < 0x7fffffffll;
 }
 
 bool sizes_ok(int batch, int tokens, int k_tokens, int H, int kv_heads) {

@@ -958,7 +958,7 @@ LVAR_FAST(fast_paged_attn) {
 // rows that the kernels address with 31 bits (axes of one element may have any stride)
 bool packed_rows(const at::Tensor* t, int dev) {
   return rows_ok(t, dev) && t->size(0) == 1 && t->size(1) <= INT32_MAX && t->size(2) <= INT32_MAX &&
-         (t->size(2) <= 1 || (t->size(2) - 1) * t->stride(2) * 2 + t->size(3) * 2 < INT32_MAX);
+         (t->size(2) <= 1 || (t->stride(2) <= (1 << 20) && (t->size(2) - 1) * t->stride(2) * 2 + t->size(3) * 2 < INT32_MAX));
 }
 lvar_tensor_t packed_view(const at::Tensor& t) {
   if (!t.defined()) return lvar_tensor_t{nullptr, 0, 0, 0};
@@ -966,10 +966,10 @@ lvar_tensor_t packed_view(const at::Tensor& t) {
 }
 bool offsets_ok(const at::Tensor* t, int dev) { return t && packed(t, dev, at::kInt) && t->dim() == 1 && t->size(0) > 1 && t->size(0) <= INT32_MAX; }
 
-// memory for a tensor [1,H,T,d] in t's own order of axes
+// memory for a tensor [1,H,T,d] in t's own order of axes, or by heads where only that can be addressed
 at::Tensor packed_like(const at::Tensor& t) {
   const int64_t H = t.size(1), T = t.size(2), d = t.size(3);
-  const bool tokens_first = H > 1 && T > 1 && t.stride(1) < t.stride(2);
+  const bool tokens_first = H > 1 && T > 1 && t.stride(1) < t.stride(2) && T * H * d * 2 < INT32_MAX && H * d <= (1 << 20);
   return at::Tensor(at::detail::empty_strided_cuda(t.sizes(), {H * T * d, tokens_first ? d : T * d, tokens_first ? H * d : d, 1}, at::kBFloat16, t.device()));
 }
 

@@ -18,20 +18,24 @@ from .sparse_attn_ops import ShapeError, _native, _on_device, _pad_head_dim, _pl
 
 __all__ = ["packed_attn", "ShapeError"]
 
-_MOST_BYTES = 2 ** 31 - 1   # of a head's rows: the kernels address them with 31 bits
-
-
-def _span(t) -> int:
-    return (t.shape[2] - 1) * t.stride(2) * 2 + t.shape[3] * 2
+def _addressable(t) -> bool:
+    """The rows of a head span less than 2^31 bytes, and two of them are at most 2^20 elements apart (a tile may end behind the last one)."""
+    return t.shape[2] <= 1 or (t.stride(2) <= 1 << 20 and (t.shape[2] - 1) * t.stride(2) * 2 + t.shape[3] * 2 < 2 ** 31 - 1)
 
 
 def _tokens(t, name: str):
     """``t`` as the kernels read it."""
     t = _rows(t, name)
-    if t.shape[2] > 1 and _span(t) >= _MOST_BYTES:
+    if not _addressable(t):
         t = t.clone(memory_format=torch.contiguous_format)
-        _require(_span(t) < _MOST_BYTES, lambda: f"{name} has {t.shape[2]} tokens: a head's rows must span less than 2^31 bytes")
+        _require(_addressable(t), lambda: f"{name} has {t.shape[2]} tokens: a head's rows must span less than 2^31 bytes")
     return t
+
+
+def _like(t):
+    """Memory for a result in t's own order of axes, or by heads where only that can be addressed."""
+    r = _rows_like(t)
+    return r if _addressable(r) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _view(t) -> _lib.LvarTensor:
@@ -51,7 +55,7 @@ def _offsets(t, name: str, device):
 
 def _launch(q, k, v, offsets, k_offsets, causal, scale):
     _, H, T, d = q.shape
-    o = _rows_like(q)
+    o = _like(q)
     M, L = torch.empty((2, 1, H, T, 1), dtype=torch.float32, device=q.device).unbind(0)
     if o.numel():
         with _on_device(q):
@@ -88,7 +92,7 @@ class _PackedAttn(torch.autograd.Function):
             _require(t.device == q.device, "saved tensors and gradient must be on the device of q")
         _, H, T, d = q.shape
         Hkv, Tk = k.shape[1:3]
-        dq, dk, dv = (_rows_like(t) if need else None for t, need in zip((q, k, v), ctx.needs_input_grad))
+        dq, dk, dv = (_like(t) if need else None for t, need in zip((q, k, v), ctx.needs_input_grad))
         lib = _lib.load()
         with _on_device(q):
             nbytes = int(lib.lvar_packed_attn_bwd_workspace_bytes(offsets.shape[0] - 1, T, Tk, H, Hkv, d, 1 if causal else 0))
@@ -108,10 +112,11 @@ def packed_attn(q, k, v, offsets, k_offsets=None, scale=None, causal: bool = Tru
     any strides: the views of a fused projection are read in place.  ``offsets`` int32 ``[B+1]``, on the device, ascending: sequence b has the
     queries ``offsets[b] .. offsets[b+1]-1``; and the keys ``k_offsets[b] .. k_offsets[b+1]-1``, the same by default.  ``causal``: row i of n queries
     sees keys ``j < m - n + i + 1`` of m, its own position and those ahead of it where n = m; otherwise all.  Sequences may be empty.  Rows that see
-    no key, and rows ahead of the first sequence or behind the last, get ``o = 0, M = -inf, L = 1``; rows of no sequence get zero gradients.
+    no key (or only scores of -infinity), and rows ahead of the first sequence or behind the last, get ``o = 0, M = -inf, L = 1``; rows of no sequence get zero gradients.
     The lengths are read by the kernels: a captured call is replayed with others.
 
-    ``head_dim`` 16, 32, 64, 128 or 256.  Scores, statistics and sums are fp32; probabilities (and in the backward pass their gradients) are rounded to
+    ``head_dim`` 16, 32, 64, 128 or 256.  Scores, statistics and sums are fp32 (a score x is off by up to 2^-24 of
+    ``|x|``, its probability by a factor of 2 to that: scores belong below 2^20); probabilities (and in the backward pass their gradients) are rounded to
     bf16 where they enter a product.  The order of all sums is fixed: the same call gives the same bits.  A value that is not finite reaches the
     rows that see it, and through them the gradients, and nothing else.  ``o`` and the gradients have the order of axes of their inputs.  Once
     differentiable, in reverse mode."""
