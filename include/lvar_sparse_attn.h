@@ -513,14 +513,14 @@ int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int
  *   lvar_kv_pages_free    entries from keep[r] on (NULL: all) become -1, their pages are counted down.
  *   lvar_kv_cache_fork    row target[i] gets the first lengths[source[i]] tokens of row source[i] (lengths [rows]): its whole pages by name,
  *                         counted up, the tokens of the page that is not whole in the lowest free page; -1 behind it.  What the row
- *                         named before is not looked at (free it first).  Pairs outside the table, and of a row with itself, are left out.
- *                         Two forks with one target, or a target that is a source, leave these rows undefined.
- * scratch: lvar_kv_pages_scratch_bytes(rows or forks, num_pages) (4-byte aligned, needs no preparation; may be 0).
+ *                         named before is not looked at (free it first).  Left out are pairs outside the table, of a row with itself, and
+ *                         (of the others) whose target is a target twice or the source of a pair.
+ * scratch: lvar_kv_pages_scratch_bytes(forks, num_pages), of lvar_kv_pages_alloc with forks = 0 (4-byte aligned, needs no preparation; may be 0).
  *   lvar_kv_cache_compact token i < n (counts[b], NULL: all n) of head h of the pages of out_table's row b gets the bytes of token
  *                         keep[b, h, i] (int32, or int64 if keep64; strides in elements) of page_table's row b; zeros where that names no token.
  *                         A page that both tables name is undefined.
  */
-int64_t lvar_kv_pages_scratch_bytes(int rows, int num_pages);
+int64_t lvar_kv_pages_scratch_bytes(int forks, int num_pages);
 int lvar_kv_pages_alloc(int32_t* refs, int num_pages, int32_t* page_table, int64_t table_stride, int rows, int max_pages, const int32_t* first,
                         const int32_t* last, void* scratch, int64_t scratch_bytes, void* stream);
 int lvar_kv_pages_free(int32_t* refs, int num_pages, int32_t* page_table, int64_t table_stride, int rows, int max_pages, const int32_t* keep,

@@ -203,8 +203,8 @@ int fill_pages(PagesParams& p, int32_t* refs, int num_pages, int32_t* table, int
   return LVAR_OK;
 }
 
-int fill_scratch(PagesParams& p, void* scratch, int64_t bytes) {
-  const int64_t ints = pages_scratch_ints(p.n, p.num_pages);
+int fill_scratch(PagesParams& p, int forks, void* scratch, int64_t bytes) {
+  const int64_t ints = pages_scratch_ints(forks, p.num_pages);
   if (ints > 0 && (!scratch || !aligned(scratch, 4) || bytes < 4 * ints)) return LVAR_EINVAL;
   p.scratch = (int32_t*)scratch;
   return LVAR_OK;
@@ -268,9 +268,9 @@ int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int
   return launch_kv_read(p, cache.head_dim, (hipStream_t)stream);
 }
 
-int64_t lvar_kv_pages_scratch_bytes(int rows, int num_pages) {
-  if (rows < 0 || num_pages <= 0) return LVAR_EINVAL;
-  return 4 * pages_scratch_ints(rows, num_pages);
+int64_t lvar_kv_pages_scratch_bytes(int forks, int num_pages) {
+  if (forks < 0 || num_pages <= 0) return LVAR_EINVAL;
+  return 4 * pages_scratch_ints(forks, num_pages);
 }
 
 int lvar_kv_pages_alloc(int32_t* refs, int num_pages, int32_t* page_table, int64_t table_stride, int rows, int max_pages, const int32_t* first,
@@ -280,7 +280,7 @@ int lvar_kv_pages_alloc(int32_t* refs, int num_pages, int32_t* page_table, int64
   if (st != LVAR_OK) return st;
   if (!first || !last || !aligned(first, 4) || !aligned(last, 4)) return LVAR_EINVAL;
   p.first = first; p.last = last; p.n = rows;
-  if ((st = fill_scratch(p, scratch, scratch_bytes)) != LVAR_OK) return st;
+  if ((st = fill_scratch(p, 0, scratch, scratch_bytes)) != LVAR_OK) return st;
   return launch_pages_alloc(p, (hipStream_t)stream);
 }
 
@@ -302,7 +302,7 @@ int lvar_kv_cache_fork(lvar_paged_cache_t cache, int32_t* refs, int32_t* page_ta
   if (st != LVAR_OK || (st = fill_pages(p, refs, cache.num_pages, page_table, cache.table_stride, rows, cache.max_pages)) != LVAR_OK) return st;
   if (!source || !target || !lengths || !aligned(source, 4) || !aligned(target, 4) || !aligned(lengths, 4) || forks <= 0 || forks > 65535) return LVAR_EINVAL;
   p.source = source; p.target = target; p.lengths = lengths; p.n = forks; p.shift = c.shift;
-  if ((st = fill_scratch(p, scratch, scratch_bytes)) != LVAR_OK) return st;
+  if ((st = fill_scratch(p, forks, scratch, scratch_bytes)) != LVAR_OK) return st;
   return launch_pages_fork(p, c, cache.head_dim * (cache.k_exp ? 1 : 2), (hipStream_t)stream);
 }
 

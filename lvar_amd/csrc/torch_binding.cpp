@@ -841,8 +841,8 @@ void count_writes(std::initializer_list<const at::Tensor*> ts) {
   for (const at::Tensor* t : ts) if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
-at::Tensor pages_scratch(int64_t rows, int64_t pages, int dev, int64_t& bytes) {
-  bytes = std::max<int64_t>(0, api.lvar_kv_pages_scratch_bytes(static_cast<int>(rows), static_cast<int>(pages)));
+at::Tensor pages_scratch(int64_t forks, int64_t pages, int dev, int64_t& bytes) {
+  bytes = std::max<int64_t>(0, api.lvar_kv_pages_scratch_bytes(static_cast<int>(forks), static_cast<int>(pages)));
   return bytes > 0 ? empty({bytes}, at::kByte, dev) : at::Tensor();
 }
 
@@ -857,7 +857,7 @@ LVAR_FAST(fast_pages_alloc) {
   const int64_t B = table->size(0);
   LVAR_NEED(per_sequence(first, B, dev) && per_sequence(last, B, dev));
   int64_t bytes;
-  const at::Tensor ws = pages_scratch(B, refs->numel(), dev, bytes);
+  const at::Tensor ws = pages_scratch(0, refs->numel(), dev, bytes);
   LVAR_NEED(api.lvar_kv_pages_alloc(refs->data_ptr<int32_t>(), static_cast<int>(refs->numel()), table->data_ptr<int32_t>(), table_stride(*table), dim(*table, 0), dim(*table, 1),
                                     ints(first), ints(last), bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream) == LVAR_OK);
   count_writes({refs, table});

@@ -471,8 +471,8 @@ def _written(*tensors) -> None:
     torch.autograd.graph.increment_version([t for t in tensors if t is not None and not t.is_inference()])
 
 
-def _scratch(rows: int, num_pages: int, device):
-    nbytes = int(_lib.load().lvar_kv_pages_scratch_bytes(rows, num_pages))
+def _scratch(forks: int, num_pages: int, device):
+    nbytes = int(_lib.load().lvar_kv_pages_scratch_bytes(forks, num_pages))
     return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None), max(0, nbytes)
 
 
@@ -488,7 +488,7 @@ def kv_pages_alloc(refs, page_table, first, last) -> None:
     first, last = _per_sequence(first, "first", B, refs.device), _per_sequence(last, "last", B, refs.device)
     _require(first is not None and last is not None, "first and last must be given")
     with _on_device(refs):
-        ws, nbytes = _scratch(B, refs.shape[0], refs.device)
+        ws, nbytes = _scratch(0, refs.shape[0], refs.device)
         st = _lib.load().lvar_kv_pages_alloc(refs.data_ptr(), refs.shape[0], page_table.data_ptr(), _table_stride(page_table), B, n, first.data_ptr(), last.data_ptr(),
                                             _ptr(ws), nbytes, _stream(refs))
     _lib.check(st, "lvar_kv_pages_alloc")
@@ -515,8 +515,8 @@ def kv_cache_fork(cache: PagedKVCache, refs, page_table, source, target, lengths
     copied to the lowest free page, so that both sequences can go on; entries behind it become -1.  In place.
 
     What the target's row named before is not looked at: give it back first (:func:`kv_pages_free`).  Where there is no free page the entry gets
-    -1.  Pairs with a row outside the table, and of a row with itself, are left out.  Two forks with the same target, or a target that is
-    the source of another, leave these rows undefined."""
+    -1.  Left out are pairs with a row outside the table, of a row with itself, and (of the others) those whose target is the target of
+    another pair as well, or the source of one."""
     fast = _native()
     if fast is not None and fast.fast_cache_fork(cache, refs, page_table, source, target, lengths):
         return

@@ -1,6 +1,8 @@
 """Plain CPU implementation, entry by entry with lists, of the life of cache pages: tables, counts of names, forks, compacted sequences."""
 from __future__ import annotations
 
+import collections
+
 import torch
 
 
@@ -30,8 +32,11 @@ def fork(refs, table, source, target, lengths, page: int):
     """(refs, table, copies (from, to, tokens))"""
     refs, out = list(refs), [list(r) for r in table]
     pages, copies = [p for p, r in enumerate(refs) if r <= 0], []
-    for s, t in zip(source, target):
-        if not (0 <= s < len(table) and 0 <= t < len(table)) or s == t:
+    pairs = [(s, t) for s, t in zip(source, target) if 0 <= s < len(table) and 0 <= t < len(table) and s != t]
+    sources, targets = {s for s, _ in pairs}, [t for _, t in pairs]
+    twice = {t for t, n in collections.Counter(targets).items() if n > 1}
+    for s, t in pairs:
+        if t in sources or t in twice:
             continue
         n = max(0, lengths[s])
         whole, rest = n // page, n % page

@@ -149,6 +149,27 @@ def test_many_forks(host_path):
     assert bool((cache.v.view(torch.int16)[fresh, 0, :5] == cache.v.view(torch.int16)[9050, 0, :5]).all())
 
 
+@pytest.mark.parametrize("rows", [6, 40, 5000])
+def test_forks_that_depend_on_each_other(rows, host_path):
+    """Targets that are named twice, or sources themselves, are left out; nothing of their rows, pages and counts changes."""
+    from lvar_amd import kv_cache_ops as kv
+    r = random.Random(rows)
+    P, width, page = 3 * rows + 7, 3, 16
+    table, refs = tables(rows, width, P, seed=rows, holes=False)
+    cache = pool(P, 1, page, 64, torch.bfloat16, seed=rows)
+    lengths = [r.randrange(width * page + 9) for _ in range(rows)]
+    pairs = [(0, 1), (1, 2), (2, 3), (0, 4), (3, 4), (5, 5)] if rows == 6 else [(r.randrange(rows), r.randrange(-1, rows + 1)) for _ in range(rows // 2)]
+    source, target = zip(*pairs)
+    gt, gr, before = i32(table), i32(refs), raw(cache)
+    kv.kv_cache_fork(cache, gr, gt, i32(source), i32(target), i32(lengths))
+    refs, table, copies = ref.fork(refs, table, source, target, lengths, page)
+    assert gt.tolist() == table and gr.tolist() == refs and (rows > 6 or len(copies) <= 1)
+    for x, y in zip(before, raw(cache)):
+        for old, new, n in copies:
+            x[new, :, :n] = x[old, :, :n]
+        assert torch.equal(x, y)
+
+
 COMPACT = [
     # B, heads, entries, page, head_dim, kept, dtype
     (1, 1, 1, 16, 64, 1, torch.bfloat16),
