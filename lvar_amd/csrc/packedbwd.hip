@@ -76,20 +76,34 @@ __device__ __forceinline__ bf16x8 pack_half(const f32x16& x, int kb) {
 
 #endif
 
+// keys in three buffers, values in two
 template <int D>
 constexpr int dq_lds(int waves) {
-  const int bufs = 4 * 64 * D * 2, out = waves * 32 * (D * 2 + 16);
+  const int bufs = 5 * 64 * D * 2, out = waves * 32 * (D * 2 + 16);
   return bufs > out ? bufs : out;
 }
 
-// ---- dq: 32 query rows per wave, tiles of 64 keys.  S^T and dP^T = V do^T with the rows of q and do as B operands in registers, so a lane
-// owns a query column, and dS^T is in the B operand's layout of dq^T += K^T dS^T as it is. ----
+#if defined(__HIP_DEVICE_COMPILE__)
+
+// the first of 16 elements in slot g of N: all of them are through their three slots at the end
+template <int N>
+struct DqSlots {
+  static constexpr int lo(int g) { return g <= 0 ? 0 : g >= N - 2 ? 16 : g * 16 / (N - 2); }
+};
+
+#endif
+
+// ---- dq: 32 query rows per wave, steps of 32 keys.  S^T and dP^T = V do^T with the rows of q and do as B operands in registers, so a lane
+// owns a query column, and dS^T is in the B operand's layout of dq^T += K^T dS^T as it is.  A step forms S and dP of the coming 32 keys on the
+// matrix cores while the vector ALU turns those of the present ones into dS, and adds them.  The barrier of a tile of 64 keys lies between its
+// two steps' products: the first S of the next tile is formed beside the second dS of this one, whose keys stay (hence three buffers). ----
 
 template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(const PackedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   using S = PackedLds<D>;
+  using P = PackedOperands<D>;
   constexpr int KS = D / 16, MTD = D / 32, TILE = S::TILE;
   const int id = __builtin_amdgcn_workgroup_id_x(), place = id / p.H;
   PackedTile w;
@@ -141,48 +155,99 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
   if (T > 0) {
     const int k_srb = (int)p.k_sr * 2, v_srb = (int)p.v_sr * 2;
     const i32x4 krsrc = packed_rsrc(kp, m, S::ROWB, k_srb), vrsrc = packed_rsrc(vp, m, S::ROWB, v_srb);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(LVAR_LDS char*)smem;
-    fill_tile<D, NW>(krsrc, k_srb, 0, lds0, wave, lane);
-    fill_tile<D, NW>(vrsrc, v_srb, 0, lds0 + 2 * TILE, wave, lane);
-    wait_fills<0>();
-    __syncthreads();
-    for (int t = 0; t < T; t++) {
-      const int par = t & 1;
-      // (behind the last tile: rows that nobody reads, or zeros)
-      fill_tile<D, NW>(krsrc, k_srb, 64 * (t + 1), lds0 + (1 - par) * TILE, wave, lane);
-      fill_tile<D, NW>(vrsrc, v_srb, 64 * (t + 1), lds0 + (3 - par) * TILE, wave, lane);
-      const char *kbuf = smem + par * TILE, *vbuf = smem + (2 + par) * TILE;
-#pragma unroll
-      for (int sub = 0; sub < 2; sub++) {
-        f32x16 s, dp;
-#pragma unroll
-        for (int i = 0; i < 16; i++) { s[i] = nl; dp[i] = nd; }
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-          s = mfma32(at.rows(kbuf, sub, ks), qf[ks], s);
-          dp = mfma32(at.rows(vbuf, sub, ks), gf[ks], dp);
-        }
-        const int lim = seen - 64 * t - 32 * sub - 4 * hh;
-        if (64 * t + 32 * (sub + 1) <= seen_first) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) s[i] = fast_exp2(s[i] * c) * dp[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float x = fast_exp2(s[i] * c) * dp[i];
-            s[i] = 8 * (i >> 2) + (i & 3) < lim ? x : 0.f;
-          }
-        }
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-          const bf16x8 ds = pack_half(s, kb);
-#pragma unroll
-          for (int i = 0; i < MTD; i++) acc[i] = mfma32(at.columns(kbuf, 2 * sub + kb, i), ds, acc[i]);
-        }
-      }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(LVAR_LDS char*)smem, k_rows = lds0 + at.row_at, v_rows = k_rows + 3 * TILE, k_cols = lds0 + at.tr_at;
+    constexpr int NS = 2 * KS, NP = 2 * MTD, NT = NS + NP, AHEAD = 2;
+    auto request = [&](int t, int k_pl) {   // tile t into the place k_pl of the keys' ring
+      fill_tile<D, NW>(krsrc, k_srb, 64 * t, lds0 + k_pl, wave, lane);
+      fill_tile<D, NW>(vrsrc, v_srb, 64 * t, lds0 + (3 + (t & 1)) * TILE, wave, lane);
+    };
+    auto land = [&]() {
       wait_fills<0>();
       __syncthreads();
-    }
+    };
+    // starting values of S and dP; -infinity for keys that a row does not see
+    auto starts = [&](auto masked, int t, int sub, f32x16& s, f32x16& dp) {
+      const int lim = seen - 64 * t - 32 * sub - 4 * hh;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        s[i] = decltype(masked)::value && 8 * (i >> 2) + (i & 3) >= lim ? -INFINITY : nl;
+        dp[i] = nd;
+      }
+    };
+    // FIRST: S and dP of 32 keys, rows at `kr` and `vr`, in ns and ndp.  SECOND: those in s and dp are turned into dS and added, keys at `kc`.
+    auto step = [&](auto first, auto second, uint32_t kr, uint32_t vr, uint32_t kc, f32x16& s, f32x16& dp, f32x16& ns, f32x16& ndp) {
+      constexpr bool FIRST = decltype(first)::value, SECOND = decltype(second)::value;
+      bf16x8 frag[NT];
+      uint32_t pw[8];
+      auto operand = [&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (i < NS) { if constexpr (FIRST) frag[i] = P::rows(i & 1 ? vr : kr, i >> 1); }
+        else if constexpr (i < NT) { if constexpr (SECOND) frag[i] = P::columns(kc, (i - NS) / MTD, (i - NS) % MTD); }
+      };
+      using Sch = DqSlots<NS>;
+      auto slot = [&](auto gc) {
+        constexpr int g = decltype(gc)::value;
+        if constexpr (SECOND) {
+          static_for<Sch::lo(g - 2), Sch::lo(g - 1)>([&](auto ec) {
+            constexpr int e = decltype(ec)::value;
+            s[e] *= dp[e];
+            if constexpr (e & 1) pw[e >> 1] = pack_bf16(s[e - 1], s[e]);
+          });
+          static_for<Sch::lo(g - 1), Sch::lo(g)>([&](auto ec) { constexpr int e = decltype(ec)::value; s[e] = fast_exp2(s[e]); });
+          static_for<Sch::lo(g), Sch::lo(g + 1)>([&](auto ec) { constexpr int e = decltype(ec)::value; s[e] *= c; });
+        }
+      };
+      static_for<FIRST ? 0 : NS, (FIRST ? 0 : NS) + AHEAD>(operand);
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<0, NS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (FIRST) {
+          operand(std::integral_constant<int, i + AHEAD>{});
+          if constexpr (i & 1) ndp = mfma32(frag[i], gf[i >> 1], ndp); else ns = mfma32(frag[i], qf[i >> 1], ns);
+        }
+        slot(ic);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (SECOND) {
+        slot(std::integral_constant<int, NS>{});
+        static_for<NS, NT>([&](auto ic) {
+          constexpr int i = decltype(ic)::value, kb = (i - NS) / MTD, x = (i - NS) % MTD;
+          operand(std::integral_constant<int, i + AHEAD>{});
+          acc[x] = mfma32(frag[i], __builtin_bit_cast(bf16x8, u32x4{pw[4 * kb], pw[4 * kb + 1], pw[4 * kb + 2], pw[4 * kb + 3]}), acc[x]);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      }
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    constexpr int SUB_ROWS = 32 * S::ROWB, SUB_COLS = 32 * S::ROWB;
+    f32x16 sa, da, sb, db;
+    int k_pl = 0, k_next = TILE;   // places of the present tile and of the next one
+    request(0, 0);
+    land();
+    if (T > 1) request(1, TILE);
+    starts(Yes{}, 0, 0, sa, da);
+    step(Yes{}, No{}, k_rows, v_rows, k_cols, sb, db, sa, da);
+    starts(Yes{}, 0, 1, sb, db);
+    step(Yes{}, Yes{}, k_rows + SUB_ROWS, v_rows + SUB_ROWS, k_cols, sa, da, sb, db);
+    auto round = [&](int t, auto masked) {   // the second step of tile t - 1, and the first of tile t
+      land();
+      const int k_last = k_pl;
+      k_pl = k_next;
+      k_next = k_pl == 2 * TILE ? 0 : k_pl + TILE;
+      if (t + 1 < T) request(t + 1, k_next);
+      const uint32_t vr = v_rows + (t & 1) * TILE;
+      starts(masked, t, 0, sa, da);
+      step(Yes{}, Yes{}, k_rows + k_pl, vr, k_cols + k_last + SUB_COLS, sb, db, sa, da);
+      starts(masked, t, 1, sb, db);
+      step(Yes{}, Yes{}, k_rows + k_pl + SUB_ROWS, vr + SUB_ROWS, k_cols + k_pl, sa, da, sb, db);
+    };
+    const int whole = min(T, seen_first >> 6);   // tiles that all rows of the wave see whole
+    int t = 1;
+    for (; t < whole; t++) round(t, No{});
+    for (; t < T; t++) round(t, Yes{});
+    step(No{}, Yes{}, k_rows, v_rows, k_cols + k_pl + SUB_COLS, sb, db, sa, da);
+    __syncthreads();
   }
   bf16_t* to = p.dq + h * p.dq_sh + (int64_t)(w.first + q0) * p.dq_sr;
   store_rows<D>(smem + wave * (32 * (D * 2 + 16)), acc, p.scale, to, p.dq_sr, w.n - q0, lane);
