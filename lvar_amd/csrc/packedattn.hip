@@ -233,29 +233,36 @@ __device__ __forceinline__ void packed_fwd_item(const PackedParams& p, char* sme
       for (int kb = 0; kb < 4; kb++)
 #pragma unroll
         for (int i = 0; i < MTD; i++) oacc[i] = mfma32(at.columns(vbuf, kb, i), pb[kb], oacc[i]);
-      __syncthreads();
     };
     using P0 = std::integral_constant<int, 0>;
     using P1 = std::integral_constant<int, 1>;
     using No = std::false_type;
     using Yes = std::true_type;
-    // tiles that all rows of the wave see whole, then the others (loops of their own: behind a branch in one loop the two bodies spill)
-    const int whole = min(T, seen_first >> 6);
+    // tiles that all rows of the wave see whole, then the others that one of them sees (loops of their own: behind a branch in one loop the two
+    // bodies spill), then those that only other waves do
+    const int mine = q0 < w.n ? (seen_by(min(q0 + 32, w.n) - 1) + 63) >> 6 : 0, whole = min(mine, seen_first >> 6);
     int t = 0;
     for (; t + 2 < whole; t += 2) {
       body(t, P0{}, No{}, sa0, sa1, sb0, sb1);
       body(t + 1, P1{}, No{}, sb0, sb1, sa0, sa1);
     }
-    for (; t + 2 < T; t += 2) {
+    for (; t + 2 < mine; t += 2) {
       body(t, P0{}, Yes{}, sa0, sa1, sb0, sb1);
       body(t + 1, P1{}, Yes{}, sb0, sb1, sa0, sa1);
     }
-    if (t + 1 < T) {
+    if (t + 1 < mine) {
       body(t, P0{}, Yes{}, sa0, sa1, sb0, sb1);
       last(P1{}, sb0, sb1);
-    } else {
+    } else if (mine > 0) {
       last(P0{}, sa0, sa1);
     }
+    for (t = max(0, mine - 1); t + 1 < T; t++) {
+      fill_tile<D, NW>(vrsrc, v_srb, 64 * (t + 1), lds0 + (2 + ((t + 1) & 1)) * TILE, wave, lane);
+      fill_tile<D, NW>(krsrc, k_srb, 64 * (t + 2), lds0 + (t & 1) * TILE, wave, lane);
+      wait_fills<0>();
+      __syncthreads();
+    }
+    __syncthreads();
   }
 
   const float ltot = xhalf_sum(lsum[0] + lsum[1]);

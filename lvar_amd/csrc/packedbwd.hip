@@ -226,27 +226,34 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
     request(0, 0);
     land();
     if (T > 1) request(1, TILE);
-    starts(Yes{}, 0, 0, sa, da);
-    step(Yes{}, No{}, k_rows, v_rows, k_cols, sb, db, sa, da);
-    starts(Yes{}, 0, 1, sb, db);
-    step(Yes{}, Yes{}, k_rows + SUB_ROWS, v_rows + SUB_ROWS, k_cols, sa, da, sb, db);
-    auto round = [&](int t, auto masked) {   // the second step of tile t - 1, and the first of tile t
+    auto arrive = [&](int t) {   // tile t is there, the next one is requested
       land();
-      const int k_last = k_pl;
       k_pl = k_next;
       k_next = k_pl == 2 * TILE ? 0 : k_pl + TILE;
       if (t + 1 < T) request(t + 1, k_next);
+    };
+    auto round = [&](int t, auto masked) {   // the second step of tile t - 1, and the first of tile t
+      const int k_last = k_pl;
+      arrive(t);
       const uint32_t vr = v_rows + (t & 1) * TILE;
       starts(masked, t, 0, sa, da);
       step(Yes{}, Yes{}, k_rows + k_pl, vr, k_cols + k_last + SUB_COLS, sb, db, sa, da);
       starts(masked, t, 1, sb, db);
       step(Yes{}, Yes{}, k_rows + k_pl + SUB_ROWS, vr + SUB_ROWS, k_cols + k_pl, sa, da, sb, db);
     };
-    const int whole = min(T, seen_first >> 6);   // tiles that all rows of the wave see whole
+    const int mine = q0 < w.n ? (seen_by(min(q0 + 32, w.n) - 1) + 63) >> 6 : 0;   // tiles that a row of the wave sees
+    const int whole = min(mine, seen_first >> 6);                                 // and that all of them see whole
     int t = 1;
-    for (; t < whole; t++) round(t, No{});
-    for (; t < T; t++) round(t, Yes{});
-    step(No{}, Yes{}, k_rows, v_rows, k_cols + k_pl + SUB_COLS, sb, db, sa, da);
+    if (mine > 0) {
+      starts(Yes{}, 0, 0, sa, da);
+      step(Yes{}, No{}, k_rows, v_rows, k_cols, sb, db, sa, da);
+      starts(Yes{}, 0, 1, sb, db);
+      step(Yes{}, Yes{}, k_rows + SUB_ROWS, v_rows + SUB_ROWS, k_cols, sa, da, sb, db);
+      for (; t < whole; t++) round(t, No{});
+      for (; t < mine; t++) round(t, Yes{});
+      step(No{}, Yes{}, k_rows, v_rows, k_cols + k_pl + SUB_COLS, sb, db, sa, da);
+    }
+    for (; t < T; t++) arrive(t);
     __syncthreads();
   }
   bf16_t* to = p.dq + h * p.dq_sh + (int64_t)(w.first + q0) * p.dq_sr;
@@ -344,6 +351,10 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
   const int t_first = (int)(T_all * share / p.shares), T = (int)(T_all * (share + 1) / p.shares) - t_first;
   const int blk_first = last - t_first / p.G, head_first = t_first % p.G;
   const int whole0 = p.causal ? max(0, k0 + 31 - shift) : 0;   // rows from here on see all keys of the wave
+  // those that see a key of this pair of waves: none of the last ones, if causal
+  const int b0_mine = p.causal ? min(max(0, k0 - shift), n) / Q::R : 0;
+  const int64_t T_mine = k0 < w.n ? (int64_t)max(0, last + 1 - b0_mine) * p.G - t_first : 0;
+  const int mine = __builtin_amdgcn_readfirstlane((int)max((int64_t)0, min(T_mine, (int64_t)T)));
   const float c = p.c;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LVAR_LDS char*)smem;
 
@@ -509,15 +520,19 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
       round(-1, Yes{}, No{}, sb, sa);   // the first round forms dP(0)
     }
     int t = 0;
-    for (; t + 2 < T; t += 2) {
+    for (; t + 2 < mine; t += 2) {
       round(t, Yes{}, Yes{}, sa, sb);
       round(t + 1, Yes{}, Yes{}, sb, sa);
     }
-    if (t + 1 < T) {
+    if (t + 1 < mine) {
       round(t, Yes{}, Yes{}, sa, sb);
       round(t + 1, No{}, Yes{}, sb, sa);
-    } else {
+    } else if (mine > 0) {
       round(t, No{}, Yes{}, sa, sb);
+    }
+    for (t = mine; t < T; t++) {
+      request();
+      settle(std::integral_constant<int, Q::LEAD - 1>{});
     }
     if constexpr (ROLE == 0) __syncthreads();   // the others' last round
     wait_fills<0>();

@@ -30,8 +30,8 @@ def test_every_instance_is_built(kernels):
 
 
 def test_spilled_registers(kernels):
-    # (256 columns: outside of the loop over the keys, or a few per tile; keys of 128 columns: rows that are formed again)
-    may = {"packed_fwd_kernel": {256: 10}, "packed_dkv_kernel": {128: 7}}
+    # (256 columns: a few per tile)
+    may = {"packed_fwd_kernel": {256: 4}}
     spilled = {n: k[".vgpr_spill_count"] for n, k in kernels.items() if k.get(".vgpr_spill_count", 0) > may.get(n[0], {}).get(n[1] if len(n) > 1 else 0, 0)}
     assert not spilled, spilled
 
