@@ -554,9 +554,11 @@ int lvar_paged_attn_fwd(lvar_tensor_t q, lvar_paged_cache_t cache, const int32_t
  * and rows of no sequence (ahead of the first offset, behind the last), get o = 0, M = -inf, L = 1.  Query head h reads key/value head
  * h / (H / kv_heads).  head_dim 64, 128 or 256; rows 16-byte aligned; a head's rows span less than 2^31 bytes.  A value that is not finite reaches
  * the rows that see it and no others.  Scores, M, L and sums are fp32; probabilities enter the second product as bf16 (2^-9).
+ * workspace: lvar_packed_attn_fwd_workspace_bytes() (often 0; 16-byte aligned, written and read by this call).
  */
+int64_t lvar_packed_attn_fwd_workspace_bytes(int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal);
 int lvar_packed_attn_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar_tensor_t o, const int32_t* offsets, const int32_t* k_offsets,
-                         float* M, float* L, int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal, float scale,
+                         float* M, float* L, void* workspace, int64_t workspace_bytes, int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal, float scale,
                          void* stream);
 
 /*

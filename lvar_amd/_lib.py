@@ -24,7 +24,7 @@ EXPORTED_SYMBOLS = (
     "lvar_paged_attn_workspace_bytes", "lvar_paged_attn_fwd",
     "lvar_qk_norm_axes_fwd", "lvar_qk_norm_axes_bwd_scratch_bytes", "lvar_qk_norm_axes_bwd", "lvar_kv_cache_append_axes",
     "lvar_kv_pages_scratch_bytes", "lvar_kv_pages_alloc", "lvar_kv_pages_free", "lvar_kv_cache_fork", "lvar_kv_cache_compact",
-    "lvar_packed_attn_fwd", "lvar_packed_attn_bwd_workspace_bytes", "lvar_packed_attn_bwd",
+    "lvar_packed_attn_fwd_workspace_bytes", "lvar_packed_attn_fwd", "lvar_packed_attn_bwd_workspace_bytes", "lvar_packed_attn_bwd",
 )
 
 
@@ -169,8 +169,10 @@ def load() -> C.CDLL:
     lib.lvar_kv_cache_fork.argtypes = [G, P, P, I, P, P, P, I, P, I64, P]
     lib.lvar_kv_cache_compact.restype = I
     lib.lvar_kv_cache_compact.argtypes = [G, P, I64, I, P, I, I64, I64, I64, P, I, I, P]
+    lib.lvar_packed_attn_fwd_workspace_bytes.restype = I64
+    lib.lvar_packed_attn_fwd_workspace_bytes.argtypes = [I] * 7
     lib.lvar_packed_attn_fwd.restype = I
-    lib.lvar_packed_attn_fwd.argtypes = [T, T, T, T, P, P, P, P, I, I, I, I, I, I, I, F, P]
+    lib.lvar_packed_attn_fwd.argtypes = [T, T, T, T, P, P, P, P, P, I64, I, I, I, I, I, I, I, F, P]
     lib.lvar_packed_attn_bwd_workspace_bytes.restype = I64
     lib.lvar_packed_attn_bwd_workspace_bytes.argtypes = [I] * 7
     lib.lvar_packed_attn_bwd.restype = I

@@ -23,12 +23,14 @@ struct PackedParams {
   bf16_t *dq, *dk, *dv;             // null: not wanted
   int64_t dq_sh, dq_sr, dk_sh, dk_sr, dv_sh, dv_sr;
   int slots;                        // set at launch: places for query tiles, see find_tile
-  int shares;                       // set at launch: workgroups that share the query rows of a key tile
-  float* parts;                     // their sums, [shares][dk, dv][Hkv][Tk][D]
+  int shares;                       // set at launch: workgroups that share the keys of a query tile, or the query rows of a key tile
+  float* parts;                     // their sums: [shares][H][T][D] of o or dq, [shares][dk, dv][Hkv][Tk][D]
+  float* part_stats;                // forward: [shares][H][T][3] what their P refers to, its sum, the maximum
   float* stats;                     // [H,2,T]: -(M + log2 L) / c (-inf: the row sees nothing), and -sum(do * o)
 };
 
-int launch_packed_fwd(PackedParams p, int head_dim, hipStream_t s);
+int64_t packed_fwd_bytes(const PackedParams& p, int head_dim);
+int launch_packed_fwd(PackedParams p, void* workspace, int head_dim, hipStream_t s);
 int64_t packed_bwd_bytes(const PackedParams& p, int head_dim);
 int launch_packed_bwd(PackedParams p, void* workspace, int head_dim, hipStream_t s);
 
@@ -36,7 +38,28 @@ int launch_packed_bwd(PackedParams p, void* workspace, int head_dim, hipStream_t
 // behind the last included, have at most these many.
 inline int64_t packed_slots(int T, int B, int R) { return (int64_t)T / R + B + 2; }
 
+// Workgroups that share the keys of a query tile of 128 rows, where query tiles alone leave compute units idle (few rows over many keys, few heads): as
+// many as fill the waves that a SIMD holds, twice that if causal, where the last tile has twice the work of the mean one.  None gets fewer than
+// SHARE_TILES tiles of the mean sequence: parts cost a launch and 8 bytes of traffic per element, about what 9 us of products are worth.  Against one
+// workgroup per tile, forward / dq, the sum of the parts included: 64 rows of 8 heads of 128 over 8192 keys 93 -> 22 / 144 -> 28 us; 16384 rows
+// of one head, causal 198 -> 91 / 302 -> 126 us; 9360 rows of 4 heads of 64, causal 95 -> 71 / 126 -> 90 us.  With shares of 4 tiles 2048 rows of 16 heads of
+// 128, causal lost: 35 -> 44 / 51 -> 55 us.
+inline int query_shares(const PackedParams& p, int waves_per_simd) {
+  constexpr int SHARE_TILES = 12;
+  const int64_t groups = ((int64_t)p.T / 128 + p.B) * p.H, slots = (int64_t)device_cus() * waves_per_simd * (p.causal ? 2 : 1);
+  const int64_t most = (int64_t)p.Tk / p.B / 64 / (p.causal ? 2 : 1) / SHARE_TILES, want = slots / (groups > 0 ? groups : 1);
+  const int64_t n = want < most ? want : most;
+  return n < 2 ? 1 : n > 32 ? 32 : (int)n;
+}
+
 #if defined(__HIP_DEVICE_COMPILE__)
+
+// Tiles t0 .. t0 + T - 1 of a share of T_all
+struct Share { int t0, T; };
+__device__ __forceinline__ Share share_of(int T_all, int share, int shares) {
+  const int t0 = (int)((int64_t)T_all * share / shares);
+  return {t0, (int)((int64_t)T_all * (share + 1) / shares) - t0};
+}
 
 // Sum over the 64 lanes, the same in all of them
 __device__ __forceinline__ int wave_sum(int x) {
@@ -235,12 +258,14 @@ __device__ __forceinline__ void fill_tile(const i32x4& rsrc, int srb, int row0, 
 // Head of place j of H: with a multiple of 8 heads, those of an XCD (workgroups are dealt to the 8 in turn) are neighbours, which share keys and values.
 __device__ __forceinline__ int packed_head(int j, int H) { return (H & 7) == 0 ? (j & 7) * (H >> 3) + (j >> 3) : j; }
 
-// Is x infinite or NaN?  On bits that the compiler cannot trace back to a float: with -fno-honor-nans it turns the test into one for infinity.
-__device__ __forceinline__ bool not_finite(float x) {
+// The bits of x, which the compiler cannot trace back to a float: with -fno-honor-nans it takes a test of them for one of a number.
+__device__ __forceinline__ uint32_t bits_of(float x) {
   uint32_t u = __builtin_bit_cast(uint32_t, x);
   asm("" : "+v"(u));
-  return (u & 0x7f800000u) == 0x7f800000u;
+  return u;
 }
+// Is x infinite or NaN?
+__device__ __forceinline__ bool not_finite(float x) { return (bits_of(x) & 0x7f800000u) == 0x7f800000u; }
 
 // The transposed accumulators of a wave, 32 rows of D columns, as bf16 rows: through LDS (32 * (2 D + 16) bytes at `buf`, this wave's
 // own), so that rows are stored in 16-byte pieces.  rows < n are stored.
@@ -267,6 +292,36 @@ __device__ __forceinline__ void store_rows(char* buf, const f32x16 (&acc)[MT], f
   }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
+}
+
+// The same sums as they are, fp32 rows of D one behind the other, half of the columns at a time through the same bytes of LDS.  (Straight from the
+// accumulators, 16 bytes of each row per instruction, the stores of three shares of 2048 rows of 16 heads of 128 took longer than their products.)
+template <int D, int MT>
+__device__ __forceinline__ void store_part(char* buf, const f32x16 (&acc)[MT], float* to, int n, int lane) {
+  static_assert(MT * 32 == D, "all columns");
+  constexpr int STR = D * 2 + 16, CPR = D / 8;   // bytes of half a row, 16-byte pieces
+  const int hh = lane >> 5, r = lane & 31;
+#pragma unroll
+  for (int half = 0; half < 2; half++) {
+#pragma unroll
+    for (int m = 0; m < MT / 2; m++)
+#pragma unroll
+      for (int a = 0; a < 4; a++) {
+        const f32x16& x = acc[half * (MT / 2) + m];
+        *(f32x4*)(buf + r * STR + (m * 32 + 8 * a + 4 * hh) * 4) = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]};
+      }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 32 * CPR / 64; i++) {
+      const int at = lane + i * 64, row = at / CPR, chunk = at - row * CPR;
+      const f32x4 x = *(const f32x4*)(buf + row * STR + chunk * 16);
+      if (row < n) *(f32x4*)(to + row * D + half * (D / 2) + chunk * 4) = x;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 #endif  // __HIP_DEVICE_COMPILE__

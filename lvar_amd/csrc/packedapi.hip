@@ -44,12 +44,22 @@ int fill(PackedParams& p, const lvar_tensor_t& q, const lvar_tensor_t& k, const 
 
 extern "C" {
 
+int64_t lvar_packed_attn_fwd_workspace_bytes(int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal) {
+  if (!sizes_ok(batch, tokens, k_tokens, H, kv_heads)) return LVAR_EINVAL;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return LVAR_EUNSUPPORTED;
+  PackedParams p{};
+  p.B = batch; p.T = tokens; p.Tk = k_tokens; p.H = H; p.Hkv = kv_heads; p.G = H / kv_heads; p.causal = causal ? 1 : 0;
+  return packed_fwd_bytes(p, head_dim);
+}
+
 int lvar_packed_attn_fwd(lvar_tensor_t q, lvar_tensor_t k, lvar_tensor_t v, lvar_tensor_t o, const int32_t* offsets, const int32_t* k_offsets, float* M,
-                         float* L, int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal, float scale, void* stream) {
+                         float* L, void* workspace, int64_t workspace_bytes, int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal, float scale, void* stream) {
   PackedParams p{};
   const int st = fill(p, q, k, v, o, offsets, k_offsets, M, L, batch, tokens, k_tokens, H, kv_heads, head_dim, causal, scale);
   if (st != LVAR_OK || tokens == 0) return st;
-  return launch_packed_fwd(p, head_dim, (hipStream_t)stream);
+  const int64_t bytes = packed_fwd_bytes(p, head_dim);
+  if (bytes > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < bytes)) return LVAR_EINVAL;
+  return launch_packed_fwd(p, workspace, head_dim, (hipStream_t)stream);
 }
 
 int64_t lvar_packed_attn_bwd_workspace_bytes(int batch, int tokens, int k_tokens, int H, int kv_heads, int head_dim, int causal) {

@@ -38,19 +38,23 @@ __device__ __forceinline__ void careful_row(const bf16_t* q, const bf16_t* k, in
   for (int e = 0; e < D / 64; e++) o[e * 64 + lane] = (bf16_t)acc[e];
 }
 
-template <int D, int NW>
-__device__ __forceinline__ void packed_fwd_item(const PackedParams& p, char* smem, const PackedTile& w, const int h) {
+template <int D, int NW, bool SPLIT>
+__device__ __forceinline__ void packed_fwd_item(const PackedParams& p, char* smem, const PackedTile& w, const int h, const int share) {
   using S = PackedLds<D>;
   constexpr int KS = D / 16, MTD = D / 32, ROWS = NW * 32, TILE = S::TILE, SLOTS = S::NI / NW;
   const int lane = __builtin_amdgcn_workitem_id_x() & 63;
   const int wave = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_workitem_id_x() >> 6);
   const int hh = lane >> 5, r = lane & 31;
   const S at(lane);
-  const int k_first = w.other_first, m = w.other_n;
+  const int m_all = w.other_n;
   const int hk = h / p.G, q0 = w.row0 + wave * 32;   // first row of the wave
-  const int shift = p.causal ? m - w.n : m;          // row i sees keys below i + shift + 1 (causal), below m
-  auto seen_by = [&](int row) { return max(0, p.causal ? min(m, row + shift + 1) : m); };
-  const int T = (seen_by(min(w.row0 + ROWS, w.n) - 1) + 63) >> 6;
+  const int shift = p.causal ? m_all - w.n : m_all;  // row i sees keys below i + shift + 1 (causal), below m_all
+  auto all_seen_by = [&](int row) { return max(0, p.causal ? min(m_all, row + shift + 1) : m_all); };
+  const int T_all = (all_seen_by(min(w.row0 + ROWS, w.n) - 1) + 63) >> 6;
+  const Share part = SPLIT ? share_of(T_all, share, p.shares) : Share{0, T_all};
+  // from here on keys are those of the share
+  const int T = part.T, k_first = w.other_first + 64 * part.t0, m = SPLIT ? max(0, min(m_all - 64 * part.t0, 64 * T)) : m_all;
+  auto seen_by = [&](int row) { return SPLIT ? max(0, min(m, all_seen_by(row) - 64 * part.t0)) : all_seen_by(row); };
   const int row = min(q0 + r, w.n - 1);
   const int seen = seen_by(row), seen_first = __builtin_amdgcn_readfirstlane(seen);   // lane 0 has the wave's first row: the fewest
 
@@ -266,7 +270,18 @@ __device__ __forceinline__ void packed_fwd_item(const PackedParams& p, char* sme
   }
 
   const float ltot = xhalf_sum(lsum[0] + lsum[1]);
-  const bool empty = __builtin_bit_cast(uint32_t, ltot) == 0u;   // no key seen
+  const bool empty = bits_of(ltot) == 0u;   // no key seen
+  if constexpr (SPLIT) {   // packed_fwd_join_kernel does the rest
+    const int64_t at_row = ((int64_t)share * p.H + h) * p.T + w.first + q0;
+    if (hh == 0 && q0 + r < w.n) {
+      float* st = p.part_stats + (at_row + r) * 3;
+      st[0] = m_ref;
+      st[1] = ltot;
+      st[2] = m_true;
+    }
+    if (T > 0) store_part<D>(smem + wave * (32 * (D * 2 + 16)), oacc, p.parts + at_row * D, w.n - q0, lane);
+    return;
+  }
   const float inv = empty ? 0.f : 1.0f / ltot;
   if (hh == 0 && q0 + r < w.n) {
     const int64_t to = (int64_t)h * p.T + w.first + q0 + r;
@@ -301,35 +316,104 @@ constexpr int packed_fwd_lds() {
   return bufs > out ? bufs : out;
 }
 
-template <int D, int NW>
+template <int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_fwd_kernel(const PackedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const int id = __builtin_amdgcn_workgroup_id_x(), place = id / p.H;
+  const int per = SPLIT ? p.H * p.shares : p.H;
+  const int id = __builtin_amdgcn_workgroup_id_x(), place = id / per, j = id - place * per;
   PackedTile w;
   // the places from the last one on: of a causal sequence the tiles with the most keys come first
   if (!find_tile<NW * 32>(p.q_off, p.T, p.k_off, p.Tk, p.B, p.slots - 1 - place, false, w)) return;
-  packed_fwd_item<D, NW>(p, smem, w, packed_head(id - place * p.H, p.H));
+  const int share = SPLIT ? j / p.H : 0;
+  packed_fwd_item<D, NW, SPLIT>(p, smem, w, packed_head(j - share * p.H, p.H), share);
 #endif
 }
 
-template <int D, int NW>
+// The rows of a launch whose workgroups shared keys, from the parts in their order: a lane per four columns.
+template <int D>
+__global__ __launch_bounds__(256) void packed_fwd_join_kernel(const PackedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int LPR = D / 4, RPG = 256 / LPR;
+  const int tid = __builtin_amdgcn_workitem_id_x(), lane = tid & 63, column = tid % LPR * 4;
+  const int64_t rows = (int64_t)p.H * p.T, x = (int64_t)__builtin_amdgcn_workgroup_id_x() * RPG + tid / LPR, at = min(x, rows - 1);
+  const int h = (int)(at / p.T), row = (int)(at - (int64_t)h * p.T);
+  const float *st = p.part_stats + at * 3, *part = p.parts + at * D + column;
+  float M = -INFINITY;
+#pragma unroll 4
+  for (int s = 0; s < p.shares; s++) M = fmaxf(M, st[s * rows * 3 + 2]);
+  float L = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  bool any = false;
+  for (int s = 0; s < p.shares; s++) {
+    const float sum = st[s * rows * 3 + 1];
+    const f32x4 y = *(const f32x4*)(part + s * rows * D);
+    const bool some = bits_of(sum) != 0u;   // a key of the share is seen (else its part may not be written)
+    any |= some;
+    const float f = some ? fast_exp2(st[s * rows * 3] - M) : 0.f;
+    L = fmaf(f, sum, L);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = fmaf(f, some ? y[e] : 0.f, o[e]);
+  }
+  const float inv = any ? 1.0f / L : 0.f;
+  bf16_t* to = p.o + h * p.o_sh + (int64_t)row * p.o_sr;
+  if (x < rows) {
+    if (column == 0) {
+      p.M[at] = M;
+      p.L[at] = any ? L : 1.0f;
+    }
+    *(u32x2*)(to + column) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+  }
+  if (!p.causal) return;
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; e++) bad |= not_finite(o[e]);
+  uint64_t left = __builtin_amdgcn_ballot_w64(bad && x < rows);
+  if (left) wait_fills<0>();   // the rows as stored above are written again
+  while (left) {
+    const int i = __builtin_ctzll(left) / LPR * LPR;   // the first lane of a row
+    left &= i + LPR < 64 ? ~0ull << (i + LPR) : 0ull;
+    const int hi = __builtin_amdgcn_readlane(h, i), ri = __builtin_amdgcn_readlane(row, i), hk = hi / p.G;
+    PackedTile w;
+    find_row(p.q_off, p.T, p.k_off, p.Tk, p.B, ri, w);
+    const int seen = max(0, min(w.other_n, w.row0 + w.other_n - w.n + 1));
+    careful_row<D>(p.q + hi * p.q_sh + (int64_t)ri * p.q_sr, p.k + hk * p.k_sh + (int64_t)w.other_first * p.k_sr, p.k_sr,
+                   p.v + hk * p.v_sh + (int64_t)w.other_first * p.v_sr, p.v_sr, seen, p.c, __shfl(M, i, 64), __shfl(inv, i, 64), p.o + hi * p.o_sh + (int64_t)ri * p.o_sr);
+  }
+#endif
+}
+
+template <int D, int NW, bool SPLIT>
 static int launch_fwd(PackedParams p, hipStream_t s) {
   constexpr int SMEM = packed_fwd_lds<D, NW>();
-  const int64_t slots = packed_slots(p.T, p.B, NW * 32), groups = slots * p.H;
-  if (groups * (NW * 64) > 0xffffffffll) return LVAR_EINVAL;
+  const int64_t slots = packed_slots(p.T, p.B, NW * 32), groups = slots * p.H * p.shares, joins = ((int64_t)p.H * p.T * (D / 4) + 255) / 256;
+  if (groups * (NW * 64) > 0xffffffffll || joins * 256 > 0xffffffffll) return LVAR_EINVAL;
   p.slots = (int)slots;
-  auto kern = packed_fwd_kernel<D, NW>;
+  auto kern = packed_fwd_kernel<D, NW, SPLIT>;
   static std::atomic<uint64_t> ready{0};
   if (!ensure_lds_limit((const void*)kern, SMEM, ready)) return LVAR_ELAUNCH;
   hipLaunchKernelGGL(kern, dim3((uint32_t)groups), dim3(NW * 64), SMEM, s, p);
+  if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
+  if (SPLIT) hipLaunchKernelGGL(packed_fwd_join_kernel<D>, dim3((uint32_t)joins), dim3(256), 0, s, p);
   return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
 }
 
-int launch_packed_fwd(PackedParams p, int head_dim, hipStream_t s) {
-  if (head_dim == 128) return launch_fwd<128, 4>(p, s);
-  if (head_dim == 64) return launch_fwd<64, 4>(p, s);
-  if (head_dim == 256) return launch_fwd<256, 4>(p, s);
+static int fwd_shares(const PackedParams& p, int head_dim) { return query_shares(p, head_dim <= 128 ? 2 : 1); }
+
+// sums and statistics of shares
+int64_t packed_fwd_bytes(const PackedParams& p, int head_dim) {
+  const int shares = fwd_shares(p, head_dim);
+  return shares > 1 ? 4 * (int64_t)shares * p.H * p.T * (head_dim + 3) : 0;
+}
+
+int launch_packed_fwd(PackedParams p, void* workspace, int head_dim, hipStream_t s) {
+  p.shares = fwd_shares(p, head_dim);
+  p.parts = (float*)workspace;
+  p.part_stats = p.parts + (int64_t)p.shares * p.H * p.T * head_dim;
+  const bool split = p.shares > 1;
+  if (head_dim == 128) return split ? launch_fwd<128, 4, true>(p, s) : launch_fwd<128, 4, false>(p, s);
+  if (head_dim == 64) return split ? launch_fwd<64, 4, true>(p, s) : launch_fwd<64, 4, false>(p, s);
+  if (head_dim == 256) return split ? launch_fwd<256, 4, true>(p, s) : launch_fwd<256, 4, false>(p, s);
   return LVAR_EUNSUPPORTED;
 }
 

@@ -52,6 +52,23 @@ struct CarefulRow {
   }
 };
 
+// Four columns of the sum of all shares, `stride` floats from one to the next, to `to` (null: nowhere).  Is one of them not finite?
+__device__ __forceinline__ bool join_part(const float* part, int64_t stride, int shares, float factor, bf16_t* to) {
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < shares; s++) {
+    const f32x4 y = *(const f32x4*)(part + s * stride);
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] += y[e];
+  }
+  if (!to) return false;
+  *(u32x2*)to = u32x2{pack_bf16(sum[0] * factor, sum[1] * factor), pack_bf16(sum[2] * factor, sum[3] * factor)};
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; e++) bad |= not_finite(sum[e]);
+  return bad;
+}
+
 template <int MT>
 __device__ __forceinline__ bool any_not_finite(const f32x16 (&acc)[MT]) {
   bool bad = false;
@@ -98,25 +115,30 @@ struct DqSlots {
 // matrix cores while the vector ALU turns those of the present ones into dS, and adds them.  The barrier of a tile of 64 keys lies between its
 // two steps' products: the first S of the next tile is formed beside the second dS of this one, whose keys stay (hence three buffers). ----
 
-template <int D, int NW>
+template <int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(const PackedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   using S = PackedLds<D>;
   using P = PackedOperands<D>;
   constexpr int KS = D / 16, MTD = D / 32, TILE = S::TILE;
-  const int id = __builtin_amdgcn_workgroup_id_x(), place = id / p.H;
+  const int per = SPLIT ? p.H * p.shares : p.H;
+  const int id = __builtin_amdgcn_workgroup_id_x(), place = id / per, j = id - place * per, share = SPLIT ? j / p.H : 0;
   PackedTile w;
   if (!find_tile<NW * 32>(p.q_off, p.T, p.k_off, p.Tk, p.B, p.slots - 1 - place, false, w)) return;
-  const int h = packed_head(id - place * p.H, p.H), hk = h / p.G;
+  const int h = packed_head(j - share * p.H, p.H), hk = h / p.G;
   const int lane = __builtin_amdgcn_workitem_id_x() & 63;
   const int wave = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_workitem_id_x() >> 6);
   const int hh = lane >> 5, r = lane & 31;
   const S at(lane);
-  const int k_first = w.other_first, m = w.other_n;
-  const int q0 = w.row0 + wave * 32, shift = p.causal ? m - w.n : m;
-  auto seen_by = [&](int row) { return max(0, p.causal ? min(m, row + shift + 1) : m); };
-  const int T = (seen_by(min(w.row0 + NW * 32, w.n) - 1) + 63) >> 6;
+  const int m_all = w.other_n;
+  const int q0 = w.row0 + wave * 32, shift = p.causal ? m_all - w.n : m_all;
+  auto all_seen_by = [&](int row) { return max(0, p.causal ? min(m_all, row + shift + 1) : m_all); };
+  const int T_all = (all_seen_by(min(w.row0 + NW * 32, w.n) - 1) + 63) >> 6;
+  const Share part = SPLIT ? share_of(T_all, share, p.shares) : Share{0, T_all};
+  // from here on keys are those of the share
+  const int T = part.T, k_first = w.other_first + 64 * part.t0, m = SPLIT ? max(0, min(m_all - 64 * part.t0, 64 * T)) : m_all;
+  auto seen_by = [&](int row) { return SPLIT ? max(0, min(m, all_seen_by(row) - 64 * part.t0)) : all_seen_by(row); };
   const int row = min(q0 + r, w.n - 1);
   const int seen = seen_by(row), seen_first = __builtin_amdgcn_readfirstlane(seen);
   const bool live = q0 + r < w.n;
@@ -140,9 +162,9 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
   delta = xhalf_sum(delta);
   const int64_t stat = (int64_t)h * p.T + trow;
   const float M = p.M[stat], L = p.L[stat];
-  const bool sees = seen > 0;
+  const bool sees = all_seen_by(row) > 0;
   const float nl = sees ? -(M + __builtin_amdgcn_logf(L)) / c : -INFINITY, nd = sees ? -delta : 0.f;
-  if (hh == 0 && live) {
+  if (hh == 0 && live && share == 0) {
     float* to = p.stats + (int64_t)h * 2 * p.T + trow;
     to[0] = nl;
     to[p.T] = nd;
@@ -256,6 +278,10 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
     for (; t < T; t++) arrive(t);
     __syncthreads();
   }
+  if constexpr (SPLIT) {   // packed_dq_join_kernel does the rest
+    store_part<D>(smem + wave * (32 * (D * 2 + 16)), acc, p.parts + (((int64_t)share * p.H + h) * p.T + w.first + q0) * D, w.n - q0, lane);
+    return;
+  }
   bf16_t* to = p.dq + h * p.dq_sh + (int64_t)(w.first + q0) * p.dq_sr;
   store_rows<D>(smem + wave * (32 * (D * 2 + 16)), acc, p.scale, to, p.dq_sr, w.n - q0, lane);
   if (p.causal) {
@@ -272,6 +298,34 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
       a.add(p.q + h * p.q_sh + x * p.q_sr, p.g + h * p.g_sh + x * p.g_sr, kp, p.k_sr, vp, p.v_sr, 0, __shfl(seen, i, 64), &nli, &ndi, c);
       a.store(a.a0, p.scale, to + i * p.dq_sr);
     }
+  }
+#endif
+}
+
+// dq of a launch whose workgroups shared keys, from the parts in their order: a lane per four columns.
+template <int D>
+__global__ __launch_bounds__(256) void packed_dq_join_kernel(const PackedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int LPR = D / 4, RPG = 256 / LPR;
+  const int tid = __builtin_amdgcn_workitem_id_x(), column = tid % LPR * 4;
+  const int64_t rows = (int64_t)p.H * p.T, x = (int64_t)__builtin_amdgcn_workgroup_id_x() * RPG + tid / LPR, at = min(x, rows - 1);
+  const int h = (int)(at / p.T), row = (int)(at - (int64_t)h * p.T);
+  uint64_t left = __builtin_amdgcn_ballot_w64(join_part(p.parts + at * D + column, rows * D, p.shares, p.scale, x < rows ? p.dq + h * p.dq_sh + (int64_t)row * p.dq_sr + column : nullptr));
+  if (!p.causal) return;
+  if (left) wait_fills<0>();   // the rows as stored above are written again
+  while (left) {
+    const int i = __builtin_ctzll(left) / LPR * LPR;   // the first lane of a row
+    left &= i + LPR < 64 ? ~0ull << (i + LPR) : 0ull;
+    const int hi = __builtin_amdgcn_readlane(h, i), ri = __builtin_amdgcn_readlane(row, i), hk = hi / p.G;
+    PackedTile w;
+    find_row(p.q_off, p.T, p.k_off, p.Tk, p.B, ri, w);
+    const int seen = max(0, min(w.other_n, w.row0 + w.other_n - w.n + 1));
+    const float* st = p.stats + (int64_t)hi * 2 * p.T + ri;
+    CarefulRow<D, false> a;
+    a.clear();
+    a.add(p.q + hi * p.q_sh + (int64_t)ri * p.q_sr, p.g + hi * p.g_sh + (int64_t)ri * p.g_sr, p.k + hk * p.k_sh + (int64_t)w.other_first * p.k_sr, p.k_sr,
+          p.v + hk * p.v_sh + (int64_t)w.other_first * p.v_sr, p.v_sr, 0, seen, st, st + p.T, p.c);
+    a.store(a.a0, p.scale, p.dq + hi * p.dq_sh + (int64_t)ri * p.dq_sr);
   }
 #endif
 }
@@ -541,8 +595,8 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
   bf16_t* out = ROLE ? p.dk : p.dv;
   if (!out) return;
   if (p.shares > 1) {   // as it is, transposed: packed_dkv_join_kernel does the rest
-    float* part = p.parts + (((int64_t)share * 2 + ROLE) * p.Hkv + hk) * p.Tk * D + (int64_t)(w.first + k0 + r) * D + 4 * hh;
-    if (k0 + r < w.n) {
+    float* part = p.parts + ((((int64_t)share * 2 + ROLE) * p.Hkv + hk) * p.Tk + w.first + k0 + r) * D + 4 * hh;
+    if (k0 + r < w.n) {   // (through LDS, as rows of dq, this spills at head_dim 256)
 #pragma unroll
       for (int m = 0; m < MTD; m++)
 #pragma unroll
@@ -580,39 +634,28 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, D <= 128 ? 2 : 1) void packed_d
 #endif
 }
 
-// dk and dv from the sums of the shares of a launch, in their order: a wave per key and head.
+// dk and dv from the sums of the shares of a launch, in their order: a lane per four columns.
 template <int D>
 __global__ __launch_bounds__(256) void packed_dkv_join_kernel(const PackedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int E = D / 64;
-  const int tid = __builtin_amdgcn_workitem_id_x(), lane = tid & 63;
-  const int64_t x = (int64_t)__builtin_amdgcn_workgroup_id_x() * 4 + __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (x >= (int64_t)p.Hkv * p.Tk) return;
-  const int hk = (int)(x / p.Tk), row = (int)(x - (int64_t)hk * p.Tk);
-  const int64_t plane = (int64_t)p.Hkv * p.Tk * D;
-#pragma unroll
-  for (int role = 0; role < 2; role++) {
-    bf16_t* out = role ? p.dk : p.dv;
-    if (!out) continue;
-    const float* part = p.parts + role * plane + x * D + lane * E;
-    float sum[E] = {};
-    for (int s = 0; s < p.shares; s++)
-#pragma unroll
-      for (int e = 0; e < E; e++) sum[e] += part[2 * s * plane + e];
-    bf16_t* to = out + hk * (role ? p.dk_sh : p.dv_sh) + (int64_t)row * (role ? p.dk_sr : p.dv_sr) + lane * E;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      bad |= not_finite(sum[e]);
-      to[e] = (bf16_t)(sum[e] * (role ? p.scale : 1.f));
-    }
-    if (p.causal && __builtin_amdgcn_ballot_w64(bad)) {
-      wait_fills<0>();   // the row as stored above is written again
-      PackedTile w;
-      find_row(p.k_off, p.Tk, p.q_off, p.T, p.B, row, w);
-      const int from = max(0, w.row0 - (w.n - w.other_n));
-      if (role) careful_key<D, 1>(p, w, hk, w.row0, from); else careful_key<D, 0>(p, w, hk, w.row0, from);
-    }
+  constexpr int LPR = D / 4, RPG = 256 / LPR;
+  const int tid = __builtin_amdgcn_workitem_id_x(), column = tid % LPR * 4, role = __builtin_amdgcn_workgroup_id_y();
+  bf16_t* out = role ? p.dk : p.dv;
+  if (!out) return;
+  const int64_t rows = (int64_t)p.Hkv * p.Tk, x = (int64_t)__builtin_amdgcn_workgroup_id_x() * RPG + tid / LPR, at = min(x, rows - 1);
+  const int hk = (int)(at / p.Tk), row = (int)(at - (int64_t)hk * p.Tk);
+  bf16_t* to = out + hk * (role ? p.dk_sh : p.dv_sh) + (int64_t)row * (role ? p.dk_sr : p.dv_sr) + column;
+  uint64_t left = __builtin_amdgcn_ballot_w64(join_part(p.parts + (role * rows + at) * D + column, 2 * rows * D, p.shares, role ? p.scale : 1.f, x < rows ? to : nullptr));
+  if (!p.causal) return;
+  if (left) wait_fills<0>();   // the rows as stored above are written again
+  while (left) {
+    const int i = __builtin_ctzll(left) / LPR * LPR;   // the first lane of a row
+    left &= i + LPR < 64 ? ~0ull << (i + LPR) : 0ull;
+    const int hi = __builtin_amdgcn_readlane(hk, i), ri = __builtin_amdgcn_readlane(row, i);
+    PackedTile w;
+    find_row(p.k_off, p.Tk, p.q_off, p.T, p.B, ri, w);
+    const int from = max(0, w.row0 - (w.n - w.other_n));
+    if (role) careful_key<D, 1>(p, w, hi, w.row0, from); else careful_key<D, 0>(p, w, hi, w.row0, from);
   }
 #endif
 }
@@ -631,32 +674,54 @@ static int dkv_shares(const PackedParams& p) {
   return n < 2 ? 1 : n > 64 ? 64 : (int)n;
 }
 
-template <int D>
-static int launch_bwd(PackedParams p, void* workspace, hipStream_t s) {
-  constexpr int NW = 4, DQ_LDS = dq_lds<D>(NW), DKV_LDS = Dkv<D>::bytes();
+template <int D, bool SPLIT>
+static int launch_dq(PackedParams p, hipStream_t s) {
+  constexpr int NW = 4, LDS = dq_lds<D>(NW);
   p.slots = (int)packed_slots(p.T, p.B, NW * 32);
-  p.shares = dkv_shares<D>(p);
-  p.stats = (float*)workspace;
-  p.parts = p.stats + ((int64_t)p.H * 2 * p.T + 3) / 4 * 4;
-  const int64_t q_groups = (int64_t)p.slots * p.H, k_groups = packed_slots(p.Tk, p.B, Dkv<D>::KEYS) * p.Hkv * p.shares, joins = ((int64_t)p.Hkv * p.Tk + 3) / 4;
-  if (q_groups * (NW * 64) > 0xffffffffll || k_groups * (Dkv<D>::WAVES * 64) > 0xffffffffll || joins * 256 > 0xffffffffll) return LVAR_EINVAL;
-  auto dq = packed_dq_kernel<D, NW>;
-  auto dkv = packed_dkv_kernel<D>;
-  static std::atomic<uint64_t> ready_q{0}, ready_k{0};
-  if (!ensure_lds_limit((const void*)dq, DQ_LDS, ready_q) || !ensure_lds_limit((const void*)dkv, DKV_LDS, ready_k)) return LVAR_ELAUNCH;
-  hipLaunchKernelGGL(dq, dim3((uint32_t)q_groups), dim3(NW * 64), DQ_LDS, s, p);
+  const int64_t groups = (int64_t)p.slots * p.H * p.shares, joins = ((int64_t)p.H * p.T * (D / 4) + 255) / 256;
+  if (groups * (NW * 64) > 0xffffffffll || joins * 256 > 0xffffffffll) return LVAR_EINVAL;
+  auto kern = packed_dq_kernel<D, NW, SPLIT>;
+  static std::atomic<uint64_t> ready{0};
+  if (!ensure_lds_limit((const void*)kern, LDS, ready)) return LVAR_ELAUNCH;
+  hipLaunchKernelGGL(kern, dim3((uint32_t)groups), dim3(NW * 64), LDS, s, p);
   if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
-  if (!p.dk && !p.dv) return LVAR_OK;
-  hipLaunchKernelGGL(dkv, dim3((uint32_t)k_groups), dim3(Dkv<D>::WAVES * 64), DKV_LDS, s, p);
-  if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
-  if (p.shares > 1 && joins > 0) hipLaunchKernelGGL(packed_dkv_join_kernel<D>, dim3((uint32_t)joins), dim3(256), 0, s, p);
+  if (SPLIT && joins > 0) hipLaunchKernelGGL(packed_dq_join_kernel<D>, dim3((uint32_t)joins), dim3(256), 0, s, p);
   return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
 }
 
-// statistics of the rows, and the sums of shares
+template <int D>
+static int launch_dkv(PackedParams p, hipStream_t s) {
+  constexpr int LDS = Dkv<D>::bytes();
+  const int64_t groups = packed_slots(p.Tk, p.B, Dkv<D>::KEYS) * p.Hkv * p.shares, joins = ((int64_t)p.Hkv * p.Tk * (D / 4) + 255) / 256;
+  if (groups * (Dkv<D>::WAVES * 64) > 0xffffffffll || joins * 256 > 0xffffffffll) return LVAR_EINVAL;
+  auto kern = packed_dkv_kernel<D>;
+  static std::atomic<uint64_t> ready{0};
+  if (!ensure_lds_limit((const void*)kern, LDS, ready)) return LVAR_ELAUNCH;
+  hipLaunchKernelGGL(kern, dim3((uint32_t)groups), dim3(Dkv<D>::WAVES * 64), LDS, s, p);
+  if (hipGetLastError() != hipSuccess) return LVAR_ELAUNCH;
+  if (p.shares > 1 && joins > 0) hipLaunchKernelGGL(packed_dkv_join_kernel<D>, dim3((uint32_t)joins, 2), dim3(256), 0, s, p);
+  return hipGetLastError() == hipSuccess ? LVAR_OK : LVAR_ELAUNCH;
+}
+
+// dq needs no shares where only its statistics are wanted
+static int dq_shares(const PackedParams& p, int head_dim, bool wanted) { return wanted ? query_shares(p, head_dim <= 128 ? 2 : 1) : 1; }
+
+template <int D>
+static int launch_bwd(PackedParams p, void* workspace, hipStream_t s) {
+  p.stats = (float*)workspace;
+  p.parts = p.stats + ((int64_t)p.H * 2 * p.T + 3) / 4 * 4;
+  p.shares = dq_shares(p, D, p.dq != nullptr);
+  const int st = p.shares > 1 ? launch_dq<D, true>(p, s) : launch_dq<D, false>(p, s);
+  if (st != LVAR_OK || (!p.dk && !p.dv)) return st;
+  p.shares = dkv_shares<D>(p);
+  return launch_dkv<D>(p, s);
+}
+
+// statistics of the rows, and the sums of shares, of dq first and then of dk and dv
 int64_t packed_bwd_bytes(const PackedParams& p, int head_dim) {
-  const int shares = head_dim == 64 ? dkv_shares<64>(p) : head_dim == 128 ? dkv_shares<128>(p) : dkv_shares<256>(p);
-  return 4 * (((int64_t)p.H * 2 * p.T + 3) / 4 * 4 + (shares > 1 ? (int64_t)shares * 2 * p.Hkv * p.Tk * head_dim : 0));
+  const int q = dq_shares(p, head_dim, true), k = head_dim == 64 ? dkv_shares<64>(p) : head_dim == 128 ? dkv_shares<128>(p) : dkv_shares<256>(p);
+  const int64_t of_q = q > 1 ? (int64_t)q * p.H * p.T * head_dim : 0, of_k = k > 1 ? (int64_t)k * 2 * p.Hkv * p.Tk * head_dim : 0;
+  return 4 * (((int64_t)p.H * 2 * p.T + 3) / 4 * 4 + (of_q > of_k ? of_q : of_k));
 }
 
 int launch_packed_bwd(PackedParams p, void* workspace, int head_dim, hipStream_t s) {

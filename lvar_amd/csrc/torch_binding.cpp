@@ -48,7 +48,7 @@ namespace {
   X(lvar_kv_cache_read) X(lvar_paged_attn_workspace_bytes) X(lvar_paged_attn_fwd)                                         \
   X(lvar_qk_norm_axes_fwd) X(lvar_qk_norm_axes_bwd_scratch_bytes) X(lvar_qk_norm_axes_bwd) X(lvar_kv_cache_append_axes)   \
   X(lvar_kv_pages_scratch_bytes) X(lvar_kv_pages_alloc) X(lvar_kv_pages_free) X(lvar_kv_cache_fork) X(lvar_kv_cache_compact) \
-  X(lvar_packed_attn_fwd) X(lvar_packed_attn_bwd_workspace_bytes) X(lvar_packed_attn_bwd)
+  X(lvar_packed_attn_fwd_workspace_bytes) X(lvar_packed_attn_fwd) X(lvar_packed_attn_bwd_workspace_bytes) X(lvar_packed_attn_bwd)
 struct Api {
 #define LVAR_FIELD(name) decltype(&::name) name = nullptr;
   LVAR_ENTRIES(LVAR_FIELD)
@@ -985,8 +985,12 @@ int packed_forward(const PackedCall& x, at::Tensor& o, at::Tensor& M, at::Tensor
   Qkv sizes{};
   sizes.B = 1; sizes.H = H; sizes.Lq = T; sizes.dev = dev;
   empty_stats(sizes, M, L);
+  const int B = dim(*x.off, 0) - 1, Tk = dim(*x.k, 2), Hkv = dim(*x.k, 1), d = dim(*x.q, 3);
+  const int64_t bytes = api.lvar_packed_attn_fwd_workspace_bytes(B, T, Tk, H, Hkv, d, x.causal);
+  at::Tensor ws;
+  if (bytes > 0) ws = empty({bytes}, at::kByte, dev);
   return api.lvar_packed_attn_fwd(packed_view(*x.q), packed_view(*x.k), packed_view(*x.v), packed_view(o), x.off->data_ptr<int32_t>(), x.k_off->data_ptr<int32_t>(),
-                                  M.data_ptr<float>(), L.data_ptr<float>(), dim(*x.off, 0) - 1, T, dim(*x.k, 2), H, dim(*x.k, 1), dim(*x.q, 3), x.causal, x.scale,
+                                  M.data_ptr<float>(), L.data_ptr<float>(), bytes > 0 ? ws.data_ptr() : nullptr, bytes > 0 ? bytes : 0, B, T, Tk, H, Hkv, d, x.causal, x.scale,
                                   c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream());
 }
 

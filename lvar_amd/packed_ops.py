@@ -58,9 +58,12 @@ def _launch(q, k, v, offsets, k_offsets, causal, scale):
     o = _like(q)
     M, L = torch.empty((2, 1, H, T, 1), dtype=torch.float32, device=q.device).unbind(0)
     if o.numel():
+        lib, sizes = _lib.load(), (offsets.shape[0] - 1, T, k.shape[2], H, k.shape[1], d, 1 if causal else 0)
         with _on_device(q):
-            st = _lib.load().lvar_packed_attn_fwd(_view(q), _view(k), _view(v), _view(o), offsets.data_ptr(), k_offsets.data_ptr(), M.data_ptr(), L.data_ptr(),
-                                                 offsets.shape[0] - 1, T, k.shape[2], H, k.shape[1], d, 1 if causal else 0, scale, _stream(q))
+            nbytes = max(0, int(lib.lvar_packed_attn_fwd_workspace_bytes(*sizes)))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+            st = lib.lvar_packed_attn_fwd(_view(q), _view(k), _view(v), _view(o), offsets.data_ptr(), k_offsets.data_ptr(), M.data_ptr(), L.data_ptr(),
+                                          _ptr(ws), nbytes, *sizes, scale, _stream(q))
         _lib.check(st, "lvar_packed_attn_fwd")
     return o, M, L
 

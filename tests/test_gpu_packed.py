@@ -65,6 +65,13 @@ CASES = [
     ([700, 40], None, 8, 1, 128, True, 1, 0),
     ([310], None, 8, 1, 256, True, 0, 0),
     ([70], None, 2, 2, 32, False, 0, 0),
+    # several workgroups share the keys of a query tile
+    ([3100], None, 2, 1, 64, True, 0, 0),
+    ([600, 7, 150], [6700, 0, 5300], 2, 2, 128, True, 3, 1),
+    ([140], [3090], 1, 1, 256, True, 0, 2),
+    ([9, 1, 0], [2500, 3000, 70], 6, 2, 128, False, 0, 0),
+    ([9, 140], [3900, 2300], 2, 1, 64, True, 0, 0),
+    ([200, 1], [130, 7000], 1, 1, 256, True, 0, 0),                   # (one sequence has far more keys than the mean, one has rows without any)
 ]
 
 

@@ -55,6 +55,9 @@ BAD = [
     ([60, 60], [70, 90], 1, 1, 128, False),
     ([600], [70], 1, 1, 64, True),          # (rows that see nothing; several workgroups share the keys)
     ([300], None, 4, 1, 128, True),         # (so they do here)
+    ([70, 3], [3300, 3000], 1, 1, 64, True),     # (several workgroups share the keys of a query tile)
+    ([9], [3100], 2, 1, 256, True),
+    ([33, 8], [900, 2900], 1, 1, 128, False),
 ]
 
 
@@ -104,7 +107,7 @@ def run(q, k, v, off, koff, go, **kw):
     return [o.detach(), M, L, *torch.autograd.grad(o, leaves, go)]
 
 
-SETS = [([300, 0, 41, 500], None, 4, 2, 128, True), ([1000, 400], [60, 10], 4, 4, 64, False), ([260], None, 8, 1, 256, True)]
+SETS = [([300, 0, 41, 500], None, 4, 2, 128, True), ([1000, 400], [60, 10], 4, 4, 64, False), ([260], None, 8, 1, 256, True), ([20, 1400], [1700, 4700], 2, 1, 128, True)]
 
 
 @pytest.mark.parametrize("case", SETS, ids=str)

@@ -98,7 +98,7 @@ def call(lib, name, **change):
     sizes = [a[n] for n in ("batch", "tokens", "k_tokens", "H", "kv_heads", "head_dim", "causal")]
     stats = [C.c_void_p(a[n] or None) for n in ("offsets", "k_offsets", "M", "L")]
     if name == "fwd":
-        return lib.lvar_packed_attn_fwd(*map(view, ("q", "k", "v", "o")), *stats, *sizes, a["scale"], None)
+        return lib.lvar_packed_attn_fwd(*map(view, ("q", "k", "v", "o")), *stats, C.c_void_p(a["workspace"] or None), a["workspace_bytes"], *sizes, a["scale"], None)
     return lib.lvar_packed_attn_bwd(*map(view, ("q", "k", "v", "o", "go")), *stats, *map(view, ("dq", "dk", "dv")), C.c_void_p(a["workspace"] or None),
                                     a["workspace_bytes"], *sizes, a["scale"], None)
 
@@ -122,3 +122,5 @@ def test_workspace(lib):
     for bad in (dict(batch=0), dict(tokens=-1), dict(k_tokens=-1), dict(H=3), dict(kv_heads=0)):
         assert size(**bad) == -1
     assert size(head_dim=80) == -2
+    fwd = lib.lvar_packed_attn_fwd_workspace_bytes
+    assert fwd(2, 8, 8, 4, 2, 128, 1) == 0 and fwd(0, 8, 8, 4, 2, 128, 1) == -1 and fwd(2, 8, 8, 4, 2, 96, 1) == -2
