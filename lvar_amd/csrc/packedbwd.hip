@@ -353,13 +353,27 @@ struct Dkv {
   static constexpr int SUB = D == 256 ? 1 : 2, R = 32 * SUB, TILE = R * D * 2;    // 32-row blocks and rows of a tile, its bytes
   // tiles of q: t-1 .. t+1 are in use, of do: t
   static constexpr int LEAD = D == 256 ? 2 : 1, Q_RING = LEAD + 3, G_RING = LEAD + 1;
-  static constexpr int G_AT = Q_RING * TILE, P_AT = G_AT + G_RING * TILE, P_WAVE = R * 32 * 2;   // P: [parity][pair]
+  static constexpr int G_AT = Q_RING * TILE, P_AT = G_AT + G_RING * TILE, P_WAVE = R * 32 * 3;   // P: [parity][pair], 24 bits each
   static constexpr int STAT_AT = P_AT + 2 * KW * P_WAVE, STAT_WAVE = Q_RING * 256;               // statistics: [wave][place in the ring]
   static constexpr int OUT = WAVES * 32 * (D * 2 + 16);
   static constexpr int bytes() { return STAT_AT + WAVES * STAT_WAVE > OUT ? STAT_AT + WAVES * STAT_WAVE : OUT; }
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
+
+// P passes between two waves as the upper 24 bits of its fp32: 16 of two elements to a word, the next 8 of four to another.  (As bf16
+// dk is off by 0.0030 of its size instead of 0.0025, which is as far as dq; rounded once, at its end, it would be by 0.0017.  It costs 5 % of the kernel at head_dim
+// 128, 15 % at 64: 272 -> 286 us, 53 -> 61 us.)
+__device__ __forceinline__ uint32_t word(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ __forceinline__ uint32_t upper16(float a, float b) { return __builtin_amdgcn_perm(word(b), word(a), 0x07060302u); }
+__device__ __forceinline__ uint32_t next8(float a, float b, float c, float d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(word(d), word(c), 0x0c0c0501u), __builtin_amdgcn_perm(word(b), word(a), 0x0c0c0501u), 0x05040100u);
+}
+// element E of a group of eight
+template <int E>
+__device__ __forceinline__ float unpack24(uint32_t upper, uint32_t next) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_perm(upper, next, (E & 1 ? 0x07060000u : 0x05040000u) | (E & 3) << 8 | 0x0cu));
+}
 
 // the first of N elements in slot g: three quarters over the NS steps of the first product, the others over the first HB of the second
 template <int N, int NS, int HB>
@@ -499,9 +513,12 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
     auto round = [&](int t, auto first, auto second, f32x16 (&s)[SUB], f32x16 (&nx)[SUB]) {
       constexpr bool FIRST = decltype(first)::value, SECOND = decltype(second)::value;
       const uint32_t rows = row_at + r_pl, cols = col_at + c_pl, pt = p_at + (t & 1) * Q::KW * Q::P_WAVE;
+      const uint32_t pt8 = pt + Q::R * 64 - lane * 8;
       bf16x8 frag[NT];
       uint32_t pw[8 * SUB];   // P or dS, packed
-      u32x4 pin[2 * SUB];     // P from the other wave
+      uint32_t up[4], lo[2];  // P for the other wave
+      u32x4 pin[2 * SUB];     // and from it
+      u32x2 pin8[2 * SUB];
       auto operand = [&](auto ic) {
         constexpr int i = decltype(ic)::value;
         if constexpr (i < NS) { if constexpr (FIRST) frag[i] = P::rows(rows + i % SUB * 32 * S::ROWB, i / SUB); }
@@ -512,9 +529,14 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
       static_assert(Sch::lo(NS - 2) >= 8 && Sch::lo(NS + MTD - 2) >= 16 && (SUB == 1 || (Sch::lo(NS + 2 * MTD - 2) >= 24 && Sch::lo(NS + 3 * MTD - 2) >= 32)));
       auto finish = [&](auto ec) {
         constexpr int e = decltype(ec)::value;
-        if constexpr (ROLE == 1) s[e / 16][e % 16] *= (e & 1) ? bf16_hi(pin[e / 8][e % 8 / 2]) : bf16_lo(pin[e / 8][e % 8 / 2]);
+        if constexpr (ROLE == 1) s[e / 16][e % 16] *= unpack24<e % 8>(pin[e / 8][e % 8 / 2], pin8[e / 8][e % 8 / 4]);
         if constexpr (e & 1) pw[e >> 1] = pack_bf16(s[e / 16][e % 16 - 1], s[e / 16][e % 16]);
-        if constexpr (ROLE == 0 && e % 8 == 7) *(LVAR_LDS u32x4*)(uintptr_t)(pt + e / 8 * 1024) = u32x4{pw[e / 2 - 3], pw[e / 2 - 2], pw[e / 2 - 1], pw[e / 2]};
+        if constexpr (ROLE == 0 && e % 2 == 1) up[e % 8 / 2] = upper16(s[e / 16][e % 16 - 1], s[e / 16][e % 16]);
+        if constexpr (ROLE == 0 && e % 4 == 3) lo[e % 8 / 4] = next8(s[e / 16][e % 16 - 3], s[e / 16][e % 16 - 2], s[e / 16][e % 16 - 1], s[e / 16][e % 16]);
+        if constexpr (ROLE == 0 && e % 8 == 7) {
+          *(LVAR_LDS u32x4*)(uintptr_t)(pt + e / 8 * 1024) = u32x4{up[0], up[1], up[2], up[3]};
+          *(LVAR_LDS u32x2*)(uintptr_t)(pt8 + e / 8 * 512) = u32x2{lo[0], lo[1]};
+        }
       };
       auto slot = [&](auto gc) {
         constexpr int g = decltype(gc)::value;
@@ -528,7 +550,10 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
       };
       if constexpr (ROLE == 1 && SECOND) {
 #pragma unroll
-        for (int i = 0; i < 2 * SUB; i++) pin[i] = *(LVAR_LDS const u32x4*)(uintptr_t)(pt + i * 1024);
+        for (int i = 0; i < 2 * SUB; i++) {
+          pin[i] = *(LVAR_LDS const u32x4*)(uintptr_t)(pt + i * 1024);
+          pin8[i] = *(LVAR_LDS const u32x2*)(uintptr_t)(pt8 + i * 512);
+        }
       }
       if constexpr (FIRST) starts(nx);
       static_for<FIRST ? 0 : NS, (FIRST ? 0 : NS) + AHEAD>(operand);
