@@ -518,7 +518,7 @@ int lvar_kv_cache_read(lvar_paged_cache_t cache, const int32_t* start, const int
  * scratch: lvar_kv_pages_scratch_bytes(forks, num_pages), of lvar_kv_pages_alloc with forks = 0 (4-byte aligned, needs no preparation; may be 0).
  *   lvar_kv_cache_compact token i < n (counts[b], NULL: all n) of head h of the pages of out_table's row b gets the bytes of token
  *                         keep[b, h, i] (int32, or int64 if keep64; strides in elements) of page_table's row b; zeros where that names no token.
- *                         A page that both tables name is undefined.
+ *                         A page that both tables name, or out_table twice, is undefined.
  */
 int64_t lvar_kv_pages_scratch_bytes(int forks, int num_pages);
 int lvar_kv_pages_alloc(int32_t* refs, int num_pages, int32_t* page_table, int64_t table_stride, int rows, int max_pages, const int32_t* first,

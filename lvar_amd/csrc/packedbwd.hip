@@ -113,7 +113,10 @@ struct DqSlots {
 // ---- dq: 32 query rows per wave, steps of 32 keys.  S^T and dP^T = V do^T with the rows of q and do as B operands in registers, so a lane
 // owns a query column, and dS^T is in the B operand's layout of dq^T += K^T dS^T as it is.  A step forms S and dP of the coming 32 keys on the
 // matrix cores while the vector ALU turns those of the present ones into dS, and adds them.  The barrier of a tile of 64 keys lies between its
-// two steps' products: the first S of the next tile is formed beside the second dS of this one, whose keys stay (hence three buffers). ----
+// two steps' products: the first S of the next tile is formed beside the second dS of this one, whose keys stay (hence three buffers).
+// 12 sequences of up to 2047 tokens, 32 heads over 8 of 128, causal: 244 us with a step's products, vector work and sums one behind the other, 228 so,
+// 222 without tiles that none of a wave's rows sees: 810 TFLOP/s, matrix cores busy 48 % of the cycles.  16384 rows of 16 heads of 64 over 811 keys in
+// four texts: 46 -> 44 us. ----
 
 template <int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(const PackedParams p) {
@@ -343,7 +346,7 @@ __global__ __launch_bounds__(256) void packed_dq_join_kernel(const PackedParams 
 //
 // Tiles come from the last rows to the first, all heads of a tile behind each other: the workgroups of a sequence, which all end at
 // its last rows, read the same tile at about the same time, from the L2 (from the first rows on, 71 % of the reads missed it); half of the reads
-// still come from further away, so tiles are requested LEAD rounds ahead. ----
+// still come from further away, so tiles are requested LEAD rounds ahead.  The same sequences 286 us, 835 TFLOP/s, matrix cores busy 50 %. ----
 
 template <int D>
 struct Dkv {
@@ -686,15 +689,15 @@ __global__ __launch_bounds__(256) void packed_dkv_join_kernel(const PackedParams
 }
 
 // Workgroups that share the query rows of a key tile, where the key tiles alone leave compute units idle (few keys under many rows, or one key
-// head under many query heads): as many as give each unit one, twice that if causal, where the first tile has twice the work of the mean one;
+// head under many query heads): as many as give each unit one (head_dim 64, where it holds two: two), twice that if causal, where the first tile has twice the work of the mean one;
 // none gets fewer than SHARE_TILES tiles of an average sequence.  Against one workgroup per tile, the sum of the parts included: 4096 rows of
 // 8 heads over one key head of 128, causal 697 -> 102 us (half as many shares 133); of 256 976 -> 192 us; two of 2048 of 8 over 2 heads of 64
-// 90 -> 48 us; 16384 rows of 16 heads of 128 over 77 keys 353 -> 52 us.
+// 90 -> 46 us (one a unit: 53); 16384 rows of 16 heads of 128 over 77 keys 353 -> 52 us, of 64 over 811 in four texts 62 -> 57 us.
 template <int D>
 static int dkv_shares(const PackedParams& p) {
   constexpr int SHARE_TILES = 8;
   const int64_t groups = ((int64_t)p.Tk / Dkv<D>::KEYS + p.B) * p.Hkv, cus = device_cus(), tiles = (int64_t)p.T / p.B * p.G / Dkv<D>::R / (p.causal ? 2 : 1);
-  const int64_t most = tiles / SHARE_TILES, want = (p.causal ? 2 : 1) * cus / (groups > 0 ? groups : 1);
+  const int64_t most = tiles / SHARE_TILES, want = (p.causal ? 2 : 1) * (D == 64 ? 2 : 1) * cus / (groups > 0 ? groups : 1);
   const int64_t n = want < most ? want : most;
   return n < 2 ? 1 : n > 64 ? 64 : (int)n;
 }
@@ -704,7 +707,7 @@ static int launch_dq(PackedParams p, hipStream_t s) {
   constexpr int NW = 4, LDS = dq_lds<D>(NW);
   p.slots = (int)packed_slots(p.T, p.B, NW * 32);
   const int64_t groups = (int64_t)p.slots * p.H * p.shares, joins = ((int64_t)p.H * p.T * (D / 4) + 255) / 256;
-  if (groups * (NW * 64) > 0xffffffffll || joins * 256 > 0xffffffffll) return LVAR_EINVAL;
+  if (groups * (NW * 64) > 0xffffffffll || (SPLIT && joins * 256 > 0xffffffffll)) return LVAR_EINVAL;
   auto kern = packed_dq_kernel<D, NW, SPLIT>;
   static std::atomic<uint64_t> ready{0};
   if (!ensure_lds_limit((const void*)kern, LDS, ready)) return LVAR_ELAUNCH;
@@ -718,7 +721,7 @@ template <int D>
 static int launch_dkv(PackedParams p, hipStream_t s) {
   constexpr int LDS = Dkv<D>::bytes();
   const int64_t groups = packed_slots(p.Tk, p.B, Dkv<D>::KEYS) * p.Hkv * p.shares, joins = ((int64_t)p.Hkv * p.Tk * (D / 4) + 255) / 256;
-  if (groups * (Dkv<D>::WAVES * 64) > 0xffffffffll || joins * 256 > 0xffffffffll) return LVAR_EINVAL;
+  if (groups * (Dkv<D>::WAVES * 64) > 0xffffffffll || (p.shares > 1 && joins * 256 > 0xffffffffll)) return LVAR_EINVAL;
   auto kern = packed_dkv_kernel<D>;
   static std::atomic<uint64_t> ready{0};
   if (!ensure_lds_limit((const void*)kern, LDS, ready)) return LVAR_ELAUNCH;

@@ -1,6 +1,9 @@
 // The life of the pages of a cache: dropping, opening and forking the pages that a table names, with a count of names per page, and copying chosen
 // tokens of a sequence to other pages.  Nothing of it comes from the host: a step captured in a graph is replayed with other lengths.
 //
+// All of it is latency: 192 samples of 48 prompts (240 rows, 1500 pages) drop 2.8, search 4.9, fork 7.5 (50 MB read and written), open 5.4 us; 4 samples of
+// one 2.5 + 3.4 + 3.4 + 2.9.
+//
 // Which free page (refs <= 0) a call hands out is fixed: the lowest ones, in the order of rows and entries.  One workgroup finds them: it adds up
 // what the rows want, scans the counts until it has as many, and deals them out.  Counts change by integer additions, whose order does not matter.
 #include "kvcache.h"
@@ -214,7 +217,8 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(const PagesParams p, co
 }
 
 // Token i of a head in the pages of `out`: token keep[b, head, i] of `c`, as its bytes are.  A row is read by `1 << per` lanes, 16 bytes each of
-// key and value.
+// key and value.  Bound by memory, and by its round trips (table and position, then the row) where it is small: 2 x 16 heads keep 1052 of 10521 tokens of
+// 128 in bf16 7.3 us, 4.7 TB/s; 8 x 8 heads up to 4001 of 8191 in e4m3 15.6 us, 3.4 TB/s of rows of 128 bytes.
 __global__ __launch_bounds__(256) void pages_compact_kernel(const CompactParams p, const int per) {
   const int lane = threadIdx.x & ((1 << per) - 1), i = (blockIdx.x << (8 - per)) + (threadIdx.x >> per);
   const int head = blockIdx.y, b = blockIdx.z;

@@ -1,7 +1,8 @@
 """Operators around a growing key/value cache: norms of queries and keys per head with the position rotation in the same pass
-(:func:`qk_norm_rope`, differentiable), a paged cache of bf16 or 8-bit keys and values (:class:`PagedKVCache`,
-:func:`kv_cache_append`, :func:`qk_norm_rope_append`, :func:`kv_cache_read`) and the attention of the newest tokens over it
-(:func:`paged_attn`).
+(:func:`qk_norm_rope`, differentiable; by tables, or by positions on several axes with :func:`axis_freqs`), a paged cache of bf16 or 8-bit keys and
+values (:class:`PagedKVCache`, :func:`kv_cache_append`, :func:`qk_norm_rope_append`, :func:`kv_cache_read`), the attention of the newest tokens over it
+(:func:`paged_attn`), and the life of its pages: opening, dropping and forking them (:func:`kv_pages_alloc`, :func:`kv_pages_free`,
+:func:`kv_cache_fork`) and keeping a part of each sequence (:func:`kv_cache_compact`).
 
 They stand between a model's fused projection and the attention operators of :mod:`lvar_amd.sparse_attn_ops`: the reference
 normalises, rotates and concatenates in eager PyTorch around every attention call (models/sparvar/basic_sparvar.py:326-350).
@@ -544,7 +545,7 @@ def kv_cache_compact(cache: PagedKVCache, page_table, keep, out_table, counts=No
     int32 ``[B, max_pages]``), as its bytes are, for the first ``counts[b]`` (int32 ``[B]``; default: all) of the n that ``keep`` (int32 or
     int64 ``[B, kv_heads, n]``; a broadcast one is read in place) lists: what :func:`lvar_amd.sparse_attn_ops.scalekv_keep_indices` selects, every
     head other tokens.  Tokens that ``page_table`` does not name become zeros; places that ``out_table`` does not name are not written.  A page
-    that both tables name is left undefined: open new pages (:func:`kv_pages_alloc`) and give the old ones back afterwards."""
+    that both tables name, or ``out_table`` twice, is left undefined: open new pages (:func:`kv_pages_alloc`) and give the old ones back afterwards."""
     fast = _native()
     if fast is not None and fast.fast_cache_compact(cache, page_table, keep, out_table, counts):
         return
