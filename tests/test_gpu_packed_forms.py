@@ -328,3 +328,40 @@ def test_gradients_against_differences():
         # (the error of the difference itself: eps^2 of the third derivative, and 2^-52 of the sum over eps)
         tol = float((r["t_" + name] * step.abs()).sum()) + 1e-6 * float((r[name].abs() * step.abs()).sum())
         assert abs(float((got[i] * step).sum()) - slope) <= tol
+
+
+def test_many_tokens(host_path):
+    """2.2 million tokens of 20000 sequences that are alike: elements beyond 31 bits, heads that are copied because they span 2^31 bytes; every sequence
+    has the bits of one alone."""
+    H, n, B, d = 8, 110, 20000, 128
+    one = [rand(1, h, n, d, seed=i).cuda() for i, h in enumerate((H, 1, 1, H))]
+    want = run(*one[:3], i32([0, n]), None, one[3])
+    many = [t.transpose(1, 2).repeat(1, B, 1, 1).transpose(1, 2) for t in one]      # [1,h,T,d], tokens first
+    got = run(*many[:3], torch.arange(B + 1, dtype=torch.int32, device="cuda") * n, None, many[3])
+    for a, b in zip(got, want):
+        a = a.view(*a.shape[:2], B, n, a.shape[3]) if a.is_contiguous() else a.transpose(1, 2).view(1, B, n, a.shape[1], a.shape[3]).permute(0, 3, 1, 2, 4)
+        assert bool((a == b[:, :, None]).all())
+
+
+def test_workspace_that_is_too_small():
+    """Where the keys of a query tile are shared, the entry point wants room for the parts."""
+    import ctypes as C
+    from lvar_amd import _lib
+    lib = _lib.load()
+    T, Tk, d = 64, 8192, 128
+    sizes = (1, T, Tk, 1, 1, d, 0)
+    need = lib.lvar_packed_attn_fwd_workspace_bytes(*sizes)
+    assert need > 0
+    q, k = rand(1, 1, T, d).cuda(), rand(1, 1, Tk, d, seed=1).cuda()
+    o, st = torch.zeros_like(q), torch.zeros(2, T, device="cuda")
+    ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    view = lambda t: _lib.LvarTensor(t.data_ptr(), 0, 0, d)  # noqa: E731
+    ptr = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    off, koff = i32([0, T]), i32([0, Tk])
+    call = lambda w, n: lib.lvar_packed_attn_fwd(view(q), view(k), view(k), view(o), ptr(off), ptr(koff), ptr(st[0]), ptr(st[1]), w, n, *sizes, 0.1,  # noqa: E731
+                                                 C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert call(None, need) == -1 and call(ptr(ws), need - 1) == -1 and call(C.c_void_p(ws.data_ptr() + 8), need) == -1
+    assert bool((o == 0).all())
+    assert call(ptr(ws), need) == 0
+    torch.cuda.synchronize()
+    assert bool((o != 0).any())
