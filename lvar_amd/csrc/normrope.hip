@@ -528,7 +528,7 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const WeightGradParam
 
 // ---- tables of the angles of a call ----
 
-// A large backward pass reads cosines and sines from tables that a launch ahead of it writes to scratch memory, with the row of every token: the
+// A large backward pass reads cosines and sines from tables that a launch ahead of it writes to scratch memory, with the row of every token where sequences differ: the
 // angles are formed once, not once per pair of heads.  Formed in place / from tables, both launches, 32 + 8 heads of 128 with three axes, pairs of
 // neighbours: 410 tokens 12.2 / 14.7 us, 3280 34.5 / 36.0, 8192 65.5 / 64.2, 32768 285 / 266; of halves 12.3 / 14.9, 35.3 / 35.3, 68.1 / 65.0, 308 / 277.
 // The forward launches, whose workgroups form them for four heads and do not loop, gain nothing (2 x 32 heads of 4096 into a cache 39.7 / 41.1).
@@ -536,7 +536,7 @@ __global__ __launch_bounds__(NR_T) void axis_tables_kernel(const NormRopeParams 
   const int quads = p.rot >> 3;                                  // of pairs
   const int64_t at = (int64_t)blockIdx.x * NR_T + threadIdx.x;
   const int64_t r = at / quads;
-  if (at < (int64_t)p.B * p.L) row_of[at] = rows == p.L ? (int)(at % p.L) : (int)at;
+  if (row_of && at < rows) row_of[at] = (int)at;
   if (r >= rows) return;
   const int q = (int)(at - r * quads), b = (int)(r / p.L), i = (int)(r - (int64_t)b * p.L);
   float s[4], c[4];
@@ -549,15 +549,15 @@ static int64_t axis_rows(const NormRopeParams& p) { return p.pos_sb ? (int64_t)p
 
 int64_t axis_table_bytes(const NormRopeParams& p) {
   if ((int64_t)p.B * p.L * (p.H + p.Hkv) < AXIS_TABLE_ROWS) return 0;
-  return axis_rows(p) * p.rot * 4 + (int64_t)p.B * p.L * 4;
+  return axis_rows(p) * p.rot * 4 + (p.pos_sb ? (int64_t)p.B * p.L * 4 : 0);
 }
 
 // Writes the tables and turns p into a call that reads them.
 int launch_axis_tables(NormRopeParams& p, void* scratch, hipStream_t s) {
-  const int64_t rows = axis_rows(p), half = p.rot >> 1, tokens = (int64_t)p.B * p.L;
+  const int64_t rows = axis_rows(p), half = p.rot >> 1;
   float *cos = (float*)scratch, *sin = cos + rows * half;
-  int32_t* row_of = (int32_t*)(sin + rows * half);
-  const int64_t threads = rows * (half >> 2) > tokens ? rows * (half >> 2) : tokens, groups = (threads + NR_T - 1) / NR_T;
+  int32_t* row_of = p.pos_sb ? (int32_t*)(sin + rows * half) : nullptr;   // (without, a token's row is its number: 250 us instead of 262 for the largest call above)
+  const int64_t groups = (rows * (half >> 2) + NR_T - 1) / NR_T;
   if (!grid_fits(groups, NR_T)) return LVAR_EINVAL;
   hipLaunchKernelGGL(axis_tables_kernel, dim3((uint32_t)groups), dim3(NR_T), 0, s, p, cos, sin, row_of, (int)rows);
   p.cos = cos; p.sin = sin; p.cs_row = half; p.table_rows = (int)rows;
