@@ -148,6 +148,17 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
   const int64_t trow = w.first + row;
   const float c = p.c;
 
+  // the first tile is requested ahead of the rows, so that one latency covers both
+  const bf16_t *kp = p.k + hk * p.k_sh + (int64_t)k_first * p.k_sr, *vp = p.v + hk * p.v_sh + (int64_t)k_first * p.v_sr;
+  const int k_srb = (int)p.k_sr * 2, v_srb = (int)p.v_sr * 2;
+  const i32x4 krsrc = packed_rsrc(kp, m, S::ROWB, k_srb), vrsrc = packed_rsrc(vp, m, S::ROWB, v_srb);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(LVAR_LDS char*)smem;
+  auto request = [&](int t, int k_pl) {   // tile t into the place k_pl of the keys' ring
+    fill_tile<D, NW>(krsrc, k_srb, 64 * t, lds0 + k_pl, wave, lane);
+    fill_tile<D, NW>(vrsrc, v_srb, 64 * t, lds0 + (3 + (t & 1)) * TILE, wave, lane);
+  };
+  if (p.dq && T > 0) request(0, 0);
+
   // q and do of the row; delta from do and o, half of the columns in each of the lanes l and l^32
   bf16x8 qf[KS], gf[KS];
   float delta = 0.f;
@@ -175,17 +186,10 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
 
   f32x16 acc[MTD];
   clear(acc);
-  const bf16_t *kp = p.k + hk * p.k_sh + (int64_t)k_first * p.k_sr, *vp = p.v + hk * p.v_sh + (int64_t)k_first * p.v_sr;
   if (!p.dq) return;
   if (T > 0) {
-    const int k_srb = (int)p.k_sr * 2, v_srb = (int)p.v_sr * 2;
-    const i32x4 krsrc = packed_rsrc(kp, m, S::ROWB, k_srb), vrsrc = packed_rsrc(vp, m, S::ROWB, v_srb);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(LVAR_LDS char*)smem, k_rows = lds0 + at.row_at, v_rows = k_rows + 3 * TILE, k_cols = lds0 + at.tr_at;
+    const uint32_t k_rows = lds0 + at.row_at, v_rows = k_rows + 3 * TILE, k_cols = lds0 + at.tr_at;
     constexpr int NS = 2 * KS, NP = 2 * MTD, NT = NS + NP, AHEAD = 2;
-    auto request = [&](int t, int k_pl) {   // tile t into the place k_pl of the keys' ring
-      fill_tile<D, NW>(krsrc, k_srb, 64 * t, lds0 + k_pl, wave, lane);
-      fill_tile<D, NW>(vrsrc, v_srb, 64 * t, lds0 + (3 + (t & 1)) * TILE, wave, lane);
-    };
     auto land = [&]() {
       wait_fills<0>();
       __syncthreads();
@@ -248,7 +252,6 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
     constexpr int SUB_ROWS = 32 * S::ROWB, SUB_COLS = 32 * S::ROWB;
     f32x16 sa, da, sb, db;
     int k_pl = 0, k_next = TILE;   // places of the present tile and of the next one
-    request(0, 0);
     land();
     if (T > 1) request(1, TILE);
     auto arrive = [&](int t) {   // tile t is there, the next one is requested
