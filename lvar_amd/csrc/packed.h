@@ -26,6 +26,7 @@ struct PackedParams {
   int shares;                       // set at launch: workgroups that share the keys of a query tile, or the query rows of a key tile
   float* parts;                     // their sums: [shares][H][T][D] of o or dq, [shares][dk, dv][Hkv][Tk][D]
   float* part_stats;                // forward: [shares][H][T][3] what their P refers to, its sum, the maximum
+  int settle;                       // set at launch: deltas of rows with few keys are corrected, see packed_dq_kernel
   float* stats;                     // [H,2,T]: -(M + log2 L) / c (-inf: the row sees nothing), and -sum(do * o)
 };
 

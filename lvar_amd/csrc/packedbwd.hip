@@ -114,8 +114,13 @@ struct DqSlots {
 // owns a query column, and dS^T is in the B operand's layout of dq^T += K^T dS^T as it is.  A step forms S and dP of the coming 32 keys on the
 // matrix cores while the vector ALU turns those of the present ones into dS, and adds them.  The barrier of a tile of 64 keys lies between its
 // two steps' products: the first S of the next tile is formed beside the second dS of this one, whose keys stay (hence three buffers).
+//
+// delta comes from o, which is rounded: sum_j P (dP - delta), which should be 0, is off.  In rows of few keys, where o is no mean of many values, that is as
+// large as the rounding of dS; waves whose rows have all their keys in one tile form that sum first and take it off (settle): dq and dk of the sequences
+// below are then off by 0.0024 of their size instead of 0.0025 (0.0024 instead of 0.0026 if they have 110 tokens each), for 1 % of the time.
+//
 // 12 sequences of up to 2047 tokens, 32 heads over 8 of 128, causal: 244 us with a step's products, vector work and sums one behind the other, 228 so,
-// 222 without tiles that none of a wave's rows sees: 810 TFLOP/s, matrix cores busy 48 % of the cycles.  16384 rows of 16 heads of 64 over 811 keys in
+// 222 without tiles that none of a wave's rows sees, 225 with settled deltas: 810 TFLOP/s, matrix cores busy 48 % of the cycles.  16384 rows of 16 heads of 64 over 811 keys in
 // four texts: 46 -> 44 us. ----
 
 template <int D, int NW, bool SPLIT>
@@ -157,7 +162,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
     fill_tile<D, NW>(krsrc, k_srb, 64 * t, lds0 + k_pl, wave, lane);
     fill_tile<D, NW>(vrsrc, v_srb, 64 * t, lds0 + (3 + (t & 1)) * TILE, wave, lane);
   };
-  if (p.dq && T > 0) request(0, 0);
+  if (T > 0) request(0, 0);
 
   // q and do of the row; delta from do and o, half of the columns in each of the lanes l and l^32
   bf16x8 qf[KS], gf[KS];
@@ -177,7 +182,8 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
   const int64_t stat = (int64_t)h * p.T + trow;
   const float M = p.M[stat], L = p.L[stat];
   const bool sees = all_seen_by(row) > 0;
-  const float nl = sees ? -(M + __builtin_amdgcn_logf(L)) / c : -INFINITY, nd = sees ? -delta : 0.f;
+  const float nl = sees ? -(M + __builtin_amdgcn_logf(L)) / c : -INFINITY;
+  float nd = sees ? -delta : 0.f;
   if (hh == 0 && live && share == 0) {
     float* to = p.stats + (int64_t)h * 2 * p.T + trow;
     to[0] = nl;
@@ -186,7 +192,8 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
 
   f32x16 acc[MTD];
   clear(acc);
-  if (!p.dq) return;
+  const bool settle = !SPLIT && p.settle;
+  if (!p.dq && (!settle || T > 3)) return;   // (beyond three tiles no wave has one alone)
   if (T > 0) {
     const uint32_t k_rows = lds0 + at.row_at, v_rows = k_rows + 3 * TILE, k_cols = lds0 + at.tr_at;
     constexpr int NS = 2 * KS, NP = 2 * MTD, NT = NS + NP, AHEAD = 2;
@@ -273,6 +280,22 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
     const int whole = min(mine, seen_first >> 6);                                 // and that all of them see whole
     int t = 1;
     if (mine > 0) {
+      if (settle && mine == 1) {
+        starts(Yes{}, 0, 0, sa, da);
+        step(Yes{}, No{}, k_rows, v_rows, k_cols, sb, db, sa, da);
+        starts(Yes{}, 0, 1, sb, db);
+        step(Yes{}, No{}, k_rows + SUB_ROWS, v_rows + SUB_ROWS, k_cols, sa, da, sb, db);
+        const int lim = seen - 4 * hh;
+        float off = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int key = 8 * (i >> 2) + (i & 3);
+          const float x = fast_exp2(sa[i] * c) * da[i], y = fast_exp2(sb[i] * c) * db[i];
+          off += (key < lim ? x : 0.f) + (key + 32 < lim ? y : 0.f);
+        }
+        nd -= xhalf_sum(off);
+        if (hh == 0 && live) p.stats[(int64_t)h * 2 * p.T + p.T + trow] = nd;
+      }
       starts(Yes{}, 0, 0, sa, da);
       step(Yes{}, No{}, k_rows, v_rows, k_cols, sb, db, sa, da);
       starts(Yes{}, 0, 1, sb, db);
@@ -288,6 +311,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
     store_part<D>(smem + wave * (32 * (D * 2 + 16)), acc, p.parts + (((int64_t)share * p.H + h) * p.T + w.first + q0) * D, w.n - q0, lane);
     return;
   }
+  if (!p.dq) return;
   bf16_t* to = p.dq + h * p.dq_sh + (int64_t)(w.first + q0) * p.dq_sr;
   store_rows<D>(smem + wave * (32 * (D * 2 + 16)), acc, p.scale, to, p.dq_sr, w.n - q0, lane);
   if (p.causal) {
@@ -368,7 +392,7 @@ struct Dkv {
 #if defined(__HIP_DEVICE_COMPILE__)
 
 // P passes between two waves as the upper 24 bits of its fp32: 16 of two elements to a word, the next 8 of four to another.  (As bf16
-// dk is off by 0.0030 of its size instead of 0.0025, which is as far as dq; rounded once, at its end, it would be by 0.0017.  It costs 5 % of the kernel at head_dim
+// dk is off by 0.0030 of its size instead of 0.0025, as dq; rounded once, at its end, it would be by 0.0017.  It costs 5 % of the kernel at head_dim
 // 128, 15 % at 64: 272 -> 286 us, 53 -> 61 us.)
 __device__ __forceinline__ uint32_t word(float x) { return __builtin_bit_cast(uint32_t, x); }
 __device__ __forceinline__ uint32_t upper16(float a, float b) { return __builtin_amdgcn_perm(word(b), word(a), 0x07060302u); }
@@ -741,6 +765,7 @@ template <int D>
 static int launch_bwd(PackedParams p, void* workspace, hipStream_t s) {
   p.stats = (float*)workspace;
   p.parts = p.stats + ((int64_t)p.H * 2 * p.T + 3) / 4 * 4;
+  p.settle = dq_shares(p, D, true) == 1;
   p.shares = dq_shares(p, D, p.dq != nullptr);
   const int st = p.shares > 1 ? launch_dq<D, true>(p, s) : launch_dq<D, false>(p, s);
   if (st != LVAR_OK || (!p.dk && !p.dv)) return st;
