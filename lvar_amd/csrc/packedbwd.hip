@@ -162,7 +162,9 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
     fill_tile<D, NW>(krsrc, k_srb, 64 * t, lds0 + k_pl, wave, lane);
     fill_tile<D, NW>(vrsrc, v_srb, 64 * t, lds0 + (3 + (t & 1)) * TILE, wave, lane);
   };
-  if (T > 0) request(0, 0);
+  // without dq: only statistics, and deltas that are settled (beyond three tiles no wave has one alone)
+  const bool settle = !SPLIT && p.settle, runs = p.dq || (settle && T <= 3);
+  if (runs && T > 0) request(0, 0);
 
   // q and do of the row; delta from do and o, half of the columns in each of the lanes l and l^32
   bf16x8 qf[KS], gf[KS];
@@ -192,8 +194,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
 
   f32x16 acc[MTD];
   clear(acc);
-  const bool settle = !SPLIT && p.settle;
-  if (!p.dq && (!settle || T > 3)) return;   // (beyond three tiles no wave has one alone)
+  if (!runs) return;
   if (T > 0) {
     const uint32_t k_rows = lds0 + at.row_at, v_rows = k_rows + 3 * TILE, k_cols = lds0 + at.tr_at;
     constexpr int NS = 2 * KS, NP = 2 * MTD, NT = NS + NP, AHEAD = 2;
