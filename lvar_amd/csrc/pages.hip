@@ -1,7 +1,7 @@
 // The life of the pages of a cache: dropping, opening and forking the pages that a table names, with a count of names per page, and copying chosen
 // tokens of a sequence to other pages.  Nothing of it comes from the host: a step captured in a graph is replayed with other lengths.
 //
-// All of it is latency: 192 samples of 48 prompts (240 rows, 1500 pages) drop 2.8, search 4.9, fork 7.5 (50 MB read and written), open 5.4 us; 4 samples of
+// All of it is latency: 192 samples of 48 prompts (240 rows, 1500 pages) drop 2.8, search 3.9, fork 7.5 (50 MB read and written), open 5.6 us; 4 samples of
 // one 2.5 + 3.4 + 3.4 + 2.9.
 //
 // Which free page (refs <= 0) a call hands out is fixed: the lowest ones, in the order of rows and entries.  One workgroup finds them: it adds up
@@ -11,7 +11,7 @@
 namespace lvar {
 
 // threads of the search; pages that it keeps in LDS; rows of a table of which pairs are checked
-constexpr int PG_FEW = 64, PG_T = 1024, PG_LIST = 4096, PG_MARKS = 65536 / 32;
+constexpr int PG_FEW = 64, PG_SOME = 256, PG_T = 1024, PG_LIST = 4096, PG_MARKS = 65536 / 32;
 
 // Sum over the workgroup ahead of this thread, and of all; `part` has a place for every wave.
 template <int T, class I>
@@ -252,11 +252,17 @@ int64_t pages_scratch_ints(int forks, int num_pages) {
   return forks + (num_pages > PG_LIST ? num_pages : 0);
 }
 
-// One wave where it sees all pages at once and needs no barrier (33 pages: the search of four forks 4.8 -> 3.4 us, of four rows 5.3 -> 2.9 us)
-static bool few(const PagesParams& p) { return p.n <= PG_FEW && p.num_pages <= 4 * PG_FEW; }
+// Threads of a search.  One wave where it sees all pages at once and needs no barrier (33 pages: the search of four forks 4.8 -> 3.4 us, of four rows 5.3
+// -> 2.9 us); four where they see them in two looks and hold all rows, 16 beyond (4 / 16 waves: 20 rows or forks on 1000 pages 3.4 / 5.1 and 3.6 / 4.6 us, 192 on 1500
+// pages, all taken but the last 5.7 / 5.4 and 5.1 / 5.1, on 4096 7.8 / 6.0 and 6.9 / 5.8).
+static int threads(const PagesParams& p) {
+  return p.n <= PG_FEW && p.num_pages <= 4 * PG_FEW ? PG_FEW : p.n <= PG_SOME && p.num_pages <= 8 * PG_SOME ? PG_SOME : PG_T;
+}
 
 int launch_pages_alloc(const PagesParams& p, hipStream_t s) {
-  if (few(p)) hipLaunchKernelGGL(pages_alloc_kernel<PG_FEW>, dim3(1), dim3(PG_FEW), 0, s, p);
+  const int t = threads(p);
+  if (t == PG_FEW) hipLaunchKernelGGL(pages_alloc_kernel<PG_FEW>, dim3(1), dim3(PG_FEW), 0, s, p);
+  else if (t == PG_SOME) hipLaunchKernelGGL(pages_alloc_kernel<PG_SOME>, dim3(1), dim3(PG_SOME), 0, s, p);
   else hipLaunchKernelGGL(pages_alloc_kernel<PG_T>, dim3(1), dim3(PG_T), 0, s, p);
   return status();
 }
@@ -267,7 +273,9 @@ int launch_pages_free(const PagesParams& p, hipStream_t s) {
 }
 
 int launch_pages_fork(const PagesParams& p, const PagedView& c, int row_bytes, hipStream_t s) {
-  if (few(p)) hipLaunchKernelGGL(pages_fork_find_kernel<PG_FEW>, dim3(1), dim3(PG_FEW), 0, s, p);
+  const int t = threads(p);
+  if (t == PG_FEW) hipLaunchKernelGGL(pages_fork_find_kernel<PG_FEW>, dim3(1), dim3(PG_FEW), 0, s, p);
+  else if (t == PG_SOME) hipLaunchKernelGGL(pages_fork_find_kernel<PG_SOME>, dim3(1), dim3(PG_SOME), 0, s, p);
   else hipLaunchKernelGGL(pages_fork_find_kernel<PG_T>, dim3(1), dim3(PG_T), 0, s, p);
   const int st = status();
   if (st != LVAR_OK) return st;

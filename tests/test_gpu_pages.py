@@ -53,7 +53,7 @@ def tables(rows, width, P, seed, holes=True):
     return table, refs
 
 
-@pytest.mark.parametrize("rows,width,P", [(1, 1, 1), (3, 5, 7), (7, 300, 4000), (64, 33, 2500), (5000, 3, 20000), (2, 9000, 20001)])
+@pytest.mark.parametrize("rows,width,P", [(1, 1, 1), (3, 5, 7), (20, 9, 300), (200, 12, 1900), (7, 300, 4000), (64, 33, 2500), (5000, 3, 20000), (2, 9000, 20001)])
 def test_free_and_alloc(rows, width, P, host_path):
     from lvar_amd import kv_cache_ops as kv
     table, refs = tables(rows, width, P, seed=rows)
@@ -149,7 +149,7 @@ def test_many_forks(host_path):
     assert bool((cache.v.view(torch.int16)[fresh, 0, :5] == cache.v.view(torch.int16)[9050, 0, :5]).all())
 
 
-@pytest.mark.parametrize("rows", [6, 40, 5000])
+@pytest.mark.parametrize("rows", [6, 40, 400, 5000])
 def test_forks_that_depend_on_each_other(rows, host_path):
     """Targets that are named twice, or sources themselves, are left out; nothing of their rows, pages and counts changes."""
     from lvar_amd import kv_cache_ops as kv
