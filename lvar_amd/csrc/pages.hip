@@ -156,6 +156,7 @@ __global__ __launch_bounds__(T) void pages_fork_find_kernel(const PagesParams p)
     return done + all;
   };
   for (int r0 = 0; r0 < p.n; r0 += T) N = wants(r0, N);
+  N = min(N, p.num_pages);   // (a list that LDS does not hold is then of a pool that has its place behind the forks, see pages_scratch_ints)
   int* list = N <= PG_LIST ? lds_list : p.scratch + p.n;
   const int found = N > 0 ? find_free<T>(p, bits, N, list, part) : 0;
   int done = 0;
