@@ -183,7 +183,8 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
   delta = xhalf_sum(delta);
   const int64_t stat = (int64_t)h * p.T + trow;
   const float M = p.M[stat], L = p.L[stat];
-  const bool sees = all_seen_by(row) > 0;
+  // (no key, or none with a weight: M and L as the forward pass writes them then; with M in the start of its sums P would be NaN)
+  const bool sees = all_seen_by(row) > 0 && !(bits_of(M) == 0xff800000u && bits_of(L) == 0x3f800000u);
   const float nl = sees ? -(M + __builtin_amdgcn_logf(L)) / c : -INFINITY;
   float nd = sees ? -delta : 0.f;
   if (hh == 0 && live && share == 0) {
