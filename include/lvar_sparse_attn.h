@@ -550,8 +550,8 @@ int lvar_paged_attn_fwd(lvar_tensor_t q, lvar_paged_cache_t cache, const int32_t
  * Attention over packed sequences.  Sequence b of `batch` has queries offsets[b] .. offsets[b+1]-1 of q [H,tokens,d] and keys
  * k_offsets[b] .. k_offsets[b+1]-1 of k, v [kv_heads,k_tokens,d] (bf16 views; stride_b is not used; int32 [batch+1] on the device,
  * ascending, the same array where queries and keys are of the same tokens).  Row i of n queries over m keys sees keys j < m - n + i + 1
- * (causal) or all m.  o = softmax(q k^T scale) v (bf16 view [H,tokens,d]), M and L fp32 [H,tokens] as everywhere here.  Rows that see no key,
- * and rows of no sequence (ahead of the first offset, behind the last), get o = 0, M = -inf, L = 1.  Query head h reads key/value head
+ * (causal) or all m.  o = softmax(q k^T scale) v (bf16 view [H,tokens,d]), M and L fp32 [H,tokens] as everywhere here.  Rows that see no key (or only
+ * scores below -10^30, -infinity among them), and rows of no sequence (ahead of the first offset, behind the last), get o = 0, M = -inf, L = 1.  Query head h reads key/value head
  * h / (H / kv_heads).  head_dim 64, 128 or 256; rows 16-byte aligned; a head's rows span less than 2^31 bytes.  A value that is not finite reaches
  * the rows that see it and no others.  Scores, M, L and sums are fp32; probabilities enter the second product as bf16 (2^-9).
  * workspace: lvar_packed_attn_fwd_workspace_bytes() (often 0; 16-byte aligned, written and read by this call).

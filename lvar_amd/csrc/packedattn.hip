@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256) void packed_fwd_join_kernel(const PackedParams
   bf16_t* to = p.o + h * p.o_sh + (int64_t)row * p.o_sr;
   if (x < rows) {
     if (column == 0) {
-      p.M[at] = M;
+      p.M[at] = any ? M : -INFINITY;
       p.L[at] = any ? L : 1.0f;
     }
     *(u32x2*)(to + column) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};

@@ -115,7 +115,7 @@ def packed_attn(q, k, v, offsets, k_offsets=None, scale=None, causal: bool = Tru
     any strides: the views of a fused projection are read in place.  ``offsets`` int32 ``[B+1]``, on the device, ascending: sequence b has the
     queries ``offsets[b] .. offsets[b+1]-1``; and the keys ``k_offsets[b] .. k_offsets[b+1]-1``, the same by default.  ``causal``: row i of n queries
     sees keys ``j < m - n + i + 1`` of m, its own position and those ahead of it where n = m; otherwise all.  Sequences may be empty.  Rows that see
-    no key (or only scores of -infinity), and rows ahead of the first sequence or behind the last, get ``o = 0, M = -inf, L = 1``; rows of no sequence get zero gradients.
+    no key (or only scores below -10^30, -infinity among them), and rows ahead of the first sequence or behind the last, get ``o = 0, M = -inf, L = 1``; rows of no sequence get zero gradients.
     The lengths are read by the kernels: a captured call is replayed with others.
 
     ``head_dim`` 16, 32, 64, 128 or 256.  Scores, statistics and sums are fp32 (a score x is off by up to 2^-24 of

@@ -90,9 +90,9 @@ def made(case):
 
 
 @pytest.mark.parametrize("case", CASES, ids=str)
-@pytest.mark.parametrize("power", [100])
+@pytest.mark.parametrize("power", [60, 100])
 def test_rows_of_finite_elements(case, power):
-    """Every fifth row meets every key at -2^200, which 32 bits do not hold."""
+    """Every fifth row meets every key at -2^120 (a number) or -2^200 (which 32 bits do not hold)."""
     q, k, v, off, koff, causal = made(case)
     k[..., 0] = 2.0 ** power
     q[..., 0] = 0
