@@ -12,7 +12,8 @@ namespace lvar {
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
-// One row of a gradient whose sums are not finite, pair by pair: 0 * infinity from a row that does not see a key must not stay in it.
+// One row of a gradient whose sums are not finite, pair by pair: 0 * infinity from a row that does not see a key, or from the zeros behind the last row
+// or key of a tile, must not stay in it.
 // x0, x1: the fixed row (of q and do, or of k and v); y0, y1: the rows of the other side, lo .. hi-1.  ds weighs y0, P weighs y1 (KEY).
 // Rare, and so plain: lanes are pairs for the products, columns for the sums.
 template <int D, bool KEY>
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void packed_dq_kernel(co
   if (!p.dq) return;
   bf16_t* to = p.dq + h * p.dq_sh + (int64_t)(w.first + q0) * p.dq_sr;
   store_rows<D>(smem + wave * (32 * (D * 2 + 16)), acc, p.scale, to, p.dq_sr, w.n - q0, lane);
-  if (p.causal) {
+  if (p.causal || m_all % 64 != 0) {
     uint64_t rows = __builtin_amdgcn_ballot_w64(any_not_finite(acc) && live);
     rows = (rows | rows >> 32) & 0xffffffffu;
     if (rows) wait_fills<0>();   // the rows as stored above are written again
@@ -343,7 +344,6 @@ __global__ __launch_bounds__(256) void packed_dq_join_kernel(const PackedParams 
   const int64_t rows = (int64_t)p.H * p.T, x = (int64_t)__builtin_amdgcn_workgroup_id_x() * RPG + tid / LPR, at = min(x, rows - 1);
   const int h = (int)(at / p.T), row = (int)(at - (int64_t)h * p.T);
   uint64_t left = __builtin_amdgcn_ballot_w64(join_part(p.parts + at * D + column, rows * D, p.shares, p.scale, x < rows ? p.dq + h * p.dq_sh + (int64_t)row * p.dq_sr + column : nullptr));
-  if (!p.causal) return;
   if (left) wait_fills<0>();   // the rows as stored above are written again
   while (left) {
     const int i = __builtin_ctzll(left) / LPR * LPR;   // the first lane of a row
@@ -351,7 +351,8 @@ __global__ __launch_bounds__(256) void packed_dq_join_kernel(const PackedParams 
     const int hi = __builtin_amdgcn_readlane(h, i), ri = __builtin_amdgcn_readlane(row, i), hk = hi / p.G;
     PackedTile w;
     find_row(p.q_off, p.T, p.k_off, p.Tk, p.B, ri, w);
-    const int seen = max(0, min(w.other_n, w.row0 + w.other_n - w.n + 1));
+    if (!p.causal && w.other_n % 64 == 0) continue;
+    const int seen = p.causal ? max(0, min(w.other_n, w.row0 + w.other_n - w.n + 1)) : w.other_n;
     const float* st = p.stats + (int64_t)hi * 2 * p.T + ri;
     CarefulRow<D, false> a;
     a.clear();
@@ -664,7 +665,7 @@ __device__ __forceinline__ void dkv_wave(const PackedParams& p, char* smem, cons
   const int64_t out_sr = ROLE ? p.dk_sr : p.dv_sr;
   bf16_t* to = out + hk * (ROLE ? p.dk_sh : p.dv_sh) + (int64_t)(w.first + k0) * out_sr;
   store_rows<D>(smem + all_waves * (32 * (D * 2 + 16)), acc, ROLE ? p.scale : 1.f, to, out_sr, w.n - k0, lane);
-  if (p.causal) {
+  if (p.causal || n % Q::R != 0) {
     uint64_t keys = __builtin_amdgcn_ballot_w64(any_not_finite(acc) && k0 + r < w.n);
     keys = (keys | keys >> 32) & 0xffffffffu;
     if (keys) wait_fills<0>();   // the rows as stored above are written again
@@ -703,7 +704,6 @@ __global__ __launch_bounds__(256) void packed_dkv_join_kernel(const PackedParams
   const int hk = (int)(at / p.Tk), row = (int)(at - (int64_t)hk * p.Tk);
   bf16_t* to = out + hk * (role ? p.dk_sh : p.dv_sh) + (int64_t)row * (role ? p.dk_sr : p.dv_sr) + column;
   uint64_t left = __builtin_amdgcn_ballot_w64(join_part(p.parts + (role * rows + at) * D + column, 2 * rows * D, p.shares, role ? p.scale : 1.f, x < rows ? to : nullptr));
-  if (!p.causal) return;
   if (left) wait_fills<0>();   // the rows as stored above are written again
   while (left) {
     const int i = __builtin_ctzll(left) / LPR * LPR;   // the first lane of a row
@@ -711,7 +711,8 @@ __global__ __launch_bounds__(256) void packed_dkv_join_kernel(const PackedParams
     const int hi = __builtin_amdgcn_readlane(hk, i), ri = __builtin_amdgcn_readlane(row, i);
     PackedTile w;
     find_row(p.k_off, p.Tk, p.q_off, p.T, p.B, ri, w);
-    const int from = max(0, w.row0 - (w.n - w.other_n));
+    if (!p.causal && w.other_n % Dkv<D>::R == 0) continue;
+    const int from = p.causal ? max(0, w.row0 - (w.n - w.other_n)) : 0;
     if (role) careful_key<D, 1>(p, w, hi, w.row0, from); else careful_key<D, 0>(p, w, hi, w.row0, from);
   }
 #endif
