@@ -41,8 +41,8 @@ inline int64_t packed_slots(int T, int B, int R) { return (int64_t)T / R + B + 2
 
 // Workgroups that share the keys of a query tile of 128 rows, where query tiles alone leave compute units idle (few rows over many keys, few heads): as
 // many as fill the waves that a SIMD holds, twice that if causal, where the last tile has twice the work of the mean one.  None gets fewer than
-// SHARE_TILES tiles of the mean sequence: parts cost a launch and 8 bytes of traffic per element, about what 9 us of products are worth.  Against one
-// workgroup per tile, forward / dq, the sum of the parts included: 64 rows of 8 heads of 128 over 8192 keys 93 -> 22 / 144 -> 28 us; 16384 rows
+// SHARE_TILES tiles of the mean sequence (lengths are on the device: one long sequence among many short ones is not shared): parts cost a launch and
+// 8 bytes of traffic per element, about what 9 us of products are worth.  Against one workgroup per tile, forward / dq, the sum of the parts included: 64 rows of 8 heads of 128 over 8192 keys 93 -> 22 / 144 -> 28 us; 16384 rows
 // of one head, causal 198 -> 91 / 302 -> 126 us; 9360 rows of 4 heads of 64, causal 95 -> 71 / 126 -> 90 us.  With shares of 4 tiles 2048 rows of 16 heads of
 // 128, causal lost: 35 -> 44 / 51 -> 55 us.
 inline int query_shares(const PackedParams& p, int waves_per_simd) {
@@ -89,7 +89,8 @@ __device__ __forceinline__ int packed_border(const int32_t* off, int B, int T, i
 // place belongs to is found among the borders without knowing the lengths in between: 64 candidates per step, and with up to 62 sequences in
 // one round trip to memory.  False: a place without a tile.
 //
-// `levels` (up to 62 sequences, a lane each): of a causal launch over key tiles those of a range differ in work, the first having the most
+// `levels` (up to 62 sequences, a lane each; beyond, the order of the places is kept, and what that costs there is not measured): of a causal launch
+// over key tiles those of a range differ in work, the first having the most
 // rows behind it, and the launch would end on whichever long one comes late: place by place the tiles with the most behind
 // them, of all ranges.  (12 sequences of up to 2047 tokens, 8 x 4 heads, in the kernel of that time:
 // 492 -> 404 us.  Query tiles, four times as many and each shorter: 3 % less for these, 2 % more for 16 prompts of up to 4096.)

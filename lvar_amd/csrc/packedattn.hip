@@ -8,9 +8,10 @@
 // maximum of S(t+1); one barrier per tile.  The maximum that P refers to is only raised where a row grows by more than 2^8 (exact: numerator and
 // denominator share it).  P is rounded to bf16 (2^-9 of each on average, and the errors of a row's keys are independent); its sum is not.
 //
-// Bound by the matrix cores at the clock that the power limit leaves: 32768 tokens of 32 heads over 8 of 128, causal, 7.22 ms, 1220 TFLOP/s with the
-// matrix cores busy 78 % of the cycles at 1.5 GHz; 16 ragged prompts of up to 4096 tokens 606 us, 1010 TFLOP/s (59 %), 12 sequences of up to 2047
-// 150 us, 795 TFLOP/s (48 %): a tile of a few keys pays for its start and end.  Every operand of a product is read from LDS, 1 KiB per product, which is what LDS gives
+// Bound by the matrix cores at the clock that the power limit leaves, which differs from card to card: 32768 tokens of 32 heads over 8 of 128, causal, 7.1 to
+// 7.6 ms, 1160 to 1240 TFLOP/s with the matrix cores busy 78 % of the cycles at 1.5 GHz; 16 ragged prompts of up to 4096 tokens 601 to 643 us, 960 to
+// 1020 TFLOP/s (59 %), 12 sequences of up to 2047 150 us, 795 TFLOP/s (48 %): a tile of a few keys pays for its start and end.
+// Every operand of a product is read from LDS, 1 KiB per product, which is what LDS gives
 // at full rate; with half of the reads left out (and wrong results) the same launches take 5 % less, so wider waves would not pay.
 #include "packed.h"
 

@@ -121,7 +121,8 @@ struct DqSlots {
 // below are then off by 0.0024 of their size instead of 0.0025 (0.0024 instead of 0.0026 if they have 110 tokens each), for 1 % of the time.
 //
 // 12 sequences of up to 2047 tokens, 32 heads over 8 of 128, causal: 244 us with a step's products, vector work and sums one behind the other, 228 so,
-// 222 without tiles that none of a wave's rows sees, 225 with settled deltas: 810 TFLOP/s, matrix cores busy 48 % of the cycles.  16384 rows of 16 heads of 64 over 811 keys in
+// 222 without tiles that none of a wave's rows sees, 225 with settled deltas (224 to 232 from card to card: 770 to 800 TFLOP/s), matrix cores busy 48 % of the
+// cycles.  16384 rows of 16 heads of 64 over 811 keys in
 // four texts: 46 -> 44 us. ----
 
 template <int D, int NW, bool SPLIT>
@@ -376,7 +377,8 @@ __global__ __launch_bounds__(256) void packed_dq_join_kernel(const PackedParams 
 //
 // Tiles come from the last rows to the first, all heads of a tile behind each other: the workgroups of a sequence, which all end at
 // its last rows, read the same tile at about the same time, from the L2 (from the first rows on, 71 % of the reads missed it); half of the reads
-// still come from further away, so tiles are requested LEAD rounds ahead.  The same sequences 286 us, 835 TFLOP/s, matrix cores busy 50 %. ----
+// still come from further away, so tiles are requested LEAD rounds ahead.  The same sequences 277 to 289 us from card to card, 825 to 860 TFLOP/s, matrix
+// cores busy 50 %. ----
 
 template <int D>
 struct Dkv {
@@ -394,9 +396,9 @@ struct Dkv {
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
-// P passes between two waves as the upper 24 bits of its fp32: 16 of two elements to a word, the next 8 of four to another.  (As bf16
-// dk is off by 0.0030 of its size instead of 0.0025, as dq; rounded once, at its end, it would be by 0.0017.  It costs 5 % of the kernel at head_dim
-// 128, 15 % at 64: 272 -> 286 us, 53 -> 61 us.)
+// P passes between two waves as the upper 24 bits of its fp32, cut (less than 2^-15 of it is lost, where dS is rounded to 2^-9): 16 of two elements to a
+// word, the next 8 of four to another.  (As bf16 dk is off by 0.0030 of its size instead of 0.0025, as dq; rounded once, at its end, it would be by
+// 0.0017.  It costs 5 % of the kernel at head_dim 128, 15 % at 64: 272 -> 286 us, 53 -> 61 us.)
 __device__ __forceinline__ uint32_t word(float x) { return __builtin_bit_cast(uint32_t, x); }
 __device__ __forceinline__ uint32_t upper16(float a, float b) { return __builtin_amdgcn_perm(word(b), word(a), 0x07060302u); }
 __device__ __forceinline__ uint32_t next8(float a, float b, float c, float d) {

@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(const PagesParams p, co
 
 // Token i of a head in the pages of `out`: token keep[b, head, i] of `c`, as its bytes are.  A row is read by `1 << per` lanes, 16 bytes each of
 // key and value.  Bound by memory, and by its round trips (table and position, then the row) where it is small: 2 x 16 heads keep 1052 of 10521 tokens of
-// 128 in bf16 7.3 us, 4.7 TB/s; 8 x 8 heads up to 4001 of 8191 in e4m3 15.6 us, 3.4 TB/s of rows of 128 bytes.
+// 128 in bf16 6.4 to 7.2 us, 4.8 to 5.4 TB/s read and written; 8 x 8 heads up to 4001 of 8191 in e4m3 15.5 us, 4.6 TB/s of rows of 128 bytes and their exponents.
 __global__ __launch_bounds__(256) void pages_compact_kernel(const CompactParams p, const int per) {
   const int lane = threadIdx.x & ((1 << per) - 1), i = (blockIdx.x << (8 - per)) + (threadIdx.x >> per);
   const int head = blockIdx.y, b = blockIdx.z;

@@ -952,7 +952,6 @@ LVAR_FAST(fast_paged_attn) {
   END_HANDLE_TH_ERRORS
 }
 
-// rows are read with 16-byte accesses: anything else is copied into a plain tensor first
 // ---- attention over packed sequences (lvar_amd.packed_ops) ----
 
 // rows that the kernels address with 31 bits (axes of one element may have any stride)
@@ -1069,6 +1068,7 @@ LVAR_FAST(fast_packed_attn) {
   END_HANDLE_TH_ERRORS
 }
 
+// rows are read with 16-byte accesses: anything else is copied into a plain tensor first
 at::Tensor as_plain(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.dim() == 4, name, " must be [B,H,L,d], got ", t.sizes());
   TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16, got ", t.scalar_type());
